@@ -1,0 +1,617 @@
+// The paged cache of include/gradhip.h: gh_cache_*.
+#include "api_error.h"
+#include "cache_attend.h"
+#include "kernels_cache.h"
+
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <memory>
+
+namespace gh {
+
+namespace {
+
+[[noreturn]] void refuse(const std::string& why) { throw ApiError{GH_ERR_INVALID_ARGUMENT, "cache: " + why}; }
+
+// The device a cache lives on is the current one while its calls run.
+struct DeviceScope {
+    int before = 0;
+    explicit DeviceScope(int device) {
+        HIP_CHECK(hipGetDevice(&before));
+        if (before != device) HIP_CHECK(hipSetDevice(device));
+        now = device;
+    }
+    ~DeviceScope() {
+        if (before != now) (void)hipSetDevice(before);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+    int now = 0;
+};
+
+struct DeviceBuffer {
+    char* at = nullptr;
+    size_t bytes = 0;
+    ~DeviceBuffer() {
+        if (at) (void)hipFree(at);
+    }
+    // Room for so many bytes, contents lost; what the stream still does with the old ones is waited for.
+    bool reserve(size_t want, hipStream_t stream) {
+        if (want <= bytes) return false;
+        HIP_CHECK(hipStreamSynchronize(stream));
+        if (at) HIP_CHECK(hipFree(at));
+        at = nullptr;
+        bytes = 0;
+        const size_t room = (want + want / 2 + 4095) / 4096 * 4096;
+        HIP_CHECK(hipMalloc(&at, room));
+        bytes = room;
+        return true;
+    }
+};
+
+// Pinned host memory that a kernel reads, two buffers in turn: a buffer is written again when the kernel that read it is done.
+struct Staging {
+    struct Slot {
+        char* at = nullptr;
+        size_t bytes = 0;
+        hipEvent_t read = nullptr;
+        bool pending = false;
+    } slots[2];
+    int turn = 0;
+
+    ~Staging() {
+        for (Slot& s : slots) {
+            if (s.at) (void)hipHostFree(s.at);
+            if (s.read) (void)hipEventDestroy(s.read);
+        }
+    }
+    char* reserve(size_t want) {
+        turn ^= 1;
+        Slot& s = slots[turn];
+        if (!s.read) HIP_CHECK(hipEventCreateWithFlags(&s.read, hipEventDisableTiming));
+        if (s.pending) HIP_CHECK(hipEventSynchronize(s.read));
+        s.pending = false;
+        if (want > s.bytes) {
+            if (s.at) HIP_CHECK(hipHostFree(s.at));
+            s.at = nullptr;
+            s.bytes = 0;
+            const size_t room = (want + want / 2 + 4095) / 4096 * 4096;
+            HIP_CHECK(hipHostMalloc(&s.at, room, hipHostMallocDefault));
+            s.bytes = room;
+        }
+        return s.at;
+    }
+    // The last reserved buffer's first bytes to the device.
+    void send(char* to, size_t bytes, hipStream_t stream) {
+        Slot& s = slots[turn];
+        const size_t words = (bytes + 15) / 16;
+        if (words == 0) return;
+        const int groups = static_cast<int>(std::min<size_t>(256, (words + 255) / 256));
+        hipLaunchKernelGGL(cache_load_kernel, dim3(groups), dim3(256), 0, stream, reinterpret_cast<const u32x4*>(s.at),
+                           reinterpret_cast<u32x4*>(to), words);
+        HIP_CHECK(hipGetLastError());
+        HIP_CHECK(hipEventRecord(s.read, stream));
+        s.pending = true;
+    }
+};
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+constexpr int kMaxHeads = 1024;
+constexpr int kMaxPageTokens = 1024;
+constexpr int kPlans = 4;
+
+}  // namespace
+
+struct Cache {
+    gh_cache_opts o{};
+    int device = 0;
+    int group = 1;
+    int bytes = 4;  // of an element
+    CacheLayout layout{};
+    PageBook book;
+    DeviceBuffer pool, speed, pass, lists, parts, arrived;
+    Staging staging;
+    hipEvent_t moved = nullptr;  // from one stream to the next
+    hipStream_t stream = nullptr;  // of the last call
+    bool used = false;             // ... if there was one
+
+    // the open pass
+    bool open = false;
+    int rows = 0;
+    std::vector<PassSeq> seqs;
+    std::vector<int> news;
+    size_t rows_at = 0, table_at = 0, items_at = 0;  // in `pass`, behind the sequences
+
+    // its attention, as it was last cut up for a mask
+    struct Plan {
+        bool valid = false;
+        bool causal = true;
+        int window = 0;
+        AttendForm form{};
+        AttendPlan cut;
+        DeviceBuffer items;             // empty for the plan that came with the pass
+        const AttendItem* at = nullptr;
+    } plans[kPlans];
+    int next_plan = 0;
+    bool last_causal = true;  // the mask of the last call: the next pass is planned for it
+    int last_window = 0;
+
+    Cache(const gh_cache_opts& opts, int pages, int page_tokens) : o(opts), book(pages, page_tokens) {}
+    ~Cache() {
+        (void)hipDeviceSynchronize();
+        if (moved) (void)hipEventDestroy(moved);
+    }
+
+    AttendForm form_for(int tiles) const {
+        return o.type == GH_F32 ? attend_form_f32(o.head_dim, tiles)
+             : o.type == GH_BF16 ? attend_form_bf16(o.head_dim, tiles)
+                                 : attend_form_f16(o.head_dim, tiles);
+    }
+
+    // Calls on one cache run in their order whatever streams they name: a call on another stream than the one before waits
+    // for what that one did.  Under capture a call would be replayed with the pages and lengths of today: refused.
+    void enter(void* hip_stream) {
+        const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        HIP_CHECK(hipStreamIsCapturing(st, &status));
+        if (status != hipStreamCaptureStatusNone)
+            throw ApiError{GH_ERR_RUNTIME, "cache: the stream is being captured into a graph; a replay would use the pages of the pass "
+                                           "that was open at capture"};
+        if (used && st != stream) {
+            if (!moved) HIP_CHECK(hipEventCreateWithFlags(&moved, hipEventDisableTiming));
+            HIP_CHECK(hipEventRecord(moved, stream));
+            HIP_CHECK(hipStreamWaitEvent(st, moved, 0));
+        }
+        stream = st;
+        used = true;
+    }
+
+    void close() {
+        open = false;
+        for (Plan& p : plans) p.valid = false;
+    }
+
+    void copy_pages(const char* from, const PageCopy* device_list, int n) {
+        if (n == 0) return;
+        const int runs = o.layers * 2 * o.kv_heads, token_bytes = o.head_dim * bytes;
+        // ~2048 workgroups: eight per compute unit
+        const int x = std::max(1, std::min(runs, 2048 / std::min(n, 2048)));
+        hipLaunchKernelGGL(cache_copy_kernel, dim3(x, std::min(n, 65535)), dim3(256), 0, stream, from, pool.at, layout.page_bytes, runs,
+                           static_cast<int>(layout.run_bytes / 16), token_bytes, device_list, n);
+        HIP_CHECK(hipGetLastError());
+    }
+
+    // How the pass's attention is cut, and room for what its parts leave.
+    void cut(Plan& plan, bool causal, int window) {
+        int most = 0;
+        for (int n : news) most = std::max(most, n * group);
+        plan.causal = causal;
+        plan.window = window;
+        plan.form = form_for(most > 16 ? 2 : 1);
+        plan.cut = plan_attend(seqs, news, group, o.kv_heads, plan.form.height, causal, window, 1024, 128);
+        const size_t part_bytes = static_cast<size_t>(plan.cut.parts) * o.kv_heads * plan.form.part_floats * sizeof(float);
+        parts.reserve(part_bytes, stream);
+        if (arrived.reserve(static_cast<size_t>(plan.cut.tiles) * o.kv_heads * sizeof(unsigned), stream))
+            HIP_CHECK(hipMemsetAsync(arrived.at, 0, arrived.bytes, stream));
+    }
+};
+
+static void check_rows(const char* what, const gh_rows* r, int heads, int dim) {
+    if (!r || !r->data) refuse(std::string(what) + " is null");
+    if (r->row_stride < 0 || r->head_stride < 0) refuse(std::string(what) + " has a negative stride");
+    (void)heads;
+    (void)dim;
+}
+
+// Rows that are written must not lie on top of one another.
+static void check_apart(const char* what, const gh_rows* r, long long rows, int heads, int dim) {
+    const long long row = r->row_stride, head = r->head_stride;
+    const bool heads_inside = (heads == 1 || head >= dim) && (rows == 1 || row >= (heads - 1) * head + dim);
+    const bool rows_inside = (rows == 1 || row >= dim) && (heads == 1 || head >= (rows - 1) * row + dim);
+    if (!heads_inside && !rows_inside) refuse(std::string(what) + "'s rows overlap");
+}
+
+static bool aligned(const gh_rows* r, int bytes, bool one_row, bool one_head) {
+    return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && (one_row || r->row_stride * bytes % 16 == 0)
+           && (one_head || r->head_stride * bytes % 16 == 0);
+}
+
+static CacheRows cache_rows(const gh_rows* r) { return CacheRows{static_cast<char*>(r->data), r->row_stride, r->head_stride}; }
+
+static gh_cache_opts checked(const gh_cache_opts& in) {
+    gh_cache_opts o = in;
+    if (o.page_tokens == 0) o.page_tokens = 64;
+    if (o.layers < 1 || o.layers > 4096) refuse("layers must be 1 to 4096");
+    if (o.kv_heads < 1 || o.heads < 1 || o.heads > kMaxHeads) refuse("heads must be 1 to 1024");
+    if (o.heads % o.kv_heads != 0) refuse("heads must be a multiple of kv_heads");
+    if (o.head_dim < 8 || o.head_dim > 256 || o.head_dim % 8 != 0) refuse("head_dim must be a multiple of 8, 8 to 256");
+    if (o.type != GH_F32 && o.type != GH_BF16 && o.type != GH_F16) refuse("unknown element type");
+    if (o.page_tokens < 16 || o.page_tokens > kMaxPageTokens || (o.page_tokens & (o.page_tokens - 1)))
+        refuse("page_tokens must be a power of two, 16 to 1024");
+    if (o.pages < 1 || o.pages > (INT_MAX - kMaxPageTokens) / o.page_tokens) refuse("pages x page_tokens must be 1 to 2^31");
+    if (!(o.rope_base >= 0.0f) || std::isinf(o.rope_base)) refuse("rope_base must be a finite number, 0 for no rotation");
+    return o;
+}
+
+static std::unique_ptr<Cache> create_cache(const gh_cache_opts& in) {
+    const gh_cache_opts o = checked(in);
+    require_gpu();
+    auto c = std::make_unique<Cache>(o, o.pages, o.page_tokens);
+    HIP_CHECK(hipGetDevice(&c->device));
+    c->group = o.heads / o.kv_heads;
+    c->bytes = o.type == GH_F32 ? 4 : 2;
+    CacheLayout& l = c->layout;
+    l.run_bytes = static_cast<size_t>(o.page_tokens) * o.head_dim * c->bytes;
+    l.page_bytes = l.run_bytes * o.kv_heads * 2 * o.layers;
+    l.kv_heads = o.kv_heads;
+    l.dim = o.head_dim;
+    l.layers = o.layers;
+    while ((1 << l.page_shift) < o.page_tokens) l.page_shift++;
+    const size_t bytes = l.page_bytes * static_cast<size_t>(o.pages);
+    const hipError_t e = hipMalloc(&c->pool.at, bytes);
+    if (e == hipErrorOutOfMemory) {
+        (void)hipGetLastError();
+        throw ApiError{GH_ERR_DEVICE, "cache: no memory for a pool of " + std::to_string(bytes) + " bytes"};
+    }
+    HIP_CHECK(e);
+    c->pool.bytes = bytes;
+    l.pool = c->pool.at;
+    if (o.rope_base > 0.0f) {
+        // in turns per position, 64 bits
+        std::vector<double> speed(static_cast<size_t>(o.head_dim) / 2);
+        for (size_t j = 0; j < speed.size(); j++)
+            speed[j] = std::pow(static_cast<double>(o.rope_base), -2.0 * static_cast<double>(j) / o.head_dim) / (2.0 * M_PI);
+        HIP_CHECK(hipMalloc(&c->speed.at, speed.size() * sizeof(double)));
+        c->speed.bytes = speed.size() * sizeof(double);
+        HIP_CHECK(hipMemcpy(c->speed.at, speed.data(), c->speed.bytes, hipMemcpyHostToDevice));
+    }
+    return c;
+}
+
+// A sequence's pages' contents into a new sequence of `to`.
+static int copy_sequence(Cache& from, Cache& to, int seq, void* stream) {
+    const PageBook::Sequence& s = from.book.at(seq);
+    const int length = s.length, n = static_cast<int>(s.pages.size());
+    if (&from != &to) from.enter(stream);
+    to.enter(stream);
+    const size_t bytes = static_cast<size_t>(n) * sizeof(PageCopy);
+    to.lists.reserve(bytes, to.stream);
+    PageCopy* list = reinterpret_cast<PageCopy*>(to.staging.reserve(bytes));
+    const int id = to.book.add_filled(length);
+    const std::vector<int>& a = from.book.at(seq).pages;
+    const std::vector<int>& b = to.book.at(id).pages;
+    for (int i = 0; i < n; i++)
+        list[i] = {a[static_cast<size_t>(i)], b[static_cast<size_t>(i)], std::min(from.o.page_tokens, length - i * from.o.page_tokens)};
+    if (n > 0) {
+        to.staging.send(to.lists.at, bytes, to.stream);
+        to.copy_pages(from.pool.at, reinterpret_cast<const PageCopy*>(to.lists.at), n);
+    }
+    return id;
+}
+
+static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, int n, void* stream) {
+    long long rows = 0, pages = 0;
+    c.close();
+    for (int i = 0; i < n; i++) {
+        const int length = c.book.at(seqs[i]).length;
+        if (counts[i] < 0) refuse("negative number of positions");
+        rows += counts[i];
+        pages += (static_cast<long long>(length) + counts[i] + c.o.page_tokens - 1) / c.o.page_tokens;
+        if (rows * c.group > (1 << 30) || pages > (1 << 30)) refuse("a pass of more than 2^30 rows");
+    }
+    c.enter(stream);
+    // everything that may be refused or find no memory comes before the pages change hands
+    c.seqs.assign(static_cast<size_t>(n), PassSeq{});
+    c.news.assign(counts, counts + n);
+    int row0 = 0, table = 0;
+    for (int i = 0; i < n; i++) {
+        const int first = c.book.at(seqs[i]).length;
+        if (counts[i] > INT_MAX - kMaxPageTokens - first) throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: a sequence of more than 2^31 positions"};
+        c.seqs[static_cast<size_t>(i)] = {first + counts[i], first, row0, table};
+        row0 += counts[i];
+        table += c.book.pages_for(first + counts[i]);
+    }
+    Cache::Plan& plan = c.plans[0];
+    c.cut(plan, c.last_causal, c.last_window);
+    c.next_plan = 1;
+    const size_t copies_at = round16(sizeof(PassSeq) * static_cast<size_t>(n));
+    const size_t rows_at = copies_at + round16(sizeof(PageCopy) * static_cast<size_t>(n));
+    const size_t table_at = rows_at + round16(sizeof(RowAt) * static_cast<size_t>(rows));
+    const size_t items_at = table_at + round16(sizeof(int) * static_cast<size_t>(table));
+    const size_t bytes = items_at + sizeof(AttendItem) * plan.cut.items.size();
+    c.pass.reserve(bytes, c.stream);
+    char* host = c.staging.reserve(bytes);
+    const std::vector<PageCopy> copies = c.book.extend(seqs, counts, n);
+
+    std::memcpy(host, c.seqs.data(), sizeof(PassSeq) * c.seqs.size());
+    if (!copies.empty()) std::memcpy(host + copies_at, copies.data(), sizeof(PageCopy) * copies.size());
+    RowAt* row = reinterpret_cast<RowAt*>(host + rows_at);
+    int* page = reinterpret_cast<int*>(host + table_at);
+    for (int i = 0; i < n; i++) {
+        const PageBook::Sequence& s = c.book.at(seqs[i]);
+        std::memcpy(page, s.pages.data(), sizeof(int) * s.pages.size());
+        page += s.pages.size();
+        for (int t = s.length - counts[i]; t < s.length; t++)
+            *row++ = {s.pages[static_cast<size_t>(t >> c.layout.page_shift)] * c.o.page_tokens + (t & (c.o.page_tokens - 1)), t};
+    }
+    if (!plan.cut.items.empty()) std::memcpy(host + items_at, plan.cut.items.data(), sizeof(AttendItem) * plan.cut.items.size());
+    c.staging.send(c.pass.at, bytes, c.stream);
+    c.copy_pages(c.pool.at, reinterpret_cast<const PageCopy*>(c.pass.at + copies_at), static_cast<int>(copies.size()));
+    plan.at = reinterpret_cast<const AttendItem*>(c.pass.at + items_at);
+    plan.valid = true;
+    c.rows_at = rows_at;
+    c.table_at = table_at;
+    c.rows = static_cast<int>(rows);
+    c.open = true;
+}
+
+static void check_pass(const Cache& c, int layer) {
+    if (!c.open)
+        throw ApiError{GH_ERR_RUNTIME, "cache: no pass is open (extend opens one; fork, truncate, drop, compact and a copy into the cache end it)"};
+    if (layer < 0 || layer >= c.o.layers) throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: no layer " + std::to_string(layer)};
+}
+
+static void append_rows(Cache& c, int layer, const gh_rows* k, const gh_rows* v, const gh_rows* q, const gh_rows* q_out, bool rotate, void* stream) {
+    check_pass(c, layer);
+    if ((q == nullptr) != (q_out == nullptr)) refuse("queries and a place for them go together");
+    if (c.rows == 0) return;
+    const int dim = c.o.head_dim;
+    check_rows("k", k, c.o.kv_heads, dim);
+    check_rows("v", v, c.o.kv_heads, dim);
+    if (q) {
+        check_rows("q", q, c.o.heads, dim);
+        check_rows("q_out", q_out, c.o.heads, dim);
+        check_apart("q_out", q_out, c.rows, c.o.heads, dim);
+    }
+    const DeviceScope on(c.device);
+    c.enter(stream);
+    AppendParams p{};
+    p.cache = c.layout;
+    p.k = cache_rows(k);
+    p.v = cache_rows(v);
+    const bool one_row = c.rows == 1, one_kv = c.o.kv_heads == 1, one_head = c.o.heads == 1;
+    p.vector_rows = aligned(k, c.bytes, one_row, one_kv) && aligned(v, c.bytes, one_row, one_kv);
+    if (q) {
+        p.q = cache_rows(q);
+        p.q_out = cache_rows(q_out);
+        p.vector_rows = p.vector_rows && aligned(q, c.bytes, one_row, one_head) && aligned(q_out, c.bytes, one_row, one_head);
+    }
+    p.rows = reinterpret_cast<const RowAt*>(c.pass.at + c.rows_at);
+    p.speed = rotate ? reinterpret_cast<const double*>(c.speed.at) : nullptr;
+    p.layer = layer;
+    p.heads = c.o.heads;
+    const auto kernel = c.o.type == GH_F32 ? cache_append_kernel<kCacheF32>
+                      : c.o.type == GH_BF16 ? cache_append_kernel<kCacheBf16>
+                                            : cache_append_kernel<kCacheF16>;
+    hipLaunchKernelGGL(kernel, dim3(c.rows), dim3(256), 0, c.stream, p);
+    HIP_CHECK(hipGetLastError());
+}
+
+static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, float scale, bool causal, int window, void* stream) {
+    check_pass(c, layer);
+    if (window < 0) refuse("negative window");
+    if (!(scale >= 0.0f) || std::isinf(scale)) refuse("scale must be a finite number, 0 for 1 / sqrt(head_dim)");
+    if (c.rows == 0) return;
+    check_rows("q", q, c.o.heads, c.o.head_dim);
+    check_rows("out", out, c.o.heads, c.o.head_dim);
+    check_apart("out", out, c.rows, c.o.heads, c.o.head_dim);
+    const DeviceScope on(c.device);
+    c.enter(stream);
+    c.last_causal = causal;
+    c.last_window = window;
+    Cache::Plan* plan = nullptr;
+    for (Cache::Plan& p : c.plans)
+        if (p.valid && p.causal == causal && p.window == window) plan = &p;
+    if (!plan) {  // another mask than the pass was planned for
+        plan = &c.plans[c.next_plan];
+        c.next_plan = c.next_plan % (kPlans - 1) + 1;  // (the first stays: its items are the pass's own)
+        plan->valid = false;
+        c.cut(*plan, causal, window);
+        const size_t bytes = sizeof(AttendItem) * plan->cut.items.size();
+        plan->items.reserve(bytes, c.stream);
+        std::memcpy(c.staging.reserve(bytes), plan->cut.items.data(), bytes);
+        c.staging.send(plan->items.at, bytes, c.stream);
+        plan->at = reinterpret_cast<const AttendItem*>(plan->items.at);
+        plan->valid = true;
+    }
+    AttendParams p{};
+    p.cache = c.layout;
+    p.q = cache_rows(q);
+    p.out = cache_rows(out);
+    p.seqs = reinterpret_cast<const PassSeq*>(c.pass.at);
+    p.table = reinterpret_cast<const int*>(c.pass.at + c.table_at);
+    p.items = plan->at;
+    p.layer = layer;
+    p.group = c.group;
+    p.scale = (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(c.o.head_dim))) * 1.44269504088896340736f;
+    p.causal = causal;
+    p.window = window;
+    p.vector_rows = aligned(q, c.bytes, c.rows == 1, c.o.heads == 1) && aligned(out, c.bytes, c.rows == 1, c.o.heads == 1);
+    p.parts = reinterpret_cast<float*>(c.parts.at);
+    p.arrived = reinterpret_cast<unsigned*>(c.arrived.at);
+    hipLaunchKernelGGL(plan->form.kernel, dim3(static_cast<unsigned>(plan->cut.items.size()), c.o.kv_heads), dim3(64 * kAttendWaves), 0, c.stream, p);
+    HIP_CHECK(hipGetLastError());
+}
+
+static void read_positions(Cache& c, int seq, int layer, int layers, int start, int count, const gh_rows* k, long long k_layer, const gh_rows* v,
+                           long long v_layer, void* stream) {
+    const PageBook::Sequence& s = c.book.at(seq);
+    if (layer < 0 || layers < 0 || layer > c.o.layers || layers > c.o.layers - layer) throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: layers out of range"};
+    if (start < 0 || count < 0 || start > s.length || count > s.length - start)
+        throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: positions out of range"};
+    if (count == 0 || layers == 0) return;
+    const int dim = c.o.head_dim, heads = c.o.kv_heads;
+    check_rows("k", k, heads, dim);
+    check_rows("v", v, heads, dim);
+    check_apart("k", k, count, heads, dim);
+    check_apart("v", v, count, heads, dim);
+    if (layers > 1)
+        for (const auto& [r, stride, name] : {std::tuple{k, k_layer, "k"}, std::tuple{v, v_layer, "v"}})
+            if (stride < (count - 1) * r->row_stride + (heads - 1) * r->head_stride + dim) refuse(std::string(name) + "'s layers overlap");
+    const DeviceScope on(c.device);
+    c.enter(stream);
+    const int first = start >> c.layout.page_shift, last = (start + count - 1) >> c.layout.page_shift;
+    const size_t bytes = sizeof(int) * static_cast<size_t>(last - first + 1);
+    c.lists.reserve(bytes, c.stream);
+    std::memcpy(c.staging.reserve(bytes), s.pages.data() + first, bytes);
+    c.staging.send(c.lists.at, bytes, c.stream);
+    ReadParams p{};
+    p.cache = c.layout;
+    p.k = cache_rows(k);
+    p.v = cache_rows(v);
+    p.k_layer = k_layer;
+    p.v_layer = v_layer;
+    p.table = reinterpret_cast<const int*>(c.lists.at);
+    p.layer = layer;
+    p.start = start;
+    p.count = count;
+    p.vector_rows = aligned(k, c.bytes, count == 1, heads == 1) && aligned(v, c.bytes, count == 1, heads == 1)
+                    && (layers == 1 || (k_layer * c.bytes % 16 == 0 && v_layer * c.bytes % 16 == 0));
+    const auto kernel = c.o.type == GH_F32 ? cache_read_kernel<kCacheF32>
+                      : c.o.type == GH_BF16 ? cache_read_kernel<kCacheBf16>
+                                            : cache_read_kernel<kCacheF16>;
+    hipLaunchKernelGGL(kernel, dim3((count + kReadPositions - 1) / kReadPositions, layers, 2), dim3(256), 0, c.stream, p);
+    HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace gh
+
+struct gh_cache {
+    std::unique_ptr<gh::Cache> impl;
+};
+
+using namespace gh;
+
+static Cache& cache_of(gh_cache* c) {
+    if (!c) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null cache"};
+    return *c->impl;
+}
+
+extern "C" {
+
+gh_status gh_cache_create(const gh_cache_opts* opts, gh_cache** out) {
+    return guard([&] {
+        if (!opts || !out) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        *out = nullptr;
+        *out = new gh_cache{create_cache(*opts)};
+    });
+}
+
+void gh_cache_free(gh_cache* c) {
+    if (!c) return;
+    (void)guard([&] {
+        const DeviceScope on(c->impl->device);
+        c->impl.reset();
+    });
+    delete c;
+}
+
+gh_status gh_cache_get_info(const gh_cache* c, gh_cache_info* out) {
+    return guard([&] {
+        if (!c || !out) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        const Cache& m = *c->impl;
+        *out = gh_cache_info{m.device, m.book.pages(), m.book.pages_free(), m.book.sequences(), m.open ? m.rows : -1, 0, m.pool.bytes};
+    });
+}
+
+gh_status gh_cache_add(gh_cache* c, int32_t* seq) {
+    return guard([&] {
+        if (!seq) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        *seq = cache_of(c).book.add();
+    });
+}
+
+int32_t gh_cache_length(const gh_cache* c, int32_t seq) {
+    int32_t length = -1;
+    if (c) (void)guard([&] { length = c->impl->book.at(seq).length; });
+    return length;
+}
+
+gh_status gh_cache_fork(gh_cache* c, int32_t seq, int32_t length, int32_t* out) {
+    return guard([&] {
+        if (!out) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        Cache& m = cache_of(c);
+        const int id = m.book.fork(seq, length == -1 ? m.book.at(seq).length : length);
+        m.close();
+        *out = id;
+    });
+}
+
+gh_status gh_cache_truncate(gh_cache* c, int32_t seq, int32_t length) {
+    return guard([&] {
+        Cache& m = cache_of(c);
+        m.book.truncate(seq, length);
+        m.close();
+    });
+}
+
+gh_status gh_cache_drop(gh_cache* c, int32_t seq) {
+    return guard([&] {
+        Cache& m = cache_of(c);
+        m.book.drop(seq);
+        m.close();
+    });
+}
+
+gh_status gh_cache_copy(gh_cache* from, int32_t seq, gh_cache* to, void* hip_stream, int32_t* out) {
+    return guard([&] {
+        if (!out) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        Cache &a = cache_of(from), &b = cache_of(to);
+        if (a.o.layers != b.o.layers || a.o.kv_heads != b.o.kv_heads || a.o.head_dim != b.o.head_dim || a.o.type != b.o.type
+            || a.o.page_tokens != b.o.page_tokens)
+            refuse("a copy between caches of different layers, kv_heads, head_dim, type or page_tokens");
+        if (a.device != b.device) refuse("a copy between devices");
+        (void)a.book.at(seq);
+        const DeviceScope on(b.device);
+        b.close();
+        *out = copy_sequence(a, b, seq, hip_stream);
+    });
+}
+
+gh_status gh_cache_compact(gh_cache* c, void* hip_stream, int32_t* pages_used) {
+    return guard([&] {
+        Cache& m = cache_of(c);
+        const DeviceScope on(m.device);
+        m.enter(hip_stream);
+        m.close();
+        const int used = m.book.pages() - m.book.pages_free();
+        const size_t most = sizeof(PageCopy) * static_cast<size_t>(std::min(used, m.book.pages_free()));
+        m.lists.reserve(most, m.stream);
+        char* host = m.staging.reserve(most);
+        const std::vector<PageCopy> moves = m.book.compact();
+        if (!moves.empty()) {
+            std::memcpy(host, moves.data(), sizeof(PageCopy) * moves.size());
+            m.staging.send(m.lists.at, sizeof(PageCopy) * moves.size(), m.stream);
+            m.copy_pages(m.pool.at, reinterpret_cast<const PageCopy*>(m.lists.at), static_cast<int>(moves.size()));
+        }
+        if (pages_used) *pages_used = used;
+    });
+}
+
+gh_status gh_cache_extend(gh_cache* c, const int32_t* seqs, const int32_t* counts, int32_t n, void* hip_stream) {
+    return guard([&] {
+        Cache& m = cache_of(c);
+        if (n < 0 || (n > 0 && (!seqs || !counts))) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        const DeviceScope on(m.device);
+        extend_cache(m, seqs, counts, n, hip_stream);
+    });
+}
+
+gh_status gh_cache_append(gh_cache* c, int32_t layer, const gh_rows* k, const gh_rows* v, const gh_rows* q, const gh_rows* q_out,
+                          int32_t rotate, void* hip_stream) {
+    return guard([&] { append_rows(cache_of(c), layer, k, v, q, q_out, rotate != 0, hip_stream); });
+}
+
+gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale, int32_t causal, int32_t window,
+                          void* hip_stream) {
+    return guard([&] { attend(cache_of(c), layer, q, out, scale, causal != 0, window, hip_stream); });
+}
+
+gh_status gh_cache_read(gh_cache* c, int32_t seq, int32_t layer, int32_t layers, int32_t start, int32_t count, const gh_rows* k,
+                        int64_t k_layer_stride, const gh_rows* v, int64_t v_layer_stride, void* hip_stream) {
+    return guard([&] { read_positions(cache_of(c), seq, layer, layers, start, count, k, k_layer_stride, v, v_layer_stride, hip_stream); });
+}
+
+}  // extern "C"

@@ -1,0 +1,8 @@
+// Attention over paged caches of bf16: the kernels of this element type.
+#include "cache_attend.h"
+
+namespace gh {
+
+AttendForm attend_form_bf16(int dim, int tiles) { return attend_form_of<kCacheBf16>(dim, tiles); }
+
+}  // namespace gh

@@ -1,0 +1,8 @@
+// Attention over paged caches of f16: the kernels of this element type.
+#include "cache_attend.h"
+
+namespace gh {
+
+AttendForm attend_form_f16(int dim, int tiles) { return attend_form_of<kCacheF16>(dim, tiles); }
+
+}  // namespace gh

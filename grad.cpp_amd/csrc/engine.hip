@@ -1,7 +1,7 @@
 // gradhip engine: device model, paged KV cache, the per-token step (eager,
 // hipGraph-replayed), the on-GPU generate loop, and the C ABI of
 // include/gradhip.h.
-#include "../../include/gradhip.h"
+#include "api_error.h"
 #include "checkpoint.h"
 #include "tokenizer.h"
 #include "kernels_attn.h"
@@ -28,59 +28,6 @@
 #include <vector>
 
 namespace gh {
-
-// ------------------------------------------------------------------ errors
-
-struct ApiError {
-    gh_status code;
-    std::string msg;
-};
-
-static thread_local std::string g_last_error;
-
-[[noreturn]] static void throw_device(hipError_t e, const char* what, const char* file, int line) {
-    throw ApiError{GH_ERR_DEVICE, std::string("HIP error in ") + what + ": " + hipGetErrorString(e)
-                                      + " (" + file + ":" + std::to_string(line) + ")"};
-}
-
-#define HIP_CHECK(expr)                                                        \
-    do {                                                                       \
-        hipError_t e_ = (expr);                                                \
-        if (e_ != hipSuccess) throw_device(e_, #expr, __FILE__, __LINE__);     \
-    } while (0)
-
-template <typename F>
-static gh_status guard(F&& f) {
-    try {
-        f();
-        return GH_OK;
-    } catch (const ApiError& e) {
-        g_last_error = e.msg;
-        return e.code;
-    } catch (const std::out_of_range& e) {
-        g_last_error = e.what();
-        return GH_ERR_OUT_OF_RANGE;
-    } catch (const std::invalid_argument& e) {
-        g_last_error = e.what();
-        return GH_ERR_INVALID_ARGUMENT;
-    } catch (const std::bad_alloc&) {
-        g_last_error = "out of host memory";
-        return GH_ERR_RUNTIME;
-    } catch (const std::exception& e) {
-        g_last_error = e.what();
-        return GH_ERR_RUNTIME;
-    }
-}
-
-static void require_gpu() {
-    int n = 0;
-    hipError_t e = hipGetDeviceCount(&n);
-    if (e != hipSuccess || n <= 0) {
-        throw ApiError{GH_ERR_DEVICE,
-                       "gradhip needs a gfx950 GPU: no HIP device is usable and there is no CPU "
-                       "fallback"};
-    }
-}
 
 // Device memory that a call is faster with and can do without, uncleared: false, and nothing
 // allocated, if there is not enough.

@@ -1,0 +1,140 @@
+// The paged cache's kernels that move data: plans to the device, new rows into the pages (rotated to their positions), pages
+// to pages, and positions back out.  All are bound by memory; none keeps anything in shared memory but the angles of a row.
+#pragma once
+
+#include "kernels_cache_attn.h"
+#include "page_book.h"
+
+namespace gh {
+
+// Words of 16 bytes out of pinned host memory.
+__global__ __launch_bounds__(256) void cache_load_kernel(const u32x4* __restrict__ host, u32x4* __restrict__ to, size_t n) {
+    for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) to[i] = host[i];
+}
+
+struct AppendParams {
+    CacheLayout cache;
+    CacheRows k, v, q, q_out;  // q.at null: no queries
+    const RowAt* rows;
+    const double* speed;  // turns per position of every pair of dims; null: keys and queries go as they are
+    int layer;
+    int heads;  // of q
+    int vector_rows;
+};
+
+template <int TYPE>
+struct Eight {
+    using T = typename CacheType<TYPE>::T;
+    T e[8];
+    __device__ __forceinline__ void load(const char* at, bool vector) {
+        if (vector) {
+            *reinterpret_cast<u32x4*>(e) = *reinterpret_cast<const u32x4*>(at);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4*>(e + 4) = *reinterpret_cast<const u32x4*>(at + 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = reinterpret_cast<const T*>(at)[i];
+        }
+    }
+    __device__ __forceinline__ void store(char* at, bool vector) const {
+        if (vector) {
+            *reinterpret_cast<u32x4*>(at) = *reinterpret_cast<const u32x4*>(e);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4*>(at + 16) = *reinterpret_cast<const u32x4*>(e + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) reinterpret_cast<T*>(at)[i] = e[i];
+        }
+    }
+    // Pairs (2j, 2j + 1) by the angles of their row, in 32 bits, rounded once.
+    __device__ __forceinline__ void turn(const float* cosine, const float* sine) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = static_cast<float>(e[2 * i]), b = static_cast<float>(e[2 * i + 1]);
+            e[2 * i] = static_cast<T>(a * cosine[i] - b * sine[i]);
+            e[2 * i + 1] = static_cast<T>(a * sine[i] + b * cosine[i]);
+        }
+    }
+};
+
+// One workgroup per row: its keys, values and queries, eight dims to a thread.  The angle position * base^(-2j / dim) is
+// formed in 64 bits, in turns, and only what is left of it below half a turn is rounded to 32: a position of a million keeps
+// all its digits.
+template <int TYPE>
+__global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p) {
+    constexpr int kBytes = CacheType<TYPE>::kBytes;
+    __shared__ float cosine[128], sine[128];
+    const long long row = blockIdx.x;
+    const RowAt at = p.rows[row];
+    if (p.speed) {
+        if (threadIdx.x < static_cast<unsigned>(p.cache.dim / 2)) {
+            const double turns = at.pos * p.speed[threadIdx.x], part = turns - rint(turns);
+            const float near = static_cast<float>(part), rest = static_cast<float>(part - near) * 6.28318530717958647692f;
+            float s, c;
+            sincospif(2.0f * near, &s, &c);
+            sine[threadIdx.x] = s + c * rest;  // (what rounding the angle left, to first order)
+            cosine[threadIdx.x] = c - s * rest;
+        }
+        __syncthreads();
+    }
+    const int eights = p.cache.dim / 8, cached = p.cache.kv_heads * eights;
+    const int page = at.slot >> p.cache.page_shift, place = at.slot & ((1 << p.cache.page_shift) - 1);
+    const int all = 2 * cached + (p.q.at ? p.heads * eights : 0);
+    for (int i = threadIdx.x; i < all; i += 256) {
+        const int which = i < cached ? 0 : i < 2 * cached ? 1 : 2;
+        const int j = i - which * cached, head = j / eights, dim = j % eights * 8;
+        const CacheRows& from = which == 0 ? p.k : which == 1 ? p.v : p.q;
+        Eight<TYPE> x;
+        x.load(from.at + (row * from.row + head * from.head + dim) * kBytes, p.vector_rows);
+        if (p.speed && which != 1) x.turn(cosine + dim / 2, sine + dim / 2);
+        if (which < 2) {
+            x.store(cache_run(p.cache, page, p.layer, which, head) + (static_cast<size_t>(place) * p.cache.dim + dim) * kBytes, true);
+        } else {
+            x.store(p.q_out.at + (row * p.q_out.row + head * p.q_out.head + dim) * kBytes, p.vector_rows);
+        }
+    }
+}
+
+// The first positions of pages into other pages (of this pool or of one of the same shape), run by run.
+__global__ __launch_bounds__(256) void cache_copy_kernel(const char* __restrict__ from, char* __restrict__ to, size_t page_bytes, int runs,
+                                                         int run_words, int token_bytes, const PageCopy* __restrict__ copies, int n) {
+    for (int c = blockIdx.y; c < n; c += gridDim.y) {
+        const PageCopy copy = copies[c];
+        const int words = copy.tokens * token_bytes / 16;
+        const u32x4* a = reinterpret_cast<const u32x4*>(from + static_cast<size_t>(copy.from) * page_bytes);
+        u32x4* b = reinterpret_cast<u32x4*>(to + static_cast<size_t>(copy.to) * page_bytes);
+        for (int run = blockIdx.x; run < runs; run += gridDim.x)
+            for (int w = threadIdx.x; w < words; w += 256)
+                b[static_cast<size_t>(run) * run_words + w] = a[static_cast<size_t>(run) * run_words + w];
+    }
+}
+
+struct ReadParams {
+    CacheLayout cache;
+    CacheRows k, v;  // position start goes to row 0
+    long long k_layer, v_layer;
+    const int* table;  // pages from start's on
+    int layer, start, count;
+    int vector_rows;
+};
+
+constexpr int kReadPositions = 16;
+
+// 16 positions of a layer, K or V, to a workgroup.
+template <int TYPE>
+__global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
+    constexpr int kBytes = CacheType<TYPE>::kBytes;
+    const int which = blockIdx.z, layer = blockIdx.y, n0 = blockIdx.x * kReadPositions;
+    const int eights = p.cache.dim / 8, tokens = min(kReadPositions, p.count - n0);
+    const CacheRows& to = which ? p.v : p.k;
+    const long long base = layer * (which ? p.v_layer : p.k_layer);
+    const int first_page = p.start >> p.cache.page_shift;
+    for (int i = threadIdx.x; i < tokens * eights * p.cache.kv_heads; i += 256) {
+        const int dim = i % eights * 8, token = i / eights % tokens, head = i / eights / tokens;
+        const int t = p.start + n0 + token;
+        const int page = p.table[(t >> p.cache.page_shift) - first_page], place = t & ((1 << p.cache.page_shift) - 1);
+        Eight<TYPE> x;
+        x.load(cache_run(p.cache, page, p.layer + layer, which, head) + (static_cast<size_t>(place) * p.cache.dim + dim) * kBytes, true);
+        x.store(to.at + (base + (n0 + token) * to.row + head * to.head + dim) * kBytes, p.vector_rows);
+    }
+}
+
+}  // namespace gh

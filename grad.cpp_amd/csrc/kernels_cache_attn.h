@@ -1,0 +1,546 @@
+// Attention of a pass's rows over a paged cache.
+//
+// For row r of a sequence (a token at position t and one of the query heads of a kv head):
+//   z_u = scale q.K_u for the visible positions u,   o = sum_u exp(z_u - m) V_u / sum_u exp(z_u - m),   m = max_u z_u,
+// in one pass over K and V: a wavefront keeps the running maximum m, its share of the sum and the unnormalised output of its
+// rows and corrects the last two when the maximum grows.
+//
+// Everything runs on the matrix cores with the rows in the COLUMNS of the products: Z^T = K Q^T and O^T = V^T P^T.  A lane
+// then holds scores of ONE row (lane & 15) in both products: the maximum, the sum and the correction are values of its own,
+// and the probabilities it made are, in the order it made them, the operand that the second product wants from it, because
+// which position goes to which of the product's k slots is free as long as K and V agree.  Nothing passes through shared
+// memory between the products.  A lane's k slots are positions 4 (lane / 16) .. + 3 of each block of 16.
+//
+//   Z^T operand K:   lane l holds position l & 15, eight (four) consecutive dims of its quarter l >> 4: one 16-byte load
+//   O^T operand V^T: lane l holds c = DH / 16 consecutive dims (l & 15) c .. of its positions: 16 lanes read one whole row of a
+//                    head; which of the c products a dim goes to is free too, so products are numbered by the place in
+//                    the run.  16-bit elements are paired up over positions in registers (v_perm).
+#pragma once
+
+#include "cache_plan.h"
+#include "kernels_common.h"
+
+namespace gh {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+enum { kCacheF32 = 0, kCacheBf16 = 1, kCacheF16 = 2 };
+
+template <int TYPE>
+struct CacheType;
+template <>
+struct CacheType<kCacheF32> {
+    using T = float;
+    static constexpr int kBytes = 4;
+    static constexpr float kLift = 0.0f;
+};
+template <>
+struct CacheType<kCacheBf16> {
+    using T = __bf16;
+    using V8 = __bf16 __attribute__((ext_vector_type(8)));
+    using V2 = __bf16 __attribute__((ext_vector_type(2)));
+    static constexpr int kBytes = 2;
+    static constexpr float kLift = 0.0f;
+    static constexpr unsigned kInf = 0x7F80u, kOne = 0x3F80u;  // infinity's and one's bits
+    static __device__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct CacheType<kCacheF16> {
+    using T = _Float16;
+    using V8 = _Float16 __attribute__((ext_vector_type(8)));
+    using V2 = _Float16 __attribute__((ext_vector_type(2)));
+    static constexpr int kBytes = 2;
+    // Probabilities are kept 2^14 times as large (the sum too): one of 2^-28 of the largest is still a normal number.
+    static constexpr float kLift = 14.0f;
+    static constexpr unsigned kInf = 0x7C00u, kOne = 0x3C00u;
+    static __device__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+    }
+};
+
+// Where things are in the pool: [page][layer][K, V][kv head][place in the page][dim].
+struct CacheLayout {
+    char* pool;
+    size_t page_bytes;
+    size_t run_bytes;  // of one (layer, K or V, head): page_tokens * dim elements
+    int kv_heads;
+    int dim;
+    int page_shift;
+    int layers;
+};
+
+__device__ __forceinline__ char* cache_run(const CacheLayout& l, int page, int layer, int which, int head) {
+    return l.pool + static_cast<size_t>(page) * l.page_bytes + (static_cast<size_t>(layer * 2 + which) * l.kv_heads + head) * l.run_bytes;
+}
+
+// Rows of heads of the caller's: element strides.
+struct CacheRows {
+    char* at;
+    long long row, head;
+};
+
+struct AttendParams {
+    CacheLayout cache;
+    CacheRows q, out;
+    const PassSeq* seqs;
+    const int* table;
+    const AttendItem* items;
+    int layer;
+    int group;
+    float scale;  // of the scores, times log2(e)
+    int causal;
+    int window;
+    int vector_rows;    // q's and out's rows can be read and written 16 bytes at a time
+    float* parts;       // [part][kv head][tile height][DH + 2]: output, maximum, sum
+    unsigned* arrived;  // [tile][kv head], zero between launches
+};
+
+constexpr int kBeyond = 0x40000000;  // past the end of any run (a run is a megabyte at most)
+constexpr int kAttendWaves = 4;
+
+// Largest value and sum over the four lanes that hold a row (lanes l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// What a wavefront reads at a time: a granule of 32 (16-bit) or 16 (fp32) positions of one head.
+template <int TYPE, int DH>
+struct Granule {
+    static constexpr bool kWide = TYPE == kCacheF32;
+    static constexpr int kTokens = kWide ? 16 : 32;
+    static constexpr int kBlocks = kTokens / 16;
+    static constexpr int kDims = DH / 16;                      // dims of a lane in V
+    static constexpr int kKeyWords = kWide ? DH / 4 : DH / 8;  // of one block
+    static constexpr int kValueWords = kWide ? kDims : kDims / 2;  // of one position
+    static constexpr int kQuarter = kWide ? 4 : 8;             // dims of 16 bytes
+    unsigned k[kBlocks][kKeyWords];
+    unsigned v[kBlocks * 4][kValueWords];
+};
+
+// FULL: the head has DH dims.  Otherwise lanes whose dims do not exist read past the end of the run: zeros.
+template <int TYPE, int DH, bool FULL>
+__device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer, const int* table, int head, int at, int end,
+                                             Granule<TYPE, DH>& g) {
+    using G = Granule<TYPE, DH>;
+    constexpr int kBytes = CacheType<TYPE>::kBytes;
+    const int lane = threadIdx.x & 63, row = cache.dim * kBytes;
+    const int key_lane = (lane & 15) * row + (lane >> 4) * 16;
+    const int value_dim = (lane & 15) * G::kDims;
+    const int value_lane = (lane >> 4) * 4 * row + value_dim * kBytes;
+#pragma unroll
+    for (int b = 0; b < G::kBlocks; b++) {
+        // a block that begins behind the last position may have no page: it reads the one before, and counts for nothing
+        const int t = at + 16 * b < end ? at + 16 * b : at;
+        const int page = table[t >> cache.page_shift];
+        const int offset = (t & ((1 << cache.page_shift) - 1)) * row;
+        const char* run = cache_run(cache, page, layer, 0, head);
+        const __amdgpu_buffer_rsrc_t ks = make_buffer(run, static_cast<unsigned>(cache.run_bytes));
+        const __amdgpu_buffer_rsrc_t vs = make_buffer(run + cache.kv_heads * cache.run_bytes, static_cast<unsigned>(cache.run_bytes));
+#pragma unroll
+        for (int c = 0; c < G::kKeyWords / 4; c++) {
+            const bool there = FULL || 4 * G::kQuarter * c + G::kQuarter * (lane >> 4) < cache.dim;
+            const u32x4 w = __builtin_bit_cast(
+                u32x4, __builtin_amdgcn_raw_buffer_load_b128(ks, there ? key_lane + 64 * c : kBeyond, offset, 0));
+            g.k[b][4 * c] = w.x;
+            g.k[b][4 * c + 1] = w.y;
+            g.k[b][4 * c + 2] = w.z;
+            g.k[b][4 * c + 3] = w.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            unsigned* to = g.v[4 * b + i];
+            if constexpr (G::kValueWords == 1) {
+                to[0] = __builtin_amdgcn_raw_buffer_load_b32(vs, FULL || value_dim < cache.dim ? value_lane : kBeyond, offset + i * row, 0);
+            } else if constexpr (G::kValueWords == 2) {
+                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(
+                                                              vs, FULL || value_dim < cache.dim ? value_lane : kBeyond, offset + i * row, 0));
+                to[0] = w.x;
+                to[1] = w.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < G::kValueWords / 4; c++) {
+                    const bool there = FULL || value_dim + G::kQuarter * c < cache.dim;
+                    const u32x4 w = __builtin_bit_cast(
+                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(vs, there ? value_lane + 16 * c : kBeyond, offset + i * row, 0));
+                    to[4 * c] = w.x;
+                    to[4 * c + 1] = w.y;
+                    to[4 * c + 2] = w.z;
+                    to[4 * c + 3] = w.w;
+                }
+            }
+        }
+    }
+}
+
+// The second product's operand for dims `word`'s low or high halves: a lane's eight positions, two to a register.
+template <int WORDS>
+__device__ __forceinline__ u32x4 value_operand(const unsigned (&v)[8][WORDS], int word, bool high) {
+    const unsigned sel = high ? 0x07060302u : 0x05040100u;
+    u32x4 r;
+    r.x = __builtin_amdgcn_perm(v[1][word], v[0][word], sel);
+    r.y = __builtin_amdgcn_perm(v[3][word], v[2][word], sel);
+    r.z = __builtin_amdgcn_perm(v[5][word], v[4][word], sel);
+    r.w = __builtin_amdgcn_perm(v[7][word], v[6][word], sel);
+    return r;
+}
+
+// Infinities and NaN among the values of a granule that some rows may not see: 0 * infinity would reach those rows
+// through the product.  Such elements leave the granule (they become zeros) and are added to the rows that do see
+// them: a product with visibility in the place of the probabilities counts them, infinity as 1, minus infinity as 64 and
+// NaN as 4096 (at most 32 positions, sums below 2^24).  Rare, and only in granules that a mask cuts.
+__device__ __forceinline__ float unbounded_sum(float n) {
+    const unsigned c = static_cast<unsigned>(n);
+    float v = c & 63u ? INFINITY : 0.0f;
+    if (c & 4032u) v -= INFINITY;
+    return c > 4095u ? NAN : v;
+}
+
+template <int TYPE, int DH, int TILES>
+__device__ __forceinline__ void add_unbounded(Granule<TYPE, DH>& g, const unsigned (&seen)[TILES], f32x4 (&o)[TILES][DH / 16]) {
+    using G = Granule<TYPE, DH>;
+    using C = CacheType<TYPE>;
+#pragma unroll
+    for (int cc = 0; cc < G::kDims; cc++) {
+        f32x4 n[TILES];
+#pragma unroll
+        for (int rt = 0; rt < TILES; rt++) n[rt] = f32x4{0, 0, 0, 0};
+        if constexpr (G::kWide) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e = __uint_as_float(g.v[i][cc]);
+                const float w = e - e == 0.0f ? 0.0f : e > 0.0f ? 1.0f : e < 0.0f ? 64.0f : 4096.0f;
+#pragma unroll
+                for (int rt = 0; rt < TILES; rt++)
+                    n[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, static_cast<float>((seen[rt] >> i) & 1u), n[rt], 0, 0, 0);
+            }
+        } else {
+            u32x4 a = value_operand(g.v, cc / 2, cc & 1);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                using T = typename C::T;
+                const typename C::V2 e = __builtin_bit_cast(typename C::V2, static_cast<unsigned>(a[w]));
+                typename C::V2 to;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const float f = static_cast<float>(e[half]);
+                    to[half] = static_cast<T>(f - f == 0.0f ? 0.0f : f > 0.0f ? 1.0f : f < 0.0f ? 64.0f : 4096.0f);
+                }
+                a[w] = __builtin_bit_cast(unsigned, to);
+            }
+#pragma unroll
+            for (int rt = 0; rt < TILES; rt++) {
+                u32x4 b;
+#pragma unroll
+                for (int w = 0; w < 4; w++) b[w] = ((seen[rt] >> (2 * w)) & 1u) * C::kOne | ((seen[rt] >> (2 * w + 1)) & 1u) * (C::kOne << 16);
+                n[rt] = C::mfma(a, b, n[rt]);
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < TILES; rt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[rt][cc][i] += unbounded_sum(n[rt][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * G::kBlocks; i++)
+#pragma unroll
+        for (int w = 0; w < G::kValueWords; w++) {
+            unsigned& e = g.v[i][w];
+            if constexpr (G::kWide) {
+                e = (e & 0x7F800000u) == 0x7F800000u ? 0u : e;
+            } else {
+                e = (e & C::kInf) == C::kInf ? e & 0xFFFF0000u : e;
+                e = (e & (C::kInf << 16)) == (C::kInf << 16) ? e & 0x0000FFFFu : e;
+            }
+        }
+}
+
+// Whether a word of the cache's type holds an infinity or NaN: the exponent's bits are all ones.
+template <int TYPE>
+__device__ __forceinline__ bool unbounded(unsigned w) {
+    using C = CacheType<TYPE>;
+    if constexpr (TYPE == kCacheF32) {
+        return (w & 0x7F800000u) == 0x7F800000u;
+    } else {
+        return (w & C::kInf) == C::kInf || (w & (C::kInf << 16)) == (C::kInf << 16);
+    }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store_four(const CacheRows& rows, long long at, bool vector, const f32x4& o) {
+    using T = typename CacheType<TYPE>::T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T4 v = __builtin_convertvector(o, T4);
+    T* to = reinterpret_cast<T*>(rows.at) + at;
+    if (vector) {
+        *reinterpret_cast<T4*>(to) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) to[e] = v[e];
+    }
+}
+
+// Tiles of 16 TILES rows; the four wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
+// A tile whose positions were dealt to several workgroups is finished by the last of them to arrive.
+template <int TYPE, int DH, bool FULL, int TILES>
+__global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const AttendParams p) {
+    using C = CacheType<TYPE>;
+    using T = typename C::T;
+    using G = Granule<TYPE, DH>;
+    constexpr int kDims = G::kDims, kPad = DH + 4;
+    __shared__ __align__(16) float meet[kAttendWaves][16][kPad];
+    __shared__ float tops[kAttendWaves][16], sums[kAttendWaves][16];
+    __shared__ unsigned last;
+
+    const AttendItem it = p.items[blockIdx.x];
+    const int head = blockIdx.y;
+    const PassSeq s = p.seqs[it.seq];
+    const int* table = p.table + s.table;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = lane >> 4;
+
+    // the rows' queries, as the first product's second operand
+    unsigned q[TILES][G::kKeyWords];
+    int pos[TILES];
+#pragma unroll
+    for (int rt = 0; rt < TILES; rt++) {
+        const int r = it.r0 + 16 * rt + (lane & 15);
+        const bool row = 16 * rt + (lane & 15) < it.rows;
+        const int token = row ? r / p.group : 0, h = row ? r % p.group : 0;
+        pos[rt] = row ? s.first + token : -1;
+        const T* from = reinterpret_cast<const T*>(p.q.at) + (s.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
+#pragma unroll
+        for (int c = 0; c < G::kKeyWords / 4; c++) {
+            const int dim = 4 * G::kQuarter * c + G::kQuarter * quarter;
+            u32x4 w{0, 0, 0, 0};
+            if (row && (FULL || dim < p.cache.dim)) {
+                if (p.vector_rows) {
+                    w = *reinterpret_cast<const u32x4*>(from + dim);
+                } else if constexpr (G::kWide) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = __float_as_uint(from[dim + e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        w[e / 2] |= static_cast<unsigned>(__builtin_bit_cast(unsigned short, from[dim + e])) << (16 * (e & 1));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) q[rt][4 * c + e] = w[e];
+        }
+    }
+    const int first = s.first + it.r0 / p.group, final = s.first + (it.r0 + it.rows - 1) / p.group;
+
+    f32x4 o[TILES][kDims];
+    float m[TILES], l[TILES];
+#pragma unroll
+    for (int rt = 0; rt < TILES; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int cc = 0; cc < kDims; cc++) o[rt][cc] = f32x4{0, 0, 0, 0};
+    }
+
+    Granule<TYPE, DH> now, next;
+    int at = it.k0 + wave * G::kTokens;
+    if (at < it.k1) load_granule<TYPE, DH, FULL>(p.cache, p.layer, table, head, at, it.k1, now);
+    while (at < it.k1) {
+        const int then = at + kAttendWaves * G::kTokens;
+        if (then < it.k1) load_granule<TYPE, DH, FULL>(p.cache, p.layer, table, head, then, it.k1, next);
+
+        // does a mask cut this granule?
+        const bool cut = at + G::kTokens > it.k1 || (p.causal && at + G::kTokens - 1 > first) || (p.window > 0 && at <= final - p.window);
+        float z[TILES][4 * G::kBlocks];
+#pragma unroll
+        for (int rt = 0; rt < TILES; rt++)
+#pragma unroll
+            for (int b = 0; b < G::kBlocks; b++) {
+                f32x4 acc{0, 0, 0, 0};
+                if constexpr (G::kWide) {
+#pragma unroll
+                    for (int w = 0; w < G::kKeyWords; w++)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][w]), __uint_as_float(q[rt][w]), acc, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < G::kKeyWords; w += 4)
+                        acc = C::mfma(u32x4{now.k[b][w], now.k[b][w + 1], now.k[b][w + 2], now.k[b][w + 3]},
+                                      u32x4{q[rt][w], q[rt][w + 1], q[rt][w + 2], q[rt][w + 3]}, acc);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[rt][4 * b + i] = acc[i] * p.scale;
+            }
+        unsigned seen[TILES];
+        bool hidden = false;
+        if (cut) {
+#pragma unroll
+            for (int rt = 0; rt < TILES; rt++) {
+                seen[rt] = 0;
+#pragma unroll
+                for (int i = 0; i < 4 * G::kBlocks; i++) {
+                    const int t = at + 16 * (i / 4) + 4 * quarter + (i & 3);
+                    const bool see = t < it.k1 && (!p.causal || t <= pos[rt]) && (p.window <= 0 || t > pos[rt] - p.window);
+                    z[rt][i] = see ? z[rt][i] : -INFINITY;
+                    seen[rt] |= see ? 1u << i : 0u;
+                }
+            }
+            // places behind the last position hold anything; a position that some rows may not see is looked at
+#pragma unroll
+            for (int i = 0; i < 4 * G::kBlocks; i++) {
+                const bool there = at + 16 * (i / 4) + 4 * quarter + (i & 3) < it.k1;
+#pragma unroll
+                for (int w = 0; w < G::kValueWords; w++) {
+                    now.v[i][w] = there ? now.v[i][w] : 0u;
+                    hidden = hidden || unbounded<TYPE>(now.v[i][w]);
+                }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < TILES; rt++) {
+            float top = z[rt][0];
+#pragma unroll
+            for (int i = 1; i < 4 * G::kBlocks; i++) top = fmaxf(top, z[rt][i]);
+            top = row_max(top);
+            if (__any(top > m[rt])) {
+                const float keep = top > m[rt] ? __builtin_amdgcn_exp2f(m[rt] - top) : 1.0f;
+                m[rt] = fmaxf(m[rt], top);
+                l[rt] *= keep;
+#pragma unroll
+                for (int cc = 0; cc < kDims; cc++) o[rt][cc] *= keep;
+            }
+            const float base = m[rt] == -INFINITY ? 0.0f : m[rt] - C::kLift;
+#pragma unroll
+            for (int i = 0; i < 4 * G::kBlocks; i++) {
+                z[rt][i] = __builtin_amdgcn_exp2f(z[rt][i] - base);
+                l[rt] += z[rt][i];
+            }
+        }
+        if (cut && __any(hidden)) add_unbounded<TYPE, DH, TILES>(now, seen, o);  // (behind the correction: infinity * 0 is none)
+        if constexpr (G::kWide) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int cc = 0; cc < kDims; cc++)
+#pragma unroll
+                    for (int rt = 0; rt < TILES; rt++)
+                        o[rt][cc] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.v[i][cc]), z[rt][i], o[rt][cc], 0, 0, 0);
+        } else {
+            // probabilities in the cache's type: off by half a step of theirs each, at random, which is what the outputs'
+            // own rounding is
+            u32x4 prob[TILES];
+#pragma unroll
+            for (int rt = 0; rt < TILES; rt++)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    prob[rt][w] = __builtin_bit_cast(unsigned, typename C::V2{static_cast<T>(z[rt][2 * w]), static_cast<T>(z[rt][2 * w + 1])});
+#pragma unroll
+            for (int cc = 0; cc < kDims; cc++) {
+                const u32x4 a = value_operand(now.v, cc / 2, cc & 1);
+#pragma unroll
+                for (int rt = 0; rt < TILES; rt++) o[rt][cc] = C::mfma(a, prob[rt], o[rt][cc]);
+            }
+        }
+        now = next;
+        at = then;
+    }
+
+    const bool only = it.parts == 1;
+    constexpr int kBlock = 16 * TILES * kPad;  // floats of a part
+    float* const parts = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
+    const size_t part_stride = static_cast<size_t>(p.cache.kv_heads) * kBlock;
+    constexpr int kChunks = DH / 4;  // of a row
+#pragma unroll
+    for (int rt = 0; rt < TILES; rt++) {
+        if (16 * rt >= it.rows) break;
+        const float sum = row_sum(l[rt]);
+        if (quarter == 0) {
+            tops[wave][lane] = m[rt];
+            sums[wave][lane] = sum;
+        }
+        __syncthreads();
+        const int mine = lane & 15;
+        float top = tops[0][mine];
+#pragma unroll
+        for (int w = 1; w < kAttendWaves; w++) top = fmaxf(top, tops[w][mine]);
+        const float keep = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int cc = 0; cc < kDims; cc++) meet[wave][mine][(4 * quarter + i) * kDims + cc] = o[rt][cc][i] * keep;
+        __syncthreads();
+        for (int e = threadIdx.x; e < 16 * kChunks; e += 64 * kAttendWaves) {
+            const int row = e / kChunks, dim = e % kChunks * 4;
+            if (16 * rt + row >= it.rows) break;
+            float high = tops[0][row], total = 0.0f;
+#pragma unroll
+            for (int w = 1; w < kAttendWaves; w++) high = fmaxf(high, tops[w][row]);
+            f32x4 out{0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kAttendWaves; w++) {
+                total += sums[w][row] * (tops[w][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[w][row] - high));
+                out += *reinterpret_cast<const f32x4*>(&meet[w][row][dim]);
+            }
+            if (only) {
+                const int r = it.r0 + 16 * rt + row;
+                if (FULL || dim < p.cache.dim)
+                    store_four<TYPE>(p.out, (s.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
+                                     p.vector_rows, out / total);
+            } else {
+                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + it.index * part_stride, kBlock * 4);
+                const int base = (16 * rt + row) * kPad * 4;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, out), rs, base + dim * 4, 0, kAuxDeviceScope);
+                if (dim == 0)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, f32x4{high, total, 0.0f, 0.0f}), rs, base + DH * 4, 0, kAuxDeviceScope);
+            }
+        }
+        __syncthreads();
+    }
+    if (only) return;
+
+    // the stores have to be out before the workgroup counts as arrived
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    unsigned* const arrived = p.arrived + static_cast<size_t>(it.tile) * p.cache.kv_heads + head;
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (last != static_cast<unsigned>(it.parts - 1)) return;
+    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int e = threadIdx.x; e < it.rows * kChunks; e += 64 * kAttendWaves) {
+        const int row = e / kChunks, dim = e % kChunks * 4, base = row * kPad * 4;
+        float top = -INFINITY, total = 0.0f;
+        f32x4 out{0, 0, 0, 0};
+        for (int j0 = 0; j0 < it.parts; j0 += 4) {  // four parts' loads in flight, folded in the order of the positions
+            v4i a[4], st[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + min(j0 + j, it.parts - 1) * part_stride, kBlock * 4);
+                a[j] = coherent_load16(rs, base + dim * 4);
+                st[j] = coherent_load16(rs, base + DH * 4);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j0 + j >= it.parts) break;
+                const float high = __int_as_float(st[j].x), sum = __int_as_float(st[j].y);
+                const float up = fmaxf(top, high);
+                const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+                const float take = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(high - up);
+                total = total * keep + sum * take;
+                out = out * keep + __builtin_bit_cast(f32x4, a[j]) * take;
+                top = up;
+            }
+        }
+        const int r = it.r0 + row;
+        if (FULL || dim < p.cache.dim)
+            store_four<TYPE>(p.out, (s.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
+                             out / total);
+    }
+}
+
+}  // namespace gh

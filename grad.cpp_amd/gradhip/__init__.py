@@ -61,6 +61,20 @@ class GhTokenizerInfo(C.Structure):
                 ("n_merges", C.c_int32), ("n_specials", C.c_int32), ("fingerprint", C.c_uint64)]
 
 
+class GhCacheOpts(C.Structure):
+    _fields_ = [("layers", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("type", C.c_int32), ("page_tokens", C.c_int32), ("pages", C.c_int32), ("rope_base", C.c_float)]
+
+
+class GhRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class GhCacheInfo(C.Structure):
+    _fields_ = [("device", C.c_int32), ("pages", C.c_int32), ("pages_free", C.c_int32), ("sequences", C.c_int32),
+                ("pass_rows", C.c_int32), ("reserved", C.c_int32), ("pool_bytes", C.c_uint64)]
+
+
 # Every symbol include/gradhip.h declares: name -> (restype, argtypes)
 _f32p, _i32p, _vp = C.POINTER(C.c_float), C.POINTER(C.c_int32), C.c_void_p
 TokenCallback = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.POINTER(C.c_int32), C.c_int32)  # gh_token_callback
@@ -107,6 +121,22 @@ SYMBOLS = {
     "gh_pretokenize": (C.c_int, [C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t), C.c_size_t,
                                  C.POINTER(C.c_size_t)]),
     "gh_codepoint_class": (C.c_int32, [C.c_uint32]),
+    "gh_cache_create": (C.c_int, [C.POINTER(GhCacheOpts), C.POINTER(_vp)]),
+    "gh_cache_free": (None, [_vp]),
+    "gh_cache_get_info": (C.c_int, [_vp, C.POINTER(GhCacheInfo)]),
+    "gh_cache_add": (C.c_int, [_vp, _i32p]),
+    "gh_cache_length": (C.c_int32, [_vp, C.c_int32]),
+    "gh_cache_fork": (C.c_int, [_vp, C.c_int32, C.c_int32, _i32p]),
+    "gh_cache_truncate": (C.c_int, [_vp, C.c_int32, C.c_int32]),
+    "gh_cache_drop": (C.c_int, [_vp, C.c_int32]),
+    "gh_cache_copy": (C.c_int, [_vp, C.c_int32, _vp, _vp, _i32p]),
+    "gh_cache_compact": (C.c_int, [_vp, _vp, _i32p]),
+    "gh_cache_extend": (C.c_int, [_vp, _i32p, _i32p, C.c_int32, _vp]),
+    "gh_cache_append": (C.c_int, [_vp, C.c_int32, C.POINTER(GhRows), C.POINTER(GhRows), C.POINTER(GhRows), C.POINTER(GhRows),
+                                  C.c_int32, _vp]),
+    "gh_cache_attend": (C.c_int, [_vp, C.c_int32, C.POINTER(GhRows), C.POINTER(GhRows), C.c_float, C.c_int32, C.c_int32, _vp]),
+    "gh_cache_read": (C.c_int, [_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(GhRows), C.c_int64,
+                                C.POINTER(GhRows), C.c_int64, _vp]),
     "gh_device_info": (C.c_int, [C.c_char_p, C.c_size_t, _i32p, _i32p]),
     "gh_device_read_bandwidth": (C.c_int, [C.c_size_t, C.c_int32, C.POINTER(C.c_double)]),
     "gh_device_reread_bandwidth": (C.c_int, [C.c_size_t, C.c_int32, C.POINTER(C.c_double)]),
@@ -476,3 +506,154 @@ class Session:
         t = GhTiming()
         _check(load_library().gh_session_last_timing(self._h, C.byref(t)))
         return {k: getattr(t, k) for k, _ in GhTiming._fields_}
+
+
+CACHE_TYPES = {"f32": 0, "bf16": 1, "f16": 2}  # GH_F32, GH_BF16, GH_F16
+_TORCH_NAMES = {"f32": "torch.float32", "bf16": "torch.bfloat16", "f16": "torch.float16"}
+
+
+class Cache:
+    """A paged cache of keys and values (gh_cache_*): sequences of their own lengths, forked, copied, rewound and
+    dropped one by one, and the attention of a pass's rows over them.
+
+    Tensors are torch's (anything with its data_ptr, shape, stride, dtype and device), of the cache's type and on its
+    device, [rows, heads, head_dim] with a dense last dimension and any other strides.  stream is a hipStream_t as an
+    int (torch.cuda.Stream.cuda_stream), 0 for the default stream; work is enqueued there and not waited for."""
+
+    def __init__(self, layers, heads, kv_heads, head_dim, pages, dtype="f32", page_tokens=0, rope_base=0.0):
+        if dtype not in CACHE_TYPES:
+            raise ValueError(f"cache: unknown element type {dtype!r}")
+        self._h = None
+        self._lib = load_library()
+        h = _vp()
+        opts = GhCacheOpts(layers, heads, kv_heads, head_dim, CACHE_TYPES[dtype], page_tokens, pages, rope_base)
+        _check(self._lib.gh_cache_create(C.byref(opts), C.byref(h)))
+        self._h = h.value
+        self.layers, self.heads, self.kv_heads, self.head_dim, self.dtype = layers, heads, kv_heads, head_dim, dtype
+        self._torch_name = _TORCH_NAMES[dtype]
+        self._device = self.info.device
+        self._rows = -1  # of the open pass
+
+    def close(self):
+        if self._h:
+            self._lib.gh_cache_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def info(self) -> GhCacheInfo:
+        out = GhCacheInfo()
+        _check(self._lib.gh_cache_get_info(self._h, C.byref(out)))
+        return out
+
+    @property
+    def pages_free(self) -> int:
+        return self.info.pages_free
+
+    def length(self, seq) -> int:
+        """Positions of a sequence."""
+        n = self._lib.gh_cache_length(self._h, seq)
+        if n < 0:
+            raise IndexError(f"cache: no sequence {seq}")
+        return n
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        out = C.c_int32()
+        _check(self._lib.gh_cache_add(self._h, C.byref(out)))
+        return out.value
+
+    def fork(self, seq, length=-1) -> int:
+        """A sequence that begins with seq's first `length` positions (-1: all of them), in the same pages."""
+        out = C.c_int32()
+        _check(self._lib.gh_cache_fork(self._h, seq, length, C.byref(out)))
+        self._rows = -1
+        return out.value
+
+    def copy(self, seq, to=None, stream=0) -> int:
+        """A sequence, of the cache `to` if one is named, with seq's contents in pages of its own."""
+        out = C.c_int32()
+        to = to or self
+        _check(self._lib.gh_cache_copy(self._h, seq, to._h, stream or None, C.byref(out)))
+        to._rows = -1
+        return out.value
+
+    def truncate(self, seq, length) -> None:
+        """Keeps seq's first `length` positions."""
+        _check(self._lib.gh_cache_truncate(self._h, seq, length))
+        self._rows = -1
+
+    def drop(self, seq) -> None:
+        """Ends seq and frees the pages that nobody else holds."""
+        _check(self._lib.gh_cache_drop(self._h, seq))
+        self._rows = -1
+
+    def compact(self, stream=0) -> int:
+        """Moves the pages in use to the front of the pool; returns how many there are."""
+        out = C.c_int32()
+        _check(self._lib.gh_cache_compact(self._h, stream or None, C.byref(out)))
+        self._rows = -1
+        return out.value
+
+    def extend(self, seqs, counts, stream=0) -> None:
+        """Opens a pass: counts[i] new positions for seqs[i].  Its rows are those positions, sequence after sequence."""
+        n = len(seqs)
+        if len(counts) != n:
+            raise ValueError("cache: a count for every sequence")
+        self._rows = -1
+        _check(self._lib.gh_cache_extend(self._h, (C.c_int32 * n)(*seqs), (C.c_int32 * n)(*counts), n, stream or None))
+        self._rows = sum(counts)
+
+    def _tensor(self, t, name, heads, rows, dims=3):
+        shape, stride = t.shape, t.stride()
+        if len(shape) != dims or shape[-2] != heads or shape[-1] != self.head_dim or shape[-3] < rows:
+            raise ValueError(f"cache: {name} of shape {tuple(shape)} where [{'layers, ' if dims == 4 else ''}{rows}, {heads}, {self.head_dim}] goes")
+        if str(t.dtype) != self._torch_name:
+            raise ValueError(f"cache: {name} is {t.dtype}, the cache {self._torch_name}")
+        device = t.device
+        if device.type != "cuda" or device.index != self._device:
+            raise ValueError(f"cache: {name} is on {device}, the cache on cuda:{self._device}")
+        if stride[-1] != 1:
+            raise ValueError(f"cache: {name}'s last dimension is not dense")
+        return GhRows(t.data_ptr(), stride[-3], stride[-2])
+
+    def append(self, layer, k, v, q=None, q_out=None, rotate=True, stream=0) -> None:
+        """Stores the pass's keys and values [rows, kv_heads, head_dim] in a layer, keys rotated to their positions if the
+        cache has a rope_base; q [rows, heads, head_dim] is rotated likewise into q_out (which may be q)."""
+        n = max(self._rows, 0)
+        args = [self._tensor(k, "k", self.kv_heads, n), self._tensor(v, "v", self.kv_heads, n)]
+        if (q is None) != (q_out is None):
+            raise ValueError("cache: queries and a place for them go together")
+        if q is not None:
+            args += [self._tensor(q, "q", self.heads, n), self._tensor(q_out, "q_out", self.heads, n)]
+        refs = [C.byref(a) for a in args] + [None] * (4 - len(args))
+        _check(self._lib.gh_cache_append(self._h, layer, *refs, 1 if rotate else 0, stream or None))
+
+    def attend(self, layer, q, out, scale=0.0, causal=True, window=0, stream=0) -> None:
+        """out = softmax(scale q.K) V for the pass's rows over what is cached of their sequences in a layer: positions up to
+        the row's own if causal, and only the last `window` of those up to it if window is not 0; scale 0 means
+        1 / sqrt(head_dim).  q and out: [rows, heads, head_dim]; rows beyond the pass's are left as they are."""
+        n = max(self._rows, 0)
+        a, b = self._tensor(q, "q", self.heads, n), self._tensor(out, "out", self.heads, n)
+        _check(self._lib.gh_cache_attend(self._h, layer, C.byref(a), C.byref(b), scale, 1 if causal else 0, window, stream or None))
+
+    def read(self, seq, k, v, start=0, layer=None, stream=0) -> None:
+        """Copies positions of seq from `start` on, as many as k and v have rows, out of the pages: k and v are
+        [rows, kv_heads, head_dim] of one layer, or [layers, rows, kv_heads, head_dim] of all."""
+        if layer is None:
+            if len(k.shape) != 4 or len(v.shape) != 4 or k.shape[0] != self.layers or v.shape[0] != self.layers:
+                raise ValueError("cache: k and v are [layers, rows, kv_heads, head_dim] unless a layer is named")
+            dims, layers, strides = 4, self.layers, (k.stride()[0], v.stride()[0])
+        else:
+            dims, layers, strides = 3, 1, (0, 0)
+        count = k.shape[-3]
+        if v.shape[-3] != count:
+            raise ValueError("cache: k and v differ in their rows")
+        a, b = self._tensor(k, "k", self.kv_heads, count, dims), self._tensor(v, "v", self.kv_heads, count, dims)
+        _check(self._lib.gh_cache_read(self._h, seq, layer or 0, layers, start, count, C.byref(a), strides[0], C.byref(b), strides[1],
+                                       stream or None))

@@ -3,7 +3,8 @@
  *
  * Plain C ABI: opaque handles, plain pointers and sizes, status codes.  Each
  * entry point names the grad.cpp interface it stands in for (paths relative to
- * the grad.cpp source tree).  All arithmetic is fp32; token ids are int32.
+ * the grad.cpp source tree).  All arithmetic is fp32 (but for gh_cache_*, which has 16-bit
+ * types too); token ids are int32.
  *
  * Threading: a model handle is immutable after creation and may be shared by
  * sessions on different host threads.  A session owns one HIP stream; calls on
@@ -333,6 +334,115 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
                           int32_t history_stride, int32_t n_history, const gh_sampling* opt,
                           const float* uniforms, uint64_t seed, int32_t pick_index, int32_t* out_ids,
                           void* hip_stream);
+
+/* --------------------------------------------------------------- paged cache */
+
+/* No counterpart in grad.cpp, whose cache is two flat vectors of one session
+ * (inference.h:42-44): a paged cache of keys and values as an object of its own, for
+ * programs that run their own layers over sequences of different lengths.  A sequence is a
+ * list of pages; a page holds page_tokens positions of every layer.  Sequences can share
+ * pages (gh_cache_fork); a shared page is copied before anybody writes into it.
+ *
+ * A pass: gh_cache_extend names the sequences that grow and by how many positions, hands
+ * out their pages and sends the pass's plan to the device, once for all layers.  Its rows
+ * are the new positions, sequence after sequence in the order named.  In each layer,
+ * gh_cache_append stores the rows' keys and values (keys and queries rotated to their
+ * positions, if the cache was made with a rope_base) and gh_cache_attend computes the
+ * attention of the rows' queries over everything cached of their sequence, the rows
+ * themselves included.  A pass stays open, and its calls can be repeated, until the next
+ * extend, or a fork, truncate, drop, compact, or copy into the cache.
+ *
+ * Data pointers are DEVICE memory of the caller's, of the cache's element type, on the
+ * cache's device (the current one at creation).  Calls that take a hip_stream (a hipStream_t,
+ * NULL for the default stream) enqueue their work there and return without waiting, except
+ * where an internal buffer has to grow.  Calls on one cache must be serialised by the caller
+ * and take effect in their order whatever streams they name: a call on another stream than
+ * the one before waits, on the device, for that one's work (so a stream that a cache was
+ * used on must live until the cache's next call or its end).  The caller's own buffers are
+ * ordered by the streams the caller names.  A stream that is being captured into a graph is
+ * refused (GH_ERR_RUNTIME): a replay would use the pages and lengths of the capture.
+ * Every size, page and position is checked on the host before anything is enqueued. */
+typedef struct gh_cache gh_cache;
+
+enum { GH_F32 = 0, GH_BF16 = 1, GH_F16 = 2 }; /* element types */
+
+typedef struct gh_cache_opts {
+    int32_t layers;      /* 1 to 4096 */
+    int32_t heads;       /* query heads, a multiple of kv_heads; 1 to 1024 */
+    int32_t kv_heads;    /* query head h reads key/value head h / (heads / kv_heads) */
+    int32_t head_dim;    /* a multiple of 8, 8 to 256 */
+    int32_t type;        /* GH_F32, GH_BF16, GH_F16: keys, values, queries and outputs.  Sums, maxima
+                          * and exponentials are 32-bit whatever the type; with the 16-bit types
+                          * probabilities are rounded to the type before they meet the values */
+    int32_t page_tokens; /* positions of a page: a power of two, 16 to 1024; 0 = 64 */
+    int32_t pages;       /* of the pool, allocated at creation: 2 * layers * kv_heads * page_tokens * head_dim elements each */
+    float rope_base;     /* rotary positions: pairs (2j, 2j + 1) by position * base^(-2j / head_dim), as
+                          * inference.cpp:169-175 but with the angles in 64 bits; 0 = no rotation */
+} gh_cache_opts;
+
+/* Rows of heads: element [row][head][dim] is at data[row * row_stride + head * head_stride + dim].
+ * Strides count elements and are not negative; what is written must not overlap itself.
+ * Any alignment of whole elements; 16 bytes of data and strides are faster. */
+typedef struct gh_rows {
+    void* data;
+    int64_t row_stride;
+    int64_t head_stride;
+} gh_rows;
+
+typedef struct gh_cache_info {
+    int32_t device;
+    int32_t pages;
+    int32_t pages_free;
+    int32_t sequences;
+    int32_t pass_rows; /* of the open pass, -1 when none is open */
+    int32_t reserved;
+    uint64_t pool_bytes;
+} gh_cache_info;
+
+gh_status gh_cache_create(const gh_cache_opts* opts, gh_cache** out);
+void gh_cache_free(gh_cache* c); /* waits for the device */
+gh_status gh_cache_get_info(const gh_cache* c, gh_cache_info* out);
+
+/* A new, empty sequence: the lowest number that no sequence has. */
+gh_status gh_cache_add(gh_cache* c, int32_t* seq);
+/* Positions of a sequence, -1 if there is none of that number. */
+int32_t gh_cache_length(const gh_cache* c, int32_t seq);
+/* A sequence whose first `length` positions (-1: all) are seq's, in the same pages. */
+gh_status gh_cache_fork(gh_cache* c, int32_t seq, int32_t length, int32_t* out);
+/* Keeps a sequence's first `length` positions; pages that nobody holds any more are free. */
+gh_status gh_cache_truncate(gh_cache* c, int32_t seq, int32_t length);
+/* Ends a sequence and frees its pages. */
+gh_status gh_cache_drop(gh_cache* c, int32_t seq);
+/* A sequence of `to` (which may be `from`) with the contents of from's seq in pages of its
+ * own.  The two caches have to agree in everything but heads, pages and rope_base. */
+gh_status gh_cache_copy(gh_cache* from, int32_t seq, gh_cache* to, void* hip_stream, int32_t* out);
+/* Moves the pages in use to the front of the pool; *pages_used (may be NULL) of them are. */
+gh_status gh_cache_compact(gh_cache* c, void* hip_stream, int32_t* pages_used);
+
+/* Opens a pass: counts[i] (0 allowed) more positions for sequence seqs[i], i < n, no sequence
+ * twice.  GH_ERR_RUNTIME when the pool has too few free pages; then no sequence has changed
+ * and no pass is open.  Until they are appended, the new positions' contents are undefined. */
+gh_status gh_cache_extend(gh_cache* c, const int32_t* seqs, const int32_t* counts, int32_t n, void* hip_stream);
+
+/* Stores the pass's keys and values (kv_heads heads per row) in `layer`.  q and q_out (both or
+ * neither NULL): the rows' queries are rotated likewise into q_out, which may be q.  rotate = 0
+ * stores (and copies) everything as it is.  k and v (and q_out) may be strided views. */
+gh_status gh_cache_append(gh_cache* c, int32_t layer, const gh_rows* k, const gh_rows* v, const gh_rows* q,
+                          const gh_rows* q_out, int32_t rotate, void* hip_stream);
+
+/* out = softmax(scale q.K) V per row and head over the positions u of the row's sequence with
+ * u <= t (causal != 0; t is the row's position) and u > t - window (window > 0).  scale 0 means
+ * 1 / sqrt(head_dim).  Rows of q and out beyond the pass's are neither read nor written.  out may
+ * be q.  What a row may not see never reaches it, infinities and NaN included; a row all of whose
+ * scores are minus infinity is NaN. */
+gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale,
+                          int32_t causal, int32_t window, void* hip_stream);
+
+/* Positions [start, start + count) of a sequence in `layers` layers from `layer` on, densely:
+ * layer i's rows begin layer_stride * i elements behind the first's. */
+gh_status gh_cache_read(gh_cache* c, int32_t seq, int32_t layer, int32_t layers, int32_t start, int32_t count,
+                        const gh_rows* k, int64_t k_layer_stride, const gh_rows* v, int64_t v_layer_stride,
+                        void* hip_stream);
 
 /* ------------------------------------------------------------ measurement */
 
