@@ -101,6 +101,7 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 constexpr int kMaxHeads = 1024;
 constexpr int kMaxPageTokens = 1024;
 constexpr int kPlans = 4;
+constexpr int kFewRows = 16;  // of a sequence: they go to a launch of their own beside longer ones
 
 }  // namespace
 
@@ -129,10 +130,21 @@ struct Cache {
         bool valid = false;
         bool causal = true;
         int window = 0;
-        AttendForm form{};
-        AttendPlan cut;
-        DeviceBuffer items;             // empty for the plan that came with the pass
+        // sequences of few rows and of many go to kernels of their own, one behind the other
+        struct Launch {
+            AttendForm form{};
+            AttendPlan cut;
+        } launches[2];
+        DeviceBuffer items;  // empty for the plan that came with the pass
         const AttendItem* at = nullptr;
+        size_t count() const { return launches[0].cut.items.size() + launches[1].cut.items.size(); }
+        size_t bytes() const { return sizeof(AttendItem) * count(); }
+        void write(char* host) const {
+            for (const Launch& l : launches) {
+                if (!l.cut.items.empty()) std::memcpy(host, l.cut.items.data(), sizeof(AttendItem) * l.cut.items.size());
+                host += sizeof(AttendItem) * l.cut.items.size();
+            }
+        }
     } plans[kPlans];
     int next_plan = 0;
     bool last_causal = true;  // the mask of the last call: the next pass is planned for it
@@ -144,10 +156,10 @@ struct Cache {
         if (moved) (void)hipEventDestroy(moved);
     }
 
-    AttendForm form_for(int tiles) const {
-        return o.type == GH_F32 ? attend_form_f32(o.head_dim, tiles)
-             : o.type == GH_BF16 ? attend_form_bf16(o.head_dim, tiles)
-                                 : attend_form_f16(o.head_dim, tiles);
+    AttendForm form_for(int rows_of_sequence) const {
+        return o.type == GH_F32 ? attend_form_f32(o.head_dim, rows_of_sequence)
+             : o.type == GH_BF16 ? attend_form_bf16(o.head_dim, rows_of_sequence)
+                                 : attend_form_f16(o.head_dim, rows_of_sequence);
     }
 
     // Calls on one cache run in their order whatever streams they name: a call on another stream than the one before waits
@@ -185,16 +197,31 @@ struct Cache {
 
     // How the pass's attention is cut, and room for what its parts leave.
     void cut(Plan& plan, bool causal, int window) {
-        int most = 0;
-        for (int n : news) most = std::max(most, n * group);
         plan.causal = causal;
         plan.window = window;
-        plan.form = form_for(most > 16 ? 2 : 1);
-        plan.cut = plan_attend(seqs, news, group, o.kv_heads, plan.form.height, causal, window, 1024, 128);
-        const size_t part_bytes = static_cast<size_t>(plan.cut.parts) * o.kv_heads * plan.form.part_floats * sizeof(float);
+        size_t part_bytes = 0, counters = 0;
+        for (int many = 0; many < 2; many++) {
+            Plan::Launch& l = plan.launches[many];
+            std::vector<int> mine(news.size(), 0);
+            int most = 0;
+            for (size_t i = 0; i < news.size(); i++)
+                if ((news[i] * group > kFewRows) == (many == 1)) {
+                    mine[i] = news[i];
+                    most = std::max(most, news[i] * group);
+                }
+            l.form = form_for(most);
+            // (a launch holds at most 2^32 threads)
+            if (static_cast<long long>(most + 15) / 16 * static_cast<long long>(news.size()) * o.kv_heads > (1 << 22)) {
+                long long tiles = 0;
+                for (int n : mine) tiles += (static_cast<long long>(n) * group + l.form.height - 1) / l.form.height;
+                if (tiles * o.kv_heads > (1 << 22)) refuse("a pass of more than 2^22 tiles of rows");
+            }
+            l.cut = plan_attend(seqs, mine, group, o.kv_heads, l.form.height, causal, window, 1024, 128);
+            part_bytes = std::max(part_bytes, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
+            counters = std::max(counters, static_cast<size_t>(l.cut.tiles) * o.kv_heads);
+        }
         parts.reserve(part_bytes, stream);
-        if (arrived.reserve(static_cast<size_t>(plan.cut.tiles) * o.kv_heads * sizeof(unsigned), stream))
-            HIP_CHECK(hipMemsetAsync(arrived.at, 0, arrived.bytes, stream));
+        if (arrived.reserve(counters * sizeof(unsigned), stream)) HIP_CHECK(hipMemsetAsync(arrived.at, 0, arrived.bytes, stream));
     }
 };
 
@@ -299,7 +326,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
         if (counts[i] < 0) refuse("negative number of positions");
         rows += counts[i];
         pages += (static_cast<long long>(length) + counts[i] + c.o.page_tokens - 1) / c.o.page_tokens;
-        if (rows * c.group > (1 << 30) || pages > (1 << 30)) refuse("a pass of more than 2^30 rows");
+        if (rows > (1 << 23) || rows * c.group > (1 << 30) || pages > (1 << 28)) refuse("a pass of more than 2^23 rows");
     }
     c.enter(stream);
     // everything that may be refused or find no memory comes before the pages change hands
@@ -320,7 +347,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     const size_t rows_at = copies_at + round16(sizeof(PageCopy) * static_cast<size_t>(n));
     const size_t table_at = rows_at + round16(sizeof(RowAt) * static_cast<size_t>(rows));
     const size_t items_at = table_at + round16(sizeof(int) * static_cast<size_t>(table));
-    const size_t bytes = items_at + sizeof(AttendItem) * plan.cut.items.size();
+    const size_t bytes = items_at + plan.bytes();
     c.pass.reserve(bytes, c.stream);
     char* host = c.staging.reserve(bytes);
     const std::vector<PageCopy> copies = c.book.extend(seqs, counts, n);
@@ -336,7 +363,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
         for (int t = s.length - counts[i]; t < s.length; t++)
             *row++ = {s.pages[static_cast<size_t>(t >> c.layout.page_shift)] * c.o.page_tokens + (t & (c.o.page_tokens - 1)), t};
     }
-    if (!plan.cut.items.empty()) std::memcpy(host + items_at, plan.cut.items.data(), sizeof(AttendItem) * plan.cut.items.size());
+    plan.write(host + items_at);
     c.staging.send(c.pass.at, bytes, c.stream);
     c.copy_pages(c.pool.at, reinterpret_cast<const PageCopy*>(c.pass.at + copies_at), static_cast<int>(copies.size()));
     plan.at = reinterpret_cast<const AttendItem*>(c.pass.at + items_at);
@@ -409,9 +436,9 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
         c.next_plan = c.next_plan % (kPlans - 1) + 1;  // (the first stays: its items are the pass's own)
         plan->valid = false;
         c.cut(*plan, causal, window);
-        const size_t bytes = sizeof(AttendItem) * plan->cut.items.size();
+        const size_t bytes = plan->bytes();
         plan->items.reserve(bytes, c.stream);
-        std::memcpy(c.staging.reserve(bytes), plan->cut.items.data(), bytes);
+        plan->write(c.staging.reserve(bytes));
         c.staging.send(plan->items.at, bytes, c.stream);
         plan->at = reinterpret_cast<const AttendItem*>(plan->items.at);
         plan->valid = true;
@@ -431,8 +458,13 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.vector_rows = aligned(q, c.bytes, c.rows == 1, c.o.heads == 1) && aligned(out, c.bytes, c.rows == 1, c.o.heads == 1);
     p.parts = reinterpret_cast<float*>(c.parts.at);
     p.arrived = reinterpret_cast<unsigned*>(c.arrived.at);
-    hipLaunchKernelGGL(plan->form.kernel, dim3(static_cast<unsigned>(plan->cut.items.size()), c.o.kv_heads), dim3(64 * kAttendWaves), 0, c.stream, p);
-    HIP_CHECK(hipGetLastError());
+    for (const Cache::Plan::Launch& l : plan->launches) {
+        if (!l.cut.items.empty()) {
+            hipLaunchKernelGGL(l.form.kernel, dim3(static_cast<unsigned>(l.cut.items.size()) * c.o.kv_heads), dim3(64 * kAttendWaves), 0, c.stream, p);
+            HIP_CHECK(hipGetLastError());
+        }
+        p.items += l.cut.items.size();
+    }
 }
 
 static void read_positions(Cache& c, int seq, int layer, int layers, int start, int count, const gh_rows* k, long long k_layer, const gh_rows* v,

@@ -1,34 +1,40 @@
 // Which attention kernel takes a pass; one translation unit per element type makes them.
 #pragma once
 
-#include "kernels_cache_attn.h"
+#include "kernels_cache_tile.h"
 
 namespace gh {
 
 using AttendKernel = void (*)(AttendParams);
 
 struct AttendForm {
-    AttendKernel kernel;
-    int height;      // rows of a tile
-    int part_floats; // of a tile's part in memory
+    AttendKernel kernel = nullptr;
+    int height = 0;       // rows of a tile
+    int part_floats = 0;  // of a tile's part in memory
 };
 
-// The form for tiles of up to 16 * tiles rows of heads of `dim` dims.
-AttendForm attend_form_f32(int dim, int tiles);
-AttendForm attend_form_bf16(int dim, int tiles);
-AttendForm attend_form_f16(int dim, int tiles);
+// The kernel for sequences of so many rows (tokens times query heads of a kv head) at heads of `dim` dims.
+AttendForm attend_form_f32(int dim, int rows);
+AttendForm attend_form_bf16(int dim, int rows);
+AttendForm attend_form_f16(int dim, int rows);
+
+template <int TYPE, int DH, bool FULL>
+AttendForm attend_form_at(int rows) {
+    const auto form = [](AttendKernel kernel, int height) { return AttendForm{kernel, height, height * (DH + 4)}; };
+    if constexpr (TYPE != kCacheF32)
+        if (rows > 64) return form(attend_tile_kernel<TYPE, DH, FULL, DH == 256 ? 32 : 64>, kTileRows);
+    if constexpr (DH < 256)
+        if (rows > 16) return form(attend_rows_kernel<TYPE, DH, FULL, 2>, 32);
+    return form(attend_rows_kernel<TYPE, DH, FULL, 1>, 16);
+}
 
 template <int TYPE>
-AttendForm attend_form_of(int dim, int tiles) {
-    const auto form = [](AttendKernel kernel, int width, int t) { return AttendForm{kernel, 16 * t, 16 * t * (width + 4)}; };
-    if (dim > 128) return form(attend_rows_kernel<TYPE, 256, false, 1>, 256, 1);
-    if (dim == 128)
-        return tiles > 1 ? form(attend_rows_kernel<TYPE, 128, true, 2>, 128, 2) : form(attend_rows_kernel<TYPE, 128, true, 1>, 128, 1);
-    if (dim > 64)
-        return tiles > 1 ? form(attend_rows_kernel<TYPE, 128, false, 2>, 128, 2) : form(attend_rows_kernel<TYPE, 128, false, 1>, 128, 1);
-    if (dim == 64)
-        return tiles > 1 ? form(attend_rows_kernel<TYPE, 64, true, 2>, 64, 2) : form(attend_rows_kernel<TYPE, 64, true, 1>, 64, 1);
-    return tiles > 1 ? form(attend_rows_kernel<TYPE, 64, false, 2>, 64, 2) : form(attend_rows_kernel<TYPE, 64, false, 1>, 64, 1);
+AttendForm attend_form_of(int dim, int rows) {
+    if (dim > 128) return attend_form_at<TYPE, 256, false>(rows);
+    if (dim == 128) return attend_form_at<TYPE, 128, true>(rows);
+    if (dim > 64) return attend_form_at<TYPE, 128, false>(rows);
+    if (dim == 64) return attend_form_at<TYPE, 64, true>(rows);
+    return attend_form_at<TYPE, 64, false>(rows);
 }
 
 }  // namespace gh

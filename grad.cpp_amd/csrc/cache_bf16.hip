@@ -3,6 +3,6 @@
 
 namespace gh {
 
-AttendForm attend_form_bf16(int dim, int tiles) { return attend_form_of<kCacheBf16>(dim, tiles); }
+AttendForm attend_form_bf16(int dim, int rows) { return attend_form_of<kCacheBf16>(dim, rows); }
 
 }  // namespace gh

@@ -3,6 +3,6 @@
 
 namespace gh {
 
-AttendForm attend_form_f32(int dim, int tiles) { return attend_form_of<kCacheF32>(dim, tiles); }
+AttendForm attend_form_f32(int dim, int rows) { return attend_form_of<kCacheF32>(dim, rows); }
 
 }  // namespace gh

@@ -64,8 +64,7 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
     const int span = static_cast<int>(std::min<long long>(std::max<long long>(least, (each + 127) / 128 * 128), 1 << 30));
     for (size_t i = 0; i < seqs.size(); i++) {
         const int all = rows[i] * group;
-        // the last rows see the most: they go first
-        for (int r0 = all > 0 ? (all - 1) / height * height : -1; r0 >= 0; r0 -= height) {
+        for (int r0 = 0; r0 < all; r0 += height) {
             const int n = std::min(height, all - r0);
             int k0, k1;
             visible_span(seqs[i], r0, n, group, causal, window, k0, k1);
@@ -82,6 +81,8 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
             }
         }
     }
+    // the longest go first: what is dealt last ends the launch
+    std::stable_sort(plan.items.begin(), plan.items.end(), [](const AttendItem& a, const AttendItem& b) { return a.k1 - a.k0 > b.k1 - b.k0; });
     return plan;
 }
 

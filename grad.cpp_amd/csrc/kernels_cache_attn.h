@@ -204,6 +204,26 @@ __device__ __forceinline__ float unbounded_sum(float n) {
     return c > 4095u ? NAN : v;
 }
 
+// Two 16-bit values: what they count for, and themselves if they are bounded and zero if not.
+template <int TYPE>
+__device__ __forceinline__ unsigned unbounded_kind(unsigned word) {
+    using C = CacheType<TYPE>;
+    const typename C::V2 e = __builtin_bit_cast(typename C::V2, word);
+    typename C::V2 to;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const float f = static_cast<float>(e[half]);
+        to[half] = static_cast<typename C::T>(f - f == 0.0f ? 0.0f : f > 0.0f ? 1.0f : f < 0.0f ? 64.0f : 4096.0f);
+    }
+    return __builtin_bit_cast(unsigned, to);
+}
+template <int TYPE>
+__device__ __forceinline__ unsigned bounded(unsigned e) {
+    using C = CacheType<TYPE>;
+    e = (e & C::kInf) == C::kInf ? e & 0xFFFF0000u : e;
+    return (e & (C::kInf << 16)) == (C::kInf << 16) ? e & 0x0000FFFFu : e;
+}
+
 template <int TYPE, int DH, int TILES>
 __device__ __forceinline__ void add_unbounded(Granule<TYPE, DH>& g, const unsigned (&seen)[TILES], f32x4 (&o)[TILES][DH / 16]) {
     using G = Granule<TYPE, DH>;
@@ -225,17 +245,7 @@ __device__ __forceinline__ void add_unbounded(Granule<TYPE, DH>& g, const unsign
         } else {
             u32x4 a = value_operand(g.v, cc / 2, cc & 1);
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                using T = typename C::T;
-                const typename C::V2 e = __builtin_bit_cast(typename C::V2, static_cast<unsigned>(a[w]));
-                typename C::V2 to;
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const float f = static_cast<float>(e[half]);
-                    to[half] = static_cast<T>(f - f == 0.0f ? 0.0f : f > 0.0f ? 1.0f : f < 0.0f ? 64.0f : 4096.0f);
-                }
-                a[w] = __builtin_bit_cast(unsigned, to);
-            }
+            for (int w = 0; w < 4; w++) a[w] = unbounded_kind<TYPE>(a[w]);
 #pragma unroll
             for (int rt = 0; rt < TILES; rt++) {
                 u32x4 b;
@@ -257,8 +267,7 @@ __device__ __forceinline__ void add_unbounded(Granule<TYPE, DH>& g, const unsign
             if constexpr (G::kWide) {
                 e = (e & 0x7F800000u) == 0x7F800000u ? 0u : e;
             } else {
-                e = (e & C::kInf) == C::kInf ? e & 0xFFFF0000u : e;
-                e = (e & (C::kInf << 16)) == (C::kInf << 16) ? e & 0x0000FFFFu : e;
+                e = bounded<TYPE>(e);
             }
         }
 }
@@ -288,6 +297,51 @@ __device__ __forceinline__ void store_four(const CacheRows& rows, long long at, 
     }
 }
 
+// The workgroup's part of a tile is in memory: the last part to arrive folds all of them, in the order of the positions, and
+// writes the tile's outputs.
+template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS>
+__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, const PassSeq& s, int head, float* parts,
+                                             size_t part_stride, unsigned& last) {
+    constexpr int kPad = DH + 4, kChunks = DH / 4, kBlock = HEIGHT * kPad;
+    // the stores have to be out before the workgroup counts as arrived
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    unsigned* const arrived = p.arrived + static_cast<size_t>(it.tile) * p.cache.kv_heads + head;
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (last != static_cast<unsigned>(it.parts - 1)) return;
+    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int e = threadIdx.x; e < it.rows * kChunks; e += THREADS) {
+        const int row = e / kChunks, dim = e % kChunks * 4, base = row * kPad * 4;
+        float top = -INFINITY, total = 0.0f;
+        f32x4 out{0, 0, 0, 0};
+        for (int j0 = 0; j0 < it.parts; j0 += 4) {  // four parts' loads in flight
+            v4i a[4], st[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + min(j0 + j, it.parts - 1) * part_stride, kBlock * 4);
+                a[j] = coherent_load16(rs, base + dim * 4);
+                st[j] = coherent_load16(rs, base + DH * 4);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j0 + j >= it.parts) break;
+                const float high = __int_as_float(st[j].x), sum = __int_as_float(st[j].y);
+                const float up = fmaxf(top, high);
+                const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+                const float take = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(high - up);
+                total = total * keep + sum * take;
+                out = out * keep + __builtin_bit_cast(f32x4, a[j]) * take;
+                top = up;
+            }
+        }
+        const int r = it.r0 + row;
+        if (FULL || dim < p.cache.dim)
+            store_four<TYPE>(p.out, (s.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
+                             out / total);
+    }
+}
+
 // Tiles of 16 TILES rows; the four wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
 // A tile whose positions were dealt to several workgroups is finished by the last of them to arrive.
 template <int TYPE, int DH, bool FULL, int TILES>
@@ -300,8 +354,8 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
     __shared__ float tops[kAttendWaves][16], sums[kAttendWaves][16];
     __shared__ unsigned last;
 
-    const AttendItem it = p.items[blockIdx.x];
-    const int head = blockIdx.y;
+    const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
+    const int head = blockIdx.x % p.cache.kv_heads;
     const PassSeq s = p.seqs[it.seq];
     const int* table = p.table + s.table;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -504,43 +558,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
     }
     if (only) return;
 
-    // the stores have to be out before the workgroup counts as arrived
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    unsigned* const arrived = p.arrived + static_cast<size_t>(it.tile) * p.cache.kv_heads + head;
-    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (last != static_cast<unsigned>(it.parts - 1)) return;
-    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int e = threadIdx.x; e < it.rows * kChunks; e += 64 * kAttendWaves) {
-        const int row = e / kChunks, dim = e % kChunks * 4, base = row * kPad * 4;
-        float top = -INFINITY, total = 0.0f;
-        f32x4 out{0, 0, 0, 0};
-        for (int j0 = 0; j0 < it.parts; j0 += 4) {  // four parts' loads in flight, folded in the order of the positions
-            v4i a[4], st[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + min(j0 + j, it.parts - 1) * part_stride, kBlock * 4);
-                a[j] = coherent_load16(rs, base + dim * 4);
-                st[j] = coherent_load16(rs, base + DH * 4);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (j0 + j >= it.parts) break;
-                const float high = __int_as_float(st[j].x), sum = __int_as_float(st[j].y);
-                const float up = fmaxf(top, high);
-                const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-                const float take = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(high - up);
-                total = total * keep + sum * take;
-                out = out * keep + __builtin_bit_cast(f32x4, a[j]) * take;
-                top = up;
-            }
-        }
-        const int r = it.r0 + row;
-        if (FULL || dim < p.cache.dim)
-            store_four<TYPE>(p.out, (s.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
-                             out / total);
-    }
+    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, s, head, parts, part_stride, last);
 }
 
 }  // namespace gh

@@ -174,7 +174,8 @@ static int plans(unsigned seed) {
                 n_tiles++;
                 const auto found = tiles.find({static_cast<int>(i), r0});
                 CHECK(found != tiles.end());
-                const std::vector<AttendItem>& t = found->second;
+                std::vector<AttendItem>& t = found->second;
+                std::sort(t.begin(), t.end(), [](const AttendItem& a, const AttendItem& b) { return a.k0 < b.k0; });
                 const int rows = std::min(height, news[i] * group - r0);
                 int low = INT_MAX, high = 0;
                 for (int r = r0; r < r0 + rows; r++) {

@@ -153,6 +153,44 @@ def test_attend_over_ragged_sequences(torch, dtype, heads):
     rig.check(seqs, counts, q, what="single tokens")
 
 
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attend_of_many_rows_beside_few(torch, dtype, heads):
+    h, kv, dim, page = HEADS[heads]
+    rig = Rig(torch, dtype, heads=h, kv_heads=kv, dim=dim, page=page, pages=4096 // page, seed=4)
+    seqs = [rig.add() for _ in range(4)]
+    rig.grow(seqs, [300, 64, 0, 5])
+    counts = [200, 1, 131, 70]
+    q = rig.grow(seqs, counts)
+    rig.check(seqs, counts, q, what="causal")
+    rig.check(seqs, counts, q, window=90, what="window")
+    rig.check(seqs, counts, q, causal=False, window=150, what="window ahead")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_never_see_what_they_may_not(torch, dtype):
+    """As below, in chunks of many rows: infinities and NaN in the chunk itself, of values and of keys."""
+    for dim, heads, kv in ((64, 2, 2), (128, 3, 1), (24, 1, 1)):
+        rig = Rig(torch, dtype, heads=heads, kv_heads=kv, dim=dim, page=16, pages=60, seed=5)
+        bad = torch.full((1, 960, kv, dim), float("nan")).to(rig.R.DTYPES[dtype])
+        bad[:, ::3] = -float("inf")
+        waste = rig.add()
+        rig.grow([waste], [960], k=bad, v=bad)
+        rig.drop(waste)
+        s = rig.add()
+        rig.grow([s], [133])
+        k, v = rig.rand(1, 250, kv, dim), rig.rand(1, 250, kv, dim)
+        v[0, 50, :, 3] = float("inf")
+        v[0, 120, :, 3] = -float("inf")
+        v[0, 120, 0, 9] = float("nan")
+        v[0, 200, :, dim - 1] = -float("inf")
+        k[0, 180, :, 1] = float("inf")
+        k[0, 230, :, 2] = float("nan")
+        q = rig.grow([s], [250], k=k, v=v)
+        rig.check([s], [250], q, what="later positions")
+        rig.check([s], [250], q, window=40, what="behind the window")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("before,new", [(0, 1), (0, 2), (0, 15), (0, 16), (0, 17), (0, 64), (0, 131), (15, 1), (16, 1), (31, 2), (63, 70), (127, 129), (1000, 1), (2047, 5)])
 def test_attend_at_the_edges_of_pages_and_tiles(torch, dtype, before, new):
