@@ -216,7 +216,15 @@ struct Cache {
                 for (int n : mine) tiles += (static_cast<long long>(n) * group + l.form.height - 1) / l.form.height;
                 if (tiles * o.kv_heads > (1 << 22)) refuse("a pass of more than 2^22 tiles of rows");
             }
-            l.cut = plan_attend(seqs, mine, group, o.kv_heads, l.form.height, causal, window, 1024, 128);
+            const bool tiles = l.form.height == kTileRows;
+            // Few rows: four workgroups to a compute unit in all, so that ragged sequences end together (16 sequences of 4 k to
+            // 32 k positions, 32/8 heads of 128 in bf16: 258 us, with one to a compute unit 289); parts below 64 KB of keys
+            // cost more to join than they save (13 sequences of up to 1 k positions, fp32: 14.5 us, 15.6 in parts of half
+            // that), and more than 64 parts of a tile are a long join (one sequence of 128 k positions: 59 us, 69 in 128).
+            // Many rows: as many as are resident at once, in the 16-bit types half of that, where joining parts of 128
+            // rows weighs more (777 rows, window 1024, fp16: 37 us, 41; 397 rows over 2 k positions, fp32: 45 us in half, 40).
+            const int workgroups = !tiles ? 1024 : bytes == 4 ? 512 : 256;
+            l.cut = plan_attend(seqs, mine, group, o.kv_heads, l.form.height, causal, window, workgroups, !tiles ? 1024 / bytes : 128, 64);
             part_bytes = std::max(part_bytes, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
             counters = std::max(counters, static_cast<size_t>(l.cut.tiles) * o.kv_heads);
         }
@@ -447,7 +455,6 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.cache = c.layout;
     p.q = cache_rows(q);
     p.out = cache_rows(out);
-    p.seqs = reinterpret_cast<const PassSeq*>(c.pass.at);
     p.table = reinterpret_cast<const int*>(c.pass.at + c.table_at);
     p.items = plan->at;
     p.layer = layer;
@@ -460,7 +467,7 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.arrived = reinterpret_cast<unsigned*>(c.arrived.at);
     for (const Cache::Plan::Launch& l : plan->launches) {
         if (!l.cut.items.empty()) {
-            hipLaunchKernelGGL(l.form.kernel, dim3(static_cast<unsigned>(l.cut.items.size()) * c.o.kv_heads), dim3(64 * kAttendWaves), 0, c.stream, p);
+            hipLaunchKernelGGL(l.form.kernel, dim3(static_cast<unsigned>(l.cut.items.size()) * c.o.kv_heads), dim3(l.form.threads), 0, c.stream, p);
             HIP_CHECK(hipGetLastError());
         }
         p.items += l.cut.items.size();

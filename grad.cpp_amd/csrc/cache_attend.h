@@ -10,6 +10,7 @@ using AttendKernel = void (*)(AttendParams);
 struct AttendForm {
     AttendKernel kernel = nullptr;
     int height = 0;       // rows of a tile
+    int threads = 0;
     int part_floats = 0;  // of a tile's part in memory
 };
 
@@ -20,12 +21,17 @@ AttendForm attend_form_f16(int dim, int rows);
 
 template <int TYPE, int DH, bool FULL>
 AttendForm attend_form_at(int rows) {
-    const auto form = [](AttendKernel kernel, int height) { return AttendForm{kernel, height, height * (DH + 4)}; };
-    if constexpr (TYPE != kCacheF32)
-        if (rows > 64) return form(attend_tile_kernel<TYPE, DH, FULL, DH == 256 ? 32 : 64>, kTileRows);
+    const auto form = [](AttendKernel kernel, int height, int waves) { return AttendForm{kernel, height, 64 * waves, height * (DH + 4)}; };
+    if (rows > 64) {
+        if constexpr (TYPE == kCacheF32) {
+            return form(attend_wide_kernel<DH, FULL, DH == 64 ? 64 : 32>, kTileRows, kTileWaves);
+        } else {
+            return form(attend_tile_kernel<TYPE, DH, FULL, DH == 256 ? 32 : 64>, kTileRows, kTileWaves);
+        }
+    }
     if constexpr (DH < 256)
-        if (rows > 16) return form(attend_rows_kernel<TYPE, DH, FULL, 2>, 32);
-    return form(attend_rows_kernel<TYPE, DH, FULL, 1>, 16);
+        if (rows > 16) return form(attend_rows_kernel<TYPE, DH, FULL, 2>, 32, attend_waves(DH, 2));
+    return form(attend_rows_kernel<TYPE, DH, FULL, 1>, 16, attend_waves(DH, 1));
 }
 
 template <int TYPE>

@@ -32,7 +32,7 @@ struct AttendItem {
     int index;  // which part this is
     int parts;
     int tile;
-    int pad[3];  // a multiple of 16 bytes
+    int first, row0, table;  // the sequence's, so that a kernel has them with the rest
 };
 
 struct AttendPlan {
@@ -49,9 +49,9 @@ inline void visible_span(const PassSeq& s, int r0, int rows, int group, bool cau
 }
 
 // Tiles of `height` rows; a tile's positions are cut into parts of one length so that the launch has about
-// `workgroups` of them over all kv heads, none shorter than `least` positions.
+// `workgroups` of them over all kv heads, none shorter than `least` positions and no tile in more than `most` parts.
 inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vector<int>& rows, int group, int kv_heads, int height,
-                              bool causal, int window, int workgroups, int least) {
+                              bool causal, int window, int workgroups, int least, int most) {
     AttendPlan plan;
     long long total = 0;
     for (size_t i = 0; i < seqs.size(); i++)
@@ -68,13 +68,13 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
             const int n = std::min(height, all - r0);
             int k0, k1;
             visible_span(seqs[i], r0, n, group, causal, window, k0, k1);
-            const int parts = std::max(1, (k1 - k0 + span - 1) / span);
+            const int parts = std::max(1, std::min(most, (k1 - k0 + span - 1) / span));
             const int part = parts > 1 ? plan.parts : -1, tile = parts > 1 ? plan.tiles : 0;
             // as even as whole runs of 32 positions allow
             const int run = (((k1 - k0 + parts - 1) / parts) + 31) / 32 * 32;
             const int made = std::max(1, (k1 - k0 + run - 1) / run);
             for (int j = 0; j < made; j++)
-                plan.items.push_back({static_cast<int>(i), r0, n, k0 + j * run, std::min(k1, k0 + (j + 1) * run), made > 1 ? part : -1, j, made, tile, {0, 0, 0}});
+                plan.items.push_back({static_cast<int>(i), r0, n, k0 + j * run, std::min(k1, k0 + (j + 1) * run), made > 1 ? part : -1, j, made, tile, seqs[i].first, seqs[i].row0, seqs[i].table});
             if (made > 1) {
                 plan.parts += made;
                 plan.tiles++;

@@ -86,7 +86,6 @@ struct CacheRows {
 struct AttendParams {
     CacheLayout cache;
     CacheRows q, out;
-    const PassSeq* seqs;
     const int* table;
     const AttendItem* items;
     int layer;
@@ -100,7 +99,6 @@ struct AttendParams {
 };
 
 constexpr int kBeyond = 0x40000000;  // past the end of any run (a run is a megabyte at most)
-constexpr int kAttendWaves = 4;
 
 // Largest value and sum over the four lanes that hold a row (lanes l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float row_max(float v) {
@@ -297,12 +295,29 @@ __device__ __forceinline__ void store_four(const CacheRows& rows, long long at, 
     }
 }
 
-// The workgroup's part of a tile is in memory: the last part to arrive folds all of them, in the order of the positions, and
-// writes the tile's outputs.
+// What a thread has folded of the parts of four output elements: their weighted sum, the maximum it is relative to, the sum.
+struct Folded {
+    f32x4 out;
+    float top, total;
+    __device__ __forceinline__ void fold(const f32x4& o, float high, float sum) {
+        const float up = fmaxf(top, high);
+        const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+        const float take = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(high - up);
+        total = total * keep + sum * take;
+        out = out * keep + o * take;
+        top = up;
+    }
+};
+
+// The workgroup's part of a tile is in memory: the last part to arrive folds all of them and writes the tile's outputs.
+// Every trip to memory is a microsecond, so a thread has AHEAD elements x parts in flight, and threads that have no element of
+// their own share the parts; the order of the folding is that of the positions whoever arrives when.
+// stash: 32 bytes of shared memory for each thread.
 template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS>
-__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, const PassSeq& s, int head, float* parts,
-                                             size_t part_stride, unsigned& last) {
-    constexpr int kPad = DH + 4, kChunks = DH / 4, kBlock = HEIGHT * kPad;
+__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, int head, float* parts,
+                                             size_t part_stride, unsigned& last, char* stash) {
+    constexpr int kPad = DH + 4, kChunks = DH / 4;
+    constexpr int kSide = HEIGHT > 64 ? 4 : 1, kDeep = HEIGHT > 64 ? 4 : 16;  // elements of a thread and parts, in flight
     // the stores have to be out before the workgroup counts as arrived
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -311,41 +326,72 @@ __device__ __forceinline__ void finish_parts(const AttendParams& p, const Attend
     __syncthreads();
     if (last != static_cast<unsigned>(it.parts - 1)) return;
     if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int e = threadIdx.x; e < it.rows * kChunks; e += THREADS) {
-        const int row = e / kChunks, dim = e % kChunks * 4, base = row * kPad * 4;
-        float top = -INFINITY, total = 0.0f;
-        f32x4 out{0, 0, 0, 0};
-        for (int j0 = 0; j0 < it.parts; j0 += 4) {  // four parts' loads in flight
-            v4i a[4], st[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + min(j0 + j, it.parts - 1) * part_stride, kBlock * 4);
-                a[j] = coherent_load16(rs, base + dim * 4);
-                st[j] = coherent_load16(rs, base + DH * 4);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (j0 + j >= it.parts) break;
-                const float high = __int_as_float(st[j].x), sum = __int_as_float(st[j].y);
-                const float up = fmaxf(top, high);
-                const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-                const float take = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(high - up);
-                total = total * keep + sum * take;
-                out = out * keep + __builtin_bit_cast(f32x4, a[j]) * take;
-                top = up;
-            }
-        }
-        const int r = it.r0 + row;
+    const int elements = it.rows * kChunks;
+    const int shares = max(1, min(THREADS / elements, (it.parts + kDeep - 1) / kDeep));  // of the parts
+    const int share = static_cast<int>(threadIdx.x) / elements;                          // (0 where there is one)
+    const int each = (it.parts + shares - 1) / shares;
+    const auto write = [&](int e, const Folded& f) {
+        const int r = it.r0 + e / kChunks, dim = e % kChunks * 4;
         if (FULL || dim < p.cache.dim)
-            store_four<TYPE>(p.out, (s.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
-                             out / total);
+            store_four<TYPE>(p.out, (it.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
+                             f.out / f.total);
+    };
+    for (int e0 = shares > 1 ? static_cast<int>(threadIdx.x) % elements : threadIdx.x; e0 < elements; e0 += kSide * THREADS) {
+        Folded f[kSide];
+#pragma unroll
+        for (int k = 0; k < kSide; k++) f[k] = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
+        const int from = shares > 1 ? min(share * each, it.parts) : 0, to = shares > 1 ? min(from + each, it.parts) : it.parts;
+        for (int j0 = from; j0 < to; j0 += kDeep) {
+            v4i a[kDeep][kSide], st[kDeep][kSide];
+#pragma unroll
+            for (int j = 0; j < kDeep; j++) {
+                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts, 0xFFFFFFFFu);
+                const unsigned place = static_cast<unsigned>(min(j0 + j, it.parts - 1) * part_stride * 4);
+#pragma unroll
+                for (int k = 0; k < kSide; k++) {
+                    const int e = min(e0 + k * THREADS, elements - 1);
+                    const unsigned base = place + e / kChunks * kPad * 4;
+                    a[j][k] = coherent_load16(rs, base + e % kChunks * 16);
+                    st[j][k] = coherent_load16(rs, base + DH * 4);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kDeep; j++)
+                if (j0 + j < to)
+#pragma unroll
+                    for (int k = 0; k < kSide; k++)
+                        f[k].fold(__builtin_bit_cast(f32x4, a[j][k]), __int_as_float(st[j][k].x), __int_as_float(st[j][k].y));
+        }
+        if (shares == 1) {
+#pragma unroll
+            for (int k = 0; k < kSide; k++)
+                if (e0 + k * THREADS < elements) write(e0 + k * THREADS, f[k]);
+        } else if (share < shares) {
+            *reinterpret_cast<f32x4*>(stash + threadIdx.x * 32) = f[0].out;
+            *reinterpret_cast<f32x4*>(stash + threadIdx.x * 32 + 16) = f32x4{f[0].top, f[0].total, 0.0f, 0.0f};
+        }
+    }
+    if (shares == 1) return;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < elements) {
+        Folded f{f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
+        for (int k = 0; k < shares; k++) {
+            const char* at = stash + (k * elements + threadIdx.x) * 32;
+            const f32x4 st = *reinterpret_cast<const f32x4*>(at + 16);
+            f.fold(*reinterpret_cast<const f32x4*>(at), st.x, st.y);
+        }
+        write(threadIdx.x, f);
     }
 }
 
-// Tiles of 16 TILES rows; the four wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
+// Wavefronts of a workgroup: eight, two on each of a compute unit's SIMDs, where 256 registers hold what one needs.
+constexpr int attend_waves(int dh, int tiles) { return dh * tiles <= 128 ? 8 : 4; }
+
+// Tiles of 16 TILES rows; the wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
 // A tile whose positions were dealt to several workgroups is finished by the last of them to arrive.
 template <int TYPE, int DH, bool FULL, int TILES>
-__global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const AttendParams p) {
+__global__ __launch_bounds__(64 * attend_waves(DH, TILES)) void attend_rows_kernel(const AttendParams p) {
+    constexpr int kAttendWaves = attend_waves(DH, TILES);
     using C = CacheType<TYPE>;
     using T = typename C::T;
     using G = Granule<TYPE, DH>;
@@ -356,8 +402,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
-    const PassSeq s = p.seqs[it.seq];
-    const int* table = p.table + s.table;
+    const int* table = p.table + it.table;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int quarter = lane >> 4;
 
@@ -369,8 +414,8 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
         const int r = it.r0 + 16 * rt + (lane & 15);
         const bool row = 16 * rt + (lane & 15) < it.rows;
         const int token = row ? r / p.group : 0, h = row ? r % p.group : 0;
-        pos[rt] = row ? s.first + token : -1;
-        const T* from = reinterpret_cast<const T*>(p.q.at) + (s.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
+        pos[rt] = row ? it.first + token : -1;
+        const T* from = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
 #pragma unroll
         for (int c = 0; c < G::kKeyWords / 4; c++) {
             const int dim = 4 * G::kQuarter * c + G::kQuarter * quarter;
@@ -391,7 +436,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
             for (int e = 0; e < 4; e++) q[rt][4 * c + e] = w[e];
         }
     }
-    const int first = s.first + it.r0 / p.group, final = s.first + (it.r0 + it.rows - 1) / p.group;
+    const int first = it.first + it.r0 / p.group, final = it.first + (it.r0 + it.rows - 1) / p.group;
 
     f32x4 o[TILES][kDims];
     float m[TILES], l[TILES];
@@ -544,7 +589,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
             if (only) {
                 const int r = it.r0 + 16 * rt + row;
                 if (FULL || dim < p.cache.dim)
-                    store_four<TYPE>(p.out, (s.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
+                    store_four<TYPE>(p.out, (it.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
                                      p.vector_rows, out / total);
             } else {
                 const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + it.index * part_stride, kBlock * 4);
@@ -558,7 +603,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_rows_kernel(const At
     }
     if (only) return;
 
-    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, s, head, parts, part_stride, last);
+    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, head, parts, part_stride, last, reinterpret_cast<char*>(meet));
 }
 
 }  // namespace gh

@@ -8,6 +8,7 @@
 // the transposing read, which hands a lane four positions of one dim (16 lanes to a cycle: four rows 32 bytes apart modulo 128).
 #pragma once
 
+#include "kernels_attn.h"
 #include "kernels_cache_attn.h"
 
 namespace gh {
@@ -45,6 +46,107 @@ __device__ __forceinline__ u32x2 read_transposed(const char* at) {
     return __builtin_bit_cast(u32x2, r);
 }
 
+// Asks the scheduler for PRODUCTS products that have READS reads from shared memory each, with DEEP products' reads under way
+// ahead of the first: on its own it reads for one product, waits, multiplies.
+template <int PRODUCTS, int READS, int DEEP>
+__device__ __forceinline__ void ahead_of_products() {
+    constexpr int kRead = 0x100, kProduct = 0x8;
+    __builtin_amdgcn_sched_group_barrier(kRead, READS * DEEP, 0);
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; i++) {
+        __builtin_amdgcn_sched_group_barrier(kProduct, 1, 0);
+        if (i + DEEP < PRODUCTS) __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
+    }
+}
+
+// A wavefront's rows [from, from + rows) of a tile, one after the other and term by term: 64 positions at a time, the scores with a
+// position to a lane, the output with a dim to a lane.  What a row may not see takes no part at all, infinities and NaN are what
+// they are.  For the tiles that hold such values (a matrix product would carry them to rows that do not see them, and make
+// NaN of an infinity's parts): an order of magnitude slower than the products.
+template <int TYPE, int DH>
+__device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, const int* table, int head, int from, int rows, float* part) {
+    using C = CacheType<TYPE>;
+    using T = typename C::T;
+    constexpr int kPad = DH + 4, kOwn = DH / 64;
+    const int lane = threadIdx.x & 63, dims = p.cache.dim, mask = (1 << p.cache.page_shift) - 1;
+    const auto at = [&](int which, int t) {
+        return reinterpret_cast<const T*>(cache_run(p.cache, table[t >> p.cache.page_shift], p.layer, which, head)) + static_cast<size_t>(t & mask) * dims;
+    };
+#pragma unroll 1
+    for (int i = from; i < from + rows; i++) {
+        const int r = it.r0 + i, token = r / p.group, h = head * p.group + r % p.group, pos = it.first + token;
+        const T* query = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + h * p.q.head;
+        const int begin = p.window > 0 ? max(it.k0, pos - p.window + 1) : it.k0, end = p.causal ? min(it.k1, pos + 1) : it.k1;
+        float m = -INFINITY, l = 0.0f, o[kOwn];
+#pragma unroll
+        for (int k = 0; k < kOwn; k++) o[k] = 0.0f;
+#pragma unroll 1
+        for (int t0 = begin; t0 < end; t0 += 64) {
+            const int n = min(64, end - t0);
+            float z = -INFINITY;
+            if (lane < n) {
+                const T* key = at(0, t0 + lane);
+                z = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < dims; d++) z = fmaf(static_cast<float>(query[d]), static_cast<float>(key[d]), z);
+                z *= p.scale;
+            }
+            const float top = fmaxf(m, wave_max(z));
+            const float keep = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+            const float prob = lane < n ? __builtin_amdgcn_exp2f(z - (top == -INFINITY ? 0.0f : top - C::kLift)) : 0.0f;
+            m = top;
+            l = l * keep + wave_sum(prob);
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) o[k] *= keep;
+#pragma unroll 1
+            for (int j = 0; j < n; j++) {
+                const float w = __shfl(prob, j);
+                const T* value = at(1, t0 + j);
+#pragma unroll
+                for (int k = 0; k < kOwn; k++)
+                    if (lane + 64 * k < dims) o[k] = fmaf(w, static_cast<float>(value[lane + 64 * k]), o[k]);
+            }
+        }
+        if (it.parts == 1) {
+            T* to = reinterpret_cast<T*>(p.out.at) + (it.row0 + token) * p.out.row + h * p.out.head;
+#pragma unroll
+            for (int k = 0; k < kOwn; k++)
+                if (lane + 64 * k < dims) to[lane + 64 * k] = static_cast<T>(o[k] / l);
+        } else {
+            float* to = part + i * kPad;
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) partial_store(to + lane + 64 * k, o[k]);
+            if (lane < 2) partial_store(to + DH + lane, lane == 0 ? m : l);
+        }
+    }
+}
+
+// A wavefront's rows, whole and to the caller, or a part of them and to the place of the part.  A lane has every other run of
+// four dims of its row.
+template <int TYPE, int DH, bool FULL>
+__device__ __forceinline__ void leave_rows(const AttendParams& p, const AttendItem& it, const f32x16 (&o)[DH / 32], float m, float l, bool row,
+                                           int token, int h, int r, int half, float* part) {
+    constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
+    if (!row) return;
+    const __amdgpu_buffer_rsrc_t rs = make_buffer(part, kBlock * 4);
+    const int base = r * kPad * 4;
+    const long long to = (it.row0 + token) * p.out.row + h * p.out.head;
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int dim = 32 * d + 8 * i + 4 * half;
+            const f32x4 four{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            if (it.parts == 1) {
+                if (FULL || dim < p.cache.dim) store_four<TYPE>(p.out, to + dim, p.vector_rows, four / l);
+            } else {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, four), rs, base + dim * 4, 0, kAuxDeviceScope);
+            }
+        }
+    if (it.parts > 1 && half == 0)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, f32x4{m, l, 0.0f, 0.0f}), rs, base + DH * 4, 0, kAuxDeviceScope);
+}
+
 // Sixteen-bit types.  TOKENS positions at a time.
 template <int TYPE, int DH, bool FULL, int TOKENS>
 __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile_kernel(const AttendParams p) {
@@ -60,8 +162,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
-    const PassSeq s = p.seqs[it.seq];
-    const int* table = p.table + s.table;
+    const int* table = p.table + it.table;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5;
 
@@ -69,10 +170,10 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     const int r = it.r0 + 32 * wave + (lane & 31);
     const bool row = 32 * wave + (lane & 31) < it.rows;
     const int token = row ? r / p.group : 0, h = row ? r % p.group : 0;
-    const int pos = row ? s.first + token : -1;
+    const int pos = row ? it.first + token : -1;
     u32x4 q[kSteps];
     {
-        const T* from = reinterpret_cast<const T*>(p.q.at) + (s.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
+        const T* from = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
 #pragma unroll
         for (int c = 0; c < kSteps; c++) {
             const int dim = 16 * c + 8 * half;
@@ -90,9 +191,9 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     }
     // positions of the tile's and of this wavefront's first and last rows
     const int rows_here = min(32, it.rows - 32 * wave);
-    const int first_all = s.first + it.r0 / p.group, final_all = s.first + (it.r0 + it.rows - 1) / p.group;
-    const int first = s.first + (it.r0 + 32 * wave) / p.group;
-    const int final = s.first + (it.r0 + 32 * wave + max(rows_here, 1) - 1) / p.group;
+    const int first_all = it.first + it.r0 / p.group, final_all = it.first + (it.r0 + it.rows - 1) / p.group;
+    const int first = it.first + (it.r0 + 32 * wave) / p.group;
+    const int final = it.first + (it.r0 + 32 * wave + max(rows_here, 1) - 1) / p.group;
 
     f32x16 o[kWide];
 #pragma unroll
@@ -101,25 +202,27 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    // a thread's units of 16 bytes: rows of one block of 16 positions for a wavefront, so one page
+    // A wavefront's loads are whole rows of one block of 16 positions, so of one page; the pages of the tile behind the next are
+    // looked up while the next one is fetched, or every load would wait for its own look at the list.
     u32x4 kr[kLoads], vr[kLoads];
-    const int bytes = p.cache.dim * 2;
+    int pages[kLoads];
+    const int bytes = p.cache.dim * 2, own_row = lane / kUnits;
+    static_assert(64 % kUnits == 0, "whole rows");
+    const int own = FULL || lane % kUnits * 8 < p.cache.dim ? own_row * bytes + lane % kUnits * 16 : kBeyond;
+    const auto row_of = [&](int i) { return 64 * (kTileWaves * i + wave) / kUnits; };
+    const auto look = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) pages[i] = table[min(at + row_of(i), it.k1 - 1) >> p.cache.page_shift];
+    };
     const auto fetch = [&](int at) {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            constexpr int kRows = 64 / kUnits > 0 ? 64 / kUnits : 1;  // of a wavefront's load (DH 512 and more: none)
-            const int unit = 64 * (kTileWaves * i + wave);
-            const int row0 = unit / kUnits;  // first row of the load
-            const int t0 = at + row0 < it.k1 ? at + row0 : at;
-            const int page = table[t0 >> p.cache.page_shift];
-            const char* run = cache_run(p.cache, page, p.layer, 0, head);
+            const char* run = cache_run(p.cache, pages[i], p.layer, 0, head);
             const __amdgpu_buffer_rsrc_t ks = make_buffer(run, static_cast<unsigned>(p.cache.run_bytes));
             const __amdgpu_buffer_rsrc_t vs = make_buffer(run + p.cache.kv_heads * p.cache.run_bytes, static_cast<unsigned>(p.cache.run_bytes));
-            const int mine = lane / kUnits, dim = lane % kUnits * 8;
-            static_assert(kRows * kUnits == 64, "whole rows");
-            const bool there = (FULL || dim < p.cache.dim) && at + row0 + mine < it.k1;
-            const int offset = there ? mine * bytes + dim * 2 : kBeyond;  // (places behind the last position: zeros)
-            const int base = (t0 & ((1 << p.cache.page_shift) - 1)) * bytes;
+            const int t = at + row_of(i);
+            const int offset = t + own_row < it.k1 ? own : kBeyond;  // (places behind the last position: zeros)
+            const int base = (t & ((1 << p.cache.page_shift) - 1)) * bytes;
             kr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ks, offset, base, 0));
             vr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vs, offset, base, 0));
         }
@@ -129,53 +232,58 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     const char* const value_at = values + (4 * half + ((lane & 15) >> 2)) * kValueRow + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
     if (threadIdx.x == 0) odd = 0;
+    look(it.k0);
     fetch(it.k0);
+    look(it.k0 + TOKENS);
     for (int at = it.k0; at < it.k1; at += TOKENS) {
         const bool cut_all = (p.causal && at + TOKENS - 1 > first_all) || (p.window > 0 && at <= final_all - p.window);
         __syncthreads();
-        bool bad = false;
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const int unit = 64 * (kTileWaves * i + wave) + lane;
             const int to = unit / kUnits, c = unit % kUnits * 16;
             *reinterpret_cast<u32x4*>(keys + to * kKeyRow + c) = kr[i];
             *reinterpret_cast<u32x4*>(values + to * kValueRow + c) = vr[i];
-            if (cut_all)
+        }
+        if (cut_all) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < kLoads; i++)
 #pragma unroll
                 for (int w = 0; w < 4; w++) bad = bad || unbounded<TYPE>(vr[i][w]);
+            if (bad) odd = 1;
         }
-        // infinities and NaN among values that some rows may not see: the positions from `at` on are marked
-        if (bad) odd = static_cast<unsigned>(at) + 1;
         __syncthreads();
-        if (at + TOKENS < it.k1) fetch(at + TOKENS);
+        // Infinities and NaN among values that some rows may not see.  (Nobody writes `odd` before everybody has read it: the next
+        // tile is put in place behind the next meeting.)
+        if (cut_all && __builtin_amdgcn_readfirstlane(odd)) break;
+        if (at + TOKENS < it.k1) {
+            fetch(at + TOKENS);
+            look(at + 2 * TOKENS);
+        }
         if (rows_here <= 0 || (p.causal && at > final) || (p.window > 0 && at + TOKENS - 1 <= first - p.window)) continue;
 
-        float z[kBlocks][16];
+        f32x16 z[kBlocks];
 #pragma unroll
-        for (int b = 0; b < kBlocks; b++) {
-            f32x16 acc;
+        for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[i] = 0.0f;
+            for (int i = 0; i < 16; i++) z[b][i] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < kSteps; c++)
-                acc = mfma32<TYPE>(*reinterpret_cast<const u32x4*>(key_at + b * 32 * kKeyRow + c * 32), q[c], acc);
+        for (int c = 0; c < kSteps; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) z[b][i] = acc[i];
-        }
+            for (int b = 0; b < kBlocks; b++)
+                z[b] = mfma32<TYPE>(*reinterpret_cast<const u32x4*>(key_at + b * 32 * kKeyRow + c * 32), q[c], z[b]);
+        ahead_of_products<kBlocks * kSteps, 1, 6>();
         const bool cut = at + TOKENS > it.k1 || (p.causal && at + TOKENS - 1 > first) || (p.window > 0 && at <= final - p.window);
-        unsigned seen[kBlocks];
         if (cut) {
 #pragma unroll
-            for (int b = 0; b < kBlocks; b++) {
-                seen[b] = 0;
+            for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int t = at + 32 * b + 8 * (i / 4) + 4 * half + (i & 3);
                     const bool see = t < it.k1 && (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window);
                     z[b][i] = see ? z[b][i] : -INFINITY;
-                    seen[b] |= see ? 1u << i : 0u;
                 }
-            }
         }
         float top = z[0][0];
 #pragma unroll
@@ -200,68 +308,337 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
                 z[b][i] = __builtin_amdgcn_exp2f(z[b][i] * p.scale - base);
                 l += z[b][i];
             }
-        const bool careful = cut && __builtin_amdgcn_readfirstlane(odd) == static_cast<unsigned>(at) + 1;
+        u32x4 prob[kBlocks][2];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                u32x4 prob;
+            for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int w = 0; w < 4; w++)
-                    prob[w] = __builtin_bit_cast(
+                    prob[b][u][w] = __builtin_bit_cast(
                         unsigned, typename C::V2{static_cast<T>(z[b][8 * u + 2 * w]), static_cast<T>(z[b][8 * u + 2 * w + 1])});
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int d = 0; d < kWide; d++) {
                     const char* v = value_at + (32 * b + 16 * u) * kValueRow + d * 64;
                     const u32x2 low = read_transposed(v), high = read_transposed(v + 8 * kValueRow);
-                    u32x4 a{low.x, low.y, high.x, high.y};
-                    if (careful) {
-                        u32x4 kind, see;
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            kind[w] = unbounded_kind<TYPE>(a[w]);
-                            a[w] = bounded<TYPE>(a[w]);
-                            const unsigned bits = seen[b] >> (8 * u + 2 * w);
-                            see[w] = (bits & 1u) * C::kOne | ((bits >> 1) & 1u) * (C::kOne << 16);
-                        }
-                        f32x16 n;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) n[i] = 0.0f;
-                        n = mfma32<TYPE>(kind, see, n);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[d][i] += unbounded_sum(n[i]);
-                    }
-                    o[d] = mfma32<TYPE>(a, prob, o[d]);
+                    o[d] = mfma32<TYPE>(u32x4{low.x, low.y, high.x, high.y}, prob[b][u], o[d]);
                 }
-            }
+        ahead_of_products<kBlocks * 2 * kWide, 2, 4>();
     }
 
     const bool only = it.parts == 1;
     constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
     float* const parts = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     const size_t part_stride = static_cast<size_t>(p.cache.kv_heads) * kBlock;
-    l = both_sum(l);
-    if (row) {
-        const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + (only ? 0 : it.index) * part_stride, kBlock * 4);
-        const int base = (32 * wave + (lane & 31)) * kPad * 4;
-        const long long to = (s.row0 + token) * p.out.row + (head * p.group + h) * p.out.head;
-#pragma unroll
-        for (int d = 0; d < kWide; d++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int dim = 32 * d + 8 * i + 4 * half;
-                const f32x4 four{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                if (only) {
-                    if (FULL || dim < p.cache.dim) store_four<TYPE>(p.out, to + dim, p.vector_rows, four / l);
-                } else {
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, four), rs, base + dim * 4, 0, kAuxDeviceScope);
-                }
-            }
-        if (!only && half == 0)
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, f32x4{m, l, 0.0f, 0.0f}), rs, base + DH * 4, 0, kAuxDeviceScope);
+    if (__builtin_amdgcn_readfirstlane(odd)) {
+        rows_one_by_one<TYPE, DH>(p, it, table, head, 32 * wave, rows_here, parts + (only ? 0 : it.index) * part_stride);
+    } else {
+        leave_rows<TYPE, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half,
+                                   parts + (only ? 0 : it.index) * part_stride);
     }
     if (only) return;
-    finish_parts<TYPE, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, s, head, parts, part_stride, last);
+    finish_parts<TYPE, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, parts, part_stride, last, keys);
+}
+
+// ---------------------------------------------------------------------- fp32
+//
+// The fp32 matrix instructions have a sixteenth of the 16-bit ones' rate, so fp32 operands are taken as sums of three bf16
+// parts, x = high + middle + low, cut off and not rounded: eight bits each, 24 together, nothing is lost and nothing can
+// overflow.  Six of the nine products of parts are formed; the three left out are below 2^-24 of the whole.  The matrix
+// core cuts sums off where fp32 rounds, so products of high parts are summed over one tile of positions, from zero, apart
+// from the small ones (whose cut-off bits count for 2^-8 of theirs), and added to the running output in fp32.
+
+struct Parts {
+    u32x2 high, middle, low;  // of four values, bf16
+};
+
+__device__ __forceinline__ unsigned high_halves(float a, float b) {  // {a's, b's} upper 16 bits
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float cut_off(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
+
+// `taint` becomes NaN if any value is infinite or NaN: its rest is.
+__device__ __forceinline__ Parts three_parts(const f32x4& x, float& taint) {
+    Parts p;
+    float r[4], s[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        r[e] = x[e] - cut_off(x[e]);
+        s[e] = r[e] - cut_off(r[e]);
+        taint = fmaf(s[e], 0.0f, taint);
+    }
+    p.high = u32x2{high_halves(x[0], x[1]), high_halves(x[2], x[3])};
+    p.middle = u32x2{high_halves(r[0], r[1]), high_halves(r[2], r[3])};
+    p.low = u32x2{high_halves(s[0], s[1]), high_halves(s[2], s[3])};
+    return p;
+}
+
+template <int DH, bool FULL, int TOKENS>
+__global__ __launch_bounds__(64 * kTileWaves, DH > 64 ? 1 : 2) void attend_wide_kernel(const AttendParams p) {
+    constexpr int kKeyRow = DH * 2 + 16, kValueRow = DH * 2 + 32;  // bytes of a part's row
+    constexpr int kKeys = TOKENS * kKeyRow, kValues = TOKENS * kValueRow;
+    constexpr int kUnits = DH / 4;                               // of four values in a row
+    constexpr int kLoads = TOKENS * kUnits / (64 * kTileWaves);  // of a thread, for K and for V
+    constexpr int kBlocks = TOKENS / 32, kSteps = DH / 16, kWide = DH / 32;
+    __shared__ __align__(16) char keys[3 * kKeys];
+    __shared__ __align__(16) char values[3 * kValues];
+    __shared__ unsigned last, odd;
+
+    const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
+    const int head = blockIdx.x % p.cache.kv_heads;
+    const int* table = p.table + it.table;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = lane >> 5;
+
+    const int r = it.r0 + 32 * wave + (lane & 31);
+    const bool row = 32 * wave + (lane & 31) < it.rows;
+    const int token = row ? r / p.group : 0, h = row ? r % p.group : 0;
+    const int pos = row ? it.first + token : -1;
+    const float* const query = reinterpret_cast<const float*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
+    u32x4 q[3][kSteps];
+    float taint = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kSteps; c++) {
+        const int dim = 16 * c + 8 * half;
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            f32x4 x{0, 0, 0, 0};
+            if (row && (FULL || dim < p.cache.dim)) {
+                if (p.vector_rows) {
+                    x = *reinterpret_cast<const f32x4*>(query + dim + 4 * side);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = query[dim + 4 * side + e];
+                }
+            }
+            const Parts parts = three_parts(x, taint);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                q[0][c][2 * side + w] = parts.high[w];
+                q[1][c][2 * side + w] = parts.middle[w];
+                q[2][c][2 * side + w] = parts.low[w];
+            }
+        }
+    }
+    const int rows_here = min(32, it.rows - 32 * wave);
+    const int first = it.first + (it.r0 + 32 * wave) / p.group;
+    const int final = it.first + (it.r0 + 32 * wave + max(rows_here, 1) - 1) / p.group;
+
+    f32x16 o[kWide];
+#pragma unroll
+    for (int d = 0; d < kWide; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    f32x4 kr[kLoads], vr[kLoads];
+    int pages[kLoads];
+    const int bytes = p.cache.dim * 4, own_row = lane / kUnits;
+    static_assert(64 % kUnits == 0, "whole rows");
+    const int own = FULL || lane % kUnits * 4 < p.cache.dim ? own_row * bytes + lane % kUnits * 16 : kBeyond;
+    const auto row_of = [&](int i) { return 64 * (kTileWaves * i + wave) / kUnits; };
+    const auto look = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) pages[i] = table[min(at + row_of(i), it.k1 - 1) >> p.cache.page_shift];
+    };
+    const auto fetch = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const char* run = cache_run(p.cache, pages[i], p.layer, 0, head);
+            const __amdgpu_buffer_rsrc_t ks = make_buffer(run, static_cast<unsigned>(p.cache.run_bytes));
+            const __amdgpu_buffer_rsrc_t vs = make_buffer(run + p.cache.kv_heads * p.cache.run_bytes, static_cast<unsigned>(p.cache.run_bytes));
+            const int t = at + row_of(i);
+            const int offset = t + own_row < it.k1 ? own : kBeyond;  // (places behind the last position: zeros)
+            const int base = (t & ((1 << p.cache.page_shift) - 1)) * bytes;
+            kr[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ks, offset, base, 0));
+            vr[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(vs, offset, base, 0));
+        }
+    };
+    const auto put = [&] {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const Parts k = three_parts(kr[i], taint), v = three_parts(vr[i], taint);
+            const int unit = 64 * (kTileWaves * i + wave) + lane;
+            char* const to_k = keys + unit / kUnits * kKeyRow + unit % kUnits * 8;
+            char* const to_v = values + unit / kUnits * kValueRow + unit % kUnits * 8;
+            *reinterpret_cast<u32x2*>(to_k) = k.high;
+            *reinterpret_cast<u32x2*>(to_k + kKeys) = k.middle;
+            *reinterpret_cast<u32x2*>(to_k + 2 * kKeys) = k.low;
+            *reinterpret_cast<u32x2*>(to_v) = v.high;
+            *reinterpret_cast<u32x2*>(to_v + kValues) = v.middle;
+            *reinterpret_cast<u32x2*>(to_v + 2 * kValues) = v.low;
+        }
+        if (taint != 0.0f) odd = 1;
+    };
+    const char* const key_at = keys + (lane & 31) * kKeyRow + half * 16;
+    const char* const value_at = values + (4 * half + ((lane & 15) >> 2)) * kValueRow + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+
+    if (threadIdx.x == 0) odd = 0;
+    look(it.k0);
+    fetch(it.k0);
+    look(it.k0 + TOKENS);
+    for (int at = it.k0; at < it.k1; at += TOKENS) {
+        __syncthreads();
+        put();
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(odd)) break;  // infinities or NaN (written again behind the next meeting only)
+        if (at + TOKENS < it.k1) {
+            fetch(at + TOKENS);
+            look(at + 2 * TOKENS);
+        }
+        if (rows_here <= 0 || (p.causal && at > final) || (p.window > 0 && at + TOKENS - 1 <= first - p.window)) continue;
+
+        float z[kBlocks][16];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+            f32x16 acc;
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[i] = 0.0f;
+            if constexpr (kSteps <= 8) {  // registers hold the parts of all dims: small products first, then the large ones
+                u32x4 k[3][kSteps];
+#pragma unroll
+                for (int c = 0; c < kSteps; c++)
+#pragma unroll
+                    for (int part = 0; part < 3; part++)
+                        k[part][c] = *reinterpret_cast<const u32x4*>(key_at + part * kKeys + b * 32 * kKeyRow + c * 32);
+#pragma unroll
+                for (int c = 0; c < kSteps; c++) {
+                    acc = mfma32<kCacheBf16>(k[2][c], q[0][c], acc);
+                    acc = mfma32<kCacheBf16>(k[1][c], q[1][c], acc);
+                    acc = mfma32<kCacheBf16>(k[0][c], q[2][c], acc);
+                }
+#pragma unroll
+                for (int c = 0; c < kSteps; c++) {
+                    acc = mfma32<kCacheBf16>(k[1][c], q[0][c], acc);
+                    acc = mfma32<kCacheBf16>(k[0][c], q[1][c], acc);
+                }
+#pragma unroll
+                for (int c = 0; c < kSteps; c++) acc = mfma32<kCacheBf16>(k[0][c], q[0][c], acc);
+#pragma unroll
+                for (int i = 0; i < 16; i++) z[b][i] = acc[i];
+            } else {  // ... or the two have sums of their own
+                f32x16 small;
+#pragma unroll
+                for (int i = 0; i < 16; i++) small[i] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < kSteps; c++) {
+                    const char* k = key_at + b * 32 * kKeyRow + c * 32;
+                    const u32x4 k0 = *reinterpret_cast<const u32x4*>(k), k1 = *reinterpret_cast<const u32x4*>(k + kKeys),
+                                k2 = *reinterpret_cast<const u32x4*>(k + 2 * kKeys);
+                    small = mfma32<kCacheBf16>(k2, q[0][c], small);
+                    small = mfma32<kCacheBf16>(k1, q[1][c], small);
+                    small = mfma32<kCacheBf16>(k0, q[2][c], small);
+                    small = mfma32<kCacheBf16>(k1, q[0][c], small);
+                    small = mfma32<kCacheBf16>(k0, q[1][c], small);
+                    acc = mfma32<kCacheBf16>(k0, q[0][c], acc);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) z[b][i] = acc[i] + small[i];
+            }
+        }
+        const bool cut = at + TOKENS > it.k1 || (p.causal && at + TOKENS - 1 > first) || (p.window > 0 && at <= final - p.window);
+        if (cut) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int t = at + 32 * b + 8 * (i / 4) + 4 * half + (i & 3);
+                    const bool see = t < it.k1 && (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window);
+                    z[b][i] = see ? z[b][i] : -INFINITY;
+                }
+        }
+        float top = z[0][0];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, z[b][i]);
+        top = both_max(top) * p.scale;
+        if (__any(top > m)) {
+            const float keep = top > m ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            m = fmaxf(m, top);
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < kWide; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= keep;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        u32x4 prob[3][kBlocks][2];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                f32x4 e;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    e[i] = __builtin_amdgcn_exp2f(z[b][4 * g + i] * p.scale - base);
+                    l += e[i];
+                }
+                float none = 0.0f;
+                const Parts parts = three_parts(e, none);
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    prob[0][b][g / 2][2 * (g & 1) + w] = parts.high[w];
+                    prob[1][b][g / 2][2 * (g & 1) + w] = parts.middle[w];
+                    prob[2][b][g / 2][2 * (g & 1) + w] = parts.low[w];
+                }
+            }
+#pragma unroll
+        for (int d = 0; d < kWide; d++) {
+            u32x4 v[3][kBlocks][2];
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int part = 0; part < 3; part++) {
+                        const char* from = value_at + part * kValues + (32 * b + 16 * u) * kValueRow + d * 64;
+                        const u32x2 low = read_transposed(from), high = read_transposed(from + 8 * kValueRow);
+                        v[part][b][u] = u32x4{low.x, low.y, high.x, high.y};
+                    }
+            f32x16 acc;
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[i] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    acc = mfma32<kCacheBf16>(v[2][b][u], prob[0][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[1][b][u], prob[1][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[0][b][u], prob[2][b][u], acc);
+                }
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    acc = mfma32<kCacheBf16>(v[1][b][u], prob[0][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[0][b][u], prob[1][b][u], acc);
+                }
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) acc = mfma32<kCacheBf16>(v[0][b][u], prob[0][b][u], acc);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] += acc[i];
+        }
+    }
+
+    const bool only = it.parts == 1;
+    constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
+    float* const parts = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
+    const size_t part_stride = static_cast<size_t>(p.cache.kv_heads) * kBlock;
+    if (__builtin_amdgcn_readfirstlane(odd)) {
+        rows_one_by_one<kCacheF32, DH>(p, it, table, head, 32 * wave, rows_here, parts + (only ? 0 : it.index) * part_stride);
+    } else {
+        leave_rows<kCacheF32, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half,
+                                        parts + (only ? 0 : it.index) * part_stride);
+    }
+    if (only) return;
+    finish_parts<kCacheF32, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, parts, part_stride, last, keys);
 }
 
 }  // namespace gh

@@ -156,7 +156,7 @@ static int plans(unsigned seed) {
         const int group = 1 + static_cast<int>(rng() % 5), height = 16 << (rng() % 3), kv = 1 + static_cast<int>(rng() % 8);
         const bool causal = rng() % 4 != 0;
         const int window = rng() % 3 ? 0 : 1 + static_cast<int>(rng() % 300);
-        const int workgroups = 1 << (rng() % 12), least = 128;
+        const int workgroups = 1 << (rng() % 12), least = 128, most = 1 + static_cast<int>(rng() % 64);
         std::vector<PassSeq> seqs;
         std::vector<int> news;
         for (int i = static_cast<int>(rng() % 5); i >= 0; i--) {
@@ -164,7 +164,7 @@ static int plans(unsigned seed) {
             seqs.push_back({first + n, first, 0, 0});
             news.push_back(n);
         }
-        const AttendPlan plan = plan_attend(seqs, news, group, kv, height, causal, window, workgroups, least);
+        const AttendPlan plan = plan_attend(seqs, news, group, kv, height, causal, window, workgroups, least, most);
         std::map<std::pair<int, int>, std::vector<AttendItem>> tiles;
         for (const AttendItem& it : plan.items) tiles[{it.seq, it.r0}].push_back(it);
         size_t n_tiles = 0;
@@ -183,6 +183,7 @@ static int plans(unsigned seed) {
                     low = std::min(low, window ? std::max(0, pos - window + 1) : 0);
                     high = std::max(high, causal ? pos + 1 : seqs[i].len);
                 }
+                CHECK(static_cast<int>(t.size()) <= most);
                 CHECK(t[0].k0 <= low && t[0].k0 % 16 == 0 && t.back().k1 == high);
                 for (size_t j = 0; j < t.size(); j++) {
                     CHECK(t[j].rows == rows && t[j].parts == static_cast<int>(t.size()) && t[j].index == static_cast<int>(j));
