@@ -217,14 +217,15 @@ struct Cache {
                 if (tiles * o.kv_heads > (1 << 22)) refuse("a pass of more than 2^22 tiles of rows");
             }
             const bool tiles = l.form.height == kTileRows;
-            // Few rows: four workgroups to a compute unit in all, so that ragged sequences end together (16 sequences of 4 k to
-            // 32 k positions, 32/8 heads of 128 in bf16: 258 us, with one to a compute unit 289); parts below 64 KB of keys
-            // cost more to join than they save (13 sequences of up to 1 k positions, fp32: 14.5 us, 15.6 in parts of half
-            // that), and more than 64 parts of a tile are a long join (one sequence of 128 k positions: 59 us, 69 in 128).
+            // Few rows: several workgroups to a compute unit, so that ragged sequences end together (16 sequences of 4 k to
+            // 32 k positions, 32/8 heads of 128 in bf16: 256 us, with half as many 262, a quarter 275); parts below 64 KB of
+            // keys cost more to join than they save (13 sequences of up to 1 k positions, fp32: 14.5 us, 15.5 in parts of
+            // half that), and more than 64 parts of a tile are a long join (one sequence of 128 k positions: 61 us, 71 in 128).
             // Many rows: as many as are resident at once, in the 16-bit types half of that, where joining parts of 128
             // rows weighs more (777 rows, window 1024, fp16: 37 us, 41; 397 rows over 2 k positions, fp32: 45 us in half, 40).
-            const int workgroups = !tiles ? 1024 : bytes == 4 ? 512 : 256;
-            l.cut = plan_attend(seqs, mine, group, o.kv_heads, l.form.height, causal, window, workgroups, !tiles ? 1024 / bytes : 128, 64);
+            const int workgroups = !tiles ? (bytes == 4 ? 1024 : 2048) : bytes == 4 ? 512 : 256;
+            const int least = tiles ? 128 : bytes == 4 ? 256 : 384;
+            l.cut = plan_attend(seqs, mine, group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64);
             part_bytes = std::max(part_bytes, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
             counters = std::max(counters, static_cast<size_t>(l.cut.tiles) * o.kv_heads);
         }

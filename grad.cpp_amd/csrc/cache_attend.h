@@ -30,8 +30,8 @@ AttendForm attend_form_at(int rows) {
         }
     }
     if constexpr (DH < 256)
-        if (rows > 16) return form(attend_rows_kernel<TYPE, DH, FULL, 2>, 32, attend_waves(DH, 2));
-    return form(attend_rows_kernel<TYPE, DH, FULL, 1>, 16, attend_waves(DH, 1));
+        if (rows > 16) return form(attend_rows_kernel<TYPE, DH, FULL, 2>, 32, attend_waves(TYPE, DH, 2));
+    return form(attend_rows_kernel<TYPE, DH, FULL, 1>, 16, attend_waves(TYPE, DH, 1));
 }
 
 template <int TYPE>

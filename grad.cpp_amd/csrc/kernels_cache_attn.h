@@ -384,14 +384,16 @@ __device__ __forceinline__ void finish_parts(const AttendParams& p, const Attend
     }
 }
 
-// Wavefronts of a workgroup: eight, two on each of a compute unit's SIMDs, where 256 registers hold what one needs.
-constexpr int attend_waves(int dh, int tiles) { return dh * tiles <= 128 ? 8 : 4; }
+// Wavefronts of a workgroup: as many as take 128 positions at a time (fp32, one token: 64 sequences of up to 2 k positions
+// 88 us, with four 91; bf16 and fp16: 32 sequences at a window of 1024, heads of 80, 15.6 us, with eight 19.2; one of
+// 128 k positions 61 and 59), where 256 registers hold what one needs.
+constexpr int attend_waves(int type, int dh, int tiles) { return type == kCacheF32 && dh * tiles <= 128 ? 8 : 4; }
 
 // Tiles of 16 TILES rows; the wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
 // A tile whose positions were dealt to several workgroups is finished by the last of them to arrive.
 template <int TYPE, int DH, bool FULL, int TILES>
-__global__ __launch_bounds__(64 * attend_waves(DH, TILES)) void attend_rows_kernel(const AttendParams p) {
-    constexpr int kAttendWaves = attend_waves(DH, TILES);
+__global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_rows_kernel(const AttendParams p) {
+    constexpr int kAttendWaves = attend_waves(TYPE, DH, TILES);
     using C = CacheType<TYPE>;
     using T = typename C::T;
     using G = Granule<TYPE, DH>;
