@@ -87,6 +87,13 @@ struct Staging {
         Slot& s = slots[turn];
         const size_t words = (bytes + 15) / 16;
         if (words == 0) return;
+        if (words <= kWordsListed) {  // with the launch itself: no trip over the bus, no event
+            WordList list;
+            std::memcpy(list.words, s.at, bytes);
+            hipLaunchKernelGGL(cache_hand_kernel, dim3(1), dim3(256), 0, stream, list, reinterpret_cast<u32x4*>(to), static_cast<int>(words));
+            HIP_CHECK(hipGetLastError());
+            return;
+        }
         const int groups = static_cast<int>(std::min<size_t>(256, (words + 255) / 256));
         hipLaunchKernelGGL(cache_load_kernel, dim3(groups), dim3(256), 0, stream, reinterpret_cast<const u32x4*>(s.at),
                            reinterpret_cast<u32x4*>(to), words);
@@ -112,7 +119,7 @@ struct Cache {
     int bytes = 4;  // of an element
     CacheLayout layout{};
     PageBook book;
-    DeviceBuffer pool, speed, pass, lists, parts, arrived;
+    DeviceBuffer pool, speed, pass, parts, arrived;
     Staging staging;
     hipEvent_t moved = nullptr;  // from one stream to the next
     hipStream_t stream = nullptr;  // of the last call
@@ -123,7 +130,7 @@ struct Cache {
     int rows = 0;
     std::vector<PassSeq> seqs;
     std::vector<int> news;
-    size_t rows_at = 0, table_at = 0, items_at = 0;  // in `pass`, behind the sequences
+    size_t rows_at = 0, table_at = 0;  // in `pass`
 
     // its attention, as it was last cut up for a mask
     struct Plan {
@@ -185,14 +192,17 @@ struct Cache {
         for (Plan& p : plans) p.valid = false;
     }
 
-    void copy_pages(const char* from, const PageCopy* device_list, int n) {
-        if (n == 0) return;
+    void copy_pages(const char* from, const std::vector<PageCopy>& copies) {
         const int runs = o.layers * 2 * o.kv_heads, token_bytes = o.head_dim * bytes;
-        // ~2048 workgroups: eight per compute unit
-        const int x = std::max(1, std::min(runs, 2048 / std::min(n, 2048)));
-        hipLaunchKernelGGL(cache_copy_kernel, dim3(x, std::min(n, 65535)), dim3(256), 0, stream, from, pool.at, layout.page_bytes, runs,
-                           static_cast<int>(layout.run_bytes / 16), token_bytes, device_list, n);
-        HIP_CHECK(hipGetLastError());
+        for (size_t at = 0; at < copies.size(); at += kListed) {
+            const int n = static_cast<int>(std::min<size_t>(kListed, copies.size() - at));
+            CopyList list;
+            std::memcpy(list.copies, copies.data() + at, sizeof(PageCopy) * static_cast<size_t>(n));
+            const int x = std::max(1, std::min(runs, 2048 / n));  // ~2048 workgroups: eight per compute unit
+            hipLaunchKernelGGL(cache_copy_kernel, dim3(x, n), dim3(256), 0, stream, from, pool.at, layout.page_bytes, runs,
+                               static_cast<int>(layout.run_bytes / 16), token_bytes, list);
+            HIP_CHECK(hipGetLastError());
+        }
     }
 
     // How the pass's attention is cut, and room for what its parts leave.
@@ -312,18 +322,13 @@ static int copy_sequence(Cache& from, Cache& to, int seq, void* stream) {
     const int length = s.length, n = static_cast<int>(s.pages.size());
     if (&from != &to) from.enter(stream);
     to.enter(stream);
-    const size_t bytes = static_cast<size_t>(n) * sizeof(PageCopy);
-    to.lists.reserve(bytes, to.stream);
-    PageCopy* list = reinterpret_cast<PageCopy*>(to.staging.reserve(bytes));
+    std::vector<PageCopy> copies(static_cast<size_t>(n));
     const int id = to.book.add_filled(length);
     const std::vector<int>& a = from.book.at(seq).pages;
     const std::vector<int>& b = to.book.at(id).pages;
     for (int i = 0; i < n; i++)
-        list[i] = {a[static_cast<size_t>(i)], b[static_cast<size_t>(i)], std::min(from.o.page_tokens, length - i * from.o.page_tokens)};
-    if (n > 0) {
-        to.staging.send(to.lists.at, bytes, to.stream);
-        to.copy_pages(from.pool.at, reinterpret_cast<const PageCopy*>(to.lists.at), n);
-    }
+        copies[static_cast<size_t>(i)] = {a[static_cast<size_t>(i)], b[static_cast<size_t>(i)], std::min(from.o.page_tokens, length - i * from.o.page_tokens)};
+    to.copy_pages(from.pool.at, copies);
     return id;
 }
 
@@ -352,17 +357,13 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     Cache::Plan& plan = c.plans[0];
     c.cut(plan, c.last_causal, c.last_window);
     c.next_plan = 1;
-    const size_t copies_at = round16(sizeof(PassSeq) * static_cast<size_t>(n));
-    const size_t rows_at = copies_at + round16(sizeof(PageCopy) * static_cast<size_t>(n));
-    const size_t table_at = rows_at + round16(sizeof(RowAt) * static_cast<size_t>(rows));
+    const size_t rows_at = 0, table_at = round16(sizeof(RowAt) * static_cast<size_t>(rows));
     const size_t items_at = table_at + round16(sizeof(int) * static_cast<size_t>(table));
     const size_t bytes = items_at + plan.bytes();
     c.pass.reserve(bytes, c.stream);
     char* host = c.staging.reserve(bytes);
     const std::vector<PageCopy> copies = c.book.extend(seqs, counts, n);
 
-    std::memcpy(host, c.seqs.data(), sizeof(PassSeq) * c.seqs.size());
-    if (!copies.empty()) std::memcpy(host + copies_at, copies.data(), sizeof(PageCopy) * copies.size());
     RowAt* row = reinterpret_cast<RowAt*>(host + rows_at);
     int* page = reinterpret_cast<int*>(host + table_at);
     for (int i = 0; i < n; i++) {
@@ -374,7 +375,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     }
     plan.write(host + items_at);
     c.staging.send(c.pass.at, bytes, c.stream);
-    c.copy_pages(c.pool.at, reinterpret_cast<const PageCopy*>(c.pass.at + copies_at), static_cast<int>(copies.size()));
+    c.copy_pages(c.pool.at, copies);
     plan.at = reinterpret_cast<const AttendItem*>(c.pass.at + items_at);
     plan.valid = true;
     c.rows_at = rows_at;
@@ -492,28 +493,33 @@ static void read_positions(Cache& c, int seq, int layer, int layers, int start, 
             if (stride < (count - 1) * r->row_stride + (heads - 1) * r->head_stride + dim) refuse(std::string(name) + "'s layers overlap");
     const DeviceScope on(c.device);
     c.enter(stream);
-    const int first = start >> c.layout.page_shift, last = (start + count - 1) >> c.layout.page_shift;
-    const size_t bytes = sizeof(int) * static_cast<size_t>(last - first + 1);
-    c.lists.reserve(bytes, c.stream);
-    std::memcpy(c.staging.reserve(bytes), s.pages.data() + first, bytes);
-    c.staging.send(c.lists.at, bytes, c.stream);
     ReadParams p{};
     p.cache = c.layout;
     p.k = cache_rows(k);
     p.v = cache_rows(v);
     p.k_layer = k_layer;
     p.v_layer = v_layer;
-    p.table = reinterpret_cast<const int*>(c.lists.at);
     p.layer = layer;
-    p.start = start;
-    p.count = count;
     p.vector_rows = aligned(k, c.bytes, count == 1, heads == 1) && aligned(v, c.bytes, count == 1, heads == 1)
                     && (layers == 1 || (k_layer * c.bytes % 16 == 0 && v_layer * c.bytes % 16 == 0));
     const auto kernel = c.o.type == GH_F32 ? cache_read_kernel<kCacheF32>
                       : c.o.type == GH_BF16 ? cache_read_kernel<kCacheBf16>
                                             : cache_read_kernel<kCacheF16>;
-    hipLaunchKernelGGL(kernel, dim3((count + kReadPositions - 1) / kReadPositions, layers, 2), dim3(256), 0, c.stream, p);
-    HIP_CHECK(hipGetLastError());
+    // as many positions to a launch as its list of pages takes
+    const int shift = c.layout.page_shift;
+    for (int at = start; at < start + count;) {
+        const int first = at >> shift, last = std::min((start + count - 1) >> shift, first + 2 * kListed - 1);
+        const int end = std::min(start + count, static_cast<int>(std::min<long long>(INT_MAX, (last + 1ll) << shift)));
+        PageList list;
+        std::memcpy(list.pages, s.pages.data() + first, sizeof(int) * static_cast<size_t>(last - first + 1));
+        p.start = at;
+        p.count = end - at;
+        hipLaunchKernelGGL(kernel, dim3((p.count + kReadPositions - 1) / kReadPositions, layers, 2), dim3(256), 0, c.stream, p, list);
+        HIP_CHECK(hipGetLastError());
+        p.k.at += static_cast<long long>(p.count) * p.k.row * c.bytes;
+        p.v.at += static_cast<long long>(p.count) * p.v.row * c.bytes;
+        at = end;
+    }
 }
 
 }  // namespace gh
@@ -617,15 +623,7 @@ gh_status gh_cache_compact(gh_cache* c, void* hip_stream, int32_t* pages_used) {
         m.enter(hip_stream);
         m.close();
         const int used = m.book.pages() - m.book.pages_free();
-        const size_t most = sizeof(PageCopy) * static_cast<size_t>(std::min(used, m.book.pages_free()));
-        m.lists.reserve(most, m.stream);
-        char* host = m.staging.reserve(most);
-        const std::vector<PageCopy> moves = m.book.compact();
-        if (!moves.empty()) {
-            std::memcpy(host, moves.data(), sizeof(PageCopy) * moves.size());
-            m.staging.send(m.lists.at, sizeof(PageCopy) * moves.size(), m.stream);
-            m.copy_pages(m.pool.at, reinterpret_cast<const PageCopy*>(m.lists.at), static_cast<int>(moves.size()));
-        }
+        m.copy_pages(m.pool.at, m.book.compact());
         if (pages_used) *pages_used = used;
     });
 }

@@ -12,6 +12,15 @@ __global__ __launch_bounds__(256) void cache_load_kernel(const u32x4* __restrict
     for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) to[i] = host[i];
 }
 
+// ... or a few that come with the launch.
+constexpr size_t kWordsListed = 224;
+struct WordList {
+    u32x4 words[kWordsListed];
+};
+__global__ __launch_bounds__(256) void cache_hand_kernel(const WordList list, u32x4* __restrict__ to, int n) {
+    if (static_cast<int>(threadIdx.x) < n) to[threadIdx.x] = list.words[threadIdx.x];
+}
+
 struct AppendParams {
     CacheLayout cache;
     CacheRows k, v, q, q_out;  // q.at null: no queries
@@ -55,14 +64,30 @@ struct Eight {
     }
 };
 
-// One workgroup per row: its keys, values and queries, eight dims to a thread.  The angle position * base^(-2j / dim) is
-// formed in 64 bits, in turns, and only what is left of it below half a turn is rounded to 32: a position of a million keeps
-// all its digits.
+// One workgroup per row: its keys, values and queries, eight dims to a thread, requested before anything is computed.  The
+// angle position * base^(-2j / dim) is formed in 64 bits, in turns, and only what is left of it below half a turn is rounded to
+// 32: a position of a million keeps all its digits.
 template <int TYPE>
 __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p) {
     constexpr int kBytes = CacheType<TYPE>::kBytes;
     __shared__ float cosine[128], sine[128];
     const long long row = blockIdx.x;
+    const int eights = p.cache.dim / 8, cached = p.cache.kv_heads * eights;
+    const int all = 2 * cached + (p.q.at ? p.heads * eights : 0);
+    const auto place_of = [&](int i, int& which, int& head, int& dim) {
+        which = i < cached ? 0 : i < 2 * cached ? 1 : 2;
+        const int j = i - which * cached;
+        head = j / eights;
+        dim = j % eights * 8;
+    };
+    const auto load = [&](int i, Eight<TYPE>& x) {
+        int which, head, dim;
+        place_of(i, which, head, dim);
+        const CacheRows& from = which == 0 ? p.k : which == 1 ? p.v : p.q;
+        x.load(from.at + (row * from.row + head * from.head + dim) * kBytes, p.vector_rows);
+    };
+    Eight<TYPE> first;
+    if (static_cast<int>(threadIdx.x) < all) load(threadIdx.x, first);
     const RowAt at = p.rows[row];
     if (p.speed) {
         if (threadIdx.x < static_cast<unsigned>(p.cache.dim / 2)) {
@@ -75,15 +100,16 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p)
         }
         __syncthreads();
     }
-    const int eights = p.cache.dim / 8, cached = p.cache.kv_heads * eights;
     const int page = at.slot >> p.cache.page_shift, place = at.slot & ((1 << p.cache.page_shift) - 1);
-    const int all = 2 * cached + (p.q.at ? p.heads * eights : 0);
     for (int i = threadIdx.x; i < all; i += 256) {
-        const int which = i < cached ? 0 : i < 2 * cached ? 1 : 2;
-        const int j = i - which * cached, head = j / eights, dim = j % eights * 8;
-        const CacheRows& from = which == 0 ? p.k : which == 1 ? p.v : p.q;
         Eight<TYPE> x;
-        x.load(from.at + (row * from.row + head * from.head + dim) * kBytes, p.vector_rows);
+        if (i == static_cast<int>(threadIdx.x)) {
+            x = first;
+        } else {
+            load(i, x);
+        }
+        int which, head, dim;
+        place_of(i, which, head, dim);
         if (p.speed && which != 1) x.turn(cosine + dim / 2, sine + dim / 2);
         if (which < 2) {
             x.store(cache_run(p.cache, page, p.layer, which, head) + (static_cast<size_t>(place) * p.cache.dim + dim) * kBytes, true);
@@ -93,25 +119,30 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p)
     }
 }
 
+// Lists of up to so many entries travel with the launch itself.
+constexpr int kListed = 256;
+struct CopyList {
+    PageCopy copies[kListed];
+};
+struct PageList {
+    int pages[2 * kListed];
+};
+
 // The first positions of pages into other pages (of this pool or of one of the same shape), run by run.
 __global__ __launch_bounds__(256) void cache_copy_kernel(const char* __restrict__ from, char* __restrict__ to, size_t page_bytes, int runs,
-                                                         int run_words, int token_bytes, const PageCopy* __restrict__ copies, int n) {
-    for (int c = blockIdx.y; c < n; c += gridDim.y) {
-        const PageCopy copy = copies[c];
-        const int words = copy.tokens * token_bytes / 16;
-        const u32x4* a = reinterpret_cast<const u32x4*>(from + static_cast<size_t>(copy.from) * page_bytes);
-        u32x4* b = reinterpret_cast<u32x4*>(to + static_cast<size_t>(copy.to) * page_bytes);
-        for (int run = blockIdx.x; run < runs; run += gridDim.x)
-            for (int w = threadIdx.x; w < words; w += 256)
-                b[static_cast<size_t>(run) * run_words + w] = a[static_cast<size_t>(run) * run_words + w];
-    }
+                                                         int run_words, int token_bytes, const CopyList list) {
+    const PageCopy copy = list.copies[blockIdx.y];
+    const int words = copy.tokens * token_bytes / 16;
+    const u32x4* a = reinterpret_cast<const u32x4*>(from + static_cast<size_t>(copy.from) * page_bytes);
+    u32x4* b = reinterpret_cast<u32x4*>(to + static_cast<size_t>(copy.to) * page_bytes);
+    for (int run = blockIdx.x; run < runs; run += gridDim.x)
+        for (int w = threadIdx.x; w < words; w += 256) b[static_cast<size_t>(run) * run_words + w] = a[static_cast<size_t>(run) * run_words + w];
 }
 
 struct ReadParams {
     CacheLayout cache;
     CacheRows k, v;  // position start goes to row 0
     long long k_layer, v_layer;
-    const int* table;  // pages from start's on
     int layer, start, count;
     int vector_rows;
 };
@@ -120,7 +151,7 @@ constexpr int kReadPositions = 16;
 
 // 16 positions of a layer, K or V, to a workgroup.
 template <int TYPE>
-__global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
+__global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p, const PageList list) {  // pages from start's on
     constexpr int kBytes = CacheType<TYPE>::kBytes;
     const int which = blockIdx.z, layer = blockIdx.y, n0 = blockIdx.x * kReadPositions;
     const int eights = p.cache.dim / 8, tokens = min(kReadPositions, p.count - n0);
@@ -130,7 +161,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
     for (int i = threadIdx.x; i < tokens * eights * p.cache.kv_heads; i += 256) {
         const int dim = i % eights * 8, token = i / eights % tokens, head = i / eights / tokens;
         const int t = p.start + n0 + token;
-        const int page = p.table[(t >> p.cache.page_shift) - first_page], place = t & ((1 << p.cache.page_shift) - 1);
+        const int page = list.pages[(t >> p.cache.page_shift) - first_page], place = t & ((1 << p.cache.page_shift) - 1);
         Eight<TYPE> x;
         x.load(cache_run(p.cache, page, p.layer + layer, which, head) + (static_cast<size_t>(place) * p.cache.dim + dim) * kBytes, true);
         x.store(to.at + (base + (n0 + token) * to.row + head * to.head + dim) * kBytes, p.vector_rows);

@@ -532,7 +532,10 @@ class Cache:
         self.layers, self.heads, self.kv_heads, self.head_dim, self.dtype = layers, heads, kv_heads, head_dim, dtype
         self._torch_name = _TORCH_NAMES[dtype]
         self._device = self.info.device
+        self._right_type = self._right_device = None
         self._rows = -1  # of the open pass
+        self._rows_of = [GhRows() for _ in range(4)]  # the call's tensors, as the library takes them
+        self._refs = [C.byref(r) for r in self._rows_of]
 
     def close(self):
         if self._h:
@@ -609,38 +612,55 @@ class Cache:
         _check(self._lib.gh_cache_extend(self._h, (C.c_int32 * n)(*seqs), (C.c_int32 * n)(*counts), n, stream or None))
         self._rows = sum(counts)
 
-    def _tensor(self, t, name, heads, rows, dims=3):
-        shape, stride = t.shape, t.stride()
+    def _fill(self, place, t, name, heads, rows, dims=3):
+        """Describes a tensor to the library, in self._rows_of[place], once it has been looked over."""
+        shape = t.shape
         if len(shape) != dims or shape[-2] != heads or shape[-1] != self.head_dim or shape[-3] < rows:
             raise ValueError(f"cache: {name} of shape {tuple(shape)} where [{'layers, ' if dims == 4 else ''}{rows}, {heads}, {self.head_dim}] goes")
-        if str(t.dtype) != self._torch_name:
-            raise ValueError(f"cache: {name} is {t.dtype}, the cache {self._torch_name}")
-        device = t.device
-        if device.type != "cuda" or device.index != self._device:
-            raise ValueError(f"cache: {name} is on {device}, the cache on cuda:{self._device}")
+        # (types and devices that were found right before are compared as they are, not by name again)
+        if t.dtype is not self._right_type:
+            if str(t.dtype) != self._torch_name:
+                raise ValueError(f"cache: {name} is {t.dtype}, the cache {self._torch_name}")
+            self._right_type = t.dtype
+        if t.device != self._right_device:
+            if t.device.type != "cuda" or t.device.index != self._device:
+                raise ValueError(f"cache: {name} is on {t.device}, the cache on cuda:{self._device}")
+            self._right_device = t.device
+        stride = t.stride()
         if stride[-1] != 1:
             raise ValueError(f"cache: {name}'s last dimension is not dense")
-        return GhRows(t.data_ptr(), stride[-3], stride[-2])
+        r = self._rows_of[place]
+        r.data = t.data_ptr()
+        r.row_stride, r.head_stride = stride[-3], stride[-2]
 
     def append(self, layer, k, v, q=None, q_out=None, rotate=True, stream=0) -> None:
         """Stores the pass's keys and values [rows, kv_heads, head_dim] in a layer, keys rotated to their positions if the
         cache has a rope_base; q [rows, heads, head_dim] is rotated likewise into q_out (which may be q)."""
-        n = max(self._rows, 0)
-        args = [self._tensor(k, "k", self.kv_heads, n), self._tensor(v, "v", self.kv_heads, n)]
-        if (q is None) != (q_out is None):
+        n = self._rows if self._rows > 0 else 0
+        self._fill(0, k, "k", self.kv_heads, n)
+        self._fill(1, v, "v", self.kv_heads, n)
+        a, b, c, d = self._refs
+        if q is None and q_out is None:
+            c = d = None
+        elif q is None or q_out is None:
             raise ValueError("cache: queries and a place for them go together")
-        if q is not None:
-            args += [self._tensor(q, "q", self.heads, n), self._tensor(q_out, "q_out", self.heads, n)]
-        refs = [C.byref(a) for a in args] + [None] * (4 - len(args))
-        _check(self._lib.gh_cache_append(self._h, layer, *refs, 1 if rotate else 0, stream or None))
+        else:
+            self._fill(2, q, "q", self.heads, n)
+            self._fill(3, q_out, "q_out", self.heads, n)
+        rc = self._lib.gh_cache_append(self._h, layer, a, b, c, d, 1 if rotate else 0, stream or None)
+        if rc:
+            _check(rc)
 
     def attend(self, layer, q, out, scale=0.0, causal=True, window=0, stream=0) -> None:
         """out = softmax(scale q.K) V for the pass's rows over what is cached of their sequences in a layer: positions up to
         the row's own if causal, and only the last `window` of those up to it if window is not 0; scale 0 means
         1 / sqrt(head_dim).  q and out: [rows, heads, head_dim]; rows beyond the pass's are left as they are."""
-        n = max(self._rows, 0)
-        a, b = self._tensor(q, "q", self.heads, n), self._tensor(out, "out", self.heads, n)
-        _check(self._lib.gh_cache_attend(self._h, layer, C.byref(a), C.byref(b), scale, 1 if causal else 0, window, stream or None))
+        n = self._rows if self._rows > 0 else 0
+        self._fill(0, q, "q", self.heads, n)
+        self._fill(1, out, "out", self.heads, n)
+        rc = self._lib.gh_cache_attend(self._h, layer, self._refs[0], self._refs[1], scale, 1 if causal else 0, window, stream or None)
+        if rc:
+            _check(rc)
 
     def read(self, seq, k, v, start=0, layer=None, stream=0) -> None:
         """Copies positions of seq from `start` on, as many as k and v have rows, out of the pages: k and v are
@@ -654,6 +674,7 @@ class Cache:
         count = k.shape[-3]
         if v.shape[-3] != count:
             raise ValueError("cache: k and v differ in their rows")
-        a, b = self._tensor(k, "k", self.kv_heads, count, dims), self._tensor(v, "v", self.kv_heads, count, dims)
-        _check(self._lib.gh_cache_read(self._h, seq, layer or 0, layers, start, count, C.byref(a), strides[0], C.byref(b), strides[1],
+        self._fill(0, k, "k", self.kv_heads, count, dims)
+        self._fill(1, v, "v", self.kv_heads, count, dims)
+        _check(self._lib.gh_cache_read(self._h, seq, layer or 0, layers, start, count, self._refs[0], strides[0], self._refs[1], strides[1],
                                        stream or None))
