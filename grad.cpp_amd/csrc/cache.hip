@@ -108,6 +108,7 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 constexpr int kMaxHeads = 1024;
 constexpr int kMaxPageTokens = 1024;
 constexpr int kPlans = 4;
+constexpr int kLeastShared = 128;  // positions of a prefix that sequences attend to in common tiles
 constexpr int kFewRows = 16;  // of a sequence: they go to a launch of their own beside longer ones
 
 }  // namespace
@@ -130,6 +131,7 @@ struct Cache {
     int rows = 0;
     std::vector<PassSeq> seqs;
     std::vector<int> news;
+    std::vector<SharedPrefix> shared;  // among sequences of few rows
     size_t rows_at = 0, table_at = 0;  // in `pass`
 
     // its attention, as it was last cut up for a mask
@@ -143,14 +145,28 @@ struct Cache {
             AttendPlan cut;
         } launches[2];
         DeviceBuffer items;  // empty for the plan that came with the pass
-        const AttendItem* at = nullptr;
-        size_t count() const { return launches[0].cut.items.size() + launches[1].cut.items.size(); }
-        size_t bytes() const { return sizeof(AttendItem) * count(); }
+        const char* at = nullptr;
+        const AttendItem* items_of(int i) const { return reinterpret_cast<const AttendItem*>(at + place(i)); }
+        const AttendJoin* joins_of(int i) const { return reinterpret_cast<const AttendJoin*>(at + place(i) + items_bytes(i)); }
+        const int* maps_of(int i) const { return reinterpret_cast<const int*>(at + place(i) + items_bytes(i) + joins_bytes(i)); }
+        size_t bytes() const { return place(2); }
         void write(char* host) const {
-            for (const Launch& l : launches) {
-                if (!l.cut.items.empty()) std::memcpy(host, l.cut.items.data(), sizeof(AttendItem) * l.cut.items.size());
-                host += sizeof(AttendItem) * l.cut.items.size();
+            for (int i = 0; i < 2; i++) {
+                const AttendPlan& c = launches[i].cut;
+                char* to = host + place(i);
+                if (!c.items.empty()) std::memcpy(to, c.items.data(), sizeof(AttendItem) * c.items.size());
+                if (!c.joins.empty()) std::memcpy(to + items_bytes(i), c.joins.data(), sizeof(AttendJoin) * c.joins.size());
+                if (!c.maps.empty()) std::memcpy(to + items_bytes(i) + joins_bytes(i), c.maps.data(), sizeof(int) * c.maps.size());
             }
+        }
+
+    private:
+        size_t items_bytes(int i) const { return sizeof(AttendItem) * launches[i].cut.items.size(); }
+        size_t joins_bytes(int i) const { return sizeof(AttendJoin) * launches[i].cut.joins.size(); }
+        size_t place(int n) const {
+            size_t sum = 0;
+            for (int i = 0; i < n; i++) sum += items_bytes(i) + joins_bytes(i) + round16(sizeof(int) * launches[i].cut.maps.size());
+            return sum;
         }
     } plans[kPlans];
     int next_plan = 0;
@@ -235,10 +251,12 @@ struct Cache {
             // rows weighs more (777 rows, window 1024, fp16: 37 us, 41; 397 rows over 2 k positions, fp32: 45 us in half, 40).
             const int workgroups = !tiles ? (bytes == 4 ? 1024 : 2048) : bytes == 4 ? 512 : 256;
             const int least = tiles ? 128 : bytes == 4 ? 256 : 384;
-            l.cut = plan_attend(seqs, mine, group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64);
+            l.cut = plan_attend(seqs, mine, AttendCut{group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64},
+                                !many && window == 0 ? shared : std::vector<SharedPrefix>{});
             part_bytes = std::max(part_bytes, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
-            counters = std::max(counters, static_cast<size_t>(l.cut.tiles) * o.kv_heads);
+            counters = std::max(counters, l.cut.joins.size() * o.kv_heads);
         }
+        if (part_bytes >> 32) refuse("a pass whose parts take more than 4 GB");
         parts.reserve(part_bytes, stream);
         if (arrived.reserve(counters * sizeof(unsigned), stream)) HIP_CHECK(hipMemsetAsync(arrived.at, 0, arrived.bytes, stream));
     }
@@ -354,6 +372,14 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
         row0 += counts[i];
         table += c.book.pages_for(first + counts[i]);
     }
+    // prefixes that sequences of few rows share are read once for all of them
+    std::vector<const std::vector<int>*> pages_of(static_cast<size_t>(n));
+    std::vector<char> few(static_cast<size_t>(n));
+    for (int i = 0; i < n; i++) {
+        pages_of[static_cast<size_t>(i)] = &c.book.at(seqs[i]).pages;
+        few[static_cast<size_t>(i)] = counts[i] > 0 && static_cast<long long>(counts[i]) * c.group <= kFewRows;
+    }
+    c.shared = shared_prefixes(pages_of, c.seqs, few, c.o.page_tokens, kLeastShared);
     Cache::Plan& plan = c.plans[0];
     c.cut(plan, c.last_causal, c.last_window);
     c.next_plan = 1;
@@ -376,7 +402,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     plan.write(host + items_at);
     c.staging.send(c.pass.at, bytes, c.stream);
     c.copy_pages(c.pool.at, copies);
-    plan.at = reinterpret_cast<const AttendItem*>(c.pass.at + items_at);
+    plan.at = c.pass.at + items_at;
     plan.valid = true;
     c.rows_at = rows_at;
     c.table_at = table_at;
@@ -450,7 +476,7 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
         plan->items.reserve(bytes, c.stream);
         plan->write(c.staging.reserve(bytes));
         c.staging.send(plan->items.at, bytes, c.stream);
-        plan->at = reinterpret_cast<const AttendItem*>(plan->items.at);
+        plan->at = plan->items.at;
         plan->valid = true;
     }
     AttendParams p{};
@@ -458,7 +484,6 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.q = cache_rows(q);
     p.out = cache_rows(out);
     p.table = reinterpret_cast<const int*>(c.pass.at + c.table_at);
-    p.items = plan->at;
     p.layer = layer;
     p.group = c.group;
     p.scale = (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(c.o.head_dim))) * 1.44269504088896340736f;
@@ -467,12 +492,14 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.vector_rows = aligned(q, c.bytes, c.rows == 1, c.o.heads == 1) && aligned(out, c.bytes, c.rows == 1, c.o.heads == 1);
     p.parts = reinterpret_cast<float*>(c.parts.at);
     p.arrived = reinterpret_cast<unsigned*>(c.arrived.at);
-    for (const Cache::Plan::Launch& l : plan->launches) {
-        if (!l.cut.items.empty()) {
-            hipLaunchKernelGGL(l.form.kernel, dim3(static_cast<unsigned>(l.cut.items.size()) * c.o.kv_heads), dim3(l.form.threads), 0, c.stream, p);
-            HIP_CHECK(hipGetLastError());
-        }
-        p.items += l.cut.items.size();
+    for (int i = 0; i < 2; i++) {
+        const Cache::Plan::Launch& l = plan->launches[i];
+        if (l.cut.items.empty()) continue;
+        p.items = plan->items_of(i);
+        p.joins = plan->joins_of(i);
+        p.maps = plan->maps_of(i);
+        hipLaunchKernelGGL(l.form.kernel, dim3(static_cast<unsigned>(l.cut.items.size()) * c.o.kv_heads), dim3(l.form.threads), 0, c.stream, p);
+        HIP_CHECK(hipGetLastError());
     }
 }
 

@@ -8,6 +8,7 @@
 #pragma once
 
 #include <algorithm>
+#include <unordered_map>
 #include <vector>
 
 namespace gh {
@@ -24,22 +25,62 @@ struct RowAt {
     int pos;
 };
 
-// One workgroup's work for one kv head: rows [r0, r0 + rows) of a sequence's tile axis over the
-// positions [k0, k1).  The parts of a tile meet through `tile`'s counter and the parts' places.
+// One workgroup's work for one kv head: `rows` rows over the positions [k0, k1) of a page list.
 struct AttendItem {
-    int seq, r0, rows, k0, k1;
-    int part;   // place of the tile's first part among all that are left in memory, -1: the only part
-    int index;  // which part this is
-    int parts;
-    int tile;
-    int first, row0, table;  // the sequence's, so that a kernel has them with the rest
+    int r0, rows;  // of a sequence's tile axis, or (map >= 0) as the map has them
+    int k0, k1;
+    int part;          // the place in memory that its result goes to, -1: it is whole and goes to the caller
+    int join, joins;   // the joins that wait for it
+    int first, row0, table;  // the sequence's; for a map, a position that sees everything
+    int map;           // rows of several sequences: where their (pass row * group + head of the group) are listed
+    int pad;           // a multiple of 16 bytes
+};
+
+// A tile whose positions were dealt to several workgroups: the last of them to finish puts it together, first the parts of a
+// prefix that it shares with other tiles (rows shared_row.. of those), then its own.
+struct AttendJoin {
+    int r0, rows, row0;
+    int part, parts;
+    int shared_part, shared_parts, shared_row;
 };
 
 struct AttendPlan {
     std::vector<AttendItem> items;
-    int parts = 0;  // places that split tiles need
-    int tiles = 0;  // counters that they need
+    std::vector<AttendJoin> joins;
+    std::vector<int> maps;
+    int parts = 0;  // places that parts need
 };
+
+// Sequences of a pass that begin with the same pages: `prefix` positions, all of them before every member's new rows.
+struct SharedPrefix {
+    int prefix;
+    std::vector<int> members;
+};
+
+// Those among the sequences with `wanted` set, by their page lists: the ones with the same first page, and as many leading
+// full pages as all of them have in common, where that is `least` positions or more.
+inline std::vector<SharedPrefix> shared_prefixes(const std::vector<const std::vector<int>*>& pages, const std::vector<PassSeq>& seqs,
+                                                 const std::vector<char>& wanted, int page_tokens, int least) {
+    std::unordered_map<int, std::vector<int>> by_first;
+    for (size_t i = 0; i < seqs.size(); i++)
+        if (wanted[i] && seqs[i].first >= std::max(least, page_tokens)) by_first[(*pages[i])[0]].push_back(static_cast<int>(i));
+    std::vector<SharedPrefix> found;
+    for (auto& [page, members] : by_first) {
+        if (members.size() < 2) continue;
+        const std::vector<int>& lead = *pages[static_cast<size_t>(members[0])];
+        int common = seqs[static_cast<size_t>(members[0])].first / page_tokens;
+        for (int m : members) {
+            const std::vector<int>& other = *pages[static_cast<size_t>(m)];
+            common = std::min(common, seqs[static_cast<size_t>(m)].first / page_tokens);
+            int n = 0;
+            while (n < common && other[static_cast<size_t>(n)] == lead[static_cast<size_t>(n)]) n++;
+            common = n;
+        }
+        if (common * page_tokens >= least) found.push_back({common * page_tokens, members});
+    }
+    std::sort(found.begin(), found.end(), [](const SharedPrefix& a, const SharedPrefix& b) { return a.members[0] < b.members[0]; });
+    return found;
+}
 
 // Positions that rows [r0, r0 + rows) see any of.
 inline void visible_span(const PassSeq& s, int r0, int rows, int group, bool causal, int window, int& k0, int& k1) {
@@ -48,39 +89,105 @@ inline void visible_span(const PassSeq& s, int r0, int rows, int group, bool cau
     k0 = window > 0 ? std::max(0, t0 - window + 1) & ~15 : 0;
 }
 
-// Tiles of `height` rows; a tile's positions are cut into parts of one length so that the launch has about
-// `workgroups` of them over all kv heads, none shorter than `least` positions and no tile in more than `most` parts.
-inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vector<int>& rows, int group, int kv_heads, int height,
-                              bool causal, int window, int workgroups, int least, int most) {
+struct AttendCut {
+    int group, kv_heads;
+    int height;      // of a tile
+    bool causal;
+    int window;
+    int workgroups;  // about as many, over all kv heads
+    int least;       // positions of a part, at least
+    int most;        // parts of a tile, at most
+};
+
+// Tiles of `height` rows; a tile's positions are cut into parts of one length.  `shared`: prefixes whose members (of at
+// most `height` rows each) meet them in common tiles; only without a window, where all their rows see all of it.
+inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vector<int>& rows, const AttendCut& cut,
+                              const std::vector<SharedPrefix>& shared = {}) {
     AttendPlan plan;
-    long long total = 0;
-    for (size_t i = 0; i < seqs.size(); i++)
-        for (int r0 = 0; r0 < rows[i] * group; r0 += height) {
-            int k0, k1;
-            visible_span(seqs[i], r0, std::min(height, rows[i] * group - r0), group, causal, window, k0, k1);
-            total += k1 - k0;
-        }
-    const long long each = (total * kv_heads + workgroups - 1) / std::max(workgroups, 1);
-    const int span = static_cast<int>(std::min<long long>(std::max<long long>(least, (each + 127) / 128 * 128), 1 << 30));
-    for (size_t i = 0; i < seqs.size(); i++) {
-        const int all = rows[i] * group;
-        for (int r0 = 0; r0 < all; r0 += height) {
-            const int n = std::min(height, all - r0);
-            int k0, k1;
-            visible_span(seqs[i], r0, n, group, causal, window, k0, k1);
-            const int parts = std::max(1, std::min(most, (k1 - k0 + span - 1) / span));
-            const int part = parts > 1 ? plan.parts : -1, tile = parts > 1 ? plan.tiles : 0;
-            // as even as whole runs of 32 positions allow
-            const int run = (((k1 - k0 + parts - 1) / parts) + 31) / 32 * 32;
-            const int made = std::max(1, (k1 - k0 + run - 1) / run);
-            for (int j = 0; j < made; j++)
-                plan.items.push_back({static_cast<int>(i), r0, n, k0 + j * run, std::min(k1, k0 + (j + 1) * run), made > 1 ? part : -1, j, made, tile, seqs[i].first, seqs[i].row0, seqs[i].table});
-            if (made > 1) {
-                plan.parts += made;
-                plan.tiles++;
+    const int height = cut.height;
+    std::vector<int> prefix(seqs.size(), 0);  // that a sequence leaves to the common tiles
+    std::vector<int> packed(shared.size(), 0);  // common tiles of a prefix: members whole, as many as fit
+    for (size_t g = 0; g < shared.size(); g++) {
+        int room = 0;
+        for (int i : shared[g].members) {
+            prefix[static_cast<size_t>(i)] = shared[g].prefix;
+            const int n = rows[static_cast<size_t>(i)] * cut.group;
+            if (n > room) {
+                packed[g]++;
+                room = height;
             }
+            room -= n;
         }
     }
+    const auto tile_span = [&](size_t i, int r0, int& n, int& k0, int& k1) {
+        n = std::min(height, rows[i] * cut.group - r0);
+        visible_span(seqs[i], r0, n, cut.group, cut.causal, cut.window, k0, k1);
+        k0 = std::max(k0, prefix[i]);
+    };
+    long long total = 0;
+    for (size_t i = 0; i < seqs.size(); i++)
+        for (int r0 = 0; r0 < rows[i] * cut.group; r0 += height) {
+            int n, k0, k1;
+            tile_span(i, r0, n, k0, k1);
+            total += k1 - k0;
+        }
+    for (size_t g = 0; g < shared.size(); g++) total += static_cast<long long>(shared[g].prefix) * packed[g];
+    const long long each = (total * cut.kv_heads + cut.workgroups - 1) / std::max(cut.workgroups, 1);
+    const int span = static_cast<int>(std::min<long long>(std::max<long long>(cut.least, (each + 127) / 128 * 128), 1 << 30));
+    // the length of the parts of [k0, k1), as even as whole runs of 32 positions allow, and their number
+    const auto cut_up = [&](int k0, int k1, int& run) {
+        const int parts = std::max(1, std::min(cut.most, (k1 - k0 + span - 1) / span));
+        run = (((k1 - k0 + parts - 1) / parts) + 31) / 32 * 32;
+        return std::max(1, (k1 - k0 + run - 1) / run);
+    };
+    const auto add_items = [&](AttendItem it, int k0, int k1, int parts, int run) {
+        for (int j = 0; j < parts; j++) {
+            it.k0 = k0 + j * run;
+            it.k1 = std::min(k1, k0 + (j + 1) * run);
+            plan.items.push_back(it);
+            if (it.part >= 0) it.part++;
+        }
+    };
+    const auto add_tile = [&](size_t i, int r0, AttendJoin join) {
+        int n, k0, k1, run;
+        tile_span(i, r0, n, k0, k1);
+        const int parts = cut_up(k0, k1, run);
+        const bool whole = parts == 1 && join.shared_parts == 0;
+        AttendItem it{r0, n, 0, 0, whole ? -1 : plan.parts, static_cast<int>(plan.joins.size()), whole ? 0 : 1,
+                      seqs[i].first, seqs[i].row0, seqs[i].table, -1, 0};
+        add_items(it, k0, k1, parts, run);
+        if (whole) return;
+        join.r0 = r0;
+        join.rows = n;
+        join.row0 = seqs[i].row0;
+        join.part = plan.parts;
+        join.parts = parts;
+        plan.joins.push_back(join);
+        plan.parts += parts;
+    };
+    for (size_t g = 0; g < shared.size(); g++) {
+        const std::vector<int>& members = shared[g].members;
+        int run;
+        const int parts = cut_up(0, shared[g].prefix, run);
+        for (size_t m = 0; m < members.size();) {
+            AttendItem it{0, 0, 0, 0, plan.parts, static_cast<int>(plan.joins.size()), 0, 1 << 30, 0,
+                          seqs[static_cast<size_t>(members[m])].table, static_cast<int>(plan.maps.size()), 0};
+            plan.parts += parts;
+            for (; m < members.size(); m++) {
+                const size_t i = static_cast<size_t>(members[m]);
+                const int n = rows[i] * cut.group;
+                if (it.rows + n > height) break;
+                for (int r = 0; r < n; r++) plan.maps.push_back((seqs[i].row0 + r / cut.group) * cut.group + r % cut.group);
+                add_tile(i, 0, AttendJoin{0, 0, 0, 0, 0, it.part, parts, it.rows});
+                it.rows += n;
+                it.joins++;
+            }
+            add_items(it, 0, shared[g].prefix, parts, run);
+        }
+    }
+    for (size_t i = 0; i < seqs.size(); i++)
+        if (prefix[i] == 0)
+            for (int r0 = 0; r0 < rows[i] * cut.group; r0 += height) add_tile(i, r0, AttendJoin{});
     // the longest go first: what is dealt last ends the launch
     std::stable_sort(plan.items.begin(), plan.items.end(), [](const AttendItem& a, const AttendItem& b) { return a.k1 - a.k0 > b.k1 - b.k0; });
     return plan;

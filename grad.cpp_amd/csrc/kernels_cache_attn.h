@@ -88,14 +88,16 @@ struct AttendParams {
     CacheRows q, out;
     const int* table;
     const AttendItem* items;
+    const AttendJoin* joins;
+    const int* maps;
     int layer;
     int group;
     float scale;  // of the scores, times log2(e)
     int causal;
     int window;
     int vector_rows;    // q's and out's rows can be read and written 16 bytes at a time
-    float* parts;       // [part][kv head][tile height][DH + 2]: output, maximum, sum
-    unsigned* arrived;  // [tile][kv head], zero between launches
+    float* parts;       // [part][kv head][tile height][DH + 4]: output, maximum, sum, two of padding
+    unsigned* arrived;  // [join][kv head], zero between launches
 };
 
 constexpr int kBeyond = 0x40000000;  // past the end of any run (a run is a megabyte at most)
@@ -309,50 +311,63 @@ struct Folded {
     }
 };
 
-// The workgroup's part of a tile is in memory: the last part to arrive folds all of them and writes the tile's outputs.
-// Every trip to memory is a microsecond, so a thread has AHEAD elements x parts in flight, and threads that have no element of
-// their own share the parts; the order of the folding is that of the positions whoever arrives when.
+constexpr int kMostJoins = 16;  // that wait for one item: it has a row of each at least
+
+struct Meeting {
+    int shared_row[kMostJoins + 1];  // where a join's rows begin among the item's
+    int last[kMostJoins];            // whether this workgroup is the last for it
+};
+
+// Puts together the joins that this workgroup is the last for.  Every trip to memory is a microsecond, so a thread has several
+// elements and parts in flight, threads that have no element of their own share the parts, and all joins are made at once; the
+// order of the folding is that of the positions, whoever arrived when.  MANY: the item's rows are of several joins.
 // stash: 32 bytes of shared memory for each thread.
-template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS>
-__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, int head, float* parts,
-                                             size_t part_stride, unsigned& last, char* stash) {
-    constexpr int kPad = DH + 4, kChunks = DH / 4;
-    constexpr int kSide = HEIGHT > 64 ? 4 : 1, kDeep = HEIGHT > 64 ? 4 : 16;  // elements of a thread and parts, in flight
-    // the stores have to be out before the workgroup counts as arrived
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    unsigned* const arrived = p.arrived + static_cast<size_t>(it.tile) * p.cache.kv_heads + head;
-    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (last != static_cast<unsigned>(it.parts - 1)) return;
-    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS, bool MANY>
+__device__ __forceinline__ void join_parts(const AttendParams& p, const AttendItem& it, int head, const Meeting& meeting, char* stash) {
+    constexpr int kPad = DH + 4, kChunks = DH / 4, kBlock = HEIGHT * kPad;
+    constexpr int kSide = HEIGHT > 64 ? 4 : 1, kDeep = HEIGHT > 64 ? 4 : MANY ? 8 : 16;  // elements of a thread and parts, in flight
+    const __amdgpu_buffer_rsrc_t rs = make_buffer(p.parts, 0xFFFFFFFFu);  // (the host keeps all parts below 4 GB)
     const int elements = it.rows * kChunks;
-    const int shares = max(1, min(THREADS / elements, (it.parts + kDeep - 1) / kDeep));  // of the parts
-    const int share = static_cast<int>(threadIdx.x) / elements;                          // (0 where there is one)
-    const int each = (it.parts + shares - 1) / shares;
-    const auto write = [&](int e, const Folded& f) {
-        const int r = it.r0 + e / kChunks, dim = e % kChunks * 4;
-        if (FULL || dim < p.cache.dim)
-            store_four<TYPE>(p.out, (it.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
-                             f.out / f.total);
+    const auto join_of = [&](int e) {
+        int j = 0;
+        if constexpr (MANY)
+            while (j + 1 < it.joins && meeting.shared_row[j + 1] <= e / kChunks) j++;
+        return it.join + j;
+    };
+    const int most = p.joins[it.join].shared_parts + p.joins[it.join].parts;  // (members' own parts of a prefix's rest: one or a few)
+    const int shares = max(1, min(THREADS / elements, (most + kDeep - 1) / kDeep));  // of the parts
+    const int share = static_cast<int>(threadIdx.x) / elements;                      // (0 where there is one)
+    const auto write = [&](int e, const f32x4& out, float total) {
+        const int dim = e % kChunks * 4, j = join_of(e);
+        if ((MANY && !meeting.last[j - it.join]) || (!FULL && dim >= p.cache.dim)) return;
+        const int r = p.joins[j].r0 + e / kChunks - (MANY ? p.joins[j].shared_row : 0);
+        store_four<TYPE>(p.out, (p.joins[j].row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
+                         p.vector_rows, out / total);
     };
     for (int e0 = shares > 1 ? static_cast<int>(threadIdx.x) % elements : threadIdx.x; e0 < elements; e0 += kSide * THREADS) {
         Folded f[kSide];
 #pragma unroll
         for (int k = 0; k < kSide; k++) f[k] = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
-        const int from = shares > 1 ? min(share * each, it.parts) : 0, to = shares > 1 ? min(from + each, it.parts) : it.parts;
+        const AttendJoin* const join = p.joins + join_of(e0);
+        const int shared_parts = join->shared_parts, shared_part = join->shared_part, own_part = join->part, shared_row = join->shared_row;
+        int all = shared_parts + join->parts;
+        if (MANY && !meeting.last[join - (p.joins + it.join)]) all = 0;
+        const int each = (all + shares - 1) / shares;
+        const int skip = MANY ? shared_row : 0;  // rows of the item before the join's
+        const int from = shares > 1 ? min(share * each, all) : 0, to = shares > 1 ? min(from + each, all) : all;
         for (int j0 = from; j0 < to; j0 += kDeep) {
             v4i a[kDeep][kSide], st[kDeep][kSide];
 #pragma unroll
             for (int j = 0; j < kDeep; j++) {
-                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts, 0xFFFFFFFFu);
-                const unsigned place = static_cast<unsigned>(min(j0 + j, it.parts - 1) * part_stride * 4);
+                const int part = min(j0 + j, all - 1), own = part - shared_parts;
+                const int place = own < 0 ? shared_part + part : own_part + own, up = (own < 0 ? shared_row : 0) - skip;
+                const unsigned block = static_cast<unsigned>(place * p.cache.kv_heads + head) * (kBlock * 4u);
 #pragma unroll
                 for (int k = 0; k < kSide; k++) {
                     const int e = min(e0 + k * THREADS, elements - 1);
-                    const unsigned base = place + e / kChunks * kPad * 4;
-                    a[j][k] = coherent_load16(rs, base + e % kChunks * 16);
-                    st[j][k] = coherent_load16(rs, base + DH * 4);
+                    const unsigned row = block + (up + e / kChunks) * (kPad * 4);
+                    a[j][k] = coherent_load16(rs, row + e % kChunks * 16);
+                    st[j][k] = coherent_load16(rs, row + DH * 4);
                 }
             }
 #pragma unroll
@@ -365,7 +380,7 @@ __device__ __forceinline__ void finish_parts(const AttendParams& p, const Attend
         if (shares == 1) {
 #pragma unroll
             for (int k = 0; k < kSide; k++)
-                if (e0 + k * THREADS < elements) write(e0 + k * THREADS, f[k]);
+                if (e0 + k * THREADS < elements) write(e0 + k * THREADS, f[k].out, f[k].total);
         } else if (share < shares) {
             *reinterpret_cast<f32x4*>(stash + threadIdx.x * 32) = f[0].out;
             *reinterpret_cast<f32x4*>(stash + threadIdx.x * 32 + 16) = f32x4{f[0].top, f[0].total, 0.0f, 0.0f};
@@ -380,8 +395,36 @@ __device__ __forceinline__ void finish_parts(const AttendParams& p, const Attend
             const f32x4 st = *reinterpret_cast<const f32x4*>(at + 16);
             f.fold(*reinterpret_cast<const f32x4*>(at), st.x, st.y);
         }
-        write(threadIdx.x, f);
+        write(threadIdx.x, f.out, f.total);
     }
+}
+
+// The workgroup's part is in memory: it arrives at the joins that wait for it and makes those it is the last for.
+template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS>
+__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, int head, Meeting& meeting, char* stash) {
+    // the stores have to be out before the workgroup counts as arrived
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < it.joins) {
+        const AttendJoin& join = p.joins[it.join + threadIdx.x];
+        unsigned* const arrived = p.arrived + static_cast<size_t>(it.join + threadIdx.x) * p.cache.kv_heads + head;
+        const bool mine = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                          == static_cast<unsigned>(join.shared_parts + join.parts - 1);
+        if (mine) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        meeting.shared_row[threadIdx.x] = join.shared_row;
+        meeting.last[threadIdx.x] = mine;
+    }
+    __syncthreads();
+    int any = 0;
+    for (int i = 0; i < it.joins; i++) any |= meeting.last[i];
+    if (__builtin_amdgcn_readfirstlane(any) == 0) return;
+    if constexpr (HEIGHT == 16) {
+        if (it.map >= 0) {
+            join_parts<TYPE, DH, FULL, HEIGHT, THREADS, true>(p, it, head, meeting, stash);
+            return;
+        }
+    }
+    join_parts<TYPE, DH, FULL, HEIGHT, THREADS, false>(p, it, head, meeting, stash);
 }
 
 // Wavefronts of a workgroup: as many as take 128 positions at a time (fp32, one token: 64 sequences of up to 2 k positions
@@ -392,7 +435,7 @@ constexpr int attend_waves(int type, int dh, int tiles) { return type == kCacheF
 // Tiles of 16 TILES rows; the wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
 // A tile whose positions were dealt to several workgroups is finished by the last of them to arrive.
 template <int TYPE, int DH, bool FULL, int TILES>
-__global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_rows_kernel(const AttendParams p) {
+__global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 64 ? 4 : 1) void attend_rows_kernel(const AttendParams p) {
     constexpr int kAttendWaves = attend_waves(TYPE, DH, TILES);
     using C = CacheType<TYPE>;
     using T = typename C::T;
@@ -400,7 +443,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_row
     constexpr int kDims = G::kDims, kPad = DH + 4;
     __shared__ __align__(16) float meet[kAttendWaves][16][kPad];
     __shared__ float tops[kAttendWaves][16], sums[kAttendWaves][16];
-    __shared__ unsigned last;
+    __shared__ Meeting meeting;
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
@@ -413,10 +456,11 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_row
     int pos[TILES];
 #pragma unroll
     for (int rt = 0; rt < TILES; rt++) {
-        const int r = it.r0 + 16 * rt + (lane & 15);
         const bool row = 16 * rt + (lane & 15) < it.rows;
-        const int token = row ? r / p.group : 0, h = row ? r % p.group : 0;
-        pos[rt] = row ? it.first + token : -1;
+        // (a map's rows are of several sequences, all of them behind all of the positions)
+        const int r = !row ? 0 : it.map >= 0 ? p.maps[it.map + 16 * rt + (lane & 15)] : it.r0 + 16 * rt + (lane & 15);
+        const int token = r / p.group, h = r % p.group;
+        pos[rt] = !row ? -1 : it.map >= 0 ? it.first : it.first + token;
         const T* from = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
 #pragma unroll
         for (int c = 0; c < G::kKeyWords / 4; c++) {
@@ -552,10 +596,9 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_row
         at = then;
     }
 
-    const bool only = it.parts == 1;
+    const bool only = it.joins == 0;
     constexpr int kBlock = 16 * TILES * kPad;  // floats of a part
-    float* const parts = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
-    const size_t part_stride = static_cast<size_t>(p.cache.kv_heads) * kBlock;
+    float* const part = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     constexpr int kChunks = DH / 4;  // of a row
 #pragma unroll
     for (int rt = 0; rt < TILES; rt++) {
@@ -594,7 +637,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_row
                     store_four<TYPE>(p.out, (it.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
                                      p.vector_rows, out / total);
             } else {
-                const __amdgpu_buffer_rsrc_t rs = make_buffer(parts + it.index * part_stride, kBlock * 4);
+                const __amdgpu_buffer_rsrc_t rs = make_buffer(part, kBlock * 4);
                 const int base = (16 * rt + row) * kPad * 4;
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, out), rs, base + dim * 4, 0, kAuxDeviceScope);
                 if (dim == 0)
@@ -605,7 +648,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES)) void attend_row
     }
     if (only) return;
 
-    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, head, parts, part_stride, last, reinterpret_cast<char*>(meet));
+    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, head, meeting, reinterpret_cast<char*>(meet));
 }
 
 }  // namespace gh

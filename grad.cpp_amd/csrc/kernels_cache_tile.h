@@ -107,7 +107,7 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
                     if (lane + 64 * k < dims) o[k] = fmaf(w, static_cast<float>(value[lane + 64 * k]), o[k]);
             }
         }
-        if (it.parts == 1) {
+        if (it.joins == 0) {
             T* to = reinterpret_cast<T*>(p.out.at) + (it.row0 + token) * p.out.row + h * p.out.head;
 #pragma unroll
             for (int k = 0; k < kOwn; k++)
@@ -137,13 +137,13 @@ __device__ __forceinline__ void leave_rows(const AttendParams& p, const AttendIt
         for (int i = 0; i < 4; i++) {
             const int dim = 32 * d + 8 * i + 4 * half;
             const f32x4 four{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            if (it.parts == 1) {
+            if (it.joins == 0) {
                 if (FULL || dim < p.cache.dim) store_four<TYPE>(p.out, to + dim, p.vector_rows, four / l);
             } else {
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, four), rs, base + dim * 4, 0, kAuxDeviceScope);
             }
         }
-    if (it.parts > 1 && half == 0)
+    if (it.joins > 0 && half == 0)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, f32x4{m, l, 0.0f, 0.0f}), rs, base + DH * 4, 0, kAuxDeviceScope);
 }
 
@@ -158,7 +158,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     constexpr int kBlocks = TOKENS / 32, kSteps = DH / 16, kWide = DH / 32;
     __shared__ __align__(16) char keys[TOKENS * kKeyRow];
     __shared__ __align__(16) char values[TOKENS * kValueRow];
-    __shared__ unsigned last, odd;
+    __shared__ Meeting meeting;
+    __shared__ unsigned odd;
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
@@ -330,18 +331,16 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
         ahead_of_products<kBlocks * 2 * kWide, 2, 4>();
     }
 
-    const bool only = it.parts == 1;
+    const bool only = it.joins == 0;
     constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
-    float* const parts = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
-    const size_t part_stride = static_cast<size_t>(p.cache.kv_heads) * kBlock;
+    float* const part = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     if (__builtin_amdgcn_readfirstlane(odd)) {
-        rows_one_by_one<TYPE, DH>(p, it, table, head, 32 * wave, rows_here, parts + (only ? 0 : it.index) * part_stride);
+        rows_one_by_one<TYPE, DH>(p, it, table, head, 32 * wave, rows_here, part);
     } else {
-        leave_rows<TYPE, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half,
-                                   parts + (only ? 0 : it.index) * part_stride);
+        leave_rows<TYPE, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }
     if (only) return;
-    finish_parts<TYPE, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, parts, part_stride, last, keys);
+    finish_parts<TYPE, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, meeting, keys);
 }
 
 // ---------------------------------------------------------------------- fp32
@@ -386,7 +385,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 64 ? 1 : 2) void attend_wide_
     constexpr int kBlocks = TOKENS / 32, kSteps = DH / 16, kWide = DH / 32;
     __shared__ __align__(16) char keys[3 * kKeys];
     __shared__ __align__(16) char values[3 * kValues];
-    __shared__ unsigned last, odd;
+    __shared__ Meeting meeting;
+    __shared__ unsigned odd;
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
@@ -627,18 +627,16 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 64 ? 1 : 2) void attend_wide_
         }
     }
 
-    const bool only = it.parts == 1;
+    const bool only = it.joins == 0;
     constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
-    float* const parts = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
-    const size_t part_stride = static_cast<size_t>(p.cache.kv_heads) * kBlock;
+    float* const part = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     if (__builtin_amdgcn_readfirstlane(odd)) {
-        rows_one_by_one<kCacheF32, DH>(p, it, table, head, 32 * wave, rows_here, parts + (only ? 0 : it.index) * part_stride);
+        rows_one_by_one<kCacheF32, DH>(p, it, table, head, 32 * wave, rows_here, part);
     } else {
-        leave_rows<kCacheF32, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half,
-                                        parts + (only ? 0 : it.index) * part_stride);
+        leave_rows<kCacheF32, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }
     if (only) return;
-    finish_parts<kCacheF32, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, parts, part_stride, last, keys);
+    finish_parts<kCacheF32, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, meeting, keys);
 }
 
 }  // namespace gh

@@ -149,53 +149,104 @@ static int refusals() {
     return 0;
 }
 
-// Every (row, position it sees) is in exactly one item of its tile, spans lie inside the sequences, parts are counted.
+// Every row of a pass gets every position that it may see from exactly one item (of its own or of a shared prefix), spans lie
+// inside the sequences, places of parts are used once, and every join knows whom it waits for.
 static int plans(unsigned seed) {
     std::mt19937 rng(seed);
-    for (int round = 0; round < 400; round++) {
-        const int group = 1 + static_cast<int>(rng() % 5), height = 16 << (rng() % 3), kv = 1 + static_cast<int>(rng() % 8);
-        const bool causal = rng() % 4 != 0;
-        const int window = rng() % 3 ? 0 : 1 + static_cast<int>(rng() % 300);
-        const int workgroups = 1 << (rng() % 12), least = 128, most = 1 + static_cast<int>(rng() % 64);
+    for (int round = 0; round < 300; round++) {
+        AttendCut cut{};
+        cut.group = 1 + static_cast<int>(rng() % 5);
+        cut.kv_heads = 1 + static_cast<int>(rng() % 8);
+        cut.height = 16 << (rng() % 3);
+        cut.causal = rng() % 4 != 0;
+        cut.window = rng() % 3 ? 0 : 1 + static_cast<int>(rng() % 300);
+        cut.workgroups = 1 << (rng() % 12);
+        cut.least = 128;
+        cut.most = 1 + static_cast<int>(rng() % 64);
+        const int T = 16;
         std::vector<PassSeq> seqs;
         std::vector<int> news;
-        for (int i = static_cast<int>(rng() % 5); i >= 0; i--) {
-            const int n = static_cast<int>(rng() % 60), first = static_cast<int>(rng() % 2000);
-            seqs.push_back({first + n, first, 0, 0});
+        std::vector<std::vector<int>> pages;
+        const int families = 1 + static_cast<int>(rng() % 3);
+        int row0 = 0, table = 0;
+        for (int i = static_cast<int>(rng() % 9); i >= 0; i--) {
+            const int n = static_cast<int>(rng() % 3 ? rng() % 5 : rng() % 60), first = static_cast<int>(rng() % 1500);
+            seqs.push_back({first + n, first, row0, table});
             news.push_back(n);
+            std::vector<int> p;
+            const int family = static_cast<int>(rng() % static_cast<unsigned>(families)), common = static_cast<int>(rng() % 80);
+            for (int k = 0; k < (first + n + T - 1) / T; k++) p.push_back(k < common ? family * 1000 + k : 100000 + 1000 * static_cast<int>(seqs.size()) + k);
+            pages.push_back(p);
+            row0 += n;
+            table += static_cast<int>(p.size());
         }
-        const AttendPlan plan = plan_attend(seqs, news, group, kv, height, causal, window, workgroups, least, most);
-        std::map<std::pair<int, int>, std::vector<AttendItem>> tiles;
-        for (const AttendItem& it : plan.items) tiles[{it.seq, it.r0}].push_back(it);
-        size_t n_tiles = 0;
-        std::set<int> places, counters;
+        std::vector<const std::vector<int>*> lists;
+        std::vector<char> few;
         for (size_t i = 0; i < seqs.size(); i++) {
-            for (int r0 = 0; r0 < news[i] * group; r0 += height) {
-                n_tiles++;
-                const auto found = tiles.find({static_cast<int>(i), r0});
-                CHECK(found != tiles.end());
-                std::vector<AttendItem>& t = found->second;
-                std::sort(t.begin(), t.end(), [](const AttendItem& a, const AttendItem& b) { return a.k0 < b.k0; });
-                const int rows = std::min(height, news[i] * group - r0);
-                int low = INT_MAX, high = 0;
-                for (int r = r0; r < r0 + rows; r++) {
-                    const int pos = seqs[i].first + r / group;
-                    low = std::min(low, window ? std::max(0, pos - window + 1) : 0);
-                    high = std::max(high, causal ? pos + 1 : seqs[i].len);
-                }
-                CHECK(static_cast<int>(t.size()) <= most);
-                CHECK(t[0].k0 <= low && t[0].k0 % 16 == 0 && t.back().k1 == high);
-                for (size_t j = 0; j < t.size(); j++) {
-                    CHECK(t[j].rows == rows && t[j].parts == static_cast<int>(t.size()) && t[j].index == static_cast<int>(j));
-                    CHECK(t[j].k0 < t[j].k1 && (j == 0 || t[j].k0 == t[j - 1].k1));
-                    CHECK((t.size() > 1) == (t[j].part >= 0));
-                    if (t.size() > 1) CHECK(places.insert(t[j].part + t[j].index).second && t[j].part + t[j].index < plan.parts && t[j].tile < plan.tiles);
-                }
-                if (t.size() > 1) CHECK(counters.insert(t[0].tile).second);
+            lists.push_back(&pages[i]);
+            few.push_back(news[i] > 0 && news[i] * cut.group <= cut.height);
+        }
+        const std::vector<SharedPrefix> shared = shared_prefixes(lists, seqs, few, T, 128);
+        for (const SharedPrefix& s : shared) {
+            CHECK(s.members.size() >= 2 && s.prefix >= 128 && s.prefix % T == 0);
+            for (int m : s.members) {
+                CHECK(few[static_cast<size_t>(m)] && s.prefix <= seqs[static_cast<size_t>(m)].first);
+                for (int k = 0; k < s.prefix / T; k++) CHECK(pages[static_cast<size_t>(m)][static_cast<size_t>(k)] == pages[static_cast<size_t>(s.members[0])][static_cast<size_t>(k)]);
             }
         }
-        CHECK(tiles.size() == n_tiles);
-        CHECK(static_cast<int>(places.size()) <= plan.parts && static_cast<int>(counters.size()) == plan.tiles);
+        const AttendPlan plan = plan_attend(seqs, news, cut, cut.window == 0 ? shared : std::vector<SharedPrefix>{});
+        // position by position: who brings (pass row, head of the group) what
+        std::map<int, std::vector<int>> brought;
+        std::map<int, std::vector<std::pair<int, int>>> from;  // ... and from which place and row of it (-1: whole)
+        for (int row = 0; row < row0 * cut.group; row++) brought[row];
+        std::set<int> places;
+        for (const AttendItem& it : plan.items) {
+            CHECK(it.rows >= 1 && it.rows <= cut.height && it.k0 < it.k1 && it.k0 >= 0 && it.k0 % 16 == 0);
+            CHECK(it.joins <= 16 || cut.height > 16);
+            CHECK((it.part < 0) == (it.joins == 0));
+            if (it.part >= 0) CHECK(it.part < plan.parts && places.insert(it.part).second);
+            size_t owner = 0;
+            while (seqs[owner].table != it.table || pages[owner].empty()) owner++;
+            CHECK(it.k1 <= static_cast<int>(pages[owner].size()) * T);
+            for (int r = 0; r < it.rows; r++) {
+                const int row = it.map >= 0 ? plan.maps[static_cast<size_t>(it.map + r)] : it.row0 * cut.group + it.r0 + r;
+                CHECK(brought.count(row));
+                for (int t = it.k0; t < it.k1; t++) brought[row].push_back(t);
+                from[row].push_back({it.part, r});
+            }
+        }
+        std::map<int, std::vector<std::pair<int, int>>> wanted;  // what the joins read
+        std::map<int, int> arrivals;
+        for (const AttendItem& it : plan.items)
+            for (int j = 0; j < it.joins; j++) arrivals[it.join + j]++;
+        for (size_t j = 0; j < plan.joins.size(); j++) {
+            const AttendJoin& join = plan.joins[j];
+            CHECK(arrivals[static_cast<int>(j)] == join.parts + join.shared_parts && join.parts >= 1);
+            for (int r = 0; r < join.rows; r++) {
+                const int row = join.row0 * cut.group + join.r0 + r;
+                for (int k = 0; k < join.shared_parts; k++) wanted[row].push_back({join.shared_part + k, join.shared_row + r});
+                for (int k = 0; k < join.parts; k++) wanted[row].push_back({join.part + k, r});
+            }
+        }
+        CHECK(arrivals.size() == plan.joins.size());
+        for (size_t i = 0; i < seqs.size(); i++)
+            for (int r = 0; r < news[i] * cut.group; r++) {
+                const int row = seqs[i].row0 * cut.group + r, pos = seqs[i].first + r / cut.group;
+                std::vector<int>& got = brought[row];
+                std::sort(got.begin(), got.end());
+                CHECK(std::adjacent_find(got.begin(), got.end()) == got.end());
+                const int low = cut.window ? std::max(0, pos - cut.window + 1) : 0, high = cut.causal ? pos + 1 : seqs[i].len;
+                CHECK(!got.empty() && got.front() <= low && got.back() >= high - 1 && got.back() < seqs[i].len);
+                CHECK(static_cast<int>(got.size()) == got.back() - got.front() + 1);
+                auto& given = from[row];
+                if (given.size() == 1 && given[0].first < 0) {
+                    CHECK(!wanted.count(row));
+                } else {
+                    std::sort(given.begin(), given.end());
+                    std::sort(wanted[row].begin(), wanted[row].end());
+                    CHECK(given == wanted[row]);
+                }
+            }
     }
     return 0;
 }

@@ -342,6 +342,47 @@ def test_forks_share_until_somebody_writes(torch, dtype):
     assert rig.cache.pages_free == 64 and rig.cache.info.sequences == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", ["mha64", "grouped128", "one-key80", "dim256"])
+def test_many_samples_of_one_prompt(torch, dtype, heads):
+    """Sequences that share most of their pages are attended to together: as many as fill several tiles, of lengths of their
+    own behind the prompt, beside others that share nothing and two families more."""
+    h, kv, dim, page = HEADS[heads]
+    rig = Rig(torch, dtype, heads=h, kv_heads=kv, dim=dim, page=page, pages=8192 // page, seed=21)
+    a, b, lone = rig.add(), rig.add(), rig.add()
+    rig.grow([a, b, lone], [700, 333, 290])
+    kids = [rig.fork(a) for _ in range(19)] + [rig.fork(a, 400), rig.fork(a, 150)]
+    rig.grow(kids[:5], [3, 70, 1, 12, 30])
+    others = [rig.fork(b) for _ in range(2)]
+    seqs = kids[:7] + [lone, b] + kids[7:] + others + [a]
+    for counts in ([1] * len(seqs), [1 + (i % 3 == 0) for i in range(len(seqs))]):
+        q = rig.grow(seqs, counts)
+        rig.check(seqs, counts, q, what="shared")
+        rig.check(seqs, counts, q, window=200, what="window")
+    counts = [40 if i == 4 else 1 for i in range(len(seqs))]  # one of them with many rows
+    q = rig.grow(seqs, counts)
+    out = rig.check(seqs, counts, q, what="beside a chunk")
+    again = rig.check(seqs, counts, q, what="again")
+    assert torch.equal(out, again)
+    rig.check_contents(kids[:3])
+
+
+def test_long_lists_of_pages(torch):
+    """More pages than a launch's own list takes: copies, reads, compaction."""
+    rig = Rig(torch, "bf16", layers=2, heads=1, kv_heads=1, dim=8, page=16, pages=3200, seed=22)
+    a, b, c = rig.add(), rig.add(), rig.add()
+    rig.grow([a, b, c], [9000, 20000, 10007])
+    twin = rig.cache.copy(c)
+    rig.ref.fork(c, twin)
+    rig.drop(a)
+    rig.drop(c)
+    rig.cache.compact()
+    rig.check_contents([b, twin])
+    part = torch.empty(9991, 1, 8, dtype=torch.bfloat16, device="cuda")
+    rig.cache.read(twin, part, torch.empty_like(part), start=13, layer=1)
+    assert torch.equal(part.cpu().double(), rig.ref.k[twin][1, 13:13 + 9991])
+
+
 def test_a_rewound_sequence_takes_other_tokens(torch):
     """Drafted tokens of which the first are kept."""
     rig = Rig(torch, "f16", heads=4, kv_heads=4, dim=64, page=16, pages=32, rope=10000.0, seed=13)
