@@ -1,6 +1,7 @@
 // The paged cache of include/gradhip.h: gh_cache_*.
 #include "api_error.h"
 #include "cache_attend.h"
+#include "cache_session.h"
 #include "kernels_cache.h"
 
 #include <climits>
@@ -124,7 +125,6 @@ struct Cache {
     Staging staging;
     hipEvent_t moved = nullptr;  // from one stream to the next
     hipStream_t stream = nullptr;  // of the last call
-    bool used = false;             // ... if there was one
 
     // the open pass
     bool open = false;
@@ -186,22 +186,31 @@ struct Cache {
     }
 
     // Calls on one cache run in their order whatever streams they name: a call on another stream than the one before waits
-    // for what that one did.  Under capture a call would be replayed with the pages and lengths of today: refused.
-    void enter(void* hip_stream) {
-        const hipStream_t st = static_cast<hipStream_t>(hip_stream);
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        HIP_CHECK(hipStreamIsCapturing(st, &status));
-        if (status != hipStreamCaptureStatusNone)
-            throw ApiError{GH_ERR_RUNTIME, "cache: the stream is being captured into a graph; a replay would use the pages of the pass "
-                                           "that was open at capture"};
-        if (used && st != stream) {
-            if (!moved) HIP_CHECK(hipEventCreateWithFlags(&moved, hipEventDisableTiming));
-            HIP_CHECK(hipEventRecord(moved, stream));
-            HIP_CHECK(hipStreamWaitEvent(st, moved, 0));
+    // for what that one did.  The older stream itself is not touched (it may be gone by then) but for the default stream: a
+    // call on any other leaves an event behind.  Under capture a call would be replayed with the pages and lengths of today:
+    // refused.
+    struct Turn {
+        Cache& c;
+        Turn(Cache& cache, void* hip_stream) : c(cache) {
+            const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+            hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+            HIP_CHECK(hipStreamIsCapturing(st, &status));
+            if (status != hipStreamCaptureStatusNone)
+                throw ApiError{GH_ERR_RUNTIME, "cache: the stream is being captured into a graph; a replay would use the pages of the "
+                                               "pass that was open at capture"};
+            if (st != c.stream) {
+                if (!c.moved) HIP_CHECK(hipEventCreateWithFlags(&c.moved, hipEventDisableTiming));
+                if (c.stream == nullptr) HIP_CHECK(hipEventRecord(c.moved, nullptr));
+                HIP_CHECK(hipStreamWaitEvent(st, c.moved, 0));
+                c.stream = st;
+            }
         }
-        stream = st;
-        used = true;
-    }
+        ~Turn() {
+            if (c.stream != nullptr) (void)hipEventRecord(c.moved, c.stream);
+        }
+        Turn(const Turn&) = delete;
+        Turn& operator=(const Turn&) = delete;
+    };
 
     void close() {
         open = false;
@@ -338,8 +347,9 @@ static std::unique_ptr<Cache> create_cache(const gh_cache_opts& in) {
 static int copy_sequence(Cache& from, Cache& to, int seq, void* stream) {
     const PageBook::Sequence& s = from.book.at(seq);
     const int length = s.length, n = static_cast<int>(s.pages.size());
-    if (&from != &to) from.enter(stream);
-    to.enter(stream);
+    const Cache::Turn turn(to, stream);
+    std::unique_ptr<Cache::Turn> other;
+    if (&from != &to) other = std::make_unique<Cache::Turn>(from, stream);
     std::vector<PageCopy> copies(static_cast<size_t>(n));
     const int id = to.book.add_filled(length);
     const std::vector<int>& a = from.book.at(seq).pages;
@@ -360,7 +370,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
         pages += (static_cast<long long>(length) + counts[i] + c.o.page_tokens - 1) / c.o.page_tokens;
         if (rows > (1 << 23) || rows * c.group > (1 << 30) || pages > (1 << 28)) refuse("a pass of more than 2^23 rows");
     }
-    c.enter(stream);
+    const Cache::Turn turn(c, stream);
     // everything that may be refused or find no memory comes before the pages change hands
     c.seqs.assign(static_cast<size_t>(n), PassSeq{});
     c.news.assign(counts, counts + n);
@@ -429,7 +439,7 @@ static void append_rows(Cache& c, int layer, const gh_rows* k, const gh_rows* v,
         check_apart("q_out", q_out, c.rows, c.o.heads, dim);
     }
     const DeviceScope on(c.device);
-    c.enter(stream);
+    const Cache::Turn turn(c, stream);
     AppendParams p{};
     p.cache = c.layout;
     p.k = cache_rows(k);
@@ -461,7 +471,7 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     check_rows("out", out, c.o.heads, c.o.head_dim);
     check_apart("out", out, c.rows, c.o.heads, c.o.head_dim);
     const DeviceScope on(c.device);
-    c.enter(stream);
+    const Cache::Turn turn(c, stream);
     c.last_causal = causal;
     c.last_window = window;
     Cache::Plan* plan = nullptr;
@@ -519,7 +529,7 @@ static void read_positions(Cache& c, int seq, int layer, int layers, int start, 
         for (const auto& [r, stride, name] : {std::tuple{k, k_layer, "k"}, std::tuple{v, v_layer, "v"}})
             if (stride < (count - 1) * r->row_stride + (heads - 1) * r->head_stride + dim) refuse(std::string(name) + "'s layers overlap");
     const DeviceScope on(c.device);
-    c.enter(stream);
+    const Cache::Turn turn(c, stream);
     ReadParams p{};
     p.cache = c.layout;
     p.k = cache_rows(k);
@@ -561,6 +571,61 @@ static Cache& cache_of(gh_cache* c) {
     if (!c) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null cache"};
     return *c->impl;
 }
+
+static void check_session(const Cache& c, const KvLayout& kv, int layers) {
+    if (c.o.type != GH_F32 || c.o.layers != layers || c.o.kv_heads != kv.heads || c.o.head_dim != kv.head_size)
+        refuse("a session's context needs a cache of GH_F32 with the model's layers, heads (as kv_heads) and head size");
+    hipPointerAttribute_t at{};
+    HIP_CHECK(hipPointerGetAttributes(&at, kv.pool));
+    if (at.device != c.device) refuse("the session is on another device");
+}
+
+static void copy_session(Cache& c, const KvLayout& kv, int layers, int seq, const std::vector<int>& pages, int length, bool to_session) {
+    SessionCopyParams p{};
+    p.cache = c.layout;
+    p.kv = kv;
+    p.seq = seq;
+    p.to_session = to_session;
+    const int shift = c.layout.page_shift;
+    for (int at = 0; at < length;) {
+        const int first = at >> shift, last = std::min((length - 1) >> shift, first + 2 * kListed - 1);
+        const int end = static_cast<int>(std::min<long long>(length, (last + 1ll) << shift));
+        PageList list;
+        std::memcpy(list.pages, pages.data() + first, sizeof(int) * static_cast<size_t>(last - first + 1));
+        p.start = at;
+        p.count = end - at;
+        hipLaunchKernelGGL(cache_session_kernel, dim3((p.count + kReadPositions - 1) / kReadPositions, layers, 2), dim3(256), 0, c.stream, p, list);
+        HIP_CHECK(hipGetLastError());
+        at = end;
+    }
+}
+
+namespace gh {
+
+int cache_from_session(gh_cache* cache, const KvLayout& kv, int layers, int seq, int length, hipStream_t stream) {
+    Cache& c = cache_of(cache);
+    check_session(c, kv, layers);
+    const DeviceScope on(c.device);
+    const Cache::Turn turn(c, stream);
+    c.close();
+    const int id = c.book.add_filled(length);
+    copy_session(c, kv, layers, seq, c.book.at(id).pages, length, /*to_session=*/false);
+    return id;
+}
+
+void cache_to_session(gh_cache* cache, const int32_t* seqs, int batch, const KvLayout& kv, int layers, int length, hipStream_t stream) {
+    Cache& c = cache_of(cache);
+    check_session(c, kv, layers);
+    for (int b = 0; b < batch; b++)
+        if (c.book.at(seqs[b]).length < length)
+            throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: sequence " + std::to_string(seqs[b]) + " holds " + std::to_string(c.book.at(seqs[b]).length)
+                                                    + " positions, " + std::to_string(length) + " are wanted"};
+    const DeviceScope on(c.device);
+    const Cache::Turn turn(c, stream);
+    for (int b = 0; b < batch; b++) copy_session(c, kv, layers, b, c.book.at(seqs[b]).pages, length, /*to_session=*/true);
+}
+
+}  // namespace gh
 
 extern "C" {
 
@@ -647,7 +712,7 @@ gh_status gh_cache_compact(gh_cache* c, void* hip_stream, int32_t* pages_used) {
     return guard([&] {
         Cache& m = cache_of(c);
         const DeviceScope on(m.device);
-        m.enter(hip_stream);
+        const Cache::Turn turn(m, hip_stream);
         m.close();
         const int used = m.book.pages() - m.book.pages_free();
         m.copy_pages(m.pool.at, m.book.compact());

@@ -2,6 +2,7 @@
 // hipGraph-replayed), the on-GPU generate loop, and the C ABI of
 // include/gradhip.h.
 #include "api_error.h"
+#include "cache_session.h"
 #include "checkpoint.h"
 #include "tokenizer.h"
 #include "kernels_attn.h"
@@ -3021,6 +3022,50 @@ gh_status gh_session_score(gh_session* sess, const int32_t* ids, const int32_t* 
         });
         check_persist_abort(s);
         std::memcpy(nll_host, s.host_ids, n * sizeof(float));
+    });
+}
+
+gh_status gh_session_store(gh_session* sess, int32_t seq, gh_cache* cache, int32_t* out) {
+    return guard([&] {
+        if (!sess || !cache || !out) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        Session& s = *sess->impl;
+        if (seq < 0 || seq >= s.B) throw ApiError{GH_ERR_OUT_OF_RANGE, "no sequence " + std::to_string(seq) + " in the session"};
+        const int id = cache_from_session(cache, kv_layout(s), s.m->shape.layers, seq, s.pos, s.stream);
+        HIP_CHECK(hipStreamSynchronize(s.stream));
+        *out = id;
+    });
+}
+
+gh_status gh_session_restore(gh_session* sess, gh_cache* cache, const int32_t* seqs, const int32_t* ids, int32_t len,
+                             float* last_logits_host) {
+    return guard([&] {
+        if (!sess || !cache || !seqs || !ids) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
+        Session& s = *sess->impl;
+        const PersistGate gate(s);  // held until this call has synchronised its launches
+        const ResidentScope scope(s);
+        if (len < 1) throw ApiError{GH_ERR_INVALID_ARGUMENT, "a context of one token at least"};
+        if (len > s.m->shape.max_len) throw ApiError{GH_ERR_RUNTIME, "InferenceSession: context exceeds max_len"};
+        check_ids(s, ids, static_cast<size_t>(s.B) * len);
+        cache_to_session(cache, seqs, s.B, kv_layout(s), s.m->shape.layers, len - 1, s.stream);
+        // as after a prompt of all tokens but the last, which is stepped: its logits are what a pick needs
+        s.pos = 0;
+        s.n_hist = 0;
+        s.picks = 0;
+        std::memcpy(s.host_ids, ids, static_cast<size_t>(s.B) * len * sizeof(int));
+        stage_ids(s, s.host_ids, len, s.hist, s.hist_stride, 0);
+        s.pos = s.n_hist = len - 1;
+        if (s.engine != GH_ENGINE_PERSISTENT) {
+            hipLaunchKernelGGL(set_state_kernel, dim3(1), dim3(1), 0, s.stream, s.st, s.pos, s.n_hist, s.picks);
+            HIP_CHECK(hipGetLastError());
+        }
+        s.ahead = Session::AHEAD_STREAM;
+        run_resident(s, [&] {
+            run_prompt(s, 1, nullptr, nullptr);
+            deliver_logits(s);
+            HIP_CHECK(hipStreamSynchronize(s.stream));
+        });
+        check_persist_abort(s);
+        if (last_logits_host) std::memcpy(last_logits_host, s.host_logits, static_cast<size_t>(s.B) * s.m->shape.vocab * sizeof(float));
     });
 }
 

@@ -168,4 +168,32 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p, con
     }
 }
 
+struct SessionCopyParams {
+    CacheLayout cache;
+    KvLayout kv;
+    int seq;           // of the session
+    int start, count;  // positions; the list of pages begins with start's
+    int to_session;
+};
+
+// 16 positions of a layer, K or V, between a session's pages and a cache's, both fp32, 16 bytes to a thread.
+__global__ __launch_bounds__(256) void cache_session_kernel(const SessionCopyParams p, const PageList list) {
+    const int which = blockIdx.z, layer = blockIdx.y, n0 = blockIdx.x * kReadPositions;
+    const int fours = p.cache.dim / 4, tokens = min(kReadPositions, p.count - n0);
+    const int first_page = p.start >> p.cache.page_shift;
+    for (int i = threadIdx.x; i < tokens * fours * p.cache.kv_heads; i += 256) {
+        const int dim = i % fours * 4, token = i / fours % tokens, head = i / fours / tokens;
+        const int t = p.start + n0 + token;
+        const int page = list.pages[(t >> p.cache.page_shift) - first_page], place = t & ((1 << p.cache.page_shift) - 1);
+        float4* const cached = reinterpret_cast<float4*>(reinterpret_cast<float*>(cache_run(p.cache, page, layer, which, head))
+                                                         + static_cast<size_t>(place) * p.cache.dim + dim);
+        float4* const session = reinterpret_cast<float4*>(p.kv.pool + kv_offset(p.kv, layer, p.seq, which, head, t) + dim);
+        if (p.to_session) {
+            *session = *cached;
+        } else {
+            *cached = *session;
+        }
+    }
+}
+
 }  // namespace gh

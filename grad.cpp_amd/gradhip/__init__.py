@@ -137,6 +137,8 @@ SYMBOLS = {
     "gh_cache_attend": (C.c_int, [_vp, C.c_int32, C.POINTER(GhRows), C.POINTER(GhRows), C.c_float, C.c_int32, C.c_int32, _vp]),
     "gh_cache_read": (C.c_int, [_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(GhRows), C.c_int64,
                                 C.POINTER(GhRows), C.c_int64, _vp]),
+    "gh_session_store": (C.c_int, [_vp, C.c_int32, _vp, _i32p]),
+    "gh_session_restore": (C.c_int, [_vp, _vp, _i32p, _i32p, C.c_int32, _f32p]),
     "gh_device_info": (C.c_int, [C.c_char_p, C.c_size_t, _i32p, _i32p]),
     "gh_device_read_bandwidth": (C.c_int, [C.c_size_t, C.c_int32, C.POINTER(C.c_double)]),
     "gh_device_reread_bandwidth": (C.c_int, [C.c_size_t, C.c_int32, C.POINTER(C.c_double)]),
@@ -422,6 +424,24 @@ class Session:
         out = np.empty(ids.shape, dtype=np.float32)
         _check(load_library().gh_session_score(self._h, ids.ctypes.data_as(_i32p), targets.ctypes.data_as(_i32p),
                                                ids.shape[1], out.ctypes.data_as(_f32p)))
+        return out
+
+    def store(self, cache, seq=0) -> int:
+        """A new sequence of a Cache with everything that sequence `seq` of the session holds."""
+        out = C.c_int32()
+        _check(load_library().gh_session_store(self._h, seq, cache._h, C.byref(out)))
+        cache._rows = -1
+        return out.value
+
+    def restore(self, cache, seqs, ids) -> np.ndarray:
+        """Sequence b becomes the tokens ids[b], all but the last of them taken from sequence seqs[b] of a Cache; the last
+        one's logits (batch, vocab)."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32).reshape(self.batch, -1)
+        seqs = np.ascontiguousarray(np.atleast_1d(seqs), dtype=np.int32)
+        assert seqs.shape == (self.batch,)
+        out = np.empty((self.batch, self.vocab), dtype=np.float32)
+        _check(load_library().gh_session_restore(self._h, cache._h, seqs.ctypes.data_as(_i32p), ids.ctypes.data_as(_i32p),
+                                                 ids.shape[1], out.ctypes.data_as(_f32p)))
         return out
 
     def read_kv(self, seq, layer, kv, pos) -> np.ndarray:

@@ -357,8 +357,7 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  * NULL for the default stream) enqueue their work there and return without waiting, except
  * where an internal buffer has to grow.  Calls on one cache must be serialised by the caller
  * and take effect in their order whatever streams they name: a call on another stream than
- * the one before waits, on the device, for that one's work (so a stream that a cache was
- * used on must live until the cache's next call or its end).  The caller's own buffers are
+ * the one before waits, on the device, for that one's work.  The caller's own buffers are
  * ordered by the streams the caller names.  A stream that is being captured into a graph is
  * refused (GH_ERR_RUNTIME): a replay would use the pages and lengths of the capture.
  * Every size, page and position is checked on the host before anything is enqueued. */
@@ -443,6 +442,20 @@ gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh
 gh_status gh_cache_read(gh_cache* c, int32_t seq, int32_t layer, int32_t layers, int32_t start, int32_t count,
                         const gh_rows* k, int64_t k_layer_stride, const gh_rows* v, int64_t v_layer_stride,
                         void* hip_stream);
+
+/* A session's context into the cache: a new sequence with everything that sequence `seq` of the
+ * session holds (gh_session_position positions, every layer).  The cache is of GH_F32 and has the
+ * model's layers, heads (kv_heads) and head size; any page size.  Returns when the copy is made.
+ * With gh_session_restore: a prompt is read once and sampled from many times, conversations are
+ * set aside and taken up again, in sessions of any batch and engine of the same model. */
+gh_status gh_session_store(gh_session* s, int32_t seq, gh_cache* cache, int32_t* out);
+
+/* A context out of the cache: sequence b of the session becomes the tokens ids[b * len ..] (their
+ * history included), whose first len - 1 positions are taken from cache sequence seqs[b] (one may
+ * be named many times) and whose last is stepped, so that the session is as after gh_session_reset
+ * and gh_session_prefill of the ids.  last_logits_host (batch * vocab floats) may be NULL. */
+gh_status gh_session_restore(gh_session* s, gh_cache* cache, const int32_t* seqs, const int32_t* ids, int32_t len,
+                             float* last_logits_host);
 
 /* ------------------------------------------------------------ measurement */
 

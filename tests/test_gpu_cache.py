@@ -492,6 +492,29 @@ def test_calls_on_several_streams_keep_their_order(torch):
         rig.R.assert_within(out, want, allowed)
 
 
+def test_a_stream_may_end_before_the_cache(torch):
+    """A call waits for the one before also where that one's stream is gone (as a session's is with the session)."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    rig = Rig(torch, "f32", heads=4, kv_heads=2, dim=64, page=16, pages=600, seed=19)
+    s = rig.add()
+    rig.grow([s], [3000])
+    for i in range(4):
+        k, v, q = rig.rand(2, 2, 64), rig.rand(2, 2, 64), rig.rand(2, 4, 64)
+        kd, vd, qd = k.cuda(), v.cuda(), q.cuda()
+        out = torch.empty_like(qd)
+        torch.cuda.synchronize()
+        for call in (lambda st: rig.cache.extend([s], [2], stream=st), lambda st: rig.cache.append(0, kd, vd, stream=st),
+                     lambda st: rig.cache.attend(0, qd, out, stream=st)):
+            made = ctypes.c_void_p()
+            assert hip.hipStreamCreate(ctypes.byref(made)) == 0
+            call(made.value)
+            assert hip.hipStreamDestroy(made) == 0
+        torch.cuda.synchronize()
+        rig.ref.extend(s, k[None], v[None])
+        want, allowed = rig.R.attention(q.double(), rig.ref.k[s][0], rig.ref.v[s][0], 3000 + 2 * i)
+        rig.R.assert_within(out, want, allowed)
+
+
 def test_two_caches_at_work_beside_each_other(torch):
     rigs = [Rig(torch, t, heads=4, kv_heads=2, dim=64, page=16, pages=600, seed=18) for t in ("f32", "bf16")]
     streams = [torch.cuda.Stream() for _ in rigs]
