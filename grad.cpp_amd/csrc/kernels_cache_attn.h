@@ -520,7 +520,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
                                       u32x4{q[rt][w], q[rt][w + 1], q[rt][w + 2], q[rt][w + 3]}, acc);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) z[rt][4 * b + i] = acc[i] * p.scale;
+                for (int i = 0; i < 4; i++) z[rt][4 * b + i] = __fmul_rn(acc[i], p.scale);  // (rounded as the maximum is)
             }
         unsigned seen[TILES];
         bool hidden = false;

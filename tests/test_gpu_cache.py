@@ -191,6 +191,44 @@ def test_many_rows_never_see_what_they_may_not(torch, dtype):
         rig.check([s], [250], q, window=40, what="behind the window")
 
 
+@pytest.mark.parametrize("case", ["huge later values", "huge later keys", "rows far apart", "dims far apart", "large", "tiny", "zeros"])
+def test_many_rows_of_any_size(torch, case):
+    """fp32 chunks whose operands do not fit one power of two per tile, or just do."""
+    for dim, heads, kv in ((64, 2, 1), (128, 2, 2), (40, 1, 1), (256, 1, 1)):
+        rig = Rig(torch, "f32", heads=heads, kv_heads=kv, dim=dim, page=16, pages=60, seed=23)
+        s = rig.add()
+        rig.grow([s], [133])
+        k, v = rig.rand(1, 250, kv, dim), rig.rand(1, 250, kv, dim)
+        if case == "huge later values":
+            v[0, 100:] *= 1e30
+        elif case == "huge later keys":
+            k[0, 120:] *= 1e12
+        elif case == "rows far apart":
+            v[0, ::7] *= 2.0 ** -30
+            k[0, ::5] *= 2.0 ** -25
+        elif case == "dims far apart":
+            v[0, :, :, ::3] *= 2.0 ** -14
+            k[0, :, :, 1::2] *= 2.0 ** -15
+        elif case == "large":
+            v *= 2.0 ** 58
+            k *= 2.0 ** 40
+        elif case == "tiny":
+            v *= 2.0 ** -58
+            k *= 2.0 ** -40
+        else:
+            v[0, 30:200] = 0.0
+            k[0, 60:] = 0.0
+        q = rig.grow([s], [250], k=k, v=v)
+        if case == "large":
+            q *= 2.0 ** -40
+        elif case == "tiny":
+            q *= 2.0 ** 40
+        elif case == "zeros":
+            q[0, 17:90] = 0.0
+        rig.check([s], [250], q, what=case)
+        rig.check([s], [250], q, window=60, what=case)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("before,new", [(0, 1), (0, 2), (0, 15), (0, 16), (0, 17), (0, 64), (0, 131), (15, 1), (16, 1), (31, 2), (63, 70), (127, 129), (1000, 1), (2047, 5)])
 def test_attend_at_the_edges_of_pages_and_tiles(torch, dtype, before, new):
