@@ -8,6 +8,7 @@
 #pragma once
 
 #include <algorithm>
+#include <climits>
 #include <unordered_map>
 #include <vector>
 
@@ -31,7 +32,7 @@ struct AttendItem {
     int k0, k1;
     int part;          // the place in memory that its result goes to, -1: it is whole and goes to the caller
     int join, joins;   // the joins that wait for it
-    int first, row0, table;  // the sequence's; for a map, a position that sees everything
+    int first, row0, table;  // the sequence's; for a map, a position behind all others
     int map;           // rows of several sequences: where their (pass row * group + head of the group) are listed
     int pad;           // a multiple of 16 bytes
 };
@@ -170,7 +171,7 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
         int run;
         const int parts = cut_up(0, shared[g].prefix, run);
         for (size_t m = 0; m < members.size();) {
-            AttendItem it{0, 0, 0, 0, plan.parts, static_cast<int>(plan.joins.size()), 0, 1 << 30, 0,
+            AttendItem it{0, 0, 0, 0, plan.parts, static_cast<int>(plan.joins.size()), 0, INT_MAX - 1024, 0,
                           seqs[static_cast<size_t>(members[m])].table, static_cast<int>(plan.maps.size()), 0};
             plan.parts += parts;
             for (; m < members.size(); m++) {

@@ -127,8 +127,16 @@ struct Granule {
 };
 
 // FULL: the head has DH dims.  Otherwise lanes whose dims do not exist read past the end of the run: zeros.
+// The pages of a granule; a block behind the last position may have none: it reads the last one's, and counts for nothing.
+template <int BLOCKS>
+__device__ __forceinline__ void look_up(const CacheLayout& cache, const int* table, int at, int end, int (&pages)[BLOCKS]) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) pages[b] = table[min(at + 16 * b, end - 1) >> cache.page_shift];
+}
+
+// `pages`: of the granule's blocks of 16 positions, looked up ahead (look_up), or the loads would wait for them one by one.
 template <int TYPE, int DH, bool FULL>
-__device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer, const int* table, int head, int at, int end,
+__device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer, const int (&pages)[Granule<TYPE, DH>::kBlocks], int head, int at,
                                              Granule<TYPE, DH>& g) {
     using G = Granule<TYPE, DH>;
     constexpr int kBytes = CacheType<TYPE>::kBytes;
@@ -138,10 +146,7 @@ __device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer
     const int value_lane = (lane >> 4) * 4 * row + value_dim * kBytes;
 #pragma unroll
     for (int b = 0; b < G::kBlocks; b++) {
-        // a block that begins behind the last position may have no page: it reads the one before, and counts for nothing
-        const int t = at + 16 * b < end ? at + 16 * b : at;
-        const int page = table[t >> cache.page_shift];
-        const int offset = (t & ((1 << cache.page_shift) - 1)) * row;
+        const int offset = ((at + 16 * b) & ((1 << cache.page_shift) - 1)) * row, page = pages[b];
         const char* run = cache_run(cache, page, layer, 0, head);
         const __amdgpu_buffer_rsrc_t ks = make_buffer(run, static_cast<unsigned>(cache.run_bytes));
         const __amdgpu_buffer_rsrc_t vs = make_buffer(run + cache.kv_heads * cache.run_bytes, static_cast<unsigned>(cache.run_bytes));
@@ -323,7 +328,8 @@ struct Meeting {
 // order of the folding is that of the positions, whoever arrived when.  MANY: the item's rows are of several joins.
 // stash: 32 bytes of shared memory for each thread.
 template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS, bool MANY>
-__device__ __forceinline__ void join_parts(const AttendParams& p, const AttendItem& it, int head, const Meeting& meeting, char* stash) {
+__device__ __forceinline__ void join_parts(const AttendParams& p, const AttendItem& it, const AttendJoin& mine, int head, const Meeting& meeting,
+                                           char* stash) {
     constexpr int kPad = DH + 4, kChunks = DH / 4, kBlock = HEIGHT * kPad;
     constexpr int kSide = HEIGHT > 64 ? 4 : 1, kDeep = HEIGHT > 64 ? 4 : MANY ? 8 : 16;  // elements of a thread and parts, in flight
     const __amdgpu_buffer_rsrc_t rs = make_buffer(p.parts, 0xFFFFFFFFu);  // (the host keeps all parts below 4 GB)
@@ -334,24 +340,25 @@ __device__ __forceinline__ void join_parts(const AttendParams& p, const AttendIt
             while (j + 1 < it.joins && meeting.shared_row[j + 1] <= e / kChunks) j++;
         return it.join + j;
     };
-    const int most = p.joins[it.join].shared_parts + p.joins[it.join].parts;  // (members' own parts of a prefix's rest: one or a few)
+    const int most = mine.shared_parts + mine.parts;  // (members' own parts of a prefix's rest: one or a few)
     const int shares = max(1, min(THREADS / elements, (most + kDeep - 1) / kDeep));  // of the parts
     const int share = static_cast<int>(threadIdx.x) / elements;                      // (0 where there is one)
     const auto write = [&](int e, const f32x4& out, float total) {
         const int dim = e % kChunks * 4, j = join_of(e);
         if ((MANY && !meeting.last[j - it.join]) || (!FULL && dim >= p.cache.dim)) return;
-        const int r = p.joins[j].r0 + e / kChunks - (MANY ? p.joins[j].shared_row : 0);
-        store_four<TYPE>(p.out, (p.joins[j].row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
-                         p.vector_rows, out / total);
+        const int r = (MANY ? p.joins[j].r0 - p.joins[j].shared_row : mine.r0) + e / kChunks, row0 = MANY ? p.joins[j].row0 : mine.row0;
+        store_four<TYPE>(p.out, (row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim, p.vector_rows,
+                         out / total);
     };
     for (int e0 = shares > 1 ? static_cast<int>(threadIdx.x) % elements : threadIdx.x; e0 < elements; e0 += kSide * THREADS) {
         Folded f[kSide];
 #pragma unroll
         for (int k = 0; k < kSide; k++) f[k] = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
-        const AttendJoin* const join = p.joins + join_of(e0);
+        const int which = join_of(e0);
+        const AttendJoin* const join = MANY ? p.joins + which : &mine;
         const int shared_parts = join->shared_parts, shared_part = join->shared_part, own_part = join->part, shared_row = join->shared_row;
         int all = shared_parts + join->parts;
-        if (MANY && !meeting.last[join - (p.joins + it.join)]) all = 0;
+        if (MANY && !meeting.last[which - it.join]) all = 0;
         const int each = (all + shares - 1) / shares;
         const int skip = MANY ? shared_row : 0;  // rows of the item before the join's
         const int from = shares > 1 ? min(share * each, all) : 0, to = shares > 1 ? min(from + each, all) : all;
@@ -401,18 +408,19 @@ __device__ __forceinline__ void join_parts(const AttendParams& p, const AttendIt
 
 // The workgroup's part is in memory: it arrives at the joins that wait for it and makes those it is the last for.
 template <int TYPE, int DH, bool FULL, int HEIGHT, int THREADS>
-__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, int head, Meeting& meeting, char* stash) {
+__device__ __forceinline__ void finish_parts(const AttendParams& p, const AttendItem& it, const AttendJoin& mine, int head, Meeting& meeting,
+                                             char* stash) {
     // the stores have to be out before the workgroup counts as arrived
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (static_cast<int>(threadIdx.x) < it.joins) {
-        const AttendJoin& join = p.joins[it.join + threadIdx.x];
+        const AttendJoin join = it.joins == 1 ? mine : p.joins[it.join + threadIdx.x];
         unsigned* const arrived = p.arrived + static_cast<size_t>(it.join + threadIdx.x) * p.cache.kv_heads + head;
-        const bool mine = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+        const bool last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
                           == static_cast<unsigned>(join.shared_parts + join.parts - 1);
-        if (mine) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         meeting.shared_row[threadIdx.x] = join.shared_row;
-        meeting.last[threadIdx.x] = mine;
+        meeting.last[threadIdx.x] = last;
     }
     __syncthreads();
     int any = 0;
@@ -420,11 +428,16 @@ __device__ __forceinline__ void finish_parts(const AttendParams& p, const Attend
     if (__builtin_amdgcn_readfirstlane(any) == 0) return;
     if constexpr (HEIGHT == 16) {
         if (it.map >= 0) {
-            join_parts<TYPE, DH, FULL, HEIGHT, THREADS, true>(p, it, head, meeting, stash);
+            join_parts<TYPE, DH, FULL, HEIGHT, THREADS, true>(p, it, mine, head, meeting, stash);
             return;
         }
     }
-    join_parts<TYPE, DH, FULL, HEIGHT, THREADS, false>(p, it, head, meeting, stash);
+    join_parts<TYPE, DH, FULL, HEIGHT, THREADS, false>(p, it, mine, head, meeting, stash);
+}
+
+// The join of an item that has one, requested early: at the end it would be one more trip to memory.
+__device__ __forceinline__ AttendJoin first_join(const AttendParams& p, const AttendItem& it) {
+    return it.joins > 0 ? p.joins[it.join] : AttendJoin{};
 }
 
 // Wavefronts of a workgroup: as many as take 128 positions at a time (fp32, one token: 64 sequences of up to 2 k positions
@@ -447,6 +460,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
+    const AttendJoin mine = first_join(p, it);
     const int* table = p.table + it.table;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int quarter = lane >> 4;
@@ -495,11 +509,19 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
     }
 
     Granule<TYPE, DH> now, next;
+    int pages[G::kBlocks];
     int at = it.k0 + wave * G::kTokens;
-    if (at < it.k1) load_granule<TYPE, DH, FULL>(p.cache, p.layer, table, head, at, it.k1, now);
+    if (at < it.k1) {
+        look_up(p.cache, table, at, it.k1, pages);
+        load_granule<TYPE, DH, FULL>(p.cache, p.layer, pages, head, at, now);
+        look_up(p.cache, table, at + kAttendWaves * G::kTokens, it.k1, pages);
+    }
     while (at < it.k1) {
         const int then = at + kAttendWaves * G::kTokens;
-        if (then < it.k1) load_granule<TYPE, DH, FULL>(p.cache, p.layer, table, head, then, it.k1, next);
+        if (then < it.k1) {
+            load_granule<TYPE, DH, FULL>(p.cache, p.layer, pages, head, then, next);
+            look_up(p.cache, table, then + kAttendWaves * G::kTokens, it.k1, pages);
+        }
 
         // does a mask cut this granule?
         const bool cut = at + G::kTokens > it.k1 || (p.causal && at + G::kTokens - 1 > first) || (p.window > 0 && at <= final - p.window);
@@ -609,15 +631,15 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
             sums[wave][lane] = sum;
         }
         __syncthreads();
-        const int mine = lane & 15;
-        float top = tops[0][mine];
+        const int own = lane & 15;
+        float top = tops[0][own];
 #pragma unroll
-        for (int w = 1; w < kAttendWaves; w++) top = fmaxf(top, tops[w][mine]);
+        for (int w = 1; w < kAttendWaves; w++) top = fmaxf(top, tops[w][own]);
         const float keep = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int cc = 0; cc < kDims; cc++) meet[wave][mine][(4 * quarter + i) * kDims + cc] = o[rt][cc][i] * keep;
+            for (int cc = 0; cc < kDims; cc++) meet[wave][own][(4 * quarter + i) * kDims + cc] = o[rt][cc][i] * keep;
         __syncthreads();
         for (int e = threadIdx.x; e < 16 * kChunks; e += 64 * kAttendWaves) {
             const int row = e / kChunks, dim = e % kChunks * 4;
@@ -648,7 +670,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
     }
     if (only) return;
 
-    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, head, meeting, reinterpret_cast<char*>(meet));
+    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, mine, head, meeting, reinterpret_cast<char*>(meet));
 }
 
 }  // namespace gh

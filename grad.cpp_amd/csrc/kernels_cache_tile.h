@@ -167,6 +167,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
+    const AttendJoin mine = first_join(p, it);
     const int* table = p.table + it.table;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
         leave_rows<TYPE, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }
     if (only) return;
-    finish_parts<TYPE, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, meeting, keys);
+    finish_parts<TYPE, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, mine, head, meeting, keys);
 }
 
 // ---------------------------------------------------------------------- fp32
@@ -426,6 +427,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
 
     const AttendItem it = p.items[blockIdx.x / p.cache.kv_heads];
     const int head = blockIdx.x % p.cache.kv_heads;
+    const AttendJoin mine = first_join(p, it);
     const int* table = p.table + it.table;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5;
@@ -705,7 +707,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
         leave_rows<kCacheF32, DH, FULL>(p, it, o, m - kLift, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }
     if (only) return;
-    finish_parts<kCacheF32, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, head, meeting, keys);
+    finish_parts<kCacheF32, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, mine, head, meeting, keys);
 }
 
 }  // namespace gh

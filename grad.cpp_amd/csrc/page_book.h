@@ -52,9 +52,10 @@ public:
 
     // A new, empty sequence: the lowest number that no sequence has.
     int add() {
-        size_t i = 0;
+        size_t i = lowest_;
         while (i < seqs_.size() && seqs_[i].live) i++;
         if (i == seqs_.size()) seqs_.emplace_back();
+        lowest_ = i + 1;
         seqs_[i].live = true;
         seqs_[i].length = 0;
         seqs_[i].pages.clear();
@@ -91,6 +92,7 @@ public:
     void drop(int seq) {
         truncate(seq, 0);
         seqs_[static_cast<size_t>(seq)].live = false;
+        lowest_ = std::min(lowest_, static_cast<size_t>(seq));
     }
 
     // counts[i] more positions for seqs[i]; the copies that have to be made before anything is
@@ -212,6 +214,7 @@ private:
     std::vector<int> held_;  // by how many sequences
     std::vector<int> free_;  // a heap, the lowest on top
     std::vector<Sequence> seqs_;
+    size_t lowest_ = 0;  // no sequence below this number is free
 };
 
 }  // namespace gh
