@@ -302,6 +302,10 @@ __device__ __forceinline__ void store_four(const CacheRows& rows, long long at, 
     }
 }
 
+// Scores go into the exponent unscaled, scale and maximum in one multiply-add, whose unrounded product may be above the rounded
+// maximum: by less than half for maxima up to this, and by the same for all.  Beyond, they are scaled, and rounded, first.
+constexpr float kFusedTop = 4194304.0f;
+
 // What a thread has folded of the parts of four output elements: their weighted sum, the maximum it is relative to, the sum.
 struct Folded {
     f32x4 out;
@@ -542,7 +546,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
                                       u32x4{q[rt][w], q[rt][w + 1], q[rt][w + 2], q[rt][w + 3]}, acc);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) z[rt][4 * b + i] = __fmul_rn(acc[i], p.scale);  // (rounded as the maximum is)
+                for (int i = 0; i < 4; i++) z[rt][4 * b + i] = acc[i];
             }
         unsigned seen[TILES];
         bool hidden = false;
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
             float top = z[rt][0];
 #pragma unroll
             for (int i = 1; i < 4 * G::kBlocks; i++) top = fmaxf(top, z[rt][i]);
-            top = row_max(top);
+            top = __fmul_rn(row_max(top), p.scale);
             if (__any(top > m[rt])) {
                 const float keep = top > m[rt] ? __builtin_amdgcn_exp2f(m[rt] - top) : 1.0f;
                 m[rt] = fmaxf(m[rt], top);
@@ -583,9 +587,15 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
                 for (int cc = 0; cc < kDims; cc++) o[rt][cc] *= keep;
             }
             const float base = m[rt] == -INFINITY ? 0.0f : m[rt] - C::kLift;
+            float scale = p.scale;
+            if (__any(fabsf(base) > kFusedTop)) {
+                scale = 1.0f;
+#pragma unroll
+                for (int i = 0; i < 4 * G::kBlocks; i++) z[rt][i] = __fmul_rn(z[rt][i], p.scale);
+            }
 #pragma unroll
             for (int i = 0; i < 4 * G::kBlocks; i++) {
-                z[rt][i] = __builtin_amdgcn_exp2f(z[rt][i] - base);
+                z[rt][i] = __builtin_amdgcn_exp2f(fmaf(z[rt][i], scale, -base));
                 l[rt] += z[rt][i];
             }
         }

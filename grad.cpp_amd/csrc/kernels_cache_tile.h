@@ -59,10 +59,6 @@ __device__ __forceinline__ void ahead_of_products() {
     }
 }
 
-// Scores go into the exponent unscaled, scale and maximum in one multiply-add, whose unrounded product may be above the rounded
-// maximum: by less than half for maxima up to this, and by the same for all.  Beyond, they are scaled, and rounded, first.
-constexpr float kFusedTop = 4194304.0f;
-
 // A wavefront's rows [from, from + rows) of a tile, one after the other and term by term: 64 positions at a time, the scores with a
 // position to a lane, the output with a dim to a lane.  What a row may not see takes no part at all, infinities and NaN are what
 // they are.  For the tiles that hold such values (a matrix product would carry them to rows that do not see them, and make
