@@ -109,8 +109,18 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 constexpr int kMaxHeads = 1024;
 constexpr int kMaxPageTokens = 1024;
 constexpr int kPlans = 4;
-constexpr int kLeastShared = 128;  // positions of a prefix that sequences attend to in common tiles
-constexpr int kFewRows = 16;  // of a sequence: they go to a launch of their own beside longer ones
+// Prefixes are read in common tiles from this many positions on and where their members would read so many bytes of them in all:
+// what common tiles leave are parts, to be joined.  us, eight samples, common and apart: fp32, 12 heads of 64: 256 positions (13 MB)
+// 11.3 and 9.1, 512 11.6 and 11.9, 1 k (50 MB) 12.1 and 13.1, 2 k 13.4 and 21.4; bf16, 8 kv heads of 128: 1 k (34 MB) 14.9 and 12.6,
+// 2 k 15.5 and 20.9, 4 k 19.0 and 30.1.
+constexpr int kLeastShared = 128;
+constexpr size_t kLeastSharedBytes = 40u << 20;
+// Few rows of sequences that hold so many bytes in all go to the tiles of many rows beside them: there a single token reads its
+// sequence 1.2 (16 bit) to 2.4 (fp32) times as slowly, but a launch of its own behind the other is some 15 us.  us, together and
+// apart: bf16, single tokens over 117 MB beside a chunk of 200 tokens 49 and 69, of 1000 101 and 110, over 234 MB 68 and 102, 176 and
+// 181, over 468 MB 133 and 168, 317 and 282; fp32, over 43 MB 31 and 36, 46 and 53, over 175 MB 51 and 62, 86 and 85, over 351 MB 88
+// and 94, 161 and 141.
+constexpr size_t kTogether16 = 320u << 20, kTogether32 = 160u << 20;
 
 }  // namespace
 
@@ -139,7 +149,7 @@ struct Cache {
         bool valid = false;
         bool causal = true;
         int window = 0;
-        // sequences of few rows and of many go to kernels of their own, one behind the other
+        // sequences of few rows and of many go to kernels of their own, one behind the other, unless the few fit beside the many
         struct Launch {
             AttendForm form{};
             AttendPlan cut;
@@ -235,12 +245,29 @@ struct Cache {
         plan.causal = causal;
         plan.window = window;
         size_t part_bytes = 0, counters = 0;
+        const std::vector<SharedPrefix> prefixes = window == 0 ? shared : std::vector<SharedPrefix>{};
+        int few = few_rows(o.type);
+        if (prefixes.empty()) {
+            size_t held = 0;  // by the sequences of few rows
+            bool many = false;
+            for (size_t i = 0; i < news.size(); i++) {
+                if (news[i] == 0) continue;
+                int k0, k1;
+                visible_span(seqs[i], 0, news[i] * group, group, causal, window, k0, k1);
+                if (news[i] * group > few) {
+                    many = true;
+                } else {
+                    held += static_cast<size_t>(k1 - k0) * o.kv_heads * o.head_dim * 2 * static_cast<size_t>(bytes);
+                }
+            }
+            if (many && held <= (bytes == 4 ? kTogether32 : kTogether16)) few = 0;
+        }
         for (int many = 0; many < 2; many++) {
             Plan::Launch& l = plan.launches[many];
             std::vector<int> mine(news.size(), 0);
             int most = 0;
             for (size_t i = 0; i < news.size(); i++)
-                if ((news[i] * group > kFewRows) == (many == 1)) {
+                if ((news[i] * group > few) == (many == 1)) {
                     mine[i] = news[i];
                     most = std::max(most, news[i] * group);
                 }
@@ -256,12 +283,17 @@ struct Cache {
             // 32 k positions, 32/8 heads of 128 in bf16: 256 us, with half as many 262, a quarter 275); parts below 64 KB of
             // keys cost more to join than they save (13 sequences of up to 1 k positions, fp32: 14.5 us, 15.5 in parts of
             // half that), and more than 64 parts of a tile are a long join (one sequence of 128 k positions: 61 us, 71 in 128).
-            // Many rows: as many as are resident at once, in the 16-bit types half of that, where joining parts of 128
-            // rows weighs more (777 rows, window 1024, fp16: 37 us, 41; 397 rows over 2 k positions, fp32: 45 us in half, 40).
-            const int workgroups = !tiles ? (bytes == 4 ? 1024 : 2048) : bytes == 4 ? 512 : 256;
+            // Many rows: as many as are resident at once and no more (1024 rows over 16 k positions, bf16: 113 us, 154 with half as
+            // many; over 4 k, fp32: 96, 111 with 576), and no more parts than the last one joins in the time that they
+            // save (128 rows, bf16: 1 k positions 31 us in 4 parts, 34 in 8; 4 k 44 in 8, 75 in 32; 16 k 75 in 16, 142 in 64;
+            // fp32 products take four times as long: 4 k 44 in 16, 51 in 8 and in 32).
+            const int resident = o.head_dim > 128 ? 256 : 512;
+            const int workgroups = tiles ? resident : bytes == 4 ? 1024 : 2048;
             const int least = tiles ? 128 : bytes == 4 ? 256 : 384;
-            l.cut = plan_attend(seqs, mine, AttendCut{group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64},
-                                !many && window == 0 ? shared : std::vector<SharedPrefix>{});
+            l.cut = plan_attend(seqs, mine,
+                                AttendCut{group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64,
+                                          !tiles ? 0 : bytes == 4 ? 16 : 64, tiles ? resident : 0},
+                                many ? std::vector<SharedPrefix>{} : prefixes);
             part_bytes = std::max(part_bytes, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
             counters = std::max(counters, l.cut.joins.size() * o.kv_heads);
         }
@@ -271,11 +303,9 @@ struct Cache {
     }
 };
 
-static void check_rows(const char* what, const gh_rows* r, int heads, int dim) {
+static void check_rows(const char* what, const gh_rows* r) {
     if (!r || !r->data) refuse(std::string(what) + " is null");
     if (r->row_stride < 0 || r->head_stride < 0) refuse(std::string(what) + " has a negative stride");
-    (void)heads;
-    (void)dim;
 }
 
 // Rows that are written must not lie on top of one another.
@@ -387,9 +417,12 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     std::vector<char> few(static_cast<size_t>(n));
     for (int i = 0; i < n; i++) {
         pages_of[static_cast<size_t>(i)] = &c.book.at(seqs[i]).pages;
-        few[static_cast<size_t>(i)] = counts[i] > 0 && static_cast<long long>(counts[i]) * c.group <= kFewRows;
+        few[static_cast<size_t>(i)] = counts[i] > 0 && static_cast<long long>(counts[i]) * c.group <= kFewTile;
     }
     c.shared = shared_prefixes(pages_of, c.seqs, few, c.o.page_tokens, kLeastShared);
+    const size_t position = static_cast<size_t>(c.o.kv_heads) * c.o.head_dim * 2 * static_cast<size_t>(c.bytes);
+    const auto slight = [&](const SharedPrefix& s) { return position * static_cast<size_t>(s.prefix) * s.members.size() < kLeastSharedBytes; };
+    c.shared.erase(std::remove_if(c.shared.begin(), c.shared.end(), slight), c.shared.end());
     Cache::Plan& plan = c.plans[0];
     c.cut(plan, c.last_causal, c.last_window);
     c.next_plan = 1;
@@ -431,11 +464,11 @@ static void append_rows(Cache& c, int layer, const gh_rows* k, const gh_rows* v,
     if ((q == nullptr) != (q_out == nullptr)) refuse("queries and a place for them go together");
     if (c.rows == 0) return;
     const int dim = c.o.head_dim;
-    check_rows("k", k, c.o.kv_heads, dim);
-    check_rows("v", v, c.o.kv_heads, dim);
+    check_rows("k", k);
+    check_rows("v", v);
     if (q) {
-        check_rows("q", q, c.o.heads, dim);
-        check_rows("q_out", q_out, c.o.heads, dim);
+        check_rows("q", q);
+        check_rows("q_out", q_out);
         check_apart("q_out", q_out, c.rows, c.o.heads, dim);
     }
     const DeviceScope on(c.device);
@@ -467,8 +500,8 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     if (window < 0) refuse("negative window");
     if (!(scale >= 0.0f) || std::isinf(scale)) refuse("scale must be a finite number, 0 for 1 / sqrt(head_dim)");
     if (c.rows == 0) return;
-    check_rows("q", q, c.o.heads, c.o.head_dim);
-    check_rows("out", out, c.o.heads, c.o.head_dim);
+    check_rows("q", q);
+    check_rows("out", out);
     check_apart("out", out, c.rows, c.o.heads, c.o.head_dim);
     const DeviceScope on(c.device);
     const Cache::Turn turn(c, stream);
@@ -521,8 +554,8 @@ static void read_positions(Cache& c, int seq, int layer, int layers, int start, 
         throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: positions out of range"};
     if (count == 0 || layers == 0) return;
     const int dim = c.o.head_dim, heads = c.o.kv_heads;
-    check_rows("k", k, heads, dim);
-    check_rows("v", v, heads, dim);
+    check_rows("k", k);
+    check_rows("v", v);
     check_apart("k", k, count, heads, dim);
     check_apart("v", v, count, heads, dim);
     if (layers > 1)

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <unordered_map>
 #include <vector>
 
@@ -98,6 +99,9 @@ struct AttendCut {
     int workgroups;  // about as many, over all kv heads
     int least;       // positions of a part, at least
     int most;        // parts of a tile, at most
+    int square = 0;    // ... and, if not 0, sqrt(positions / square): the last part to end joins them all, so n parts take
+                       // positions / n + square n.  A tile of 1 / r-th the height has a join of 1 / r-th the time
+    int resident = 0;  // if not 0: no more workgroups than this many where there are fewer tiles (one more is a round of its own)
 };
 
 // Tiles of `height` rows; a tile's positions are cut into parts of one length.  `shared`: prefixes whose members (of at
@@ -134,13 +138,29 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
         }
     for (size_t g = 0; g < shared.size(); g++) total += static_cast<long long>(shared[g].prefix) * packed[g];
     const long long each = (total * cut.kv_heads + cut.workgroups - 1) / std::max(cut.workgroups, 1);
-    const int span = static_cast<int>(std::min<long long>(std::max<long long>(cut.least, (each + 127) / 128 * 128), 1 << 30));
+    long long span = std::max<long long>(cut.least, (each + 127) / 128 * 128);
     // the length of the parts of [k0, k1), as even as whole runs of 32 positions allow, and their number
-    const auto cut_up = [&](int k0, int k1, int& run) {
-        const int parts = std::max(1, std::min(cut.most, (k1 - k0 + span - 1) / span));
+    const auto cut_up = [&](int n, int k0, int k1, int& run) {
+        int most = cut.most;
+        if (cut.square > 0) most = std::min(most, static_cast<int>(std::sqrt(static_cast<double>(k1 - k0) * height / n / cut.square) + 0.5));
+        const int parts = std::max(1, static_cast<int>(std::min<long long>(most, (k1 - k0 + span - 1) / span)));
         run = (((k1 - k0 + parts - 1) / parts) + 31) / 32 * 32;
         return std::max(1, (k1 - k0 + run - 1) / run);
     };
+    if (cut.resident > 0) {
+        const auto count = [&](bool whole) {
+            long long items = 0;
+            for (size_t i = 0; i < seqs.size(); i++)
+                for (int r0 = 0; r0 < rows[i] * cut.group; r0 += height) {
+                    int n, k0, k1, run;
+                    tile_span(i, r0, n, k0, k1);
+                    items += whole ? 1 : cut_up(n, k0, k1, run);
+                }
+            return items * cut.kv_heads;
+        };
+        if (count(true) <= cut.resident)
+            while (count(false) > cut.resident) span += std::max(32ll, span / 8 / 32 * 32);
+    }
     const auto add_items = [&](AttendItem it, int k0, int k1, int parts, int run) {
         for (int j = 0; j < parts; j++) {
             it.k0 = k0 + j * run;
@@ -152,7 +172,7 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
     const auto add_tile = [&](size_t i, int r0, AttendJoin join) {
         int n, k0, k1, run;
         tile_span(i, r0, n, k0, k1);
-        const int parts = cut_up(k0, k1, run);
+        const int parts = cut_up(n, k0, k1, run);
         const bool whole = parts == 1 && join.shared_parts == 0;
         AttendItem it{r0, n, 0, 0, whole ? -1 : plan.parts, static_cast<int>(plan.joins.size()), whole ? 0 : 1,
                       seqs[i].first, seqs[i].row0, seqs[i].table, -1, 0};
@@ -169,7 +189,7 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
     for (size_t g = 0; g < shared.size(); g++) {
         const std::vector<int>& members = shared[g].members;
         int run;
-        const int parts = cut_up(0, shared[g].prefix, run);
+        const int parts = cut_up(height, 0, shared[g].prefix, run);
         for (size_t m = 0; m < members.size();) {
             AttendItem it{0, 0, 0, 0, plan.parts, static_cast<int>(plan.joins.size()), 0, INT_MAX - 1024, 0,
                           seqs[static_cast<size_t>(members[m])].table, static_cast<int>(plan.maps.size()), 0};

@@ -229,40 +229,31 @@ __device__ __forceinline__ unsigned bounded(unsigned e) {
     return (e & (C::kInf << 16)) == (C::kInf << 16) ? e & 0x0000FFFFu : e;
 }
 
-template <int TYPE, int DH, int TILES>
-__device__ __forceinline__ void add_unbounded(Granule<TYPE, DH>& g, const unsigned (&seen)[TILES], f32x4 (&o)[TILES][DH / 16]) {
+template <int TYPE, int DH>
+__device__ __forceinline__ void add_unbounded(Granule<TYPE, DH>& g, unsigned seen, f32x4 (&o)[DH / 16]) {
     using G = Granule<TYPE, DH>;
     using C = CacheType<TYPE>;
 #pragma unroll
     for (int cc = 0; cc < G::kDims; cc++) {
-        f32x4 n[TILES];
-#pragma unroll
-        for (int rt = 0; rt < TILES; rt++) n[rt] = f32x4{0, 0, 0, 0};
+        f32x4 n{0, 0, 0, 0};
         if constexpr (G::kWide) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float e = __uint_as_float(g.v[i][cc]);
                 const float w = e - e == 0.0f ? 0.0f : e > 0.0f ? 1.0f : e < 0.0f ? 64.0f : 4096.0f;
-#pragma unroll
-                for (int rt = 0; rt < TILES; rt++)
-                    n[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, static_cast<float>((seen[rt] >> i) & 1u), n[rt], 0, 0, 0);
+                n = __builtin_amdgcn_mfma_f32_16x16x4f32(w, static_cast<float>((seen >> i) & 1u), n, 0, 0, 0);
             }
         } else {
             u32x4 a = value_operand(g.v, cc / 2, cc & 1);
 #pragma unroll
             for (int w = 0; w < 4; w++) a[w] = unbounded_kind<TYPE>(a[w]);
+            u32x4 b;
 #pragma unroll
-            for (int rt = 0; rt < TILES; rt++) {
-                u32x4 b;
-#pragma unroll
-                for (int w = 0; w < 4; w++) b[w] = ((seen[rt] >> (2 * w)) & 1u) * C::kOne | ((seen[rt] >> (2 * w + 1)) & 1u) * (C::kOne << 16);
-                n[rt] = C::mfma(a, b, n[rt]);
-            }
+            for (int w = 0; w < 4; w++) b[w] = ((seen >> (2 * w)) & 1u) * C::kOne | ((seen >> (2 * w + 1)) & 1u) * (C::kOne << 16);
+            n = C::mfma(a, b, n);
         }
 #pragma unroll
-        for (int rt = 0; rt < TILES; rt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[rt][cc][i] += unbounded_sum(n[rt][i]);
+        for (int i = 0; i < 4; i++) o[cc][i] += unbounded_sum(n[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4 * G::kBlocks; i++)
@@ -447,13 +438,13 @@ __device__ __forceinline__ AttendJoin first_join(const AttendParams& p, const At
 // Wavefronts of a workgroup: as many as take 128 positions at a time (fp32, one token: 64 sequences of up to 2 k positions
 // 88 us, with four 91; bf16 and fp16: 32 sequences at a window of 1024, heads of 80, 15.6 us, with eight 19.2; one of
 // 128 k positions 61 and 59), where 256 registers hold what one needs.
-constexpr int attend_waves(int type, int dh, int tiles) { return type == kCacheF32 && dh * tiles <= 128 ? 8 : 4; }
+constexpr int attend_waves(int type, int dh) { return type == kCacheF32 && dh <= 128 ? 8 : 4; }
 
-// Tiles of 16 TILES rows; the wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
+// Tiles of 16 rows; the wavefronts of a workgroup share the positions, granule by granule, and meet at the end.
 // A tile whose positions were dealt to several workgroups is finished by the last of them to arrive.
-template <int TYPE, int DH, bool FULL, int TILES>
-__global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 64 ? 4 : 1) void attend_rows_kernel(const AttendParams p) {
-    constexpr int kAttendWaves = attend_waves(TYPE, DH, TILES);
+template <int TYPE, int DH, bool FULL>
+__global__ __launch_bounds__(64 * attend_waves(TYPE, DH), DH <= 64 ? 4 : 1) void attend_rows_kernel(const AttendParams p) {
+    constexpr int kAttendWaves = attend_waves(TYPE, DH);
     using C = CacheType<TYPE>;
     using T = typename C::T;
     using G = Granule<TYPE, DH>;
@@ -470,47 +461,38 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
     const int quarter = lane >> 4;
 
     // the rows' queries, as the first product's second operand
-    unsigned q[TILES][G::kKeyWords];
-    int pos[TILES];
+    unsigned q[G::kKeyWords];
+    const bool row = (lane & 15) < it.rows;
+    // (a map's rows are of several sequences, all of them behind all of the positions)
+    const int r = !row ? 0 : it.map >= 0 ? p.maps[it.map + (lane & 15)] : it.r0 + (lane & 15);
+    const int token = r / p.group, h = r % p.group;
+    const int pos = !row ? -1 : it.map >= 0 ? it.first : it.first + token;
+    const T* from = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
 #pragma unroll
-    for (int rt = 0; rt < TILES; rt++) {
-        const bool row = 16 * rt + (lane & 15) < it.rows;
-        // (a map's rows are of several sequences, all of them behind all of the positions)
-        const int r = !row ? 0 : it.map >= 0 ? p.maps[it.map + 16 * rt + (lane & 15)] : it.r0 + 16 * rt + (lane & 15);
-        const int token = r / p.group, h = r % p.group;
-        pos[rt] = !row ? -1 : it.map >= 0 ? it.first : it.first + token;
-        const T* from = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
+    for (int c = 0; c < G::kKeyWords / 4; c++) {
+        const int dim = 4 * G::kQuarter * c + G::kQuarter * quarter;
+        u32x4 w{0, 0, 0, 0};
+        if (row && (FULL || dim < p.cache.dim)) {
+            if (p.vector_rows) {
+                w = *reinterpret_cast<const u32x4*>(from + dim);
+            } else if constexpr (G::kWide) {
 #pragma unroll
-        for (int c = 0; c < G::kKeyWords / 4; c++) {
-            const int dim = 4 * G::kQuarter * c + G::kQuarter * quarter;
-            u32x4 w{0, 0, 0, 0};
-            if (row && (FULL || dim < p.cache.dim)) {
-                if (p.vector_rows) {
-                    w = *reinterpret_cast<const u32x4*>(from + dim);
-                } else if constexpr (G::kWide) {
+                for (int e = 0; e < 4; e++) w[e] = __float_as_uint(from[dim + e]);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = __float_as_uint(from[dim + e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        w[e / 2] |= static_cast<unsigned>(__builtin_bit_cast(unsigned short, from[dim + e])) << (16 * (e & 1));
-                }
+                for (int e = 0; e < 8; e++)
+                    w[e / 2] |= static_cast<unsigned>(__builtin_bit_cast(unsigned short, from[dim + e])) << (16 * (e & 1));
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) q[rt][4 * c + e] = w[e];
         }
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[4 * c + e] = w[e];
     }
     const int first = it.first + it.r0 / p.group, final = it.first + (it.r0 + it.rows - 1) / p.group;
 
-    f32x4 o[TILES][kDims];
-    float m[TILES], l[TILES];
+    f32x4 o[kDims];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < TILES; rt++) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.0f;
-#pragma unroll
-        for (int cc = 0; cc < kDims; cc++) o[rt][cc] = f32x4{0, 0, 0, 0};
-    }
+    for (int cc = 0; cc < kDims; cc++) o[cc] = f32x4{0, 0, 0, 0};
 
     Granule<TYPE, DH> now, next;
     int pages[G::kBlocks];
@@ -529,38 +511,38 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
 
         // does a mask cut this granule?
         const bool cut = at + G::kTokens > it.k1 || (p.causal && at + G::kTokens - 1 > first) || (p.window > 0 && at <= final - p.window);
-        float z[TILES][4 * G::kBlocks];
+        float z[4 * G::kBlocks];
 #pragma unroll
-        for (int rt = 0; rt < TILES; rt++)
+        for (int b = 0; b < G::kBlocks; b++) {
+            f32x4 acc{0, 0, 0, 0};
+            if constexpr (G::kWide) {
+                // 64 dims to a chain of products, chains added in fp32: one chain of 256 dims is off by three times a sum in pairs
 #pragma unroll
-            for (int b = 0; b < G::kBlocks; b++) {
-                f32x4 acc{0, 0, 0, 0};
-                if constexpr (G::kWide) {
+                for (int from = 0; from < G::kKeyWords; from += 16) {
+                    f32x4 chain{0, 0, 0, 0};
 #pragma unroll
-                    for (int w = 0; w < G::kKeyWords; w++)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][w]), __uint_as_float(q[rt][w]), acc, 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int w = 0; w < G::kKeyWords; w += 4)
-                        acc = C::mfma(u32x4{now.k[b][w], now.k[b][w + 1], now.k[b][w + 2], now.k[b][w + 3]},
-                                      u32x4{q[rt][w], q[rt][w + 1], q[rt][w + 2], q[rt][w + 3]}, acc);
+                    for (int w = from; w < from + 16; w++)
+                        chain = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][w]), __uint_as_float(q[w]), chain, 0, 0, 0);
+                    acc = from == 0 ? chain : acc + chain;
                 }
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) z[rt][4 * b + i] = acc[i];
+                for (int w = 0; w < G::kKeyWords; w += 4)
+                    acc = C::mfma(u32x4{now.k[b][w], now.k[b][w + 1], now.k[b][w + 2], now.k[b][w + 3]},
+                                  u32x4{q[w], q[w + 1], q[w + 2], q[w + 3]}, acc);
             }
-        unsigned seen[TILES];
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[4 * b + i] = acc[i];
+        }
+        unsigned seen = 0;
         bool hidden = false;
         if (cut) {
 #pragma unroll
-            for (int rt = 0; rt < TILES; rt++) {
-                seen[rt] = 0;
-#pragma unroll
-                for (int i = 0; i < 4 * G::kBlocks; i++) {
-                    const int t = at + 16 * (i / 4) + 4 * quarter + (i & 3);
-                    const bool see = t < it.k1 && (!p.causal || t <= pos[rt]) && (p.window <= 0 || t > pos[rt] - p.window);
-                    z[rt][i] = see ? z[rt][i] : -INFINITY;
-                    seen[rt] |= see ? 1u << i : 0u;
-                }
+            for (int i = 0; i < 4 * G::kBlocks; i++) {
+                const int t = at + 16 * (i / 4) + 4 * quarter + (i & 3);
+                const bool see = t < it.k1 && (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window);
+                z[i] = see ? z[i] : -INFINITY;
+                seen |= see ? 1u << i : 0u;
             }
             // places behind the last position hold anything; a position that some rows may not see is looked at
 #pragma unroll
@@ -573,55 +555,47 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
                 }
             }
         }
+        float top = z[0];
 #pragma unroll
-        for (int rt = 0; rt < TILES; rt++) {
-            float top = z[rt][0];
+        for (int i = 1; i < 4 * G::kBlocks; i++) top = fmaxf(top, z[i]);
+        top = __fmul_rn(row_max(top), p.scale);
+        if (__any(top > m)) {
+            const float keep = top > m ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            m = fmaxf(m, top);
+            l *= keep;
 #pragma unroll
-            for (int i = 1; i < 4 * G::kBlocks; i++) top = fmaxf(top, z[rt][i]);
-            top = __fmul_rn(row_max(top), p.scale);
-            if (__any(top > m[rt])) {
-                const float keep = top > m[rt] ? __builtin_amdgcn_exp2f(m[rt] - top) : 1.0f;
-                m[rt] = fmaxf(m[rt], top);
-                l[rt] *= keep;
-#pragma unroll
-                for (int cc = 0; cc < kDims; cc++) o[rt][cc] *= keep;
-            }
-            const float base = m[rt] == -INFINITY ? 0.0f : m[rt] - C::kLift;
-            float scale = p.scale;
-            if (__any(fabsf(base) > kFusedTop)) {
-                scale = 1.0f;
-#pragma unroll
-                for (int i = 0; i < 4 * G::kBlocks; i++) z[rt][i] = __fmul_rn(z[rt][i], p.scale);
-            }
-#pragma unroll
-            for (int i = 0; i < 4 * G::kBlocks; i++) {
-                z[rt][i] = __builtin_amdgcn_exp2f(fmaf(z[rt][i], scale, -base));
-                l[rt] += z[rt][i];
-            }
+            for (int cc = 0; cc < kDims; cc++) o[cc] *= keep;
         }
-        if (cut && __any(hidden)) add_unbounded<TYPE, DH, TILES>(now, seen, o);  // (behind the correction: infinity * 0 is none)
+        const float base = m == -INFINITY ? 0.0f : m - C::kLift;
+        float scale = p.scale;
+        if (__any(fabsf(base) > kFusedTop)) {
+            scale = 1.0f;
+#pragma unroll
+            for (int i = 0; i < 4 * G::kBlocks; i++) z[i] = __fmul_rn(z[i], p.scale);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * G::kBlocks; i++) {
+            z[i] = __builtin_amdgcn_exp2f(fmaf(z[i], scale, -base));
+            l += z[i];
+        }
+        if (cut && __any(hidden)) add_unbounded<TYPE, DH>(now, seen, o);  // (behind the correction: infinity * 0 is none)
         if constexpr (G::kWide) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int cc = 0; cc < kDims; cc++)
-#pragma unroll
-                    for (int rt = 0; rt < TILES; rt++)
-                        o[rt][cc] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.v[i][cc]), z[rt][i], o[rt][cc], 0, 0, 0);
+                    o[cc] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.v[i][cc]), z[i], o[cc], 0, 0, 0);
         } else {
             // probabilities in the cache's type: off by half a step of theirs each, at random, which is what the outputs'
             // own rounding is
-            u32x4 prob[TILES];
+            u32x4 prob;
 #pragma unroll
-            for (int rt = 0; rt < TILES; rt++)
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-                    prob[rt][w] = __builtin_bit_cast(unsigned, typename C::V2{static_cast<T>(z[rt][2 * w]), static_cast<T>(z[rt][2 * w + 1])});
+            for (int w = 0; w < 4; w++)
+                prob[w] = __builtin_bit_cast(unsigned, typename C::V2{static_cast<T>(z[2 * w]), static_cast<T>(z[2 * w + 1])});
 #pragma unroll
             for (int cc = 0; cc < kDims; cc++) {
                 const u32x4 a = value_operand(now.v, cc / 2, cc & 1);
-#pragma unroll
-                for (int rt = 0; rt < TILES; rt++) o[rt][cc] = C::mfma(a, prob[rt], o[rt][cc]);
+                o[cc] = C::mfma(a, prob, o[cc]);
             }
         }
         now = next;
@@ -629,58 +603,54 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH, TILES), DH * TILES <= 6
     }
 
     const bool only = it.joins == 0;
-    constexpr int kBlock = 16 * TILES * kPad;  // floats of a part
+    constexpr int kBlock = 16 * kPad;  // floats of a part
     float* const part = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     constexpr int kChunks = DH / 4;  // of a row
-#pragma unroll
-    for (int rt = 0; rt < TILES; rt++) {
-        if (16 * rt >= it.rows) break;
-        const float sum = row_sum(l[rt]);
-        if (quarter == 0) {
-            tops[wave][lane] = m[rt];
-            sums[wave][lane] = sum;
-        }
-        __syncthreads();
-        const int own = lane & 15;
-        float top = tops[0][own];
-#pragma unroll
-        for (int w = 1; w < kAttendWaves; w++) top = fmaxf(top, tops[w][own]);
-        const float keep = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int cc = 0; cc < kDims; cc++) meet[wave][own][(4 * quarter + i) * kDims + cc] = o[rt][cc][i] * keep;
-        __syncthreads();
-        for (int e = threadIdx.x; e < 16 * kChunks; e += 64 * kAttendWaves) {
-            const int row = e / kChunks, dim = e % kChunks * 4;
-            if (16 * rt + row >= it.rows) break;
-            float high = tops[0][row], total = 0.0f;
-#pragma unroll
-            for (int w = 1; w < kAttendWaves; w++) high = fmaxf(high, tops[w][row]);
-            f32x4 out{0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < kAttendWaves; w++) {
-                total += sums[w][row] * (tops[w][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[w][row] - high));
-                out += *reinterpret_cast<const f32x4*>(&meet[w][row][dim]);
-            }
-            if (only) {
-                const int r = it.r0 + 16 * rt + row;
-                if (FULL || dim < p.cache.dim)
-                    store_four<TYPE>(p.out, (it.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
-                                     p.vector_rows, out / total);
-            } else {
-                const __amdgpu_buffer_rsrc_t rs = make_buffer(part, kBlock * 4);
-                const int base = (16 * rt + row) * kPad * 4;
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, out), rs, base + dim * 4, 0, kAuxDeviceScope);
-                if (dim == 0)
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, f32x4{high, total, 0.0f, 0.0f}), rs, base + DH * 4, 0, kAuxDeviceScope);
-            }
-        }
-        __syncthreads();
+    const float sum = row_sum(l);
+    if (quarter == 0) {
+        tops[wave][lane] = m;
+        sums[wave][lane] = sum;
     }
+    __syncthreads();
+    const int own = lane & 15;
+    float top = tops[0][own];
+#pragma unroll
+    for (int w = 1; w < kAttendWaves; w++) top = fmaxf(top, tops[w][own]);
+    const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int cc = 0; cc < kDims; cc++) meet[wave][own][(4 * quarter + i) * kDims + cc] = o[cc][i] * keep;
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * kChunks; e += 64 * kAttendWaves) {
+        const int row = e / kChunks, dim = e % kChunks * 4;
+        if (row >= it.rows) break;
+        float high = tops[0][row], total = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kAttendWaves; w++) high = fmaxf(high, tops[w][row]);
+        f32x4 out{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kAttendWaves; w++) {
+            total += sums[w][row] * (tops[w][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[w][row] - high));
+            out += *reinterpret_cast<const f32x4*>(&meet[w][row][dim]);
+        }
+        if (only) {
+            const int r = it.r0 + row;
+            if (FULL || dim < p.cache.dim)
+                store_four<TYPE>(p.out, (it.row0 + r / p.group) * p.out.row + (head * p.group + r % p.group) * p.out.head + dim,
+                                 p.vector_rows, out / total);
+        } else {
+            const __amdgpu_buffer_rsrc_t rs = make_buffer(part, kBlock * 4);
+            const int base = row * kPad * 4;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, out), rs, base + dim * 4, 0, kAuxDeviceScope);
+            if (dim == 0)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, f32x4{high, total, 0.0f, 0.0f}), rs, base + DH * 4, 0, kAuxDeviceScope);
+        }
+    }
+    __syncthreads();
     if (only) return;
 
-    finish_parts<TYPE, DH, FULL, 16 * TILES, 64 * kAttendWaves>(p, it, mine, head, meeting, reinterpret_cast<char*>(meet));
+    finish_parts<TYPE, DH, FULL, 16, 64 * kAttendWaves>(p, it, mine, head, meeting, reinterpret_cast<char*>(meet));
 }
 
 }  // namespace gh

@@ -152,7 +152,7 @@ static int refusals() {
 // Every row of a pass gets every position that it may see from exactly one item (of its own or of a shared prefix), spans lie
 // inside the sequences, places of parts are used once, and every join knows whom it waits for.
 static int plans(unsigned seed) {
-    std::mt19937 rng(seed);
+    std::mt19937 rng(seed), more(seed + 1000);
     for (int round = 0; round < 300; round++) {
         AttendCut cut{};
         cut.group = 1 + static_cast<int>(rng() % 5);
@@ -163,6 +163,8 @@ static int plans(unsigned seed) {
         cut.workgroups = 1 << (rng() % 12);
         cut.least = 128;
         cut.most = 1 + static_cast<int>(rng() % 64);
+        cut.square = more() % 2 ? 1 << (more() % 8) : 0;
+        cut.resident = more() % 2 ? 16 << (more() % 6) : 0;
         const int T = 16;
         std::vector<PassSeq> seqs;
         std::vector<int> news;
@@ -195,6 +197,12 @@ static int plans(unsigned seed) {
             }
         }
         const AttendPlan plan = plan_attend(seqs, news, cut, cut.window == 0 ? shared : std::vector<SharedPrefix>{});
+        if (cut.resident > 0 && (cut.window != 0 || shared.empty())) {
+            size_t tiles = 0;
+            for (int n : news) tiles += static_cast<size_t>((n * cut.group + cut.height - 1) / cut.height);
+            const size_t kv = static_cast<size_t>(cut.kv_heads), most = static_cast<size_t>(cut.resident);
+            CHECK(plan.items.size() >= tiles && (tiles * kv > most || plan.items.size() * kv <= most));
+        }
         // position by position: who brings (pass row, head of the group) what
         std::map<int, std::vector<int>> brought;
         std::map<int, std::vector<std::pair<int, int>>> from;  // ... and from which place and row of it (-1: whole)

@@ -405,6 +405,27 @@ def test_many_samples_of_one_prompt(torch, dtype, heads):
     rig.check_contents(kids[:3])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", ["mha64", "grouped128", "one-key80", "dim256"])
+def test_many_samples_of_a_long_prompt(torch, dtype, heads):
+    """Prefixes of so many bytes that they are read for all members together, in several common tiles: 33 samples, among
+    them one that only shares a shorter part, beside a sequence of its own."""
+    h, kv, dim, page = HEADS[heads]
+    size = 4 if dtype == "f32" else 2
+    prompt = max(300, 50_000_000 // (33 * 2 * kv * dim * size)) // page * page + 5
+    rig = Rig(torch, dtype, heads=h, kv_heads=kv, dim=dim, page=page, pages=(2 * prompt + 40 * 128) // page + 50, seed=31)
+    a, lone = rig.add(), rig.add()
+    rig.grow([a, lone], [prompt, 290])
+    kids = [rig.fork(a) for _ in range(32)] + [rig.fork(a, prompt - page - 7)]
+    rig.grow(kids[:3], [3, 17, 1])
+    seqs = kids[:20] + [lone] + kids[20:]
+    for counts in ([1] * len(seqs), [1 + (i % 3 == 0) for i in range(len(seqs))]):
+        q = rig.grow(seqs, counts)
+        out = rig.check(seqs, counts, q, what="shared")
+        assert torch.equal(out, rig.check(seqs, counts, q, what="again"))
+    rig.check_contents(kids[:2])
+
+
 def test_long_lists_of_pages(torch):
     """More pages than a launch's own list takes: copies, reads, compaction."""
     rig = Rig(torch, "bf16", layers=2, heads=1, kv_heads=1, dim=8, page=16, pages=3200, seed=22)
