@@ -233,7 +233,8 @@ struct Cache {
             const int n = static_cast<int>(std::min<size_t>(kListed, copies.size() - at));
             CopyList list;
             std::memcpy(list.copies, copies.data() + at, sizeof(PageCopy) * static_cast<size_t>(n));
-            const int x = std::max(1, std::min(runs, 2048 / n));  // ~2048 workgroups: eight per compute unit
+            const long long pieces = static_cast<long long>(runs) * static_cast<long long>((layout.run_bytes + 4095) / 4096);
+            const int x = static_cast<int>(std::max(1ll, std::min<long long>(pieces, 2048 / n)));  // ~2048 workgroups: eight per compute unit
             hipLaunchKernelGGL(cache_copy_kernel, dim3(x, n), dim3(256), 0, stream, from, pool.at, layout.page_bytes, runs,
                                static_cast<int>(layout.run_bytes / 16), token_bytes, list);
             HIP_CHECK(hipGetLastError());

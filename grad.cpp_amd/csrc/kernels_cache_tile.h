@@ -6,6 +6,11 @@
 // Shared memory holds K and V as they are in the pages, position by position, with a stride that spreads what a product's
 // lanes read over all banks: K rows are read 16 bytes to a lane (eight lanes to a cycle: rows 16 bytes apart modulo 128), V through
 // the transposing read, which hands a lane four positions of one dim (16 lanes to a cycle: four rows 32 bytes apart modulo 128).
+//
+// Bound by the products and the softmax between them, which a wavefront does in turn: four sequences of 2048 rows onto 6 k positions,
+// 32/8 heads of 128 in bf16, 962 GFLOP: 1.07 to 1.16 ms, 830 to 900 TFLOP/s where a large plain product reaches 1124; of
+// a SIMD's cycles 36 % have a product under way and 38 % a vector instruction.  A position that a wavefront fetches itself would be fetched four
+// times: 3.6 ms with the 16-row tiles' kernel.
 #pragma once
 
 #include "kernels_attn.h"
