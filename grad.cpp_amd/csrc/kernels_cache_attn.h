@@ -305,8 +305,9 @@ struct Folded {
         const float up = fmaxf(top, high);
         const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
         const float take = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(high - up);
-        total = total * keep + sum * take;
-        out = out * keep + o * take;
+        total = fmaf(total, keep, sum * take);
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = fmaf(out[i], keep, o[i] * take);
         top = up;
     }
 };
@@ -336,7 +337,9 @@ __device__ __forceinline__ void join_parts(const AttendParams& p, const AttendIt
         return it.join + j;
     };
     const int most = mine.shared_parts + mine.parts;  // (members' own parts of a prefix's rest: one or a few)
-    const int shares = max(1, min(THREADS / elements, (most + kDeep - 1) / kDeep));  // of the parts
+    // shares of the parts.  (One where a prefix is among them: its items and the members' own end in any order, have different rows,
+    // and have to fold alike.)
+    const int shares = MANY || mine.shared_parts > 0 ? 1 : max(1, min(THREADS / elements, (most + kDeep - 1) / kDeep));
     const int share = static_cast<int>(threadIdx.x) / elements;                      // (0 where there is one)
     const auto write = [&](int e, const f32x4& out, float total) {
         const int dim = e % kChunks * 4, j = join_of(e);

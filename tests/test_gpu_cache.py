@@ -426,6 +426,21 @@ def test_many_samples_of_a_long_prompt(torch, dtype, heads):
     rig.check_contents(kids[:2])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_contexts_beside_a_chunk(torch, dtype):
+    """Single tokens over so much that they get a launch of their own beside the chunk's: with a common prefix (no window)
+    and without (a window), and the other way round, a chunk of one of them."""
+    rig = Rig(torch, dtype, heads=16, kv_heads=8, dim=128, page=64, pages=180, seed=32)
+    a, chunk = rig.add(), rig.add()
+    rig.grow([a, chunk], [5500, 70])
+    kids = [rig.fork(a) for _ in range(17)]
+    for seqs, counts in ((kids[:9] + [chunk] + kids[9:], [1] * 9 + [90] + [1] * 8), ([chunk] + kids, [3, 1, 75] + [1] * 15)):
+        q = rig.grow(seqs, counts)
+        for window in (0, 5200):
+            out = rig.check(seqs, counts, q, window=window, what=f"window {window}")
+            assert torch.equal(out, rig.check(seqs, counts, q, window=window, what="again"))
+
+
 def test_long_lists_of_pages(torch):
     """More pages than a launch's own list takes: copies, reads, compaction."""
     rig = Rig(torch, "bf16", layers=2, heads=1, kv_heads=1, dim=8, page=16, pages=3200, seed=22)
