@@ -359,58 +359,39 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
 
 // ---------------------------------------------------------------------- fp32
 //
-// The fp32 matrix instructions have a sixteenth of the 16-bit ones' rate, so fp32 operands are taken as pairs of fp16 parts,
-// x s = high + low with a power of two s that brings the largest of a query, or of a tile's keys or values, into
-// [2^14, 2^15): each part has 11 bits and the second a sign, so a pair is off by 2^-24 of its value, and by 2^-38 of the
-// largest where a value is less than 2^-16 of it.  Three of the four products of parts are formed, the fourth is below 2^-22
-// of the whole and of either sign.  (Ootomo and Yokota, 2022, published the scheme.)  The matrix core cuts sums off where
-// fp32 rounds: the small products are summed first, a tile of positions from zero, and added to the running output in fp32.
-// Probabilities are kept 2^14 times as large, so they are such values as they are.
-// What does not fit (rows of keys or values more than 2^16 below the tile's largest, maxima beyond 2^+-60, infinities, NaN) goes
-// row by row.  (Three bf16 parts, six products: 181 us for 16 x 1024 rows of 12 heads of 64 where pairs take 147.)
+// The fp32 matrix instructions have a sixteenth of the 16-bit ones' rate, so fp32 operands, probabilities among them, are taken as
+// sums of three bf16 parts, x = high + middle + low, each the rest rounded to bf16: the last one is exact.  The parts of an element are
+// its own: nothing is lost whatever its neighbours are, and nothing overflows (below 2^-103 low parts are subnormal: at
+// most 2^-125 times the other factor is lost).  Six of the nine products of parts are formed; the three left out are below
+// 2^-26 of the whole.  The matrix core cuts sums off where fp32 rounds, so the small products are summed before
+// the large ones, whose cut-off bits they would share, a tile of positions from zero, and added to the running output in fp32.
+// Infinities and NaN have no parts: their items go row by row.  16 x 1024 rows of 12 heads of 64: 187 us, 138 TFLOP/s where plain fp32
+// products reach 153.  (Pairs of fp16 parts, three products, take 150, but need a power of two that neighbours share: an element
+// 2^24 below the largest of its row or tile has lost digits, one 2^40 below it all of them.)
 
-struct Pair {
-    u32x2 high, low;  // of four values, fp16
+struct Parts {
+    u32x2 high, middle, low;  // of four values, bf16
 };
 
-__device__ __forceinline__ Pair two_parts(const f32x4& x, float scale) {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    Pair p;
+// `taint` becomes NaN if any value is infinite, NaN or rounded up to infinity: its rest is.
+__device__ __forceinline__ Parts three_parts(const f32x4& x, float& taint) {
+    Parts p;
 #pragma unroll
     for (int w = 0; w < 2; w++) {
-        const f32x2 y{x[2 * w] * scale, x[2 * w + 1] * scale};
-        const f16x2 high = __builtin_convertvector(y, f16x2);
-        const f32x2 rest{y.x - static_cast<float>(high.x), y.y - static_cast<float>(high.y)};
-        p.high[w] = __builtin_bit_cast(unsigned, high);
-        p.low[w] = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
+        float a = x[2 * w], b = x[2 * w + 1];
+        const auto part = [&] {  // of both, which keep their rests
+            const unsigned two = __builtin_bit_cast(unsigned, CacheType<kCacheBf16>::V2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
+            a -= __uint_as_float(two << 16);
+            b -= __uint_as_float(two & 0xFFFF0000u);
+            return two;
+        };
+        p.high[w] = part();
+        p.middle[w] = part();
+        taint = fmaf(a, 0.0f, fmaf(b, 0.0f, taint));
+        p.low[w] = __builtin_bit_cast(unsigned, CacheType<kCacheBf16>::V2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
     }
     return p;
 }
-
-// The largest magnitude of four values, as bits: ordered like the values, infinities and NaN above all numbers.
-__device__ __forceinline__ unsigned size_bits(const f32x4& x) {
-    unsigned b[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) b[e] = __float_as_uint(x[e]) & 0x7FFFFFFFu;
-    return max(max(b[0], b[1]), max(b[2], b[3]));
-}
-// ... over LANES consecutive lanes (16, 32 or 64), in all of them.
-template <int LANES>
-__device__ __forceinline__ unsigned span_max(unsigned v) {
-    v = max(v, static_cast<unsigned>(dpp_move_int<0xB1, 0xF>(static_cast<int>(v))));
-    v = max(v, static_cast<unsigned>(dpp_move_int<0x4E, 0xF>(static_cast<int>(v))));
-    v = max(v, static_cast<unsigned>(dpp_move_int<0x141, 0xF>(static_cast<int>(v))));
-    v = max(v, static_cast<unsigned>(dpp_move_int<0x140, 0xF>(static_cast<int>(v))));
-    if constexpr (LANES >= 32) v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), 16)));
-    if constexpr (LANES >= 64) v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), 32)));
-    return v;
-}
-
-// Whether pairs hold values whose largest has these bits, and the exponent that the largest is brought to 2^14 by.
-__device__ __forceinline__ bool pairs_hold(unsigned bits) { return bits == 0u || (bits >> 23 >= 67u && bits >> 23 <= 187u); }
-__device__ __forceinline__ int pair_shift(unsigned bits) { return bits == 0u ? 0 : 14 + 127 - static_cast<int>(bits >> 23); }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<unsigned>(e + 127) << 23); }
 
 template <int DH, bool FULL, int TOKENS>
 __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide_kernel(const AttendParams p) {
@@ -419,10 +400,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     constexpr int kUnits = DH / 4;                               // of four values in a row
     constexpr int kLoads = TOKENS * kUnits / (64 * kTileWaves);  // of a thread, for K and for V
     constexpr int kBlocks = TOKENS / 32, kSteps = DH / 16, kWide = DH / 32;
-    constexpr float kLift = 14.0f;  // of the probabilities
-    __shared__ __align__(16) char keys[2 * kKeys];
-    __shared__ __align__(16) char values[2 * kValues];
-    __shared__ unsigned largest[2][kTileWaves];  // of the tile's keys and values, by wavefront
+    __shared__ __align__(16) char keys[3 * kKeys];
+    __shared__ __align__(16) char values[3 * kValues];
     __shared__ Meeting meeting;
     __shared__ unsigned odd;
 
@@ -438,44 +417,30 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     const int token = row ? r / p.group : 0, h = row ? r % p.group : 0;
     const int pos = row ? it.first + token : -1;
     const float* const query = reinterpret_cast<const float*>(p.q.at) + (it.row0 + token) * p.q.row + (head * p.group + h) * p.q.head;
-    u32x4 q[2][kSteps];
-    float own_scale;  // of the scores, with the query's power of two taken back
-    bool bad;
-    {
-        f32x4 x[kSteps][2];
-        unsigned bits = 0;
+    u32x4 q[3][kSteps];
+    float taint = 0.0f;
 #pragma unroll
-        for (int c = 0; c < kSteps; c++) {
-            const int dim = 16 * c + 8 * half;
+    for (int c = 0; c < kSteps; c++) {
+        const int dim = 16 * c + 8 * half;
 #pragma unroll
-            for (int side = 0; side < 2; side++) {
-                x[c][side] = f32x4{0, 0, 0, 0};
-                if (row && (FULL || dim < p.cache.dim)) {
-                    if (p.vector_rows) {
-                        x[c][side] = *reinterpret_cast<const f32x4*>(query + dim + 4 * side);
-                    } else {
+        for (int side = 0; side < 2; side++) {
+            f32x4 x{0, 0, 0, 0};
+            if (row && (FULL || dim < p.cache.dim)) {
+                if (p.vector_rows) {
+                    x = *reinterpret_cast<const f32x4*>(query + dim + 4 * side);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x[c][side][e] = query[dim + 4 * side + e];
-                    }
+                    for (int e = 0; e < 4; e++) x[e] = query[dim + 4 * side + e];
                 }
-                bits = max(bits, size_bits(x[c][side]));
+            }
+            const Parts parts = three_parts(x, taint);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                q[0][c][2 * side + w] = parts.high[w];
+                q[1][c][2 * side + w] = parts.middle[w];
+                q[2][c][2 * side + w] = parts.low[w];
             }
         }
-        bits = max(bits, static_cast<unsigned>(__shfl_xor(static_cast<int>(bits), 32)));
-        bad = !pairs_hold(bits);
-        const int shift = bad ? 0 : pair_shift(bits);
-        own_scale = p.scale * power_of_two(-shift);
-#pragma unroll
-        for (int c = 0; c < kSteps; c++)
-#pragma unroll
-            for (int side = 0; side < 2; side++) {
-                const Pair parts = two_parts(x[c][side], power_of_two(shift));
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    q[0][c][2 * side + w] = parts.high[w];
-                    q[1][c][2 * side + w] = parts.low[w];
-                }
-            }
     }
     const int rows_here = min(32, it.rows - 32 * wave);
     const int first = it.first + (it.r0 + 32 * wave) / p.group;
@@ -519,54 +484,21 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     fetch(it.k0);
     look(it.k0 + TOKENS);
     for (int at = it.k0; at < it.k1; at += TOKENS) {
-        // the largest key and value of the tile, and of this thread's rows
-        unsigned key_rows[kLoads], value_rows[kLoads], key_bits = 0, value_bits = 0;
-#pragma unroll
-        for (int i = 0; i < kLoads; i++) {
-            key_rows[i] = span_max<kUnits>(size_bits(kr[i]));
-            value_rows[i] = span_max<kUnits>(size_bits(vr[i]));
-            key_bits = max(key_bits, key_rows[i]);
-            value_bits = max(value_bits, value_rows[i]);
-        }
-        if constexpr (kUnits < 32) {
-            key_bits = max(key_bits, static_cast<unsigned>(__shfl_xor(static_cast<int>(key_bits), 16)));
-            value_bits = max(value_bits, static_cast<unsigned>(__shfl_xor(static_cast<int>(value_bits), 16)));
-        }
-        if constexpr (kUnits < 64) {
-            key_bits = max(key_bits, static_cast<unsigned>(__shfl_xor(static_cast<int>(key_bits), 32)));
-            value_bits = max(value_bits, static_cast<unsigned>(__shfl_xor(static_cast<int>(value_bits), 32)));
-        }
-        if (lane == 0) {
-            largest[0][wave] = key_bits;
-            largest[1][wave] = value_bits;
-        }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kTileWaves; w++) {
-            key_bits = max(key_bits, largest[0][w]);
-            value_bits = max(value_bits, largest[1][w]);
-        }
-        key_bits = __builtin_amdgcn_readfirstlane(key_bits);
-        value_bits = __builtin_amdgcn_readfirstlane(value_bits);
-        bad = bad || !pairs_hold(key_bits) || !pairs_hold(value_bits);
-#pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            bad = bad || (key_rows[i] != 0u && (key_rows[i] >> 23) + 16u < key_bits >> 23);
-            bad = bad || (value_rows[i] != 0u && (value_rows[i] >> 23) + 16u < value_bits >> 23);
-        }
-        const int key_shift = pairs_hold(key_bits) ? pair_shift(key_bits) : 0, value_shift = pairs_hold(value_bits) ? pair_shift(value_bits) : 0;
-#pragma unroll
-        for (int i = 0; i < kLoads; i++) {
-            const Pair k = two_parts(kr[i], power_of_two(key_shift)), v = two_parts(vr[i], power_of_two(value_shift));
+            const Parts k = three_parts(kr[i], taint), v = three_parts(vr[i], taint);
             const int unit = 64 * (kTileWaves * i + wave) + lane;
             char* const to_k = keys + unit / kUnits * kKeyRow + unit % kUnits * 8;
             char* const to_v = values + unit / kUnits * kValueRow + unit % kUnits * 8;
             *reinterpret_cast<u32x2*>(to_k) = k.high;
-            *reinterpret_cast<u32x2*>(to_k + kKeys) = k.low;
+            *reinterpret_cast<u32x2*>(to_k + kKeys) = k.middle;
+            *reinterpret_cast<u32x2*>(to_k + 2 * kKeys) = k.low;
             *reinterpret_cast<u32x2*>(to_v) = v.high;
-            *reinterpret_cast<u32x2*>(to_v + kValues) = v.low;
+            *reinterpret_cast<u32x2*>(to_v + kValues) = v.middle;
+            *reinterpret_cast<u32x2*>(to_v + 2 * kValues) = v.low;
         }
-        if (bad) odd = 1;
+        if (taint != 0.0f) odd = 1;
         __syncthreads();
         if (__builtin_amdgcn_readfirstlane(odd)) break;  // (written again behind the next meeting only)
         if (at + TOKENS < it.k1) {
@@ -581,20 +513,26 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
             f32x16 acc;
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[i] = 0.0f;
-            if constexpr (kSteps <= 8) {  // registers hold the parts of all dims: small products first, then the large ones
-                u32x4 k[2][kSteps];
+            if constexpr (kSteps <= 4) {  // registers hold the parts of all dims: small products first, then the large ones
+                u32x4 k[3][kSteps];
 #pragma unroll
                 for (int c = 0; c < kSteps; c++)
 #pragma unroll
-                    for (int part = 0; part < 2; part++)
+                    for (int part = 0; part < 3; part++)
                         k[part][c] = *reinterpret_cast<const u32x4*>(key_at + part * kKeys + b * 32 * kKeyRow + c * 32);
 #pragma unroll
                 for (int c = 0; c < kSteps; c++) {
-                    acc = mfma32<kCacheF16>(k[1][c], q[0][c], acc);
-                    acc = mfma32<kCacheF16>(k[0][c], q[1][c], acc);
+                    acc = mfma32<kCacheBf16>(k[2][c], q[0][c], acc);
+                    acc = mfma32<kCacheBf16>(k[1][c], q[1][c], acc);
+                    acc = mfma32<kCacheBf16>(k[0][c], q[2][c], acc);
                 }
 #pragma unroll
-                for (int c = 0; c < kSteps; c++) acc = mfma32<kCacheF16>(k[0][c], q[0][c], acc);
+                for (int c = 0; c < kSteps; c++) {
+                    acc = mfma32<kCacheBf16>(k[1][c], q[0][c], acc);
+                    acc = mfma32<kCacheBf16>(k[0][c], q[1][c], acc);
+                }
+#pragma unroll
+                for (int c = 0; c < kSteps; c++) acc = mfma32<kCacheBf16>(k[0][c], q[0][c], acc);
             } else {  // ... or the two have sums of their own
                 f32x16 small;
 #pragma unroll
@@ -602,10 +540,14 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
 #pragma unroll
                 for (int c = 0; c < kSteps; c++) {
                     const char* k = key_at + b * 32 * kKeyRow + c * 32;
-                    const u32x4 k0 = *reinterpret_cast<const u32x4*>(k), k1 = *reinterpret_cast<const u32x4*>(k + kKeys);
-                    small = mfma32<kCacheF16>(k1, q[0][c], small);
-                    small = mfma32<kCacheF16>(k0, q[1][c], small);
-                    acc = mfma32<kCacheF16>(k0, q[0][c], acc);
+                    const u32x4 k0 = *reinterpret_cast<const u32x4*>(k), k1 = *reinterpret_cast<const u32x4*>(k + kKeys),
+                                k2 = *reinterpret_cast<const u32x4*>(k + 2 * kKeys);
+                    small = mfma32<kCacheBf16>(k2, q[0][c], small);
+                    small = mfma32<kCacheBf16>(k1, q[1][c], small);
+                    small = mfma32<kCacheBf16>(k0, q[2][c], small);
+                    small = mfma32<kCacheBf16>(k1, q[0][c], small);
+                    small = mfma32<kCacheBf16>(k0, q[1][c], small);
+                    acc = mfma32<kCacheBf16>(k0, q[0][c], acc);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[i] += small[i];
@@ -623,7 +565,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
                     z[b][i] = see ? z[b][i] : -INFINITY;
                 }
         }
-        float scale = own_scale * power_of_two(-key_shift);
+        float scale = p.scale;
         float top = z[0][0];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
@@ -639,7 +581,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= keep;
         }
-        const float base = m == -INFINITY ? 0.0f : m - kLift;
+        const float base = m == -INFINITY ? 0.0f : m;
         if (__any(fabsf(base) > kFusedTop)) {
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
@@ -647,7 +589,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
                 for (int i = 0; i < 16; i++) z[b][i] = __fmul_rn(z[b][i], scale);
             scale = 1.0f;
         }
-        u32x4 prob[2][kBlocks][2];
+        u32x4 prob[3][kBlocks][2];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
@@ -658,23 +600,24 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
                     e[i] = __builtin_amdgcn_exp2f(fmaf(z[b][4 * g + i], scale, -base));
                     l += e[i];
                 }
-                const Pair parts = two_parts(e, 1.0f);
+                float none = 0.0f;
+                const Parts parts = three_parts(e, none);
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
                     prob[0][b][g / 2][2 * (g & 1) + w] = parts.high[w];
-                    prob[1][b][g / 2][2 * (g & 1) + w] = parts.low[w];
+                    prob[1][b][g / 2][2 * (g & 1) + w] = parts.middle[w];
+                    prob[2][b][g / 2][2 * (g & 1) + w] = parts.low[w];
                 }
             }
-        const float value_scale = power_of_two(-value_shift);
 #pragma unroll
         for (int d = 0; d < kWide; d++) {
-            u32x4 v[2][kBlocks][2];
+            u32x4 v[3][kBlocks][2];
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int part = 0; part < 2; part++) {
+                    for (int part = 0; part < 3; part++) {
                         const char* from = value_at + part * kValues + (32 * b + 16 * u) * kValueRow + d * 64;
                         const u32x2 low = read_transposed(from), high = read_transposed(from + 8 * kValueRow);
                         v[part][b][u] = u32x4{low.x, low.y, high.x, high.y};
@@ -686,15 +629,23 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    acc = mfma32<kCacheF16>(v[1][b][u], prob[0][b][u], acc);
-                    acc = mfma32<kCacheF16>(v[0][b][u], prob[1][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[2][b][u], prob[0][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[1][b][u], prob[1][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[0][b][u], prob[2][b][u], acc);
                 }
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-                for (int u = 0; u < 2; u++) acc = mfma32<kCacheF16>(v[0][b][u], prob[0][b][u], acc);
+                for (int u = 0; u < 2; u++) {
+                    acc = mfma32<kCacheBf16>(v[1][b][u], prob[0][b][u], acc);
+                    acc = mfma32<kCacheBf16>(v[0][b][u], prob[1][b][u], acc);
+                }
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[d][i] = fmaf(acc[i], value_scale, o[d][i]);
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) acc = mfma32<kCacheBf16>(v[0][b][u], prob[0][b][u], acc);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] += acc[i];
         }
     }
 
@@ -704,8 +655,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     if (__builtin_amdgcn_readfirstlane(odd)) {
         rows_one_by_one<kCacheF32, DH>(p, it, table, head, 32 * wave, rows_here, part);
     } else {
-        // (sum and output are relative to 2^(m - lift))
-        leave_rows<kCacheF32, DH, FULL>(p, it, o, m - kLift, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
+        leave_rows<kCacheF32, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }
     if (only) return;
     finish_parts<kCacheF32, DH, FULL, kTileRows, 64 * kTileWaves>(p, it, mine, head, meeting, keys);

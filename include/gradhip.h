@@ -372,7 +372,9 @@ typedef struct gh_cache_opts {
     int32_t head_dim;    /* a multiple of 8, 8 to 256 */
     int32_t type;        /* GH_F32, GH_BF16, GH_F16: keys, values, queries and outputs.  Sums, maxima
                           * and exponentials are 32-bit whatever the type; with the 16-bit types
-                          * probabilities are rounded to the type before they meet the values */
+                          * probabilities are rounded to the type before they meet the values.
+                          * GH_F32's products are fp32 ones, or for many rows of a sequence sums of
+                          * products of three bf16 parts, off by less than fp32's own rounding */
     int32_t page_tokens; /* positions of a page: a power of two, 16 to 1024; 0 = 64 */
     int32_t pages;       /* of the pool, allocated at creation: 2 * layers * kv_heads * page_tokens * head_dim elements each */
     float rope_base;     /* rotary positions: pairs (2j, 2j + 1) by position * base^(-2j / head_dim), as
