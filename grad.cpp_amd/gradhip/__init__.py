@@ -7,6 +7,7 @@ library has not been built, and every compute call fails when no GPU is usable.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 
 import numpy as np
@@ -429,7 +430,7 @@ class Session:
     def store(self, cache, seq=0) -> int:
         """A new sequence of a Cache with everything that sequence `seq` of the session holds."""
         out = C.c_int32()
-        _check(load_library().gh_session_store(self._h, seq, cache._h, C.byref(out)))
+        _check(load_library().gh_session_store(self._h, _int32(seq, "sequence"), cache._h, C.byref(out)))
         cache._rows = -1
         return out.value
 
@@ -437,10 +438,11 @@ class Session:
         """Sequence b becomes the tokens ids[b], all but the last of them taken from sequence seqs[b] of a Cache; the last
         one's logits (batch, vocab)."""
         ids = np.ascontiguousarray(ids, dtype=np.int32).reshape(self.batch, -1)
-        seqs = np.ascontiguousarray(np.atleast_1d(seqs), dtype=np.int32)
-        assert seqs.shape == (self.batch,)
+        seqs = _int32s(np.atleast_1d(seqs).tolist(), "sequence")
+        if len(seqs) != self.batch:
+            raise ValueError("cache: a sequence for each of the session's")
         out = np.empty((self.batch, self.vocab), dtype=np.float32)
-        _check(load_library().gh_session_restore(self._h, cache._h, seqs.ctypes.data_as(_i32p), ids.ctypes.data_as(_i32p),
+        _check(load_library().gh_session_restore(self._h, cache._h, seqs, ids.ctypes.data_as(_i32p),
                                                  ids.shape[1], out.ctypes.data_as(_f32p)))
         return out
 
@@ -532,6 +534,22 @@ CACHE_TYPES = {"f32": 0, "bf16": 1, "f16": 2}  # GH_F32, GH_BF16, GH_F16
 _TORCH_NAMES = {"f32": "torch.float32", "bf16": "torch.bfloat16", "f16": "torch.float16"}
 
 
+def _int32(value, name):
+    """A number as an argument of 32 bits, which ctypes would cut it down to."""
+    value = operator.index(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"cache: {name} {value} is beyond 32 bits")
+    return value
+
+
+def _int32s(values, name):
+    values = list(map(operator.index, values))
+    if values:
+        _int32(min(values), name)
+        _int32(max(values), name)
+    return (C.c_int32 * len(values))(*values)
+
+
 class Cache:
     """A paged cache of keys and values (gh_cache_*): sequences of their own lengths, forked, copied, rewound and
     dropped one by one, and the attention of a pass's rows over them.
@@ -546,7 +564,9 @@ class Cache:
         self._h = None
         self._lib = load_library()
         h = _vp()
-        opts = GhCacheOpts(layers, heads, kv_heads, head_dim, CACHE_TYPES[dtype], page_tokens, pages, rope_base)
+        layers, heads, kv_heads, head_dim = (_int32(n, what) for n, what in ((layers, "layers"), (heads, "heads"), (kv_heads, "kv_heads"),
+                                                                             (head_dim, "head_dim")))
+        opts = GhCacheOpts(layers, heads, kv_heads, head_dim, CACHE_TYPES[dtype], _int32(page_tokens, "page_tokens"), _int32(pages, "pages"), rope_base)
         _check(self._lib.gh_cache_create(C.byref(opts), C.byref(h)))
         self._h = h.value
         self.layers, self.heads, self.kv_heads, self.head_dim, self.dtype = layers, heads, kv_heads, head_dim, dtype
@@ -580,7 +600,7 @@ class Cache:
 
     def length(self, seq) -> int:
         """Positions of a sequence."""
-        n = self._lib.gh_cache_length(self._h, seq)
+        n = self._lib.gh_cache_length(self._h, _int32(seq, "sequence"))
         if n < 0:
             raise IndexError(f"cache: no sequence {seq}")
         return n
@@ -594,7 +614,7 @@ class Cache:
     def fork(self, seq, length=-1) -> int:
         """A sequence that begins with seq's first `length` positions (-1: all of them), in the same pages."""
         out = C.c_int32()
-        _check(self._lib.gh_cache_fork(self._h, seq, length, C.byref(out)))
+        _check(self._lib.gh_cache_fork(self._h, _int32(seq, "sequence"), _int32(length, "length"), C.byref(out)))
         self._rows = -1
         return out.value
 
@@ -602,18 +622,18 @@ class Cache:
         """A sequence, of the cache `to` if one is named, with seq's contents in pages of its own."""
         out = C.c_int32()
         to = to or self
-        _check(self._lib.gh_cache_copy(self._h, seq, to._h, stream or None, C.byref(out)))
+        _check(self._lib.gh_cache_copy(self._h, _int32(seq, "sequence"), to._h, stream or None, C.byref(out)))
         to._rows = -1
         return out.value
 
     def truncate(self, seq, length) -> None:
         """Keeps seq's first `length` positions."""
-        _check(self._lib.gh_cache_truncate(self._h, seq, length))
+        _check(self._lib.gh_cache_truncate(self._h, _int32(seq, "sequence"), _int32(length, "length")))
         self._rows = -1
 
     def drop(self, seq) -> None:
         """Ends seq and frees the pages that nobody else holds."""
-        _check(self._lib.gh_cache_drop(self._h, seq))
+        _check(self._lib.gh_cache_drop(self._h, _int32(seq, "sequence")))
         self._rows = -1
 
     def compact(self, stream=0) -> int:
@@ -625,12 +645,15 @@ class Cache:
 
     def extend(self, seqs, counts, stream=0) -> None:
         """Opens a pass: counts[i] new positions for seqs[i].  Its rows are those positions, sequence after sequence."""
-        n = len(seqs)
-        if len(counts) != n:
+        seqs, counts = _int32s(seqs, "sequence"), _int32s(counts, "count")
+        if len(counts) != len(seqs):
             raise ValueError("cache: a count for every sequence")
         self._rows = -1
-        _check(self._lib.gh_cache_extend(self._h, (C.c_int32 * n)(*seqs), (C.c_int32 * n)(*counts), n, stream or None))
+        _check(self._lib.gh_cache_extend(self._h, seqs, counts, len(seqs), stream or None))
         self._rows = sum(counts)
+
+    def _pass_rows(self) -> int:
+        return self._rows if self._rows >= 0 else max(self.info.pass_rows, 0)
 
     def _fill(self, place, t, name, heads, rows, dims=3):
         """Describes a tensor to the library, in self._rows_of[place], once it has been looked over."""
@@ -656,7 +679,7 @@ class Cache:
     def append(self, layer, k, v, q=None, q_out=None, rotate=True, stream=0) -> None:
         """Stores the pass's keys and values [rows, kv_heads, head_dim] in a layer, keys rotated to their positions if the
         cache has a rope_base; q [rows, heads, head_dim] is rotated likewise into q_out (which may be q)."""
-        n = self._rows if self._rows > 0 else 0
+        layer, n = _int32(layer, "layer"), self._pass_rows()
         self._fill(0, k, "k", self.kv_heads, n)
         self._fill(1, v, "v", self.kv_heads, n)
         a, b, c, d = self._refs
@@ -675,7 +698,8 @@ class Cache:
         """out = softmax(scale q.K) V for the pass's rows over what is cached of their sequences in a layer: positions up to
         the row's own if causal, and only the last `window` of those up to it if window is not 0; scale 0 means
         1 / sqrt(head_dim).  q and out: [rows, heads, head_dim]; rows beyond the pass's are left as they are."""
-        n = self._rows if self._rows > 0 else 0
+        layer, n = _int32(layer, "layer"), self._pass_rows()
+        window = _int32(window, "window")
         self._fill(0, q, "q", self.heads, n)
         self._fill(1, out, "out", self.heads, n)
         rc = self._lib.gh_cache_attend(self._h, layer, self._refs[0], self._refs[1], scale, 1 if causal else 0, window, stream or None)
@@ -691,10 +715,10 @@ class Cache:
             dims, layers, strides = 4, self.layers, (k.stride()[0], v.stride()[0])
         else:
             dims, layers, strides = 3, 1, (0, 0)
-        count = k.shape[-3]
+        seq, first, start, count = _int32(seq, "sequence"), _int32(layer or 0, "layer"), _int32(start, "position"), _int32(k.shape[-3], "rows")
         if v.shape[-3] != count:
             raise ValueError("cache: k and v differ in their rows")
         self._fill(0, k, "k", self.kv_heads, count, dims)
         self._fill(1, v, "v", self.kv_heads, count, dims)
-        _check(self._lib.gh_cache_read(self._h, seq, layer or 0, layers, start, count, self._refs[0], strides[0], self._refs[1], strides[1],
+        _check(self._lib.gh_cache_read(self._h, seq, first, layers, start, count, self._refs[0], strides[0], self._refs[1], strides[1],
                                        stream or None))
