@@ -383,6 +383,7 @@ static int copy_sequence(Cache& from, Cache& to, int seq, void* stream) {
     if (&from != &to) other = std::make_unique<Cache::Turn>(from, stream);
     std::vector<PageCopy> copies(static_cast<size_t>(n));
     const int id = to.book.add_filled(length);
+    to.close();  // (a refusal leaves the open pass)
     const std::vector<int>& a = from.book.at(seq).pages;
     const std::vector<int>& b = to.book.at(id).pages;
     for (int i = 0; i < n; i++)
@@ -641,8 +642,8 @@ int cache_from_session(gh_cache* cache, const KvLayout& kv, int layers, int seq,
     check_session(c, kv, layers);
     const DeviceScope on(c.device);
     const Cache::Turn turn(c, stream);
-    c.close();
     const int id = c.book.add_filled(length);
+    c.close();
     copy_session(c, kv, layers, seq, c.book.at(id).pages, length, /*to_session=*/false);
     return id;
 }
@@ -737,7 +738,6 @@ gh_status gh_cache_copy(gh_cache* from, int32_t seq, gh_cache* to, void* hip_str
         if (a.device != b.device) refuse("a copy between devices");
         (void)a.book.at(seq);
         const DeviceScope on(b.device);
-        b.close();
         *out = copy_sequence(a, b, seq, hip_stream);
     });
 }
@@ -747,9 +747,10 @@ gh_status gh_cache_compact(gh_cache* c, void* hip_stream, int32_t* pages_used) {
         Cache& m = cache_of(c);
         const DeviceScope on(m.device);
         const Cache::Turn turn(m, hip_stream);
-        m.close();
         const int used = m.book.pages() - m.book.pages_free();
-        m.copy_pages(m.pool.at, m.book.compact());
+        const std::vector<PageCopy> moves = m.book.compact();
+        m.close();
+        m.copy_pages(m.pool.at, moves);
         if (pages_used) *pages_used = used;
     });
 }

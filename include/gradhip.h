@@ -350,7 +350,8 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  * positions, if the cache was made with a rope_base) and gh_cache_attend computes the
  * attention of the rows' queries over everything cached of their sequence, the rows
  * themselves included.  A pass stays open, and its calls can be repeated, until the next
- * extend, or a fork, truncate, drop, compact, or copy into the cache.
+ * extend, or a fork, truncate, drop, compact, or copy into the cache.  A refused call changes
+ * nothing, except that a refused extend ends the open pass.
  *
  * Data pointers are DEVICE memory of the caller's, of the cache's element type, on the
  * cache's device (the current one at creation).  Calls that take a hip_stream (a hipStream_t,
