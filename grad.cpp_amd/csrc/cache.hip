@@ -15,6 +15,10 @@ namespace {
 
 [[noreturn]] void refuse(const std::string& why) { throw ApiError{GH_ERR_INVALID_ARGUMENT, "cache: " + why}; }
 
+[[noreturn]] void no_workspace(size_t bytes) {
+    throw ApiError{GH_ERR_DEVICE, "cache: no memory for a workspace of " + std::to_string(bytes) + " bytes"};
+}
+
 // The device a cache lives on is the current one while its calls run.
 struct DeviceScope {
     int before = 0;
@@ -37,17 +41,30 @@ struct DeviceBuffer {
     ~DeviceBuffer() {
         if (at) (void)hipFree(at);
     }
-    // Room for so many bytes, contents lost; what the stream still does with the old ones is waited for.
-    bool reserve(size_t want, hipStream_t stream) {
-        if (want <= bytes) return false;
+    enum Outcome { kThere, kMoved, kNone };
+    // Room for so many bytes, contents lost if they have to move; what the stream still does with the old ones is waited for.
+    // kNone: there is no memory, not even the old.
+    Outcome reserve(size_t want, hipStream_t stream) {
+        if (want <= bytes) return kThere;
         HIP_CHECK(hipStreamSynchronize(stream));
         if (at) HIP_CHECK(hipFree(at));
         at = nullptr;
         bytes = 0;
-        const size_t room = (want + want / 2 + 4095) / 4096 * 4096;
-        HIP_CHECK(hipMalloc(&at, room));
-        bytes = room;
-        return true;
+        for (const size_t room : {want + want / 2, want}) {
+            const size_t whole = (room + 4095) / 4096 * 4096;
+            const hipError_t e = hipMalloc(&at, whole);
+            if (e == hipSuccess) {
+                bytes = whole;
+                return kMoved;
+            }
+            at = nullptr;
+            if (e != hipErrorOutOfMemory) HIP_CHECK(e);
+            (void)hipGetLastError();
+        }
+        return kNone;
+    }
+    void need(size_t want, hipStream_t stream) {
+        if (reserve(want, stream) == kNone) no_workspace(want);
     }
 };
 
@@ -114,6 +131,8 @@ constexpr int kPlans = 4;
 // 11.3 and 9.1, 512 11.6 and 11.9, 1 k (50 MB) 12.1 and 13.1, 2 k 13.4 and 21.4; bf16, 8 kv heads of 128: 1 k (34 MB) 14.9 and 12.6,
 // 2 k 15.5 and 20.9, 4 k 19.0 and 30.1.
 constexpr int kLeastShared = 128;
+// ... unless the parts take more than this: each member leaves one of 16 rows at least, whatever it has.  (One kv head of 128 dims: 8 KB.)
+constexpr size_t kMostSharedParts = 512u << 20;
 constexpr size_t kLeastSharedBytes = 40u << 20;
 // Few rows of sequences that hold so many bytes in all go to the tiles of many rows beside them: there a single token reads its
 // sequence 1.2 (16 bit) to 2.4 (fp32) times as slowly, but a launch of its own behind the other is some 15 us.  us, together and
@@ -241,12 +260,39 @@ struct Cache {
         }
     }
 
-    // How the pass's attention is cut, and room for what its parts leave.
+    // How the pass's attention is cut, and room for what its parts leave: with common prefixes, or without them where those would
+    // leave more than there is room for.
     void cut(Plan& plan, bool causal, int window) {
         plan.causal = causal;
         plan.window = window;
-        size_t part_bytes = 0, counters = 0;
-        const std::vector<SharedPrefix> prefixes = window == 0 ? shared : std::vector<SharedPrefix>{};
+        if (window == 0 && !shared.empty()) {
+            const Room room = cut_with(plan, shared);
+            if (room.parts <= kMostSharedParts && reserve(room)) return;
+        }
+        const Room room = cut_with(plan, {});
+        if (room.parts >> 32) refuse("a pass whose parts take more than 4 GB");
+        if (!reserve(room)) no_workspace(room.parts);
+    }
+
+private:
+    struct Room {
+        size_t parts = 0, counters = 0;  // bytes
+    };
+
+    // false, and no plan is valid any more, if there is no memory.
+    bool reserve(const Room& room) {
+        const bool there = parts.reserve(room.parts, stream) != DeviceBuffer::kNone;
+        const auto counted = there ? arrived.reserve(room.counters, stream) : DeviceBuffer::kNone;
+        if (counted == DeviceBuffer::kMoved) HIP_CHECK(hipMemsetAsync(arrived.at, 0, arrived.bytes, stream));
+        if (counted == DeviceBuffer::kNone)
+            for (Plan& p : plans) p.valid = false;
+        return counted != DeviceBuffer::kNone;
+    }
+
+    Room cut_with(Plan& plan, const std::vector<SharedPrefix>& prefixes) const {
+        const bool causal = plan.causal;
+        const int window = plan.window;
+        Room room;
         int few = few_rows(o.type);
         if (prefixes.empty()) {
             size_t held = 0;  // by the sequences of few rows
@@ -295,12 +341,10 @@ struct Cache {
                                 AttendCut{group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64,
                                           !tiles ? 0 : bytes == 4 ? 16 : 64, tiles ? resident : 0},
                                 many ? std::vector<SharedPrefix>{} : prefixes);
-            part_bytes = std::max(part_bytes, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
-            counters = std::max(counters, l.cut.joins.size() * o.kv_heads);
+            room.parts = std::max(room.parts, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
+            room.counters = std::max(room.counters, l.cut.joins.size() * o.kv_heads * sizeof(unsigned));
         }
-        if (part_bytes >> 32) refuse("a pass whose parts take more than 4 GB");
-        parts.reserve(part_bytes, stream);
-        if (arrived.reserve(counters * sizeof(unsigned), stream)) HIP_CHECK(hipMemsetAsync(arrived.at, 0, arrived.bytes, stream));
+        return room;
     }
 };
 
@@ -431,7 +475,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     const size_t rows_at = 0, table_at = round16(sizeof(RowAt) * static_cast<size_t>(rows));
     const size_t items_at = table_at + round16(sizeof(int) * static_cast<size_t>(table));
     const size_t bytes = items_at + plan.bytes();
-    c.pass.reserve(bytes, c.stream);
+    c.pass.need(bytes, c.stream);
     char* host = c.staging.reserve(bytes);
     const std::vector<PageCopy> copies = c.book.extend(seqs, counts, n);
 
@@ -518,7 +562,7 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
         plan->valid = false;
         c.cut(*plan, causal, window);
         const size_t bytes = plan->bytes();
-        plan->items.reserve(bytes, c.stream);
+        plan->items.need(bytes, c.stream);
         plan->write(c.staging.reserve(bytes));
         c.staging.send(plan->items.at, bytes, c.stream);
         plan->at = plan->items.at;

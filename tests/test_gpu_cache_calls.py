@@ -50,3 +50,22 @@ def test_a_refused_session_leaves_the_open_pass(torch):
     rows = torch.zeros(20, 2, 64, device="cuda")
     cache.append(0, rows, rows)
     cache.attend(0, rows, rows)
+
+
+def test_a_prefix_shared_by_thousands(torch):
+    """4096 single tokens behind one prefix, 64 heads of 256: what they would leave for the prefix's joins is more than a workspace
+    holds, so each reads the prefix itself."""
+    rig = Rig(torch, "bf16", heads=64, kv_heads=64, dim=256, page=16, pages=4200, seed=51)
+    parent = rig.add()
+    rig.grow([parent], [256])
+    kids = [rig.cache.fork(parent) for _ in range(4096)]
+    rig.cache.extend(kids, [1] * 4096)
+    gen = torch.Generator(device="cuda").manual_seed(52)
+    k, v, q = (torch.randn(4096, 64, 256, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(3))
+    out = torch.empty_like(q)
+    rig.cache.append(0, k, v)
+    rig.cache.attend(0, q, out)
+    for i in (0, 1, 15, 16, 2047, 4095):
+        keys, values = (torch.cat((old, new[i:i + 1].cpu().double())) for old, new in ((rig.ref.k[parent][0], k), (rig.ref.v[parent][0], v)))
+        want, allowed = rig.R.attention(q[i:i + 1].cpu().double(), keys, values, 256, dtype="bf16")
+        rig.R.assert_within(out[i:i + 1], want, allowed, f"sequence {i}")
