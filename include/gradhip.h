@@ -357,10 +357,11 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  * cache's device (the current one at creation).  Calls that take a hip_stream (a hipStream_t,
  * NULL for the default stream) enqueue their work there and return without waiting, except
  * where an internal buffer has to grow.  Calls on one cache must be serialised by the caller
- * and take effect in their order whatever streams they name: a call on another stream than
- * the one before waits, on the device, for that one's work.  The caller's own buffers are
+ * and take effect in their order whatever streams they name: each waits, on the device, for the
+ * one before, whose stream may have been destroyed since.  The caller's own buffers are
  * ordered by the streams the caller names.  A stream that is being captured into a graph is
- * refused (GH_ERR_RUNTIME): a replay would use the pages and lengths of the capture.
+ * refused (GH_ERR_RUNTIME): a replay would use the pages and lengths of the capture.  So is
+ * hipStreamPerThread (GH_ERR_INVALID_ARGUMENT), one handle for as many streams as threads.
  * Every size, page and position is checked on the host before anything is enqueued. */
 typedef struct gh_cache gh_cache;
 
