@@ -547,6 +547,8 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     check_pass(c, layer);
     if (window < 0) refuse("negative window");
     if (!(scale >= 0.0f) || std::isinf(scale)) refuse("scale must be a finite number, 0 for 1 / sqrt(head_dim)");
+    const float scale2 = (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(c.o.head_dim))) * 1.44269504088896340736f;  // for powers of two
+    if (std::isinf(scale2)) refuse("scale must be below 2.35e38");  // (2^128 / log2(e): infinity times a score of zero is none)
     if (c.rows == 0) return;
     check_rows("q", q);
     check_rows("out", out);
@@ -577,7 +579,7 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.table = reinterpret_cast<const int*>(c.pass.at + c.table_at);
     p.layer = layer;
     p.group = c.group;
-    p.scale = (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(c.o.head_dim))) * 1.44269504088896340736f;
+    p.scale = scale2;
     p.causal = causal;
     p.window = window;
     p.vector_rows = aligned(q, c.bytes, c.rows == 1, c.o.heads == 1) && aligned(out, c.bytes, c.rows == 1, c.o.heads == 1);

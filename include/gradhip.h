@@ -434,8 +434,8 @@ gh_status gh_cache_append(gh_cache* c, int32_t layer, const gh_rows* k, const gh
                           const gh_rows* q_out, int32_t rotate, void* hip_stream);
 
 /* out = softmax(scale q.K) V per row and head over the positions u of the row's sequence with
- * u <= t (causal != 0; t is the row's position) and u > t - window (window > 0).  scale 0 means
- * 1 / sqrt(head_dim).  Rows of q and out beyond the pass's are neither read nor written.  out may
+ * u <= t (causal != 0; t is the row's position) and u > t - window (window > 0).  scale is 0, which means
+ * 1 / sqrt(head_dim), or positive and below 2.35e38.  Rows of q and out beyond the pass's are neither read nor written.  out may
  * be q.  What a row may not see never reaches it, infinities and NaN included; a row all of whose
  * scores are minus infinity is NaN. */
 gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale,

@@ -69,3 +69,17 @@ def test_a_prefix_shared_by_thousands(torch):
         keys, values = (torch.cat((old, new[i:i + 1].cpu().double())) for old, new in ((rig.ref.k[parent][0], k), (rig.ref.v[parent][0], v)))
         want, allowed = rig.R.attention(q[i:i + 1].cpu().double(), keys, values, 256, dtype="bf16")
         rig.R.assert_within(out[i:i + 1], want, allowed, f"sequence {i}")
+
+
+@pytest.mark.parametrize("dtype", base.TYPES)
+def test_scales_at_the_ends_of_their_range(torch, dtype):
+    rig = Rig(torch, dtype, heads=2, kv_heads=1, dim=64, page=16, pages=40, seed=54)
+    s = rig.add()
+    rig.grow([s], [30])
+    q = rig.grow([s], [100])
+    q[:] = 0.0
+    for scale in (1e-45, 1e-38, 2.3e38):  # scores of zero, whatever they are multiplied by
+        rig.check([s], [100], q, scale=scale, what=f"scale {scale:g}")
+    for scale in (2.4e38, 3.4e38):  # finite, but not in the base that the exponentials are taken in
+        with pytest.raises(ValueError, match="scale"):
+            rig.cache.attend(0, q[0], torch.empty_like(q[0]), scale=scale)
