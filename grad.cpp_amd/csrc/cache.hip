@@ -131,15 +131,15 @@ constexpr int kPlans = 4;
 // 11.3 and 9.1, 512 11.6 and 11.9, 1 k (50 MB) 12.1 and 13.1, 2 k 13.4 and 21.4; bf16, 8 kv heads of 128: 1 k (34 MB) 14.9 and 12.6,
 // 2 k 15.5 and 20.9, 4 k 19.0 and 30.1.
 constexpr int kLeastShared = 128;
+constexpr size_t kLeastSharedBytes = 40u << 20;
 // ... unless the parts take more than this: each member leaves one of 16 rows at least, whatever it has.  (One kv head of 128 dims: 8 KB.)
 constexpr size_t kMostSharedParts = 512u << 20;
-constexpr size_t kLeastSharedBytes = 40u << 20;
 // Few rows of sequences that hold so many bytes in all go to the tiles of many rows beside them: there a single token reads its
 // sequence 1.2 (16 bit) to 2.4 (fp32) times as slowly, but a launch of its own behind the other is some 15 us.  us, together and
-// apart: bf16, single tokens over 117 MB beside a chunk of 200 tokens 49 and 69, of 1000 101 and 110, over 234 MB 68 and 102, 176 and
-// 181, over 468 MB 133 and 168, 317 and 282; fp32, over 43 MB 31 and 36, 46 and 53, over 175 MB 51 and 62, 86 and 85, over 351 MB 88
-// and 94, 161 and 141.
-constexpr size_t kTogether16 = 320u << 20, kTogether32 = 160u << 20;
+// apart: bf16, beside a chunk of 200 tokens over 64 MB 49 and 69, over 111 MB 68 and 102, over 269 MB 133 and 168, beside 1000 over 68 MB
+// 101 and 110, over 154 MB 176 and 181, over 254 MB 317 and 282; fp32, beside 200 over 27 MB 33 and 38, over 96 MB 60 and 68, over
+// 167 MB 99 and 99, beside 1000 over 31 MB 51 and 57, over 101 MB 103 and 95, over 230 MB 190 and 158.
+constexpr size_t kTogether16 = 320u << 20, kTogether32 = 100u << 20;
 
 }  // namespace
 
@@ -333,9 +333,9 @@ private:
             // keys cost more to join than they save (13 sequences of up to 1 k positions, fp32: 14.5 us, 15.5 in parts of
             // half that), and more than 64 parts of a tile are a long join (one sequence of 128 k positions: 61 us, 71 in 128).
             // Many rows: as many as are resident at once and no more (1024 rows over 16 k positions, bf16: 113 us, 154 with half as
-            // many; over 4 k, fp32: 96, 111 with 576), and no more parts than the last one joins in the time that they
+            // many; over 4 k, fp32: 106, 140 with 576), and no more parts than the last one joins in the time that they
             // save (128 rows, bf16: 1 k positions 31 us in 4 parts, 34 in 8; 4 k 44 in 8, 75 in 32; 16 k 75 in 16, 142 in 64;
-            // fp32 products take four times as long: 4 k 44 in 16, 51 in 8 and in 32).
+            // fp32 products take some six times as long: 4 k 48 in 16, 57 in 8, 54 in 32; 16 k 90 in 32, 98 in 16, 121 in 64).
             const int resident = o.head_dim > 128 ? 256 : 512;
             const int workgroups = tiles ? resident : bytes == 4 ? 1024 : 2048;
             const int least = tiles ? 128 : bytes == 4 ? 256 : 384;

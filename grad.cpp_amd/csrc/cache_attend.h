@@ -18,8 +18,8 @@ struct AttendForm {
 // themselves, take it; more go to tiles of 128 rows that share what is read.  Tiles of 16 rows read the cache once each, which
 // is nearly free for one sequence (its rows are in the L2s) and is not for many.  us, tiles of 16 and of 128: bf16, 32/8 heads of 128,
 // 16 sequences of 4 k positions: 16 rows 77 and 93, 32 rows 108 and 95, 64 rows 166 and 83; one sequence: 32 rows 17 and 28, 64 rows
-// 25 and 32.  fp32, 12 heads of 64, 16 sequences of 2 k positions: 32 rows 72 and 107, 64 rows 115 and 117, 128 rows 194 and 107; one
-// sequence: 64 rows 16 and 24, 128 rows over 4 k positions 37 and 44, over 16 k 92 and 77.
+// 25 and 32.  fp32, 12 heads of 64, 16 sequences of 2 k positions: 32 rows 65 and 100, 64 rows 112 and 115, 128 rows 203 and 124; one
+// sequence: 64 rows 17 and 29, 128 rows over 4 k positions 36 and 48, over 16 k 105 and 90.
 constexpr int few_rows(int type) { return type == kCacheF32 ? 64 : 32; }
 constexpr int kFewTile = 16;
 

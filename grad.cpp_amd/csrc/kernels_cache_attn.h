@@ -126,7 +126,6 @@ struct Granule {
     unsigned v[kBlocks * 4][kValueWords];
 };
 
-// FULL: the head has DH dims.  Otherwise lanes whose dims do not exist read past the end of the run: zeros.
 // The pages of a granule; a block behind the last position may have none: it reads the last one's, and counts for nothing.
 template <int BLOCKS>
 __device__ __forceinline__ void look_up(const CacheLayout& cache, const int* table, int at, int end, int (&pages)[BLOCKS]) {
@@ -134,6 +133,7 @@ __device__ __forceinline__ void look_up(const CacheLayout& cache, const int* tab
     for (int b = 0; b < BLOCKS; b++) pages[b] = table[min(at + 16 * b, end - 1) >> cache.page_shift];
 }
 
+// FULL: the head has DH dims.  Otherwise lanes whose dims do not exist read past the end of the run: zeros.
 // `pages`: of the granule's blocks of 16 positions, looked up ahead (look_up), or the loads would wait for them one by one.
 template <int TYPE, int DH, bool FULL>
 __device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer, const int (&pages)[Granule<TYPE, DH>::kBlocks], int head, int at,

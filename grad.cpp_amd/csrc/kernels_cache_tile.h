@@ -67,7 +67,8 @@ __device__ __forceinline__ void ahead_of_products() {
 // A wavefront's rows [from, from + rows) of a tile, one after the other and term by term: 64 positions at a time, the scores with a
 // position to a lane, the output with a dim to a lane.  What a row may not see takes no part at all, infinities and NaN are what
 // they are.  For the tiles that hold such values (a matrix product would carry them to rows that do not see them, and make
-// NaN of an infinity's parts): an order of magnitude slower than the products.
+// NaN of an infinity's parts): 40 to 100 times as slow as the products (397 rows at 1.6 k with one infinity among the chunk's values:
+// fp32, 12 heads of 64, 1.9 ms where 48 us do without; bf16, 32/8 heads of 128, 5.6 ms and 58 us).
 template <int TYPE, int DH>
 __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, const int* table, int head, int from, int rows, float* part) {
     using C = CacheType<TYPE>;
