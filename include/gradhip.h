@@ -356,7 +356,8 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  * Data pointers are DEVICE memory of the caller's, of the cache's element type, on the
  * cache's device (the current one at creation).  Calls that take a hip_stream (a hipStream_t,
  * NULL for the default stream) enqueue their work there and return without waiting, except
- * where an internal buffer has to grow.  Calls on one cache must be serialised by the caller
+ * where an internal buffer has to grow, and a pass whose plan is more than 3.5 KB for the plan of the
+ * one before the last to have been read.  Calls on one cache must be serialised by the caller
  * and take effect in their order whatever streams they name: each waits, on the device, for the
  * one before, whose stream may have been destroyed since.  The caller's own buffers are
  * ordered by the streams the caller names.  A stream that is being captured into a graph is
@@ -374,7 +375,10 @@ typedef struct gh_cache_opts {
     int32_t head_dim;    /* a multiple of 8, 8 to 256 */
     int32_t type;        /* GH_F32, GH_BF16, GH_F16: keys, values, queries and outputs.  Sums, maxima
                           * and exponentials are 32-bit whatever the type; with the 16-bit types
-                          * probabilities are rounded to the type before they meet the values.
+                          * probabilities are rounded to the type before they meet the values
+                          * (GH_F16: those below 2^-28 of a row's largest to multiples of 2^-38
+                          * of it).  Values' sums are formed before they are divided: those of
+                          * 2^128 over the number of positions and more may overflow.
                           * GH_F32's products are fp32 ones, or for many rows of a sequence sums of
                           * products of three bf16 parts, off by less than fp32's own rounding */
     int32_t page_tokens; /* positions of a page: a power of two, 16 to 1024; 0 = 64 */
