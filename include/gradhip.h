@@ -440,8 +440,9 @@ gh_status gh_cache_append(gh_cache* c, int32_t layer, const gh_rows* k, const gh
 /* out = softmax(scale q.K) V per row and head over the positions u of the row's sequence with
  * u <= t (causal != 0; t is the row's position) and u > t - window (window > 0).  scale is 0, which means
  * 1 / sqrt(head_dim), or positive and below 2.35e38.  Rows of q and out beyond the pass's are neither read nor written.  out may
- * be q.  What a row may not see never reaches it, infinities and NaN included; a row all of whose
- * scores are minus infinity is NaN. */
+ * be q.  What a row may not see never reaches it, infinities and NaN included; an infinite value
+ * that it does see makes its output infinite, or NaN where the probability rounds to zero (GH_F16:
+ * below 2^-39 of the largest); a row all of whose scores are minus infinity is NaN. */
 gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale,
                           int32_t causal, int32_t window, void* hip_stream);
 
