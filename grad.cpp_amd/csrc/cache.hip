@@ -159,7 +159,9 @@ struct Cache {
     bool open = false;
     int rows = 0;
     std::vector<PassSeq> seqs;
+    std::vector<int> numbers;          // theirs in the book
     std::vector<int> news;
+    std::vector<int> forgetful;        // which of them have forgotten positions
     std::vector<SharedPrefix> shared;  // among sequences of few rows
     size_t rows_at = 0, table_at = 0;  // in `pass`
 
@@ -167,7 +169,7 @@ struct Cache {
     struct Plan {
         bool valid = false;
         bool causal = true;
-        int window = 0;
+        int window = 0, sinks = 0;
         // sequences of few rows and of many go to kernels of their own, one behind the other, unless the few fit beside the many
         struct Launch {
             AttendForm form{};
@@ -200,7 +202,7 @@ struct Cache {
     } plans[kPlans];
     int next_plan = 0;
     bool last_causal = true;  // the mask of the last call: the next pass is planned for it
-    int last_window = 0;
+    int last_window = 0, last_sinks = 0;
 
     Cache(const gh_cache_opts& opts, int pages, int page_tokens) : o(opts), book(pages, page_tokens) {}
     ~Cache() {
@@ -208,7 +210,11 @@ struct Cache {
         if (done) (void)hipEventDestroy(done);
     }
 
-    AttendForm form_for(int rows_of_sequence) const {
+    AttendForm form_for(int rows_of_sequence, bool sinks) const {
+        if (sinks)
+            return o.type == GH_F32 ? attend_form_sinks_f32(o.head_dim, rows_of_sequence)
+                 : o.type == GH_BF16 ? attend_form_sinks_bf16(o.head_dim, rows_of_sequence)
+                                     : attend_form_sinks_f16(o.head_dim, rows_of_sequence);
         return o.type == GH_F32 ? attend_form_f32(o.head_dim, rows_of_sequence)
              : o.type == GH_BF16 ? attend_form_bf16(o.head_dim, rows_of_sequence)
                                  : attend_form_f16(o.head_dim, rows_of_sequence);
@@ -264,9 +270,10 @@ struct Cache {
 
     // How the pass's attention is cut, and room for what its parts leave: with common prefixes, or without them where those would
     // leave more than there is room for.
-    void cut(Plan& plan, bool causal, int window) {
+    void cut(Plan& plan, bool causal, int window, int sinks) {
         plan.causal = causal;
         plan.window = window;
+        plan.sinks = sinks;
         if (window == 0 && !shared.empty()) {
             const Room room = cut_with(plan, shared);
             if (room.parts <= kMostSharedParts && reserve(room)) return;
@@ -293,7 +300,7 @@ private:
 
     Room cut_with(Plan& plan, const std::vector<SharedPrefix>& prefixes) const {
         const bool causal = plan.causal;
-        const int window = plan.window;
+        const int window = plan.window, sinks = plan.sinks;
         Room room;
         int few = few_rows(o.type);
         if (prefixes.empty()) {
@@ -306,7 +313,7 @@ private:
                 if (news[i] * group > few) {
                     many = true;
                 } else {
-                    held += static_cast<size_t>(k1 - k0) * o.kv_heads * o.head_dim * 2 * static_cast<size_t>(bytes);
+                    held += static_cast<size_t>(k1 - k0 + std::min(sinks, k0)) * o.kv_heads * o.head_dim * 2 * static_cast<size_t>(bytes);
                 }
             }
             if (many && held <= (bytes == 4 ? kTogether32 : kTogether16)) few = 0;
@@ -320,7 +327,7 @@ private:
                     mine[i] = news[i];
                     most = std::max(most, news[i] * group);
                 }
-            l.form = form_for(most);
+            l.form = form_for(most, sinks > 0);
             // (a launch holds at most 2^32 threads)
             if (static_cast<long long>(most + 15) / 16 * static_cast<long long>(news.size()) * o.kv_heads > (1 << 22)) {
                 long long tiles = 0;
@@ -341,7 +348,7 @@ private:
             const int least = tiles ? 128 : bytes == 4 ? 256 : 384;
             l.cut = plan_attend(seqs, mine,
                                 AttendCut{group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64,
-                                          !tiles ? 0 : bytes == 4 ? 16 : 64, tiles ? resident : 0},
+                                          !tiles ? 0 : bytes == 4 ? 16 : 64, tiles ? resident : 0, sinks},
                                 many ? std::vector<SharedPrefix>{} : prefixes);
             room.parts = std::max(room.parts, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
             room.counters = std::max(room.counters, l.cut.joins.size() * o.kv_heads * sizeof(unsigned));
@@ -422,18 +429,18 @@ static std::unique_ptr<Cache> create_cache(const gh_cache_opts& in) {
 
 // A sequence's pages' contents into a new sequence of `to`.
 static int copy_sequence(Cache& from, Cache& to, int seq, void* stream) {
-    const PageBook::Sequence& s = from.book.at(seq);
-    const int length = s.length, n = static_cast<int>(s.pages.size());
+    const int length = from.book.at(seq).length;
     const Cache::Turn turn(to, stream);
     std::unique_ptr<Cache::Turn> other;
     if (&from != &to) other = std::make_unique<Cache::Turn>(from, stream);
-    std::vector<PageCopy> copies(static_cast<size_t>(n));
-    const int id = to.book.add_filled(length);
+    std::vector<PageCopy> copies;
+    copies.reserve(from.book.at(seq).pages.size());
+    const int id = to.book.add_like(from.book.at(seq));
     to.close();  // (a refusal leaves the open pass)
     const std::vector<int>& a = from.book.at(seq).pages;
     const std::vector<int>& b = to.book.at(id).pages;
-    for (int i = 0; i < n; i++)
-        copies[static_cast<size_t>(i)] = {a[static_cast<size_t>(i)], b[static_cast<size_t>(i)], std::min(from.o.page_tokens, length - i * from.o.page_tokens)};
+    for (size_t i = 0; i < a.size(); i++)
+        if (a[i] != PageBook::kNone) copies.push_back({a[i], b[i], std::min(from.o.page_tokens, length - static_cast<int>(i) * from.o.page_tokens)});
     to.copy_pages(from.pool.at, copies);
     return id;
 }
@@ -452,6 +459,8 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     // everything that may be refused or find no memory comes before the pages change hands
     c.seqs.assign(static_cast<size_t>(n), PassSeq{});
     c.news.assign(counts, counts + n);
+    c.numbers.assign(seqs, seqs + n);
+    c.forgetful.clear();
     int row0 = 0, table = 0;
     for (int i = 0; i < n; i++) {
         const int first = c.book.at(seqs[i]).length;
@@ -465,14 +474,17 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     std::vector<char> few(static_cast<size_t>(n));
     for (int i = 0; i < n; i++) {
         pages_of[static_cast<size_t>(i)] = &c.book.at(seqs[i]).pages;
-        few[static_cast<size_t>(i)] = counts[i] > 0 && static_cast<long long>(counts[i]) * c.group <= kFewTile;
+        const PageBook::Sequence& s = c.book.at(seqs[i]);
+        const bool whole = s.gone_from == s.gone_to;
+        if (!whole && counts[i] > 0) c.forgetful.push_back(i);
+        few[static_cast<size_t>(i)] = whole && counts[i] > 0 && static_cast<long long>(counts[i]) * c.group <= kFewTile;
     }
     c.shared = shared_prefixes(pages_of, c.seqs, few, c.o.page_tokens, kLeastShared);
     const size_t position = static_cast<size_t>(c.o.kv_heads) * c.o.head_dim * 2 * static_cast<size_t>(c.bytes);
     const auto slight = [&](const SharedPrefix& s) { return position * static_cast<size_t>(s.prefix) * s.members.size() < kLeastSharedBytes; };
     c.shared.erase(std::remove_if(c.shared.begin(), c.shared.end(), slight), c.shared.end());
     Cache::Plan& plan = c.plans[0];
-    c.cut(plan, c.last_causal, c.last_window);
+    c.cut(plan, c.last_causal, c.last_window, c.last_sinks);
     c.next_plan = 1;
     const size_t rows_at = 0, table_at = round16(sizeof(RowAt) * static_cast<size_t>(rows));
     const size_t items_at = table_at + round16(sizeof(int) * static_cast<size_t>(table));
@@ -485,8 +497,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     int* page = reinterpret_cast<int*>(host + table_at);
     for (int i = 0; i < n; i++) {
         const PageBook::Sequence& s = c.book.at(seqs[i]);
-        std::memcpy(page, s.pages.data(), sizeof(int) * s.pages.size());
-        page += s.pages.size();
+        for (int p : s.pages) *page++ = p == PageBook::kNone ? 0 : p;  // (of a forgotten page nothing is read)
         for (int t = s.length - counts[i]; t < s.length; t++)
             *row++ = {s.pages[static_cast<size_t>(t >> c.layout.page_shift)] * c.o.page_tokens + (t & (c.o.page_tokens - 1)), t};
     }
@@ -503,7 +514,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
 
 static void check_pass(const Cache& c, int layer) {
     if (!c.open)
-        throw ApiError{GH_ERR_RUNTIME, "cache: no pass is open (extend opens one; fork, truncate, drop, compact and a copy into the cache end it)"};
+        throw ApiError{GH_ERR_RUNTIME, "cache: no pass is open (extend opens one; fork, truncate, forget, drop, compact and a copy into the cache end it)"};
     if (layer < 0 || layer >= c.o.layers) throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: no layer " + std::to_string(layer)};
 }
 
@@ -543,9 +554,23 @@ static void append_rows(Cache& c, int layer, const gh_rows* k, const gh_rows* v,
     HIP_CHECK(hipGetLastError());
 }
 
-static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, float scale, bool causal, int window, void* stream) {
+// Rows see nothing that is forgotten: it lies between the sinks and the first row's window.
+static void check_forgotten(const Cache& c, int window, int sinks) {
+    for (int i : c.forgetful) {
+        const PassSeq& s = c.seqs[static_cast<size_t>(i)];
+        const PageBook::Sequence& held = c.book.at(c.numbers[static_cast<size_t>(i)]);
+        const int low = window > 0 ? std::max(0, s.first - window + 1) : 0;
+        if (window == 0 || held.gone_from < sinks || held.gone_to > low)
+            throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: sequence " + std::to_string(c.numbers[static_cast<size_t>(i)]) + " has forgotten positions "
+                                                    + std::to_string(held.gone_from) + " to " + std::to_string(held.gone_to) + ", which a row would see"};
+    }
+}
+
+static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, float scale, bool causal, int window, int sinks, void* stream) {
     check_pass(c, layer);
     if (window < 0) refuse("negative window");
+    if (sinks < 0) refuse("negative number of sinks");
+    sinks = window == 0 ? 0 : std::min(sinks, INT_MAX - 15);  // (rounded up to 16, and behind any position)
     if (!(scale >= 0.0f) || std::isinf(scale)) refuse("scale must be a finite number, 0 for 1 / sqrt(head_dim)");
     const float scale2 = (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(c.o.head_dim))) * 1.44269504088896340736f;  // for powers of two
     if (std::isinf(scale2)) refuse("scale must be below 2.35e38");  // (2^128 / log2(e): infinity times a score of zero is none)
@@ -553,18 +578,20 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     check_rows("q", q);
     check_rows("out", out);
     check_apart("out", out, c.rows, c.o.heads, c.o.head_dim);
+    check_forgotten(c, window, sinks);
     const DeviceScope on(c.device);
     const Cache::Turn turn(c, stream);
     c.last_causal = causal;
     c.last_window = window;
+    c.last_sinks = sinks;
     Cache::Plan* plan = nullptr;
     for (Cache::Plan& p : c.plans)
-        if (p.valid && p.causal == causal && p.window == window) plan = &p;
+        if (p.valid && p.causal == causal && p.window == window && p.sinks == sinks) plan = &p;
     if (!plan) {  // another mask than the pass was planned for
         plan = &c.plans[c.next_plan];
         c.next_plan = c.next_plan % (kPlans - 1) + 1;  // (the first stays: its items are the pass's own)
         plan->valid = false;
-        c.cut(*plan, causal, window);
+        c.cut(*plan, causal, window, sinks);
         const size_t bytes = plan->bytes();
         plan->items.need(bytes, c.stream);
         plan->write(c.staging.reserve(bytes));
@@ -582,6 +609,8 @@ static void attend(Cache& c, int layer, const gh_rows* q, const gh_rows* out, fl
     p.scale = scale2;
     p.causal = causal;
     p.window = window;
+    p.sinks = sinks;
+    p.lead = sinks_lead(sinks);
     p.vector_rows = aligned(q, c.bytes, c.rows == 1, c.o.heads == 1) && aligned(out, c.bytes, c.rows == 1, c.o.heads == 1);
     p.parts = reinterpret_cast<float*>(c.parts.at);
     p.arrived = reinterpret_cast<unsigned*>(c.arrived.at);
@@ -602,6 +631,9 @@ static void read_positions(Cache& c, int seq, int layer, int layers, int start, 
     if (layer < 0 || layers < 0 || layer > c.o.layers || layers > c.o.layers - layer) throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: layers out of range"};
     if (start < 0 || count < 0 || start > s.length || count > s.length - start)
         throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: positions out of range"};
+    if (s.forgot(start, start + count))
+        throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: sequence " + std::to_string(seq) + " has forgotten positions " + std::to_string(s.gone_from) + " to "
+                                                + std::to_string(s.gone_to)};
     if (count == 0 || layers == 0) return;
     const int dim = c.o.head_dim, heads = c.o.kv_heads;
     check_rows("k", k);
@@ -700,6 +732,9 @@ void cache_to_session(gh_cache* cache, const int32_t* seqs, int batch, const KvL
     Cache& c = cache_of(cache);
     check_session(c, kv, layers);
     for (int b = 0; b < batch; b++)
+        if (c.book.at(seqs[b]).forgot(0, length))
+            throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: sequence " + std::to_string(seqs[b]) + " has forgotten some of its positions"};
+    for (int b = 0; b < batch; b++)
         if (c.book.at(seqs[b]).length < length)
             throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: sequence " + std::to_string(seqs[b]) + " holds " + std::to_string(c.book.at(seqs[b]).length)
                                                     + " positions, " + std::to_string(length) + " are wanted"};
@@ -768,6 +803,14 @@ gh_status gh_cache_truncate(gh_cache* c, int32_t seq, int32_t length) {
     });
 }
 
+gh_status gh_cache_forget(gh_cache* c, int32_t seq, int32_t start, int32_t end) {
+    return guard([&] {
+        Cache& m = cache_of(c);
+        m.book.forget(seq, start, end);
+        m.close();
+    });
+}
+
 gh_status gh_cache_drop(gh_cache* c, int32_t seq) {
     return guard([&] {
         Cache& m = cache_of(c);
@@ -819,7 +862,12 @@ gh_status gh_cache_append(gh_cache* c, int32_t layer, const gh_rows* k, const gh
 
 gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale, int32_t causal, int32_t window,
                           void* hip_stream) {
-    return guard([&] { attend(cache_of(c), layer, q, out, scale, causal != 0, window, hip_stream); });
+    return guard([&] { attend(cache_of(c), layer, q, out, scale, causal != 0, window, 0, hip_stream); });
+}
+
+gh_status gh_cache_attend_sinks(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale, int32_t causal, int32_t window,
+                                int32_t sinks, void* hip_stream) {
+    return guard([&] { attend(cache_of(c), layer, q, out, scale, causal != 0, window, sinks, hip_stream); });
 }
 
 gh_status gh_cache_read(gh_cache* c, int32_t seq, int32_t layer, int32_t layers, int32_t start, int32_t count, const gh_rows* k,

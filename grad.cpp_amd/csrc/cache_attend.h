@@ -27,27 +27,31 @@ constexpr int kFewTile = 16;
 AttendForm attend_form_f32(int dim, int rows);
 AttendForm attend_form_bf16(int dim, int rows);
 AttendForm attend_form_f16(int dim, int rows);
+// ... whose rows see the first positions beside a window.
+AttendForm attend_form_sinks_f32(int dim, int rows);
+AttendForm attend_form_sinks_bf16(int dim, int rows);
+AttendForm attend_form_sinks_f16(int dim, int rows);
 
-template <int TYPE, int DH, bool FULL>
+template <int TYPE, int DH, bool FULL, bool SINKS>
 AttendForm attend_form_at(int rows) {
     const auto form = [](AttendKernel kernel, int height, int waves) { return AttendForm{kernel, height, 64 * waves, height * (DH + 4)}; };
     if (rows > few_rows(TYPE)) {
         if constexpr (TYPE == kCacheF32) {
-            return form(attend_wide_kernel<DH, FULL, DH == 64 ? 64 : 32>, kTileRows, kTileWaves);
+            return form(attend_wide_kernel<DH, FULL, DH == 64 ? 64 : 32, SINKS>, kTileRows, kTileWaves);
         } else {
-            return form(attend_tile_kernel<TYPE, DH, FULL, DH == 256 ? 32 : 64>, kTileRows, kTileWaves);
+            return form(attend_tile_kernel<TYPE, DH, FULL, DH == 256 ? 32 : 64, SINKS>, kTileRows, kTileWaves);
         }
     }
-    return form(attend_rows_kernel<TYPE, DH, FULL>, kFewTile, attend_waves(TYPE, DH));
+    return form(attend_rows_kernel<TYPE, DH, FULL, SINKS>, kFewTile, attend_waves(TYPE, DH));
 }
 
-template <int TYPE>
+template <int TYPE, bool SINKS>
 AttendForm attend_form_of(int dim, int rows) {
-    if (dim > 128) return attend_form_at<TYPE, 256, false>(rows);
-    if (dim == 128) return attend_form_at<TYPE, 128, true>(rows);
-    if (dim > 64) return attend_form_at<TYPE, 128, false>(rows);
-    if (dim == 64) return attend_form_at<TYPE, 64, true>(rows);
-    return attend_form_at<TYPE, 64, false>(rows);
+    if (dim > 128) return attend_form_at<TYPE, 256, false, SINKS>(rows);
+    if (dim == 128) return attend_form_at<TYPE, 128, true, SINKS>(rows);
+    if (dim > 64) return attend_form_at<TYPE, 128, false, SINKS>(rows);
+    if (dim == 64) return attend_form_at<TYPE, 64, true, SINKS>(rows);
+    return attend_form_at<TYPE, 64, false, SINKS>(rows);
 }
 
 }  // namespace gh

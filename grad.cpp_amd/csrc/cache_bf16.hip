@@ -3,6 +3,6 @@
 
 namespace gh {
 
-AttendForm attend_form_bf16(int dim, int rows) { return attend_form_of<kCacheBf16>(dim, rows); }
+AttendForm attend_form_bf16(int dim, int rows) { return attend_form_of<kCacheBf16, false>(dim, rows); }
 
 }  // namespace gh

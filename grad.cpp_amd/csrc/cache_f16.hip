@@ -3,6 +3,6 @@
 
 namespace gh {
 
-AttendForm attend_form_f16(int dim, int rows) { return attend_form_of<kCacheF16>(dim, rows); }
+AttendForm attend_form_f16(int dim, int rows) { return attend_form_of<kCacheF16, false>(dim, rows); }
 
 }  // namespace gh

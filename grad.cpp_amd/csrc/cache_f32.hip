@@ -3,6 +3,6 @@
 
 namespace gh {
 
-AttendForm attend_form_f32(int dim, int rows) { return attend_form_of<kCacheF32>(dim, rows); }
+AttendForm attend_form_f32(int dim, int rows) { return attend_form_of<kCacheF32, false>(dim, rows); }
 
 }  // namespace gh

@@ -27,7 +27,9 @@ struct RowAt {
     int pos;
 };
 
-// One workgroup's work for one kv head: `rows` rows over the positions [k0, k1) of a page list.
+// One workgroup's work for one kv head: `rows` rows over the positions [k0, k1) of a page list.  Where rows see a sequence's first
+// positions beside a window far from them, [k0, k1) counts the positions that are left when what lies between is taken out:
+// those from `lead` (the sinks, rounded up to 16) on are `gap` further on.
 struct AttendItem {
     int r0, rows;  // of a sequence's tile axis, or (map >= 0) as the map has them
     int k0, k1;
@@ -35,7 +37,7 @@ struct AttendItem {
     int join, joins;   // the joins that wait for it
     int first, row0, table;  // the sequence's; for a map, a position behind all others
     int map;           // rows of several sequences: where their (pass row * group + head of the group) are listed
-    int pad;           // a multiple of 16 bytes
+    int gap;           // a multiple of 16
 };
 
 // A tile whose positions were dealt to several workgroups: the last of them to finish puts it together, first the parts of a
@@ -91,6 +93,8 @@ inline void visible_span(const PassSeq& s, int r0, int rows, int group, bool cau
     k0 = window > 0 ? std::max(0, t0 - window + 1) & ~15 : 0;
 }
 
+constexpr int sinks_lead(int sinks) { return (sinks + 15) & ~15; }
+
 struct AttendCut {
     int group, kv_heads;
     int height;      // of a tile
@@ -102,6 +106,7 @@ struct AttendCut {
     int square = 0;    // ... and, if not 0, sqrt(positions / square): the last part to end joins them all, so n parts take
                        // positions / n + square n.  A tile of 1 / r-th the height has a join of 1 / r-th the time
     int resident = 0;  // if not 0: no more workgroups than this many where there are fewer tiles (one more is a round of its own)
+    int sinks = 0;     // first positions that rows see beside their window; only with a window
 };
 
 // Tiles of `height` rows; a tile's positions are cut into parts of one length.  `shared`: prefixes whose members (of at
@@ -124,10 +129,16 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
             room -= n;
         }
     }
-    const auto tile_span = [&](size_t i, int r0, int& n, int& k0, int& k1) {
+    const int lead = sinks_lead(cut.sinks);
+    const auto tile_span = [&](size_t i, int r0, int& n, int& k0, int& k1) {  // returns the gap
         n = std::min(height, rows[i] * cut.group - r0);
         visible_span(seqs[i], r0, n, cut.group, cut.causal, cut.window, k0, k1);
         k0 = std::max(k0, prefix[i]);
+        if (lead == 0) return 0;
+        const int gap = std::max(0, k0 - lead);
+        k0 = 0;
+        k1 -= gap;
+        return gap;
     };
     long long total = 0;
     for (size_t i = 0; i < seqs.size(); i++)
@@ -171,11 +182,11 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
     };
     const auto add_tile = [&](size_t i, int r0, AttendJoin join) {
         int n, k0, k1, run;
-        tile_span(i, r0, n, k0, k1);
+        const int gap = tile_span(i, r0, n, k0, k1);
         const int parts = cut_up(n, k0, k1, run);
         const bool whole = parts == 1 && join.shared_parts == 0;
         AttendItem it{r0, n, 0, 0, whole ? -1 : plan.parts, static_cast<int>(plan.joins.size()), whole ? 0 : 1,
-                      seqs[i].first, seqs[i].row0, seqs[i].table, -1, 0};
+                      seqs[i].first, seqs[i].row0, seqs[i].table, -1, gap};
         add_items(it, k0, k1, parts, run);
         if (whole) return;
         join.r0 = r0;

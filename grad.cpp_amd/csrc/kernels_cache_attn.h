@@ -95,6 +95,7 @@ struct AttendParams {
     float scale;  // of the scores, times log2(e)
     int causal;
     int window;
+    int sinks, lead;    // first positions that rows see beside their window, and those rounded up to 16 (AttendItem)
     int vector_rows;    // q's and out's rows can be read and written 16 bytes at a time
     float* parts;       // [part][kv head][tile height][DH + 4]: output, maximum, sum, two of padding
     unsigned* arrived;  // [join][kv head], zero between launches
@@ -112,6 +113,29 @@ __device__ __forceinline__ float row_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// The position that an item's place v is.  Places of one block of 16 are neighbours.
+template <bool SINKS>
+__device__ __forceinline__ int position_of(const AttendParams& p, const AttendItem& it, int v) {
+    return SINKS && v >= p.lead ? v + it.gap : v;
+}
+template <bool SINKS>
+__device__ __forceinline__ bool sees(const AttendParams& p, int t, int pos) {
+    return (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window || (SINKS && t < p.sinks));
+}
+// Whether a mask cuts `tokens` places from `at` on, for rows at positions first to final; whether none of the rows sees any of them.
+// Without conditional evaluation: where a branch of its own stands between a matrix product and what reads the result, the compiler puts
+// the product's wait states on one of the two paths only.
+template <bool SINKS>
+__device__ __forceinline__ bool cuts(const AttendParams& p, const AttendItem& it, int at, int tokens, int first, int final) {
+    const int u0 = position_of<SINKS>(p, it, at), u1 = position_of<SINKS>(p, it, at + tokens - 1);
+    return ((p.causal != 0) & (u1 > first)) | ((p.window > 0) & (u0 <= final - p.window) & (!SINKS || u1 >= p.sinks));
+}
+template <bool SINKS>
+__device__ __forceinline__ bool hides(const AttendParams& p, const AttendItem& it, int at, int tokens, int first, int final) {
+    const int u0 = position_of<SINKS>(p, it, at), u1 = position_of<SINKS>(p, it, at + tokens - 1);
+    return ((p.causal != 0) & (u0 > final)) | ((p.window > 0) & (u1 <= first - p.window) & (!SINKS || u0 >= p.sinks));
+}
+
 // What a wavefront reads at a time: a granule of 32 (16-bit) or 16 (fp32) positions of one head.
 template <int TYPE, int DH>
 struct Granule {
@@ -127,18 +151,19 @@ struct Granule {
 };
 
 // The pages of a granule; a block behind the last position may have none: it reads the last one's, and counts for nothing.
-template <int BLOCKS>
-__device__ __forceinline__ void look_up(const CacheLayout& cache, const int* table, int at, int end, int (&pages)[BLOCKS]) {
+template <bool SINKS, int BLOCKS>
+__device__ __forceinline__ void look_up(const AttendParams& p, const AttendItem& it, const int* table, int at, int (&pages)[BLOCKS]) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) pages[b] = table[min(at + 16 * b, end - 1) >> cache.page_shift];
+    for (int b = 0; b < BLOCKS; b++) pages[b] = table[position_of<SINKS>(p, it, min(at + 16 * b, it.k1 - 1)) >> p.cache.page_shift];
 }
 
 // FULL: the head has DH dims.  Otherwise lanes whose dims do not exist read past the end of the run: zeros.
 // `pages`: of the granule's blocks of 16 positions, looked up ahead (look_up), or the loads would wait for them one by one.
-template <int TYPE, int DH, bool FULL>
-__device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer, const int (&pages)[Granule<TYPE, DH>::kBlocks], int head, int at,
-                                             Granule<TYPE, DH>& g) {
+template <int TYPE, int DH, bool FULL, bool SINKS>
+__device__ __forceinline__ void load_granule(const AttendParams& p, const AttendItem& it, const int (&pages)[Granule<TYPE, DH>::kBlocks], int head,
+                                             int at, Granule<TYPE, DH>& g) {
     using G = Granule<TYPE, DH>;
+    const CacheLayout& cache = p.cache;
     constexpr int kBytes = CacheType<TYPE>::kBytes;
     const int lane = threadIdx.x & 63, row = cache.dim * kBytes;
     const int key_lane = (lane & 15) * row + (lane >> 4) * 16;
@@ -146,8 +171,8 @@ __device__ __forceinline__ void load_granule(const CacheLayout& cache, int layer
     const int value_lane = (lane >> 4) * 4 * row + value_dim * kBytes;
 #pragma unroll
     for (int b = 0; b < G::kBlocks; b++) {
-        const int offset = ((at + 16 * b) & ((1 << cache.page_shift) - 1)) * row, page = pages[b];
-        const char* run = cache_run(cache, page, layer, 0, head);
+        const int offset = (position_of<SINKS>(p, it, at + 16 * b) & ((1 << cache.page_shift) - 1)) * row, page = pages[b];
+        const char* run = cache_run(cache, page, p.layer, 0, head);
         const __amdgpu_buffer_rsrc_t ks = make_buffer(run, static_cast<unsigned>(cache.run_bytes));
         const __amdgpu_buffer_rsrc_t vs = make_buffer(run + cache.kv_heads * cache.run_bytes, static_cast<unsigned>(cache.run_bytes));
 #pragma unroll
@@ -450,7 +475,7 @@ constexpr int attend_waves(int type, int dh) { return type == kCacheF32 && dh <=
 // sequences of 4 k to 32 k positions, 32/8 heads of 128 in bf16, 1.41 GB: 258 us, 5.5 TB/s of the 5.8 that a plain read reaches; 64 of up
 // to 2 k, 12 heads of 64 in fp32, 457 MB: 85 us, 5.4 TB/s).  A short pass is bound by its trips one behind the other, items, pages, keys
 // and values, joins (one token over 96 positions 5.8 us, of which a launch that does nothing is 4.5).
-template <int TYPE, int DH, bool FULL>
+template <int TYPE, int DH, bool FULL, bool SINKS>
 __global__ __launch_bounds__(64 * attend_waves(TYPE, DH), DH <= 64 ? 4 : 1) void attend_rows_kernel(const AttendParams p) {
     constexpr int kAttendWaves = attend_waves(TYPE, DH);
     using C = CacheType<TYPE>;
@@ -506,19 +531,19 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH), DH <= 64 ? 4 : 1) void
     int pages[G::kBlocks];
     int at = it.k0 + wave * G::kTokens;
     if (at < it.k1) {
-        look_up(p.cache, table, at, it.k1, pages);
-        load_granule<TYPE, DH, FULL>(p.cache, p.layer, pages, head, at, now);
-        look_up(p.cache, table, at + kAttendWaves * G::kTokens, it.k1, pages);
+        look_up<SINKS>(p, it, table, at, pages);
+        load_granule<TYPE, DH, FULL, SINKS>(p, it, pages, head, at, now);
+        look_up<SINKS>(p, it, table, at + kAttendWaves * G::kTokens, pages);
     }
     while (at < it.k1) {
         const int then = at + kAttendWaves * G::kTokens;
         if (then < it.k1) {
-            load_granule<TYPE, DH, FULL>(p.cache, p.layer, pages, head, then, next);
-            look_up(p.cache, table, then + kAttendWaves * G::kTokens, it.k1, pages);
+            load_granule<TYPE, DH, FULL, SINKS>(p, it, pages, head, then, next);
+            look_up<SINKS>(p, it, table, then + kAttendWaves * G::kTokens, pages);
         }
 
         // does a mask cut this granule?
-        const bool cut = at + G::kTokens > it.k1 || (p.causal && at + G::kTokens - 1 > first) || (p.window > 0 && at <= final - p.window);
+        const bool cut = (at + G::kTokens > it.k1) | cuts<SINKS>(p, it, at, G::kTokens, first, final);
         float z[4 * G::kBlocks];
 #pragma unroll
         for (int b = 0; b < G::kBlocks; b++) {
@@ -547,8 +572,8 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH), DH <= 64 ? 4 : 1) void
         if (cut) {
 #pragma unroll
             for (int i = 0; i < 4 * G::kBlocks; i++) {
-                const int t = at + 16 * (i / 4) + 4 * quarter + (i & 3);
-                const bool see = t < it.k1 && (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window);
+                const int place = 4 * quarter + (i & 3), t = position_of<SINKS>(p, it, at + 16 * (i / 4)) + place;
+                const bool see = at + 16 * (i / 4) + place < it.k1 && sees<SINKS>(p, t, pos);
                 z[i] = see ? z[i] : -INFINITY;
                 seen |= see ? 1u << i : 0u;
             }

@@ -69,7 +69,7 @@ __device__ __forceinline__ void ahead_of_products() {
 // they are.  For the tiles that hold such values (a matrix product would carry them to rows that do not see them, and make
 // NaN of an infinity's parts): 40 to 100 times as slow as the products (397 rows at 1.6 k with one infinity among the chunk's values:
 // fp32, 12 heads of 64, 1.9 ms where 48 us do without; bf16, 32/8 heads of 128, 5.6 ms and 58 us).
-template <int TYPE, int DH>
+template <int TYPE, int DH, bool SINKS>
 __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, const int* table, int head, int from, int rows, float* part) {
     using C = CacheType<TYPE>;
     using T = typename C::T;
@@ -82,7 +82,8 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
     for (int i = from; i < from + rows; i++) {
         const int r = it.r0 + i, token = r / p.group, h = head * p.group + r % p.group, pos = it.first + token;
         const T* query = reinterpret_cast<const T*>(p.q.at) + (it.row0 + token) * p.q.row + h * p.q.head;
-        const int begin = p.window > 0 ? max(it.k0, pos - p.window + 1) : it.k0, end = p.causal ? min(it.k1, pos + 1) : it.k1;
+        // (with sinks, places that the row does not see lie among those that it does)
+        const int begin = !SINKS && p.window > 0 ? max(it.k0, pos - p.window + 1) : it.k0, end = !SINKS && p.causal ? min(it.k1, pos + 1) : it.k1;
         float m = -INFINITY, l = 0.0f, o[kOwn];
 #pragma unroll
         for (int k = 0; k < kOwn; k++) o[k] = 0.0f;
@@ -90,8 +91,9 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
         for (int t0 = begin; t0 < end; t0 += 64) {
             const int n = min(64, end - t0);
             float z = -INFINITY;
-            if (lane < n) {
-                const T* key = at(0, t0 + lane);
+            const bool seen = lane < n && (!SINKS || sees<true>(p, position_of<true>(p, it, t0 + lane), pos));
+            if (seen) {
+                const T* key = at(0, position_of<SINKS>(p, it, t0 + lane));
                 z = 0.0f;
 #pragma unroll 1
                 for (int d = 0; d < dims; d++) z = fmaf(static_cast<float>(query[d]), static_cast<float>(key[d]), z);
@@ -99,15 +101,16 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
             }
             const float top = fmaxf(m, wave_max(z));
             const float keep = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-            const float prob = lane < n ? __builtin_amdgcn_exp2f(z - (top == -INFINITY ? 0.0f : top - C::kLift)) : 0.0f;
+            const float prob = seen ? __builtin_amdgcn_exp2f(z - (top == -INFINITY ? 0.0f : top - C::kLift)) : 0.0f;
             m = top;
             l = l * keep + wave_sum(prob);
 #pragma unroll
             for (int k = 0; k < kOwn; k++) o[k] *= keep;
 #pragma unroll 1
             for (int j = 0; j < n; j++) {
+                if (SINKS && __shfl(static_cast<int>(seen), j) == 0) continue;
                 const float w = __shfl(prob, j);
-                const T* value = at(1, t0 + j);
+                const T* value = at(1, position_of<SINKS>(p, it, t0 + j));
 #pragma unroll
                 for (int k = 0; k < kOwn; k++)
                     if (lane + 64 * k < dims) o[k] = fmaf(w, static_cast<float>(value[lane + 64 * k]), o[k]);
@@ -154,7 +157,7 @@ __device__ __forceinline__ void leave_rows(const AttendParams& p, const AttendIt
 }
 
 // Sixteen-bit types.  TOKENS positions at a time.
-template <int TYPE, int DH, bool FULL, int TOKENS>
+template <int TYPE, int DH, bool FULL, int TOKENS, bool SINKS>
 __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile_kernel(const AttendParams p) {
     using C = CacheType<TYPE>;
     using T = typename C::T;
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     const auto row_of = [&](int i) { return 64 * (kTileWaves * i + wave) / kUnits; };
     const auto look = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < kLoads; i++) pages[i] = table[min(at + row_of(i), it.k1 - 1) >> p.cache.page_shift];
+        for (int i = 0; i < kLoads; i++) pages[i] = table[position_of<SINKS>(p, it, min(at + row_of(i), it.k1 - 1)) >> p.cache.page_shift];
     };
     const auto fetch = [&](int at) {
 #pragma unroll
@@ -230,7 +233,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
             const __amdgpu_buffer_rsrc_t vs = make_buffer(run + p.cache.kv_heads * p.cache.run_bytes, static_cast<unsigned>(p.cache.run_bytes));
             const int t = at + row_of(i);
             const int offset = t + own_row < it.k1 ? own : kBeyond;  // (places behind the last position: zeros)
-            const int base = (t & ((1 << p.cache.page_shift) - 1)) * bytes;
+            const int base = (position_of<SINKS>(p, it, t) & ((1 << p.cache.page_shift) - 1)) * bytes;
             kr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ks, offset, base, 0));
             vr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vs, offset, base, 0));
         }
@@ -244,7 +247,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     fetch(it.k0);
     look(it.k0 + TOKENS);
     for (int at = it.k0; at < it.k1; at += TOKENS) {
-        const bool cut_all = (p.causal && at + TOKENS - 1 > first_all) || (p.window > 0 && at <= final_all - p.window);
+        const bool cut_all = cuts<SINKS>(p, it, at, TOKENS, first_all, final_all);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
             fetch(at + TOKENS);
             look(at + 2 * TOKENS);
         }
-        if (rows_here <= 0 || (p.causal && at > final) || (p.window > 0 && at + TOKENS - 1 <= first - p.window)) continue;
+        if ((rows_here <= 0) | hides<SINKS>(p, it, at, TOKENS, first, final)) continue;
 
         f32x16 z[kBlocks];
 #pragma unroll
@@ -282,14 +285,14 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
             for (int b = 0; b < kBlocks; b++)
                 z[b] = mfma32<TYPE>(*reinterpret_cast<const u32x4*>(key_at + b * 32 * kKeyRow + c * 32), q[c], z[b]);
         ahead_of_products<kBlocks * kSteps, 1, 6>();
-        const bool cut = at + TOKENS > it.k1 || (p.causal && at + TOKENS - 1 > first) || (p.window > 0 && at <= final - p.window);
+        const bool cut = (at + TOKENS > it.k1) | cuts<SINKS>(p, it, at, TOKENS, first, final);
         if (cut) {
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int t = at + 32 * b + 8 * (i / 4) + 4 * half + (i & 3);
-                    const bool see = t < it.k1 && (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window);
+                    const int block = at + 32 * b + 16 * (i / 8), place = 8 * (i / 4 & 1) + 4 * half + (i & 3);
+                    const bool see = block + place < it.k1 && sees<SINKS>(p, position_of<SINKS>(p, it, block) + place, pos);
                     z[b][i] = see ? z[b][i] : -INFINITY;
                 }
         }
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
     float* const part = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     if (__builtin_amdgcn_readfirstlane(odd)) {
-        rows_one_by_one<TYPE, DH>(p, it, table, head, 32 * wave, rows_here, part);
+        rows_one_by_one<TYPE, DH, SINKS>(p, it, table, head, 32 * wave, rows_here, part);
     } else {
         leave_rows<TYPE, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }
@@ -394,7 +397,7 @@ __device__ __forceinline__ Parts three_parts(const f32x4& x, float& taint) {
     return p;
 }
 
-template <int DH, bool FULL, int TOKENS>
+template <int DH, bool FULL, int TOKENS, bool SINKS>
 __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide_kernel(const AttendParams p) {
     constexpr int kKeyRow = DH * 2 + 16, kValueRow = DH * 2 + 32;  // bytes of a part's row
     constexpr int kKeys = TOKENS * kKeyRow, kValues = TOKENS * kValueRow;
@@ -462,7 +465,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     const auto row_of = [&](int i) { return 64 * (kTileWaves * i + wave) / kUnits; };
     const auto look = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < kLoads; i++) pages[i] = table[min(at + row_of(i), it.k1 - 1) >> p.cache.page_shift];
+        for (int i = 0; i < kLoads; i++) pages[i] = table[position_of<SINKS>(p, it, min(at + row_of(i), it.k1 - 1)) >> p.cache.page_shift];
     };
     const auto fetch = [&](int at) {
 #pragma unroll
@@ -472,7 +475,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
             const __amdgpu_buffer_rsrc_t vs = make_buffer(run + p.cache.kv_heads * p.cache.run_bytes, static_cast<unsigned>(p.cache.run_bytes));
             const int t = at + row_of(i);
             const int offset = t + own_row < it.k1 ? own : kBeyond;  // (places behind the last position: zeros)
-            const int base = (t & ((1 << p.cache.page_shift) - 1)) * bytes;
+            const int base = (position_of<SINKS>(p, it, t) & ((1 << p.cache.page_shift) - 1)) * bytes;
             kr[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ks, offset, base, 0));
             vr[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(vs, offset, base, 0));
         }
@@ -506,7 +509,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
             fetch(at + TOKENS);
             look(at + 2 * TOKENS);
         }
-        if (rows_here <= 0 || (p.causal && at > final) || (p.window > 0 && at + TOKENS - 1 <= first - p.window)) continue;
+        if ((rows_here <= 0) | hides<SINKS>(p, it, at, TOKENS, first, final)) continue;
 
         f32x16 z[kBlocks];
 #pragma unroll
@@ -555,14 +558,14 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
             }
             z[b] = acc;
         }
-        const bool cut = at + TOKENS > it.k1 || (p.causal && at + TOKENS - 1 > first) || (p.window > 0 && at <= final - p.window);
+        const bool cut = (at + TOKENS > it.k1) | cuts<SINKS>(p, it, at, TOKENS, first, final);
         if (cut) {
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int t = at + 32 * b + 8 * (i / 4) + 4 * half + (i & 3);
-                    const bool see = t < it.k1 && (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window);
+                    const int block = at + 32 * b + 16 * (i / 8), place = 8 * (i / 4 & 1) + 4 * half + (i & 3);
+                    const bool see = block + place < it.k1 && sees<SINKS>(p, position_of<SINKS>(p, it, block) + place, pos);
                     z[b][i] = see ? z[b][i] : -INFINITY;
                 }
         }
@@ -654,7 +657,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     constexpr int kPad = DH + 4, kBlock = kTileRows * kPad;
     float* const part = p.parts + (static_cast<size_t>(only ? 0 : it.part) * p.cache.kv_heads + head) * kBlock;
     if (__builtin_amdgcn_readfirstlane(odd)) {
-        rows_one_by_one<kCacheF32, DH>(p, it, table, head, 32 * wave, rows_here, part);
+        rows_one_by_one<kCacheF32, DH, SINKS>(p, it, table, head, 32 * wave, rows_here, part);
     } else {
         leave_rows<kCacheF32, DH, FULL>(p, it, o, m, both_sum(l), row, token, head * p.group + h, 32 * wave + (lane & 31), half, part);
     }

@@ -6,6 +6,8 @@
 // that were forked share pages; a page held more than once is never written: the position that
 // would go into it goes into a copy (Copy, made by extend).  The lowest free page is handed out
 // first, so that the pages in use stay near the front and the same calls give the same pages.
+// A sequence can forget a stretch of its positions: the pages that lie wholly inside are nobody's
+// any more (kNone in its list); the positions keep their numbers.
 #pragma once
 
 #include <algorithm>
@@ -26,10 +28,14 @@ struct PageCopy {
 
 class PageBook {
 public:
+    static constexpr int kNone = -1;
+
     struct Sequence {
         bool live = false;
         int length = 0;
         std::vector<int> pages;
+        int gone_from = 0, gone_to = 0;  // positions that are forgotten
+        bool forgot(int from, int to) const { return std::max(from, gone_from) < std::min(to, gone_to); }  // any of those
     };
 
     PageBook(int pages, int page_tokens) : page_tokens_(page_tokens), held_(static_cast<size_t>(pages), 0) {
@@ -59,6 +65,7 @@ public:
         seqs_[i].live = true;
         seqs_[i].length = 0;
         seqs_[i].pages.clear();
+        seqs_[i].gone_from = seqs_[i].gone_to = 0;
         return static_cast<int>(i);
     }
 
@@ -69,11 +76,16 @@ public:
             throw std::out_of_range("cache: a fork of " + std::to_string(length) + " positions of a sequence of "
                                     + std::to_string(from.length));
         std::vector<int> pages(from.pages.begin(), from.pages.begin() + pages_for(length));
+        const int gone_from = from.gone_from, gone_to = from.gone_to;
         const int id = add();
         Sequence& s = seqs_[static_cast<size_t>(id)];
         s.pages = std::move(pages);
         s.length = length;
-        for (int p : s.pages) held_[static_cast<size_t>(p)]++;
+        s.gone_from = gone_from;
+        s.gone_to = gone_to;
+        cut_gone(s);
+        for (int p : s.pages)
+            if (p != kNone) held_[static_cast<size_t>(p)]++;
         return id;
     }
 
@@ -83,10 +95,34 @@ public:
                                     + std::to_string(at(seq).length));
         Sequence& s = seqs_[static_cast<size_t>(seq)];
         while (static_cast<int>(s.pages.size()) > pages_for(length)) {
-            release(s.pages.back());
+            if (s.pages.back() != kNone) release(s.pages.back());
             s.pages.pop_back();
         }
         s.length = length;
+        cut_gone(s);
+    }
+
+    // Gives up positions [from, to); with those given up before they have to make one stretch.
+    void forget(int seq, int from, int to) {
+        (void)at(seq);
+        Sequence& s = seqs_[static_cast<size_t>(seq)];
+        if (from >= to) return;
+        if (from < 0 || to > s.length)
+            throw std::out_of_range("cache: positions " + std::to_string(from) + " to " + std::to_string(to) + " forgotten of a sequence of "
+                                    + std::to_string(s.length));
+        if (s.gone_from < s.gone_to && (from > s.gone_to || to < s.gone_from))
+            throw std::invalid_argument("cache: sequence " + std::to_string(seq) + " has forgotten positions " + std::to_string(s.gone_from) + " to "
+                                        + std::to_string(s.gone_to) + ": what else it forgets has to touch them");
+        const bool any = s.gone_from < s.gone_to;
+        s.gone_from = any ? std::min(s.gone_from, from) : from;
+        s.gone_to = any ? std::max(s.gone_to, to) : to;
+        // (only pages with a position of this call can have become wholly forgotten)
+        const int first = std::max(pages_for(s.gone_from), from / page_tokens_), end = std::min(s.gone_to / page_tokens_, pages_for(to));
+        for (int i = first; i < end; i++) {
+            int& p = s.pages[static_cast<size_t>(i)];
+            if (p != kNone) release(p);
+            p = kNone;
+        }
     }
 
     void drop(int seq) {
@@ -111,15 +147,15 @@ public:
             need += pages_for(s.length + counts[i]) - pages_for(s.length);
             if (s.length % page_tokens_ != 0) {
                 const int last = s.pages.back();
-                if (held_[static_cast<size_t>(last)] - leaving[last] > 1) {
+                if (last == kNone) {  // (cut off inside what was forgotten)
+                    need++;
+                } else if (held_[static_cast<size_t>(last)] - leaving[last] > 1) {
                     leaving[last]++;
                     need++;
                 }
             }
         }
-        if (need > pages_free())
-            throw std::runtime_error("cache: out of pages (" + std::to_string(need) + " wanted, " + std::to_string(pages_free()) + " of "
-                                     + std::to_string(pages()) + " free)");
+        check_free(need);
         std::vector<PageCopy> copies;
         copies.reserve(static_cast<size_t>(n));
         for (int i = 0; i < n; i++) {  // (memory for the page lists first: what follows does not throw)
@@ -130,7 +166,9 @@ public:
             if (counts[i] == 0) continue;
             Sequence& s = seqs_[static_cast<size_t>(seqs[i])];
             const int used = s.length % page_tokens_;
-            if (used != 0 && held_[static_cast<size_t>(s.pages.back())] > 1) {
+            if (used != 0 && s.pages.back() == kNone) {
+                s.pages.back() = take();
+            } else if (used != 0 && held_[static_cast<size_t>(s.pages.back())] > 1) {
                 const int from = s.pages.back();
                 s.pages.back() = take();
                 held_[static_cast<size_t>(from)]--;
@@ -151,6 +189,22 @@ public:
             drop(id);
             throw;
         }
+        return id;
+    }
+
+    // A sequence like one of this or another book, in pages of its own, contents to be written by the caller.
+    int add_like(const Sequence& other) {
+        std::vector<int> pages = other.pages;
+        const int length = other.length, gone_from = other.gone_from, gone_to = other.gone_to;
+        check_free(static_cast<long long>(pages.size()) - std::count(pages.begin(), pages.end(), kNone));
+        const int id = add();
+        Sequence& s = seqs_[static_cast<size_t>(id)];
+        for (int& p : pages)
+            if (p != kNone) p = take();
+        s.pages = std::move(pages);
+        s.length = length;
+        s.gone_from = gone_from;
+        s.gone_to = gone_to;
         return id;
     }
 
@@ -175,7 +229,7 @@ public:
         for (const Sequence& s : seqs_)
             if (s.live)
                 for (size_t i = 0; i < s.pages.size(); i++)
-                    filled[static_cast<size_t>(s.pages[i])] =
+                    if (s.pages[i] != kNone) filled[static_cast<size_t>(s.pages[i])] =
                         std::max(filled[static_cast<size_t>(s.pages[i])], std::min(page_tokens_, s.length - static_cast<int>(i) * page_tokens_));
         for (PageCopy& m : moves) m.tokens = filled[static_cast<size_t>(m.from)];
         std::vector<int> rest;
@@ -197,6 +251,15 @@ public:
     int page_tokens() const { return page_tokens_; }
 
 private:
+    void check_free(long long need) const {
+        if (need > pages_free())
+            throw std::runtime_error("cache: out of pages (" + std::to_string(need) + " wanted, " + std::to_string(pages_free()) + " of "
+                                     + std::to_string(pages()) + " free)");
+    }
+    static void cut_gone(Sequence& s) {
+        s.gone_to = std::min(s.gone_to, s.length);
+        if (s.gone_from >= s.gone_to) s.gone_from = s.gone_to = 0;
+    }
     int take() {
         std::pop_heap(free_.begin(), free_.end(), std::greater<int>());
         const int p = free_.back();

@@ -129,6 +129,7 @@ SYMBOLS = {
     "gh_cache_length": (C.c_int32, [_vp, C.c_int32]),
     "gh_cache_fork": (C.c_int, [_vp, C.c_int32, C.c_int32, _i32p]),
     "gh_cache_truncate": (C.c_int, [_vp, C.c_int32, C.c_int32]),
+    "gh_cache_forget": (C.c_int, [_vp, C.c_int32, C.c_int32, C.c_int32]),
     "gh_cache_drop": (C.c_int, [_vp, C.c_int32]),
     "gh_cache_copy": (C.c_int, [_vp, C.c_int32, _vp, _vp, _i32p]),
     "gh_cache_compact": (C.c_int, [_vp, _vp, _i32p]),
@@ -136,6 +137,8 @@ SYMBOLS = {
     "gh_cache_append": (C.c_int, [_vp, C.c_int32, C.POINTER(GhRows), C.POINTER(GhRows), C.POINTER(GhRows), C.POINTER(GhRows),
                                   C.c_int32, _vp]),
     "gh_cache_attend": (C.c_int, [_vp, C.c_int32, C.POINTER(GhRows), C.POINTER(GhRows), C.c_float, C.c_int32, C.c_int32, _vp]),
+    "gh_cache_attend_sinks": (C.c_int, [_vp, C.c_int32, C.POINTER(GhRows), C.POINTER(GhRows), C.c_float, C.c_int32, C.c_int32, C.c_int32,
+                                        _vp]),
     "gh_cache_read": (C.c_int, [_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(GhRows), C.c_int64,
                                 C.POINTER(GhRows), C.c_int64, _vp]),
     "gh_session_store": (C.c_int, [_vp, C.c_int32, _vp, _i32p]),
@@ -631,6 +634,12 @@ class Cache:
         _check(self._lib.gh_cache_truncate(self._h, _int32(seq, "sequence"), _int32(length, "length")))
         self._rows = -1
 
+    def forget(self, seq, start, end) -> None:
+        """Gives up seq's positions start to end - 1 for good; they keep their numbers, and no row may see them.  All that a
+        sequence has forgotten has to be one stretch."""
+        _check(self._lib.gh_cache_forget(self._h, _int32(seq, "sequence"), _int32(start, "position"), _int32(end, "position")))
+        self._rows = -1
+
     def drop(self, seq) -> None:
         """Ends seq and frees the pages that nobody else holds."""
         _check(self._lib.gh_cache_drop(self._h, _int32(seq, "sequence")))
@@ -694,15 +703,18 @@ class Cache:
         if rc:
             _check(rc)
 
-    def attend(self, layer, q, out, scale=0.0, causal=True, window=0, stream=0) -> None:
+    def attend(self, layer, q, out, scale=0.0, causal=True, window=0, stream=0, sinks=0) -> None:
         """out = softmax(scale q.K) V for the pass's rows over what is cached of their sequences in a layer: positions up to
-        the row's own if causal, and only the last `window` of those up to it if window is not 0; scale 0 means
-        1 / sqrt(head_dim).  q and out: [rows, heads, head_dim]; rows beyond the pass's are left as they are."""
+        the row's own if causal, and only the last `window` of those up to it, and the sequence's first `sinks`, if window is
+        not 0; scale 0 means 1 / sqrt(head_dim).  q and out: [rows, heads, head_dim]; rows beyond the pass's are left as they are."""
         layer, n = _int32(layer, "layer"), self._pass_rows()
-        window = _int32(window, "window")
+        window, sinks = _int32(window, "window"), _int32(sinks, "number of sinks")
         self._fill(0, q, "q", self.heads, n)
         self._fill(1, out, "out", self.heads, n)
-        rc = self._lib.gh_cache_attend(self._h, layer, self._refs[0], self._refs[1], scale, 1 if causal else 0, window, stream or None)
+        if sinks:
+            rc = self._lib.gh_cache_attend_sinks(self._h, layer, self._refs[0], self._refs[1], scale, 1 if causal else 0, window, sinks, stream or None)
+        else:
+            rc = self._lib.gh_cache_attend(self._h, layer, self._refs[0], self._refs[1], scale, 1 if causal else 0, window, stream or None)
         if rc:
             _check(rc)
 

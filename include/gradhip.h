@@ -350,7 +350,7 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  * positions, if the cache was made with a rope_base) and gh_cache_attend computes the
  * attention of the rows' queries over everything cached of their sequence, the rows
  * themselves included.  A pass stays open, and its calls can be repeated, until the next
- * extend, or a fork, truncate, drop, compact, or copy into the cache.  A refused call changes
+ * extend, or a fork, truncate, forget, drop, compact, or copy into the cache.  A refused call changes
  * nothing, except that a refused extend ends the open pass.
  *
  * Data pointers are DEVICE memory of the caller's, of the cache's element type, on the
@@ -418,6 +418,12 @@ int32_t gh_cache_length(const gh_cache* c, int32_t seq);
 gh_status gh_cache_fork(gh_cache* c, int32_t seq, int32_t length, int32_t* out);
 /* Keeps a sequence's first `length` positions; pages that nobody holds any more are free. */
 gh_status gh_cache_truncate(gh_cache* c, int32_t seq, int32_t length);
+/* Gives up positions start to end - 1 of a sequence for good (nothing where end <= start): pages that nobody else holds and
+ * that lie wholly among forgotten positions are free.  The others keep their numbers, and the sequence its length.  What a
+ * sequence has forgotten is one stretch: a further call's has to touch it (GH_ERR_INVALID_ARGUMENT).  Forgotten positions are not
+ * read, restored, or seen by a row (GH_ERR_OUT_OF_RANGE, see gh_cache_attend_sinks); forks and copies have forgotten
+ * them too.  A truncation to fewer positions ends what lies behind it; new positions there are ordinary ones. */
+gh_status gh_cache_forget(gh_cache* c, int32_t seq, int32_t start, int32_t end);
 /* Ends a sequence and frees its pages. */
 gh_status gh_cache_drop(gh_cache* c, int32_t seq);
 /* A sequence of `to` (which may be `from`) with the contents of from's seq in pages of its
@@ -445,6 +451,13 @@ gh_status gh_cache_append(gh_cache* c, int32_t layer, const gh_rows* k, const gh
  * below 2^-39 of the largest); a row all of whose scores are minus infinity is NaN. */
 gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale,
                           int32_t causal, int32_t window, void* hip_stream);
+
+/* gh_cache_attend whose rows see, beside the last `window` positions, the first `sinks` of their sequence: positions u with
+ * u > t - window or u < sinks (and u <= t if causal).  What lies between is not read.  window = 0 sees everything, whatever
+ * `sinks` is; sinks = 0 is gh_cache_attend.  A row that would see a position that its sequence has forgotten is refused
+ * (GH_ERR_OUT_OF_RANGE): with a window, what lies from `sinks` on and before the window of the pass's first row may be forgotten. */
+gh_status gh_cache_attend_sinks(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale, int32_t causal,
+                                int32_t window, int32_t sinks, void* hip_stream);
 
 /* Positions [start, start + count) of a sequence in `layers` layers from `layer` on, densely:
  * layer i's rows begin layer_stride * i elements behind the first's. */
