@@ -2,6 +2,7 @@
 #include "api_error.h"
 #include "cache_attend.h"
 #include "cache_session.h"
+#include "device_scope.h"
 #include "kernels_cache.h"
 
 #include <climits>
@@ -18,22 +19,6 @@ namespace {
 [[noreturn]] void no_workspace(size_t bytes) {
     throw ApiError{GH_ERR_DEVICE, "cache: no memory for a workspace of " + std::to_string(bytes) + " bytes"};
 }
-
-// The device a cache lives on is the current one while its calls run.
-struct DeviceScope {
-    int before = 0;
-    explicit DeviceScope(int device) {
-        HIP_CHECK(hipGetDevice(&before));
-        if (before != device) HIP_CHECK(hipSetDevice(device));
-        now = device;
-    }
-    ~DeviceScope() {
-        if (before != now) (void)hipSetDevice(before);
-    }
-    DeviceScope(const DeviceScope&) = delete;
-    DeviceScope& operator=(const DeviceScope&) = delete;
-    int now = 0;
-};
 
 struct DeviceBuffer {
     char* at = nullptr;

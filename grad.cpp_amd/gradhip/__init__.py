@@ -76,6 +76,13 @@ class GhCacheInfo(C.Structure):
                 ("pass_rows", C.c_int32), ("reserved", C.c_int32), ("pool_bytes", C.c_uint64)]
 
 
+class GhSampleArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64), ("type", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32),
+                ("reserved", C.c_int32), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("uniforms", C.c_void_p), ("ids", C.c_void_p), ("probs", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 # Every symbol include/gradhip.h declares: name -> (restype, argtypes)
 _f32p, _i32p, _vp = C.POINTER(C.c_float), C.POINTER(C.c_int32), C.c_void_p
 TokenCallback = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.POINTER(C.c_int32), C.c_int32)  # gh_token_callback
@@ -108,6 +115,8 @@ SYMBOLS = {
                                       C.c_uint64, _i32p, _i32p, _f32p, _i32p]),
     "gh_pick_noalloc": (C.c_int, [_vp, C.c_int32, C.c_int32, _vp, C.c_int32, C.c_int32, C.POINTER(GhSampling), _vp,
                                   C.c_uint64, C.c_int32, _vp, _vp]),
+    "gh_sample_workspace": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
+    "gh_sample": (C.c_int, [C.POINTER(GhSampleArgs), _vp]),
     "gh_session_last_timing": (C.c_int, [_vp, C.POINTER(GhTiming)]),
     "gh_tokenizer_load": (C.c_int, [C.c_char_p, C.POINTER(_vp)]),
     "gh_tokenizer_from_merges": (C.c_int, [_i32p, C.c_int32, C.POINTER(C.c_char_p), _i32p, C.c_int32,
@@ -537,11 +546,11 @@ CACHE_TYPES = {"f32": 0, "bf16": 1, "f16": 2}  # GH_F32, GH_BF16, GH_F16
 _TORCH_NAMES = {"f32": "torch.float32", "bf16": "torch.bfloat16", "f16": "torch.float16"}
 
 
-def _int32(value, name):
+def _int32(value, name, of="cache"):
     """A number as an argument of 32 bits, which ctypes would cut it down to."""
     value = operator.index(value)
     if not -2 ** 31 <= value < 2 ** 31:
-        raise ValueError(f"cache: {name} {value} is beyond 32 bits")
+        raise ValueError(f"{of}: {name} {value} is beyond 32 bits")
     return value
 
 
@@ -734,3 +743,61 @@ class Cache:
         self._fill(1, v, "v", self.kv_heads, count, dims)
         _check(self._lib.gh_cache_read(self._h, seq, first, layers, start, count, self._refs[0], strides[0], self._refs[1], strides[1],
                                        stream or None))
+
+
+def sample_workspace(rows, vocab, dtype="f32") -> int:
+    """Bytes of the workspace that sample() wants for so many rows of logits."""
+    if dtype not in CACHE_TYPES:
+        raise ValueError(f"sample: unknown element type {dtype!r}")
+    out = C.c_size_t()
+    _check(load_library().gh_sample_workspace(CACHE_TYPES[dtype], _int32(rows, "rows", "sample"), _int32(vocab, "vocab", "sample"), C.byref(out)))
+    return out.value
+
+
+_TYPES_OF_TORCH = {name: CACHE_TYPES[key] for key, name in _TORCH_NAMES.items()}
+
+
+def sample(logits, uniforms, ids, temperature=None, top_k=None, top_p=None, min_p=None, probs=None, workspace=None, stream=0) -> None:
+    """Picks a token from every row of logits [rows, vocab] (gh_sample): ids [rows] of int32 receives them, probs [rows] of float32 (may be None) the
+    probability that each had among the tokens kept.  uniforms, temperature, top_p, min_p [rows] are float32, top_k [rows] int32; None is
+    off.  workspace: sample_workspace(...) bytes of any dense tensor.
+
+    Tensors are torch's (anything with its data_ptr, shape, stride, dtype and device), on one GPU; the logits have a dense last dimension
+    and any other stride, the rest is dense.  stream is a hipStream_t as an int; work is enqueued there and not waited for."""
+    shape, device = logits.shape, logits.device
+    if len(shape) != 2:
+        raise ValueError(f"sample: logits of shape {tuple(shape)} where [rows, vocab] goes")
+    kind = _TYPES_OF_TORCH.get(str(logits.dtype))
+    if kind is None:
+        raise ValueError(f"sample: logits are {logits.dtype}")
+    if device.type != "cuda":
+        raise ValueError(f"sample: logits are on {device}")
+    rows, vocab = _int32(shape[0], "rows", "sample"), _int32(shape[1], "vocab", "sample")
+    stride = logits.stride()
+    if vocab > 1 and stride[1] != 1:
+        raise ValueError("sample: the logits' last dimension is not dense")
+    at = []
+    for t, name, want in ((temperature, "temperature", "torch.float32"), (top_k, "top_k", "torch.int32"), (top_p, "top_p", "torch.float32"),
+                          (min_p, "min_p", "torch.float32"), (uniforms, "uniforms", "torch.float32"), (ids, "ids", "torch.int32"),
+                          (probs, "probs", "torch.float32")):
+        if t is None:
+            if name in ("uniforms", "ids"):
+                raise ValueError(f"sample: {name} are missing")
+            at.append(None)
+            continue
+        if str(t.dtype) != want:
+            raise ValueError(f"sample: {name} is {t.dtype}, not {want}")
+        if len(t.shape) != 1 or t.shape[0] != rows or (rows > 1 and t.stride()[0] != 1):
+            raise ValueError(f"sample: {name} of shape {tuple(t.shape)} where dense [{rows}] goes")
+        if t.device != device:
+            raise ValueError(f"sample: {name} is on {t.device}, the logits on {device}")
+        at.append(t.data_ptr())
+    room = 0
+    if workspace is not None:
+        if workspace.device != device or not workspace.is_contiguous():
+            raise ValueError(f"sample: the workspace is on {workspace.device} or not dense, the logits on {device}")
+        room = workspace.numel() * workspace.element_size()
+    args = GhSampleArgs(logits.data_ptr(), stride[0], kind, rows, vocab, 0, *at, workspace.data_ptr() if room else None, room)
+    rc = load_library().gh_sample(C.byref(args), stream or None)
+    if rc:
+        _check(rc)

@@ -20,7 +20,7 @@ HIPCC_FLAGS = [
     "-fno-fast-math", "-Wall", "-Wno-unused-function", *os.environ.get("GRADHIP_EXTRA_FLAGS", "").split(),
 ]
 SOURCES = ["engine.hip", "persist.hip", "xcd.hip", "resident.hip", "rows.hip", "pairs.hip", "cache.hip", "cache_f32.hip", "cache_bf16.hip",
-           "cache_f16.hip", "cache_sinks_f32.hip", "cache_sinks_bf16.hip", "cache_sinks_f16.hip", "checkpoint.cpp", "tokenizer.cpp"]
+           "cache_f16.hip", "cache_sinks_f32.hip", "cache_sinks_bf16.hip", "cache_sinks_f16.hip", "sample.hip", "checkpoint.cpp", "tokenizer.cpp"]
 OBJ_DIR = os.path.join(PKG, "build")
 
 

@@ -3,8 +3,8 @@
  *
  * Plain C ABI: opaque handles, plain pointers and sizes, status codes.  Each
  * entry point names the grad.cpp interface it stands in for (paths relative to
- * the grad.cpp source tree).  All arithmetic is fp32 (but for gh_cache_*, which has 16-bit
- * types too); token ids are int32.
+ * the grad.cpp source tree).  All arithmetic is fp32 (but for gh_cache_* and gh_sample, which have
+ * 16-bit types too); token ids are int32.
  *
  * Threading: a model handle is immutable after creation and may be shared by
  * sessions on different host threads.  A session owns one HIP stream; calls on
@@ -334,6 +334,48 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
                           int32_t history_stride, int32_t n_history, const gh_sampling* opt,
                           const float* uniforms, uint64_t seed, int32_t pick_index, int32_t* out_ids,
                           void* hip_stream);
+
+/* ------------------------------------------------------- sampling, row by row */
+
+/* No counterpart in grad.cpp, whose sampler takes one set of options (text_gen.cpp:135-209): picks from
+ * logits that a program of its own layers has on the device, every row (request) with its own
+ * settings.  With x the row's logits and M the largest of them, w[i] = exp((x[i] - M) / temperature), in this order:
+ *   top_k   keeps the k largest logits, of equal ones the lowest indices (0 and less, or vocab and more: all);
+ *   top_p   keeps of those, in the same order, the shortest leading stretch whose w sum to p times
+ *           the sum of all of them, one at least (1 and more: all);
+ *   min_p   keeps of those the ones with w >= min_p (0 and less: all; above 1 counts as 1);
+ *   the pick is the lowest kept index up to which the kept w sum to the row's uniform times
+ *   their whole sum (a uniform of 0 and less, or NaN: the first that is kept; of 1 and more: the last).
+ * A temperature of 0 and less, or NaN, picks the largest logit, of equal ones the first, with probability 1.  NaN in a setting is
+ * as if it were off.  NaN among the logits is never picked, nor is minus infinity: a row that has nothing else
+ * gives -1 with probability 0.  Infinite logits share the row among themselves.  w below 2^-44 count as nothing.
+ * Sums and exponentials are 64-bit: a pick is the definition's wherever the uniform is not within some 2^-40
+ * of a border.  The same call gives the same bits.
+ *
+ * Every pointer is DEVICE memory of the caller's, on one device, which need not be the current one.  The work is enqueued
+ * on hip_stream (a hipStream_t of that device, NULL for its default stream) and the call returns without waiting; nothing
+ * is allocated, so a call may be captured into a graph.  Nothing is kept between calls. */
+typedef struct gh_sample_args {
+    const void* logits;       /* row r's begin at logits + r * row_stride (elements); any alignment of whole elements */
+    int64_t row_stride;       /* not negative; 0: every row is the same logits */
+    int32_t type;             /* GH_F32, GH_BF16, GH_F16 (of the paged cache, below): of the logits */
+    int32_t rows;             /* 0 to 2^24 */
+    int32_t vocab;            /* 1 to 2^20 */
+    int32_t reserved;         /* 0 */
+    const float* temperature; /* [rows] each, or NULL: 1, off, off, off */
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* uniforms;    /* [rows], from [0, 1) */
+    int32_t* ids;             /* [rows]: the picks */
+    float* probs;             /* [rows], or NULL: w of the pick over the sum of the kept w */
+    void* workspace;          /* of gh_sample_workspace bytes (NULL if that is 0), of any contents, aligned to 16 bytes; not shared
+                               * by calls that may overlap in time */
+    size_t workspace_bytes;
+} gh_sample_args;
+
+gh_status gh_sample_workspace(int32_t type, int32_t rows, int32_t vocab, size_t* bytes);
+gh_status gh_sample(const gh_sample_args* args, void* hip_stream);
 
 /* --------------------------------------------------------------- paged cache */
 
