@@ -8,8 +8,13 @@
 // 16-bit row has thousands) share one error, and one draw in a hundred from 128 k tokens of a flat row would be
 // another token than the definition's.  The card's 64-bit instructions have the rate of plain 32-bit ones.
 //
-// No order is ever sorted out over the whole row: a cut is found by histograms, of counts or of w, over buckets of x.  w are whole
-// numbers there (multiples of 2^-scale of the largest), so that the atomics' order does not matter.
+// The row is read once, in chunks: largest logits of groups of 64; where the sum of all w matters (no top-k), sums of segments of 512
+// relative to the chunk's largest; with top-p, w by buckets of x.  From these follows a bound below which nothing is kept:
+//   top-k: k groups have a logit of at least the k-th largest of the groups' largest;
+//   top-p: the bucket in which the running sum of w reaches p of the whole;   min-p: the logarithm.
+// Only groups that reach the bound are looked at again, the tokens above it become a list, are sorted, cut and drawn from.  What does not fit a list
+// (a nucleus of thousands of tokens) is cut by the bucket's tokens alone, or, where that is not enough, by histograms over the row,
+// and drawn from segment by segment.
 #pragma once
 
 #include "kernels_cache_attn.h"
@@ -19,8 +24,18 @@ namespace gh {
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kMaxSampleVocab = 1 << 20;
-constexpr int kBuckets = 2048;
-constexpr double kLeastPower = 44.0;  // w below 2^-44 of the largest are nothing: all of a million tokens together are below 2^-24
+constexpr int kVec = 8;                       // logits of a lane
+constexpr int kGroup = 64;                    // of eight lanes
+constexpr int kSegment = 64 * kVec;           // of a wavefront
+constexpr int kRound = kSampleThreads * kVec; // of the workgroup
+constexpr int kMaxRounds = 4;                 // in registers: a chunk
+constexpr int kMaxSegments = kMaxSampleVocab / kSegment;
+constexpr int kListed = 2048;                 // tokens that are sorted
+constexpr int kBuckets = 2048;                // of the histograms over the row
+constexpr double kLeastPower = 44.0;          // w below 2^-44 of the largest are nothing: all of a million tokens together are below 2^-24
+// w by buckets of x: so many to a power of two, on a grid that all chunks share
+constexpr int kMassBuckets = 1024;
+constexpr double kMassFine = 40.0;
 
 struct SampleParams {
     const void* logits;
@@ -34,41 +49,58 @@ struct SampleParams {
     const float* uniforms;
     int* ids;
     float* probs;
+    int first_row;
+    // what the chunks leave, of every row: [groups], [chunks], [segments], [chunks][kMassBuckets]
+    int chunks;
+    float* group_tops;
+    float* chunk_tops;
+    double* segment_sums;
+    unsigned long long* masses;
 };
+
+constexpr int groups_of(int vocab) { return (vocab + kGroup - 1) / kGroup; }
+constexpr int segments_of(int vocab) { return (vocab + kSegment - 1) / kSegment; }
 
 // Order-preserving whole numbers of floats.
 __device__ __forceinline__ unsigned order_key(float x) {
     const unsigned b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_move(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = dpp_move_int<CTRL, ROW_MASK>(static_cast<int>(b)), hi = dpp_move_int<CTRL, ROW_MASK>(static_cast<int>(b >> 32));
+    return __longlong_as_double(static_cast<long long>(hi) << 32 | static_cast<unsigned>(lo));
+}
+// Running total over the lanes, this lane's included.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += dpp_move<0x111, 0xF>(v);  // row_shr:1
+    v += dpp_move<0x112, 0xF>(v);
+    v += dpp_move<0x114, 0xF>(v);
+    v += dpp_move<0x118, 0xF>(v);
+    v += dpp_move<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp_move<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
+__device__ __forceinline__ unsigned long long wave_scan(unsigned long long v) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(v, d);
+        const unsigned long long o = __shfl_up(v, d);
         if (lane >= d) v += o;
     }
     return v;
 }
-// Total of the lanes before this one.
-template <typename T>
-__device__ __forceinline__ T wave_scan_before(T inclusive) {
-    const T o = __shfl_up(inclusive, 1);
-    return (threadIdx.x & 63) == 0 ? T(0) : o;
-}
+__device__ __forceinline__ int wave_scan(int v) { return wave_inclusive_scan(v); }
+
 // Totals over the workgroup's threads: of those before this one (exactly zero where they hold nothing), and of all.  `waves` is
 // scratch; every thread calls.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T* waves, T& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const T upto = wave_scan(v);
+    const T upto = wave_scan(v), shifted = __shfl_up(upto, 1);
     __syncthreads();
     if (lane == 63) waves[wave] = upto;
     __syncthreads();
@@ -79,44 +111,49 @@ __device__ __forceinline__ T block_scan(T v, T* waves, T& all) {
         sum += waves[w];
     }
     all = sum;
-    return before + wave_scan_before(upto);
+    return before + (lane == 0 ? T(0) : shifted);
 }
 
+// A row's logits, eight neighbours to a lane; NaN and what is behind the row are minus infinity, zeros of either sign are equal.
+// (Rows begin anywhere: loads of 16 bytes need no alignment.)
 template <int TYPE>
 struct SampleRow {
     using T = typename CacheType<TYPE>::T;
-    static constexpr int kVec = 16 / CacheType<TYPE>::kBytes;
     const T* at;
     int vocab;
-    int vectors;
-    __device__ __forceinline__ SampleRow(const SampleParams& p, int row)
-        : at(static_cast<const T*>(p.logits) + row * p.row_stride), vocab(p.vocab), vectors((p.vocab + kVec - 1) / kVec) {}
-    // Vector j's logits; NaN and what is behind the row are minus infinity.  (Rows begin anywhere: loads of 16 bytes need no alignment.)
-    __device__ __forceinline__ void load(int j, float (&x)[kVec]) const {
-        T e[kVec];
-        if ((j + 1) * kVec <= vocab) {
-            __builtin_memcpy(e, at + j * kVec, 16);
-#pragma unroll
-            for (int i = 0; i < kVec; i++) x[i] = static_cast<float>(e[i]);
+    __device__ __forceinline__ SampleRow(const SampleParams& p, int row) : at(static_cast<const T*>(p.logits) + row * p.row_stride), vocab(p.vocab) {}
+    static __device__ __forceinline__ float clean(T e) {
+        const float x = static_cast<float>(e);
+        return x == x ? x + 0.0f : -INFINITY;
+    }
+    __device__ __forceinline__ void load_raw(int i0, T (&e)[kVec]) const {
+        if (i0 + kVec <= vocab) {
+            __builtin_memcpy(e, at + i0, sizeof(e));
         } else {
 #pragma unroll
-            for (int i = 0; i < kVec; i++) x[i] = j * kVec + i < vocab ? static_cast<float>(at[j * kVec + i]) : -INFINITY;
+            for (int i = 0; i < kVec; i++) e[i] = i0 + i < vocab ? at[i0 + i] : static_cast<T>(-INFINITY);
         }
-#pragma unroll
-        for (int i = 0; i < kVec; i++) x[i] = x[i] == x[i] ? x[i] + 0.0f : -INFINITY;  // (zeros of either sign are equal)
     }
+    __device__ __forceinline__ void load(int i0, float (&x)[kVec]) const {
+        T e[kVec];
+        load_raw(i0, e);
+#pragma unroll
+        for (int i = 0; i < kVec; i++) x[i] = clean(e[i]);
+    }
+    __device__ __forceinline__ float one(int i) const { return i < vocab ? clean(at[i]) : -INFINITY; }
+    // Every logit, in any order.
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
-        for (int j = threadIdx.x; j < vectors; j += kSampleThreads) {
+        for (int i0 = threadIdx.x * kVec; i0 < vocab; i0 += kRound) {
             float x[kVec];
-            load(j, x);
+            load(i0, x);
 #pragma unroll
-            for (int i = 0; i < kVec; i++) f(x[i], j * kVec + i);
+            for (int i = 0; i < kVec; i++) f(x[i], i0 + i);
         }
     }
 };
 
-// What is kept: keys above `key`, and of those equal to it the indices up to `index`; of these, w of at least `least`.
+// What is kept: keys above `key`, and of those equal to it the indices up to `index`.
 struct Cut {
     unsigned key = 0;
     int index = 0x7FFFFFFF;
@@ -124,28 +161,145 @@ struct Cut {
 };
 
 struct SampleShared {
-    unsigned long long bins[kBuckets];
+    union {
+        unsigned long long bins[kBuckets];
+        unsigned counts[kBuckets];
+    };
+    unsigned long long list[kListed];
+    union {
+        double segments[kMaxSegments];
+        int hot[kListed];  // groups
+        double kept_weights[kListed];
+    };
+    double powers[64];  // 2^(j / 64)
+    float group_tops[kMaxRounds * kRound / kGroup];
     unsigned long long scan[kSampleWaves];
     double sums[kSampleWaves];
+    int ints[kSampleWaves];
     float tops[kSampleWaves];
-    int indices[kSampleWaves];
     unsigned low, high;
     unsigned long long above;  // of the histogram, before the bucket that was found
-    int bucket;
-    int found;
+    double mass_above;
+    int bucket, found, listed;
 };
 
+// exp((x - top) / T).  2^y for y = n / 64 + r, |r| <= 1 / 128: 2^(n / 64) from a table and the series of 2^r, cut off behind the
+// fourth power (relative error below 5e-14).  Exactly 1 at the top.
 struct SampleWeights {
     float top;
-    double turn;  // log2(e) / temperature
-    double scale;
-    __device__ __forceinline__ double power(float x) const { return x == top ? 0.0 : (static_cast<double>(x) - top) * turn; }
+    double turn;  // 64 log2(e) / T
+    const double* powers;
+    __device__ __forceinline__ double power64(float x) const { return x == top ? 0.0 : (static_cast<double>(x) - top) * turn; }
     __device__ __forceinline__ double weight(float x) const {
-        const double y = power(x);
-        return y > -kLeastPower ? exp2(y) : 0.0;
+        constexpr double kMagic = 0x1.8p52;
+        constexpr double l = 0.69314718055994530942 / 64, c2 = l * l / 2, c3 = l * l * l / 6, c4 = l * l * l * l / 24;
+        const double z = power64(x), t = z + kMagic, r = z - (t - kMagic);
+        const int n = static_cast<int>(__double_as_longlong(t));
+        const double head = powers[n & 63];
+        const double tail = r * fma(r, fma(r, fma(r, c4, c3), c2), l);
+        const double w = ldexp(fma(head, tail, head), n >> 6);
+        return z > -64.0 * kLeastPower ? w : 0.0;
     }
-    __device__ __forceinline__ unsigned long long whole(double w) const { return static_cast<unsigned long long>(__double_as_longlong(fma(w, scale, 0x1p52))) & 0xFFFFFFFFFFFFFull; }
 };
+
+__device__ __forceinline__ unsigned long long whole_number(double w, double scale) {
+    return static_cast<unsigned long long>(__double_as_longlong(fma(w, scale, 0x1p52))) & 0xFFFFFFFFFFFFFull;
+}
+
+// What a row's settings come to.
+struct SampleSettings {
+    float temperature;
+    int top_k;      // 0: off
+    double top_p;   // 1: off
+    double min_p;   // 0: off
+    __device__ __forceinline__ SampleSettings(const SampleParams& p, int r) {
+        temperature = p.temperature ? p.temperature[r] : 1.0f;
+        top_k = p.top_k ? p.top_k[r] : 0;
+        if (top_k < 0 || top_k >= p.vocab) top_k = 0;
+        const float tp = p.top_p ? p.top_p[r] : 1.0f, mp = p.min_p ? p.min_p[r] : 0.0f;
+        top_p = tp < 1.0f ? tp : 1.0f;
+        min_p = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
+    }
+    __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f); }
+    __device__ __forceinline__ double turn() const { return 64 * 1.44269504088896340736 / temperature; }
+    // the whole row's sum: by segments; by buckets as well
+    __device__ __forceinline__ bool sums() const { return !greedy() && top_k == 0 && (top_p < 1.0 || min_p == 0.0); }
+    __device__ __forceinline__ bool masses() const { return !greedy() && top_k == 0 && top_p < 1.0; }
+    // places are whole numbers below 2^31, a chunk's where the row's largest is below 2^29
+    __device__ __forceinline__ bool on_grid(float top, double limit = 0x1p30) const { return fabs(top * grid()) < limit; }
+    __device__ __forceinline__ double grid() const { return kMassFine * 1.44269504088896340736 / temperature; }
+};
+
+// The place on the grid: larger logits have larger ones.
+__device__ __forceinline__ int grid_place(float x, double grid) { return static_cast<int>(__double_as_longlong(fma(static_cast<double>(x), grid, 0x1.8p52))); }
+
+__device__ __forceinline__ void fill_powers(SampleShared& sh) {
+    if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(threadIdx.x / 64.0);
+}
+
+__device__ __forceinline__ float block_top(float v, SampleShared& sh) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.tops[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh.tops[0];
+#pragma unroll
+    for (int w = 1; w < kSampleWaves; w++) v = fmaxf(v, sh.tops[w]);
+    return v;
+}
+
+// One chunk of a row: [first, first + ROUNDS * kRound).  Leaves the groups' largest logits in sh.group_tops, and where they are wanted the segments'
+// sums, relative to the largest of the chunk, in sh.segments, and w by buckets of x, from the chunk's largest down, in sh.bins.  Returns the largest.
+// The powers have to be there.
+template <int TYPE, int ROUNDS>
+__device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, SampleShared& sh) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    typename SampleRow<TYPE>::T raw[ROUNDS][kVec];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) row.load_raw(first + r * kRound + static_cast<int>(threadIdx.x) * kVec, raw[r]);
+    fill_powers(sh);
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) {
+        float high = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kVec; i++) high = fmaxf(high, SampleRow<TYPE>::clean(raw[r][i]));
+        high = fmaxf(high, dpp_move<0xB1, 0xF>(high, high));   // over the eight lanes of a group
+        high = fmaxf(high, dpp_move<0x4E, 0xF>(high, high));
+        high = fmaxf(high, dpp_move<0x141, 0xF>(high, high));  // row_half_mirror
+        if ((lane & 7) == 0) sh.group_tops[r * (kRound / kGroup) + (threadIdx.x >> 3)] = high;
+        top = fmaxf(top, high);
+    }
+    top = block_top(top, sh);
+    if (!set.sums() || top == -INFINITY) return top;
+    const SampleWeights w{top, set.turn(), sh.powers};
+    const bool masses = set.masses() && set.on_grid(top);
+    const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52), grid = set.grid();
+    const int place = grid_place(top, grid);
+    if (masses) {
+        sh.bins[threadIdx.x] = 0;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            const float x = SampleRow<TYPE>::clean(raw[r][i]);
+            const double v = w.weight(x);
+            sum += v;
+            if (masses) {
+                const unsigned b = static_cast<unsigned>(place - grid_place(x, grid));
+                if (v > 0.0) atomicAdd(&sh.bins[min(b, kMassBuckets - 1u)], whole_number(v, scale));
+            }
+        }
+        sum = wave_scan(sum);
+        if (lane == 63) sh.segments[r * kSampleWaves + wave] = sum;
+    }
+    return top;
+}
+
+// ---------------------------------------------------------- histograms over the row
 
 // The bucket in which the running total of sh.bins, from bucket 0 on, reaches `target`, or all there is if that is less; for targets of zero
 // and less the first that holds anything.  The totals before it and of all are left in sh.above and `all`.
@@ -172,19 +326,20 @@ __device__ __forceinline__ int find_bucket(SampleShared& sh, double target, unsi
 // `target`.  Buckets of x relative to the largest first, then of the keys of one bucket, finer and finer, then equal keys by
 // their index.  Tokens whose w are nothing are left out.
 template <int TYPE, bool MASS>
-__device__ __forceinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, const Cut& kept, double target, SampleShared& sh) {
-    const double fine = kBuckets / kLeastPower;
-    const auto bucket_of = [&](float x) { return min(static_cast<int>(-w.power(x) * fine), kBuckets - 1); };
+__device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, double scale, const Cut& kept, double target, SampleShared& sh) {
+    const double fine = kBuckets / kLeastPower / 64;
+    const auto counts = [&](float x) { return w.power64(x) > -64 * kLeastPower; };
+    const auto bucket_of = [&](float x) { return min(static_cast<int>(-w.power64(x) * fine), kBuckets - 1); };
     const auto clear = [&] {
         __syncthreads();
         sh.bins[2 * threadIdx.x] = 0;
         sh.bins[2 * threadIdx.x + 1] = 0;
         __syncthreads();
     };
-    const auto amount = [&](float x) { return MASS ? w.whole(w.weight(x)) : 1ull; };
+    const auto amount = [&](float x) { return MASS ? whole_number(w.weight(x), scale) : 1ull; };
     clear();
     row.each([&](float x, int i) {
-        if (w.power(x) > -kLeastPower && kept.keeps(order_key(x), i)) atomicAdd(&sh.bins[bucket_of(x)], amount(x));
+        if (counts(x) && kept.keeps(order_key(x), i)) atomicAdd(&sh.bins[bucket_of(x)], amount(x));
     });
     unsigned long long all;
     const int bucket = find_bucket(sh, target, all);
@@ -196,7 +351,7 @@ __device__ __forceinline__ Cut find_cut(const SampleRow<TYPE>& row, const Sample
     }
     __syncthreads();
     row.each([&](float x, int i) {
-        if (w.power(x) > -kLeastPower && bucket_of(x) == bucket && kept.keeps(order_key(x), i)) {
+        if (counts(x) && bucket_of(x) == bucket && kept.keeps(order_key(x), i)) {
             atomicMin(&sh.low, order_key(x));
             atomicMax(&sh.high, order_key(x));
         }
@@ -216,117 +371,160 @@ __device__ __forceinline__ Cut find_cut(const SampleRow<TYPE>& row, const Sample
         if (high - low > (1u << shift) - 1) low = high - ((1u << shift) - 1);
     }
     // equal keys: so many of them, the lowest indices
-    const float x0 = __uint_as_float(low & 0x80000000u ? low ^ 0x80000000u : ~low);
-    const double each = static_cast<double>(amount(x0));
+    const double each = static_cast<double>(amount(key_value(low)));
     const double wanted = ceil((target - static_cast<double>(above)) / each);
     const int take = wanted < 1.0 ? 1 : wanted > 1e9 ? 1000000000 : static_cast<int>(wanted);
     Cut cut;
     cut.key = low;
     if (threadIdx.x == 0) sh.found = 0x7FFFFFFF;
     int counted = 0;
-    for (int j0 = 0; j0 < row.vectors && counted < take; j0 += kSampleThreads) {
-        const int j = j0 + threadIdx.x;
-        float x[SampleRow<TYPE>::kVec];
+    for (int from = 0; from < row.vocab && counted < take; from += kRound) {
+        const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
+        float x[kVec];
         unsigned equal = 0;
-        if (j < row.vectors) {
-            row.load(j, x);
+        if (i0 < row.vocab) {
+            row.load(i0, x);
 #pragma unroll
-            for (int i = 0; i < SampleRow<TYPE>::kVec; i++) {
-                const int index = j * SampleRow<TYPE>::kVec + i;
-                if (index < row.vocab && order_key(x[i]) == low && kept.keeps(low, index)) equal |= 1u << i;
-            }
+            for (int i = 0; i < kVec; i++)
+                if (i0 + i < row.vocab && order_key(x[i]) == low && kept.keeps(low, i0 + i)) equal |= 1u << i;
         }
-        const int before = counted + static_cast<int>(block_scan(static_cast<unsigned long long>(__popc(equal)), sh.scan, all));
+        int here;
+        const int before = counted + block_scan(static_cast<int>(__popc(equal)), sh.ints, here);
         if (before < take && before + __popc(equal) >= take) {
             for (int n = take - before; n > 1; n--) equal &= equal - 1;
-            sh.found = j * SampleRow<TYPE>::kVec + __ffs(equal) - 1;
+            sh.found = i0 + __ffs(equal) - 1;
         }
-        counted += static_cast<int>(all);
+        counted += here;
     }
     __syncthreads();
     cut.index = sh.found;
     return cut;
 }
 
-// One workgroup per row.
-template <int TYPE>
-__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const SampleParams p) {
-    using Row = SampleRow<TYPE>;
-    constexpr int kVec = Row::kVec;
-    constexpr int kSegments = kMaxSampleVocab / (64 * 4);
-    __shared__ SampleShared sh;
-    __shared__ double segments[kSegments];
-    const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Row row(p, r);
+// ------------------------------------------------------------------------ lists
 
-    // the largest logit and the lowest index that has it
-    float top = -INFINITY;
-    int first = 0x7FFFFFFF;
-    row.each([&](float x, int i) {
-        if (x > top) {
-            top = x;
-            first = i;
+// n numbers of sh.list in ascending order; what lies behind them, up to the next power of two, is overwritten.
+__device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
+    int size = 64;
+    while (size < n) size *= 2;
+    for (int i = n + static_cast<int>(threadIdx.x); i < size; i += kSampleThreads) sh.list[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            for (int i = threadIdx.x; i < size / 2; i += kSampleThreads) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;
+                const unsigned long long u = sh.list[a], v = sh.list[b];
+                if ((u > v) == ((a & k) == 0)) {
+                    sh.list[a] = v;
+                    sh.list[b] = u;
+                }
+            }
+            __syncthreads();
         }
-    });
-    wave_first_max(top, first);
-    if (lane == 0) {
-        sh.tops[wave] = top;
-        sh.indices[wave] = first;
+}
+
+// A place for each lane that `wants` one, counted in *count; one atomic for all of them.
+__device__ __forceinline__ int take_places(bool wants, int* count) {
+    const unsigned long long all = __ballot(wants);
+    if (all == 0) return 0;
+    int first = 0;
+    if ((threadIdx.x & 63) == 0) first = atomicAdd(count, __popcll(all));
+    first = __builtin_amdgcn_readfirstlane(first);
+    return first + __popcll(all & ((1ull << (threadIdx.x & 63)) - 1));
+}
+
+// The tokens that `may`, of the groups whose largest logit has `group_may`, into sh.list, by (key descending, index).  Returns how many; more
+// than kListed: the list is not whole.  Groups that hold one that `may` have `group_may`; `both`: the two are the same.
+template <int TYPE, typename TOPS, typename G, typename F>
+__device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS& group_top, SampleShared& sh, bool both, G&& group_may, F&& may) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = groups_of(row.vocab);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = sh.found = 0;
+    __syncthreads();
+    for (int g0 = 64 * wave; g0 < groups; g0 += kSampleThreads) {
+        const int g = g0 + lane;
+        const float t = g < groups ? group_top(g) : -INFINITY;
+        const bool hot = t > -INFINITY && group_may(t);
+        const int at = take_places(hot, &sh.found);
+        if (hot && at < kListed) sh.hot[at] = g;
     }
     __syncthreads();
-    for (int w = 0; w < kSampleWaves; w++)
-        if (sh.tops[w] > top || (sh.tops[w] == top && sh.indices[w] < first)) {
-            top = sh.tops[w];
-            first = sh.indices[w];
-        }
-    const float temperature = p.temperature ? p.temperature[r] : 1.0f;
-    if (top == -INFINITY || !(temperature > 0.0f)) {
-        if (threadIdx.x == 0) {
-            p.ids[r] = top == -INFINITY ? -1 : first;
-            if (p.probs) p.probs[r] = top == -INFINITY ? 0.0f : 1.0f;
-        }
-        return;
-    }
-    SampleWeights w{top, 1.44269504088896340736 / temperature, __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52)};
-
-    Cut cut;
-    const int top_k = p.top_k ? p.top_k[r] : 0;
-    if (top_k > 0 && top_k < p.vocab) cut = find_cut<TYPE, false>(row, w, cut, top_k, sh);
-    const float top_p = p.top_p ? p.top_p[r] : 1.0f;
-    if (top_p < 1.0f) {
-        unsigned long long mine = 0;
-        row.each([&](float x, int i) {
-            if (cut.keeps(order_key(x), i)) mine += w.whole(w.weight(x));
-        });
-        unsigned long long all;
-        (void)block_scan(mine, sh.scan, all);
-        cut = find_cut<TYPE, true>(row, w, cut, static_cast<double>(top_p) * static_cast<double>(all), sh);
-    }
-    const float min_p = p.min_p ? p.min_p[r] : 0.0f;
-    const double least = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
-    const auto kept = [&](float x, int i) {
-        const double v = cut.keeps(order_key(x), i) ? w.weight(x) : 0.0;
-        return v >= least ? v : 0.0;
+    const int hot = sh.found;
+    const auto add = [&](float x, int index) {
+        const bool wants = x > -INFINITY && may(x);
+        const int at = take_places(wants, &sh.listed);
+        if (wants && at < kListed) sh.list[at] = static_cast<unsigned long long>(~order_key(x)) << 32 | static_cast<unsigned>(index);
     };
-
-    // sums of what a wavefront reads at a time, in the order of the indices; the one in which the draw falls
-    const int count = (row.vectors + 63) / 64;
-    for (int s = wave; s < count; s += kSampleWaves) {
-        double sum = 0.0;
-        const int j = s * 64 + lane;
-        if (j < row.vectors) {
-            float x[kVec];
-            row.load(j, x);
+    if (hot <= kListed) {
+        for (int h = wave; h < hot; h += 4 * kSampleWaves) {
+            float x[4];
+            int index[4];
 #pragma unroll
-            for (int i = 0; i < kVec; i++) sum += kept(x[i], j * kVec + i);
+            for (int k = 0; k < 4; k++) {
+                const int g = h + k * kSampleWaves;
+                index[k] = g < hot ? sh.hot[g] * kGroup + lane : row.vocab;
+                x[k] = row.one(index[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) add(x[k], index[k]);
         }
-        sum = wave_sum(sum);
-        if (lane == 0) segments[s] = sum;
+    } else if (both) {
+        return hot;  // (each holds one at least)
+    } else {
+        for (int from = 0; from < row.vocab; from += kRound) {
+            const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
+            float x[kVec];
+            row.load(i0, x);
+#pragma unroll
+            for (int i = 0; i < kVec; i++) add(x[i], i0 + i);
+        }
     }
+    __syncthreads();
+    return sh.listed;
+}
+
+// Draws from the sorted list's first `kept` tokens, whose w are in sh.kept_weights: by their indices.
+__device__ __forceinline__ void draw_listed(const SampleParams& p, int r, int kept, SampleShared& sh) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kept; i += kSampleThreads) sh.list[i] = sh.list[i] << 32 | static_cast<unsigned>(i);  // (the key goes)
+    __syncthreads();
+    sort_list(sh, kept);
+    double v[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int i = 2 * threadIdx.x + k;
+        v[k] = i < kept ? sh.kept_weights[static_cast<unsigned>(sh.list[i])] : 0.0;
+    }
+    double total;
+    const double before = block_scan(v[0] + v[1], sh.sums, total);
+    const float u = p.uniforms[r];
+    const double target = (u > 0.0f ? static_cast<double>(u) : 0.0) * total;  // (NaN: 0)
+    if (threadIdx.x == 0) {
+        sh.low = 0xFFFFFFFFu;
+        sh.found = 0;
+    }
+    __syncthreads();
+    if (v[1] > 0.0 && before + v[0] + v[1] >= target) atomicMin(&sh.low, 2 * threadIdx.x + 1);
+    if (v[0] > 0.0 && before + v[0] >= target) atomicMin(&sh.low, 2 * threadIdx.x);
+    if (v[0] > 0.0) atomicMax(&sh.found, 2 * threadIdx.x + (v[1] > 0.0));
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int at = sh.low != 0xFFFFFFFFu ? static_cast<int>(sh.low) : sh.found;
+        p.ids[r] = static_cast<int>(sh.list[at] >> 32);
+        if (p.probs) p.probs[r] = static_cast<float>(sh.kept_weights[static_cast<unsigned>(sh.list[at])] / total);
+    }
+}
+
+// ------------------------------------------------------------- segments of the row
+
+// Draws from what `weight` keeps, segment by segment; sh.segments holds the segments' sums of it.
+template <int TYPE, typename F>
+__device__ __forceinline__ void draw_segments(const SampleParams& p, int r, const SampleRow<TYPE>& row, SampleShared& sh, F&& weight) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = segments_of(row.vocab);
     __syncthreads();
     const int each = (count + kSampleThreads - 1) / kSampleThreads, from = min(count, static_cast<int>(threadIdx.x) * each), to = min(count, from + each);
     double mine = 0.0;
-    for (int s = from; s < to; s++) mine += segments[s];
+    for (int s = from; s < to; s++) mine += sh.segments[s];
     if (threadIdx.x == 0) sh.found = -1;
     double total;
     const double before = block_scan(mine, sh.sums, total);
@@ -335,49 +533,314 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const Sample
     // the last segment whose running total before it is below the target, among those that hold anything
     double below = before;
     for (int s = from; s < to; s++) {
-        if (segments[s] > 0.0 && (below < target || below == 0.0)) atomicMax(&sh.found, s);
-        below += segments[s];
+        if (sh.segments[s] > 0.0 && (below < target || below == 0.0)) atomicMax(&sh.found, s);
+        below += sh.segments[s];
     }
     __syncthreads();
     const int segment = sh.found;
     if (segment >= from && segment < to) {
         below = before;
-        for (int s = from; s < segment; s++) below += segments[s];
+        for (int s = from; s < segment; s++) below += sh.segments[s];
         sh.sums[0] = below;
     }
     __syncthreads();
     if (wave != 0) return;
-    const int j = segment * 64 + lane;
+    const int i0 = segment * kSegment + lane * kVec;
     double v[kVec], sum = 0.0;
     float x[kVec];
+    row.load(i0, x);
 #pragma unroll
-    for (int i = 0; i < kVec; i++) v[i] = 0.0;
-    if (j < row.vectors) {
-        row.load(j, x);
-#pragma unroll
-        for (int i = 0; i < kVec; i++) sum += v[i] = kept(x[i], j * kVec + i);
-    }
-    double running = sh.sums[0] + wave_scan_before(wave_scan(sum));
-    int mine_hit = 0x7FFFFFFF, mine_last = -1;
+    for (int i = 0; i < kVec; i++) sum += v[i] = weight(x[i], i0 + i);
+    const double upto = wave_scan(sum), shifted = __shfl_up(upto, 1);
+    double running = sh.sums[0] + (lane == 0 ? 0.0 : shifted);
+    int hit = -1, last = -1;
     double hit_weight = 0.0, last_weight = 0.0;
 #pragma unroll
     for (int i = 0; i < kVec; i++) {
         running += v[i];
         if (v[i] > 0.0) {
-            mine_last = i;
+            last = i;
             last_weight = v[i];
-            if (running >= target && mine_hit == 0x7FFFFFFF) {
-                mine_hit = i;
+            if (running >= target && hit < 0) {
+                hit = i;
                 hit_weight = v[i];
             }
         }
     }
-    const unsigned long long hits = __ballot(mine_hit != 0x7FFFFFFF), lasts = __ballot(mine_last >= 0);
+    const unsigned long long hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
     const int chosen = hits ? __ffsll(hits) - 1 : 63 - __clzll(lasts);
     if (lane == chosen) {
-        p.ids[r] = j * kVec + (hits ? mine_hit : mine_last);
+        p.ids[r] = i0 + (hits ? hit : last);
         if (p.probs) p.probs[r] = static_cast<float>((hits ? hit_weight : last_weight) / total);
     }
+}
+
+// ----------------------------------------------------------------------- a row
+
+// From what the chunks left to the pick.  group_top(g), chunk_top(c), segment_sum(s) and mass(c, b), the last two relative to their chunk's
+// largest and only there where that is not minus infinity.
+template <int TYPE, typename GROUP, typename CHUNK, typename SEGMENT, typename MASS>
+__device__ __forceinline__ void pick_row(const SampleParams& p, int r, const SampleRow<TYPE>& row, const SampleSettings& set, int chunk, int chunks,
+                                         const GROUP& group_top, const CHUNK& chunk_top, const SEGMENT& segment_sum, const MASS& mass, SampleShared& sh) {
+    const int groups = groups_of(p.vocab);
+    float top = -INFINITY, low = INFINITY;  // of the groups' largest
+    for (int g = threadIdx.x; g < groups; g += kSampleThreads) {
+        const float t = group_top(g);
+        top = fmaxf(top, t);
+        if (t > -INFINITY) low = fminf(low, t);
+    }
+    top = block_top(top, sh);
+    if (top == -INFINITY) {
+        if (threadIdx.x == 0) {
+            p.ids[r] = -1;
+            if (p.probs) p.probs[r] = 0.0f;
+        }
+        return;
+    }
+    if (set.greedy()) {
+        if (threadIdx.x == 0) sh.low = 0xFFFFFFFFu;
+        __syncthreads();
+        for (int g = threadIdx.x; g < groups; g += kSampleThreads)
+            if (group_top(g) == top) atomicMin(&sh.low, static_cast<unsigned>(g));
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int g = static_cast<int>(sh.low);
+            const unsigned long long here = __ballot(row.one(g * kGroup + static_cast<int>(threadIdx.x)) == top);
+            if (threadIdx.x == 0) {
+                p.ids[r] = g * kGroup + __ffsll(here) - 1;
+                if (p.probs) p.probs[r] = 1.0f;
+            }
+        }
+        return;
+    }
+    const SampleWeights w{top, set.turn(), sh.powers};
+    const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52);
+    const int segments = segments_of(p.vocab);
+    const auto sum_of = [&](int s) {
+        const double share = w.weight(chunk_top(s * kSegment / chunk));
+        return share > 0.0 ? segment_sum(s) * share : 0.0;
+    };
+
+    if (set.sums() && set.top_p == 1.0) {  // nothing is cut
+        constexpr int kOwn = kMaxSegments / kSampleThreads;
+        double own[kOwn];
+#pragma unroll
+        for (int k = 0; k < kOwn; k++) {
+            const int s = static_cast<int>(threadIdx.x) + k * kSampleThreads;
+            own[k] = s < segments ? sum_of(s) : 0.0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kOwn; k++) sh.segments[threadIdx.x + k * kSampleThreads] = own[k];
+        draw_segments(p, r, row, sh, [&](float x, int) { return w.weight(x); });
+        return;
+    }
+
+    Cut cut;
+    double total = 0.0;  // of what top-p is a share of
+    int listed = kListed + 1;
+    if (set.top_k > 0) {
+        // buckets of the logits, from the largest down, and the one that holds the k-th largest of the groups' largest, or of all where groups are few
+        if (set.top_k <= kListed) {
+            low = -block_top(-low, sh);
+            double fine = 0.0;
+            const auto bucket_of = [&](float x) { return x == top ? 0 : static_cast<int>(fmin((static_cast<double>(top) - x) * fine, 1e9)); };
+            int bound = kBuckets;
+            for (int by_group = 4 * set.top_k <= 3 * groups; by_group >= 0 && bound == kBuckets; by_group--) {
+                fine = by_group ? (kBuckets - 1) / fmax(static_cast<double>(top) - low, 1e-300) : kBuckets / kLeastPower / 64 * w.turn;
+                __syncthreads();
+                sh.counts[threadIdx.x] = 0;
+                sh.counts[threadIdx.x + kSampleThreads] = 0;
+                if (threadIdx.x == 0) sh.bucket = kBuckets;
+                __syncthreads();
+                const auto count = [&](float x, int) {
+                    if (!(x > -INFINITY)) return;
+                    if (const int b = bucket_of(x); b < kBuckets) atomicAdd(&sh.counts[b], 1u);
+                };
+                if (by_group) {
+                    for (int g = threadIdx.x; g < groups; g += kSampleThreads) count(group_top(g), 0);
+                } else {
+                    row.each(count);
+                }
+                __syncthreads();
+                const int a = static_cast<int>(sh.counts[2 * threadIdx.x]), b = static_cast<int>(sh.counts[2 * threadIdx.x + 1]);
+                int all;
+                const int before = block_scan(a + b, sh.ints, all);
+                if (before < set.top_k && before + a >= set.top_k) sh.bucket = 2 * threadIdx.x;
+                if (before + a < set.top_k && before + a + b >= set.top_k) sh.bucket = 2 * threadIdx.x + 1;
+                __syncthreads();
+                bound = sh.bucket;
+            }
+            // (none: fewer than k tokens have a w)
+            const auto may = [&](float x) { return bucket_of(x) <= bound; };
+            listed = make_list(row, group_top, sh, true, may, may);
+        }
+        if (listed > kListed) {
+            cut = find_cut<TYPE, false>(row, w, scale, cut, set.top_k, sh);
+            if (set.top_p < 1.0) {
+                unsigned long long mine = 0, all;
+                row.each([&](float x, int i) {
+                    if (cut.keeps(order_key(x), i)) mine += whole_number(w.weight(x), scale);
+                });
+                (void)block_scan(mine, sh.scan, all);
+                cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
+            }
+        }
+    } else if (set.top_p < 1.0) {
+        double mine = 0.0;
+        for (int s = threadIdx.x; s < segments; s += kSampleThreads) mine += sum_of(s);
+        (void)block_scan(mine, sh.sums, total);
+        const double target = set.top_p * total;
+        int bound = kMassBuckets;
+        const double grid = set.grid();
+        const int place = grid_place(top, grid);
+        if (set.on_grid(top, 0x1p29)) {
+            // w by buckets, of all chunks, and the one in which their running sum reaches the target
+            double own = 0.0;
+            for (int c = 0; c < chunks; c++) {
+                const float t = chunk_top(c);
+                const double share = w.weight(t);
+                if (!(share > 0.0)) continue;
+                const int b = static_cast<int>(threadIdx.x) - (place - grid_place(t, grid));
+                if (b >= 0) own += static_cast<double>(mass(c, b)) * share;
+            }
+            own /= scale;
+            if (threadIdx.x == 0) sh.bucket = kMassBuckets;
+            double all;
+            const double before = block_scan(own, sh.sums, all);
+            if (own > 0.0 && (before < target || before == 0.0) && before + own >= target) {
+                sh.bucket = threadIdx.x;
+                sh.mass_above = before;
+            }
+            __syncthreads();
+            bound = sh.bucket;
+        }
+        if (bound < kMassBuckets - 1) {  // (a chunk's last bucket holds what is further down as well)
+            const double above = sh.mass_above;
+            const auto bucket_of = [&](float x) { return w.power64(x) > -64 * kLeastPower ? place - grid_place(x, grid) : kMassBuckets; };
+            const auto reaches = [&](float x) { return bucket_of(x) <= bound; };
+            const auto may = [&](float x) { return reaches(x) && w.weight(x) >= set.min_p; };
+            listed = make_list(row, group_top, sh, true, may, may);
+            if (listed > kListed) {  // the bucket's own tokens say where the cut is
+                const int own = make_list(row, group_top, sh, false, reaches, [&](float x) { return bucket_of(x) == bound; });
+                if (own <= kListed) {
+                    sort_list(sh, own);
+                    double v[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int i = 2 * static_cast<int>(threadIdx.x) + k;
+                        v[k] = i < own ? w.weight(key_value(~static_cast<unsigned>(sh.list[i] >> 32))) : 0.0;
+                    }
+                    double all;
+                    const double before = above + block_scan(v[0] + v[1], sh.sums, all);
+                    if (threadIdx.x == 0) sh.found = 0;
+                    __syncthreads();
+                    if (v[1] > 0.0 && before + v[0] < target) atomicMax(&sh.found, 2 * static_cast<int>(threadIdx.x) + 1);
+                    if (v[0] > 0.0 && before < target) atomicMax(&sh.found, 2 * static_cast<int>(threadIdx.x));
+                    __syncthreads();
+                    cut.key = ~static_cast<unsigned>(sh.list[sh.found] >> 32);
+                    cut.index = static_cast<int>(static_cast<unsigned>(sh.list[sh.found]));
+                    bound = -1;
+                }
+            }
+        }
+        if (listed > kListed && bound >= 0) {
+            unsigned long long whole = 0, all;
+            row.each([&](float x, int) { whole += whole_number(w.weight(x), scale); });
+            (void)block_scan(whole, sh.scan, all);
+            cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
+        }
+    } else {
+        const auto may = [&](float x) { return w.weight(x) >= set.min_p; };
+        listed = make_list(row, group_top, sh, true, may, may);
+    }
+
+    if (listed <= kListed) {
+        sort_list(sh, listed);
+        if (set.top_k > 0) listed = min(listed, set.top_k);
+        double v[2], all;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = 2 * static_cast<int>(threadIdx.x) + k;
+            v[k] = i < listed ? w.weight(key_value(~static_cast<unsigned>(sh.list[i] >> 32))) : 0.0;
+        }
+        const double before = block_scan(v[0] + v[1], sh.sums, all);
+        if (set.top_k > 0) total = all;
+        const double target = set.top_p < 1.0 ? set.top_p * total : INFINITY;
+        // (all cuts leave the first of what there is: v falls and the sum before it grows)
+        const int kept0 = v[0] > 0.0 && (threadIdx.x == 0 || (before < target && v[0] >= set.min_p));
+        const int kept1 = v[1] > 0.0 && before + v[0] < target && v[1] >= set.min_p;
+        int kept;
+        (void)block_scan(kept0 + kept1, sh.ints, kept);
+        __syncthreads();
+        sh.kept_weights[2 * threadIdx.x] = v[0];
+        sh.kept_weights[2 * threadIdx.x + 1] = v[1];
+        draw_listed(p, r, kept, sh);
+        return;
+    }
+    const auto weight = [&](float x, int i) {
+        const double v = cut.keeps(order_key(x), i) ? w.weight(x) : 0.0;
+        return v >= set.min_p ? v : 0.0;
+    };
+    __syncthreads();
+    for (int s = threadIdx.x >> 6; s < segments; s += kSampleWaves) {
+        const int i0 = s * kSegment + static_cast<int>(threadIdx.x & 63) * kVec;
+        float x[kVec];
+        row.load(i0, x);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kVec; i++) sum += weight(x[i], i0 + i);
+        sum = wave_scan(sum);
+        if ((threadIdx.x & 63) == 63) sh.segments[s] = sum;
+    }
+    draw_segments(p, r, row, sh, weight);
+}
+
+// A row of one chunk, from its logits to the pick.
+template <int TYPE, int ROUNDS>
+__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const SampleParams p) {
+    __shared__ SampleShared sh;
+    const int r = p.first_row + static_cast<int>(blockIdx.x);
+    const SampleRow<TYPE> row(p, r);
+    const SampleSettings set(p, r);
+    const float top = scan_chunk<TYPE, ROUNDS>(p, row, set, 0, sh);
+    __syncthreads();
+    pick_row(p, r, row, set, ROUNDS * kRound, 1, [&](int g) { return sh.group_tops[g]; }, [&](int) { return top; },
+             [&](int s) { return sh.segments[s]; }, [&](int, int b) { return sh.bins[b]; }, sh);
+}
+
+// One chunk of a row, for sample_pick_kernel.
+template <int TYPE, int ROUNDS>
+__global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(const SampleParams p) {
+    __shared__ SampleShared sh;
+    const int c = static_cast<int>(blockIdx.x) % p.chunks, r = p.first_row + static_cast<int>(blockIdx.x) / p.chunks;
+    const SampleRow<TYPE> row(p, r);
+    const SampleSettings set(p, r);
+    const float top = scan_chunk<TYPE, ROUNDS>(p, row, set, c * ROUNDS * kRound, sh);
+    __syncthreads();
+    constexpr int kGroups = ROUNDS * kRound / kGroup, kSegments = ROUNDS * kRound / kSegment;
+    const int t = threadIdx.x;
+    if (const int g = c * kGroups + t; t < kGroups && g < groups_of(p.vocab)) p.group_tops[static_cast<size_t>(r) * groups_of(p.vocab) + g] = sh.group_tops[t];
+    if (t == 0) p.chunk_tops[static_cast<size_t>(r) * p.chunks + c] = top;
+    if (top == -INFINITY) return;
+    if (const int s = c * kSegments + t; set.sums() && t < kSegments && s < segments_of(p.vocab))
+        p.segment_sums[static_cast<size_t>(r) * segments_of(p.vocab) + s] = sh.segments[t];
+    if (set.masses() && set.on_grid(top)) p.masses[(static_cast<size_t>(r) * p.chunks + c) * kMassBuckets + t] = sh.bins[t];
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(const SampleParams p, int chunk) {
+    __shared__ SampleShared sh;
+    const int r = p.first_row + static_cast<int>(blockIdx.x);
+    const SampleRow<TYPE> row(p, r);
+    const SampleSettings set(p, r);
+    fill_powers(sh);
+    const float* const group_tops = p.group_tops + static_cast<size_t>(r) * groups_of(p.vocab);
+    const float* const chunk_tops = p.chunk_tops + static_cast<size_t>(r) * p.chunks;
+    const double* const segment_sums = p.segment_sums + static_cast<size_t>(r) * segments_of(p.vocab);
+    const unsigned long long* const masses = p.masses + static_cast<size_t>(r) * p.chunks * kMassBuckets;
+    pick_row(p, r, row, set, chunk, p.chunks, [&](int g) { return group_tops[g]; }, [&](int c) { return chunk_tops[c]; },
+             [&](int s) { return segment_sums[s]; }, [&](int c, int b) { return masses[c * kMassBuckets + b]; }, sh);
 }
 
 }  // namespace gh

@@ -12,17 +12,62 @@ static void check_sizes(int type, int rows, int vocab) {
     if (vocab < 1 || vocab > kMaxSampleVocab) refuse("vocab must be 1 to 2^20");
 }
 
-static size_t sample_workspace(int type, int rows, int vocab) {
-    check_sizes(type, rows, vocab);
-    return 0;
+// Rows of one chunk are picked from by the workgroup that reads them.  Longer ones are read in chunks by as many workgroups, large chunks where
+// they keep every compute unit busy.
+struct SampleForm {
+    int rounds = 0;
+    int chunks = 1;
+    size_t group_tops = 0, chunk_tops = 0, segment_sums = 0, masses = 0, bytes = 0;  // places in the workspace
+};
+
+static SampleForm form_of(int rows, int vocab) {
+    SampleForm f;
+    if (vocab <= kMaxRounds * kRound) {
+        f.rounds = vocab <= kRound ? 1 : vocab <= 2 * kRound ? 2 : 4;
+        return f;
+    }
+    const auto chunks = [&](int rounds) { return (vocab + rounds * kRound - 1) / (rounds * kRound); };
+    f.rounds = static_cast<long long>(rows) * chunks(4) >= 256 ? 4 : 1;
+    f.chunks = chunks(f.rounds);
+    const auto place = [&](size_t per_row) {
+        const size_t at = f.bytes;
+        f.bytes += (per_row * static_cast<size_t>(rows) + 15) / 16 * 16;
+        return at;
+    };
+    f.group_tops = place(sizeof(float) * groups_of(vocab));
+    f.chunk_tops = place(sizeof(float) * f.chunks);
+    f.segment_sums = place(sizeof(double) * segments_of(vocab));
+    f.masses = place(sizeof(unsigned long long) * kMassBuckets * f.chunks);
+    return f;
+}
+
+template <int TYPE>
+static void launch_sample(SampleParams p, const SampleForm& f, int rows, hipStream_t stream) {
+    // (a launch holds at most 2^32 threads)
+    const int slice = (1 << 21) / f.chunks;
+    for (p.first_row = 0; p.first_row < rows; p.first_row += slice) {
+        const int n = std::min(slice, rows - p.first_row);
+        if (f.chunks == 1) {
+            const auto kernel = f.rounds == 1 ? sample_row_kernel<TYPE, 1> : f.rounds == 2 ? sample_row_kernel<TYPE, 2> : sample_row_kernel<TYPE, 4>;
+            hipLaunchKernelGGL(kernel, dim3(n), dim3(kSampleThreads), 0, stream, p);
+        } else {
+            const auto kernel = f.rounds == 1 ? sample_scan_kernel<TYPE, 1> : sample_scan_kernel<TYPE, 4>;
+            hipLaunchKernelGGL(kernel, dim3(n * f.chunks), dim3(kSampleThreads), 0, stream, p);
+            HIP_CHECK(hipGetLastError());
+            hipLaunchKernelGGL(sample_pick_kernel<TYPE>, dim3(n), dim3(kSampleThreads), 0, stream, p, f.rounds * kRound);
+        }
+        HIP_CHECK(hipGetLastError());
+    }
 }
 
 static void sample(const gh_sample_args& a, hipStream_t stream) {
-    const size_t need = sample_workspace(a.type, a.rows, a.vocab);
+    check_sizes(a.type, a.rows, a.vocab);
+    const SampleForm f = form_of(a.rows, a.vocab);
     if (a.row_stride < 0) refuse("negative row_stride");
     if (a.rows == 0) return;
     if (!a.logits || !a.uniforms || !a.ids) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
-    if (need > 0 && (!a.workspace || a.workspace_bytes < need)) refuse("a workspace of " + std::to_string(need) + " bytes is needed");
+    if (f.bytes > 0 && (!a.workspace || a.workspace_bytes < f.bytes)) refuse("a workspace of " + std::to_string(f.bytes) + " bytes is needed");
+    if (f.bytes > 0 && reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) refuse("the workspace is not aligned to 16 bytes");
     require_gpu();
     hipPointerAttribute_t at{};
     if (hipPointerGetAttributes(&at, a.logits) != hipSuccess || (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)) {
@@ -44,9 +89,15 @@ static void sample(const gh_sample_args& a, hipStream_t stream) {
     p.uniforms = a.uniforms;
     p.ids = a.ids;
     p.probs = a.probs;
-    const auto kernel = a.type == GH_F32 ? sample_row_kernel<kCacheF32> : a.type == GH_BF16 ? sample_row_kernel<kCacheBf16> : sample_row_kernel<kCacheF16>;
-    hipLaunchKernelGGL(kernel, dim3(a.rows), dim3(kSampleThreads), 0, stream, p);
-    HIP_CHECK(hipGetLastError());
+    char* const work = static_cast<char*>(a.workspace);
+    p.chunks = f.chunks;
+    p.group_tops = reinterpret_cast<float*>(work + f.group_tops);
+    p.chunk_tops = reinterpret_cast<float*>(work + f.chunk_tops);
+    p.segment_sums = reinterpret_cast<double*>(work + f.segment_sums);
+    p.masses = reinterpret_cast<unsigned long long*>(work + f.masses);
+    if (a.type == GH_F32) launch_sample<kCacheF32>(p, f, a.rows, stream);
+    else if (a.type == GH_BF16) launch_sample<kCacheBf16>(p, f, a.rows, stream);
+    else launch_sample<kCacheF16>(p, f, a.rows, stream);
 }
 
 }  // namespace gh
@@ -58,7 +109,8 @@ extern "C" {
 gh_status gh_sample_workspace(int32_t type, int32_t rows, int32_t vocab, size_t* bytes) {
     return guard([&] {
         if (!bytes) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
-        *bytes = sample_workspace(type, rows, vocab);
+        check_sizes(type, rows, vocab);
+        *bytes = form_of(rows, vocab).bytes;
     });
 }
 
