@@ -21,14 +21,15 @@
 
 namespace gh {
 
-constexpr int kSampleThreads = 1024;
+constexpr int kSampleThreads = 256;  // that pick: most of it is steps one behind the other, which four wavefronts take in less time than sixteen
 constexpr int kSampleWaves = kSampleThreads / 64;
+constexpr int kWideThreads = 1024;  // that read large chunks
 constexpr int kMaxSampleVocab = 1 << 20;
-constexpr int kVec = 8;                       // logits of a lane
-constexpr int kGroup = 64;                    // of eight lanes
-constexpr int kSegment = 64 * kVec;           // of a wavefront
-constexpr int kRound = kSampleThreads * kVec; // of the workgroup
-constexpr int kMaxRounds = 4;                 // in registers: a chunk
+constexpr int kVec = 8;               // logits of a lane
+constexpr int kGroup = 64;            // of eight lanes
+constexpr int kSegment = 64 * kVec;   // of a wavefront
+constexpr int kRounds = 4;            // vectors of a thread, in registers: a chunk
+constexpr int kChunk = kSampleThreads * kVec * kRounds, kWideChunk = kWideThreads * kVec * kRounds;
 constexpr int kMaxSegments = kMaxSampleVocab / kSegment;
 constexpr int kListed = 2048;                 // tokens that are sorted
 constexpr int kBuckets = 2048;                // of the histograms over the row
@@ -50,6 +51,7 @@ struct SampleParams {
     int* ids;
     float* probs;
     int first_row;
+    double powers[64];  // 2^(j / 64)
     // what the chunks leave, of every row: [groups], [chunks], [segments], [chunks][kMassBuckets]
     int chunks;
     float* group_tops;
@@ -96,7 +98,7 @@ __device__ __forceinline__ unsigned long long wave_scan(unsigned long long v) {
 __device__ __forceinline__ int wave_scan(int v) { return wave_inclusive_scan(v); }
 
 // Totals over the workgroup's threads: of those before this one (exactly zero where they hold nothing), and of all.  `waves` is
-// scratch; every thread calls.
+// scratch; every thread calls.  (Of the threads that pick.)
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T* waves, T& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -141,14 +143,20 @@ struct SampleRow {
         for (int i = 0; i < kVec; i++) x[i] = clean(e[i]);
     }
     __device__ __forceinline__ float one(int i) const { return i < vocab ? clean(at[i]) : -INFINITY; }
-    // Every logit, in any order.
+    // Every logit, in any order, f called by all threads alike; many loads at a time, or each would be a trip to memory of its own.
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
-        for (int i0 = threadIdx.x * kVec; i0 < vocab; i0 += kRound) {
-            float x[kVec];
-            load(i0, x);
+        constexpr int kDeep = 16;
+        for (int from = 0; from < vocab; from += kDeep * kSampleThreads * kVec) {
+            T e[kDeep][kVec];
 #pragma unroll
-            for (int i = 0; i < kVec; i++) f(x[i], i0 + i);
+            for (int k = 0; k < kDeep; k++) load_raw(from + (k * kSampleThreads + static_cast<int>(threadIdx.x)) * kVec, e[k]);
+#pragma unroll
+            for (int k = 0; k < kDeep; k++) {
+                if (from + k * kSampleThreads * kVec >= vocab) break;
+#pragma unroll
+                for (int i = 0; i < kVec; i++) f(clean(e[k][i]), from + (k * kSampleThreads + static_cast<int>(threadIdx.x)) * kVec + i);
+            }
         }
     }
 };
@@ -160,7 +168,17 @@ struct Cut {
     __device__ __forceinline__ bool keeps(unsigned k, int i) const { return k > key || (k == key && i <= index); }
 };
 
-struct SampleShared {
+// What a chunk leaves.
+template <int THREADS>
+struct ChunkShared {
+    unsigned long long masses[kMassBuckets];
+    double segments[THREADS * kVec * kRounds / kSegment];
+    double powers[64];  // 2^(j / 64)
+    float group_tops[THREADS * kVec * kRounds / kGroup];
+    float tops[THREADS / 64];
+};
+
+struct PickShared {
     union {
         unsigned long long bins[kBuckets];
         unsigned counts[kBuckets];
@@ -169,10 +187,12 @@ struct SampleShared {
     union {
         double segments[kMaxSegments];
         int hot[kListed];  // groups
-        double kept_weights[kListed];
+        double weights[kListed];
     };
-    double powers[64];  // 2^(j / 64)
-    float group_tops[kMaxRounds * kRound / kGroup];
+    unsigned ranks[kSampleThreads];
+    double powers[64];
+    double chunk_sums[kMaxSampleVocab / kChunk];
+    float chunk_tops[kMaxSampleVocab / kChunk];
     unsigned long long scan[kSampleWaves];
     double sums[kSampleWaves];
     int ints[kSampleWaves];
@@ -233,68 +253,67 @@ struct SampleSettings {
 // The place on the grid: larger logits have larger ones.
 __device__ __forceinline__ int grid_place(float x, double grid) { return static_cast<int>(__double_as_longlong(fma(static_cast<double>(x), grid, 0x1.8p52))); }
 
-__device__ __forceinline__ void fill_powers(SampleShared& sh) {
-    if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(threadIdx.x / 64.0);
+__device__ __forceinline__ void fill_powers(const SampleParams& p, double* powers) {
+    if (threadIdx.x < 64) powers[threadIdx.x] = p.powers[threadIdx.x];
 }
 
-__device__ __forceinline__ float block_top(float v, SampleShared& sh) {
+template <int THREADS>
+__device__ __forceinline__ float block_top(float v, float* tops) {
     v = wave_max(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.tops[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = sh.tops[0];
+    v = tops[0];
 #pragma unroll
-    for (int w = 1; w < kSampleWaves; w++) v = fmaxf(v, sh.tops[w]);
+    for (int w = 1; w < THREADS / 64; w++) v = fmaxf(v, tops[w]);
     return v;
 }
 
-// One chunk of a row: [first, first + ROUNDS * kRound).  Leaves the groups' largest logits in sh.group_tops, and where they are wanted the segments'
-// sums, relative to the largest of the chunk, in sh.segments, and w by buckets of x, from the chunk's largest down, in sh.bins.  Returns the largest.
-// The powers have to be there.
-template <int TYPE, int ROUNDS>
-__device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, SampleShared& sh) {
+// One chunk of a row, from `first` on.  Leaves the groups' largest logits, and where they are wanted the segments' sums, relative to the largest of
+// the chunk, and w by buckets of x, from the chunk's largest down.  Returns the largest.
+template <int TYPE, int THREADS>
+__device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, ChunkShared<THREADS>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    typename SampleRow<TYPE>::T raw[ROUNDS][kVec];
+    typename SampleRow<TYPE>::T raw[kRounds][kVec];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; r++) row.load_raw(first + r * kRound + static_cast<int>(threadIdx.x) * kVec, raw[r]);
-    fill_powers(sh);
+    for (int r = 0; r < kRounds; r++) row.load_raw(first + (r * THREADS + static_cast<int>(threadIdx.x)) * kVec, raw[r]);
+    fill_powers(p, sh.powers);
     float top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < ROUNDS; r++) {
+    for (int r = 0; r < kRounds; r++) {
         float high = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kVec; i++) high = fmaxf(high, SampleRow<TYPE>::clean(raw[r][i]));
         high = fmaxf(high, dpp_move<0xB1, 0xF>(high, high));   // over the eight lanes of a group
         high = fmaxf(high, dpp_move<0x4E, 0xF>(high, high));
         high = fmaxf(high, dpp_move<0x141, 0xF>(high, high));  // row_half_mirror
-        if ((lane & 7) == 0) sh.group_tops[r * (kRound / kGroup) + (threadIdx.x >> 3)] = high;
+        if ((lane & 7) == 0) sh.group_tops[r * (THREADS * kVec / kGroup) + (threadIdx.x >> 3)] = high;
         top = fmaxf(top, high);
     }
-    top = block_top(top, sh);
+    const bool masses = set.masses();
+    if (masses)
+        for (int b = threadIdx.x; b < kMassBuckets; b += THREADS) sh.masses[b] = 0;
+    top = block_top<THREADS>(top, sh.tops);
     if (!set.sums() || top == -INFINITY) return top;
     const SampleWeights w{top, set.turn(), sh.powers};
-    const bool masses = set.masses() && set.on_grid(top);
     const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52), grid = set.grid();
     const int place = grid_place(top, grid);
-    if (masses) {
-        sh.bins[threadIdx.x] = 0;
-        __syncthreads();
-    }
+    const bool counts = masses && set.on_grid(top);
 #pragma unroll
-    for (int r = 0; r < ROUNDS; r++) {
+    for (int r = 0; r < kRounds; r++) {
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < kVec; i++) {
             const float x = SampleRow<TYPE>::clean(raw[r][i]);
             const double v = w.weight(x);
             sum += v;
-            if (masses) {
+            if (counts && v > 0.0) {
                 const unsigned b = static_cast<unsigned>(place - grid_place(x, grid));
-                if (v > 0.0) atomicAdd(&sh.bins[min(b, kMassBuckets - 1u)], whole_number(v, scale));
+                atomicAdd(&sh.masses[min(b, kMassBuckets - 1u)], whole_number(v, scale));
             }
         }
         sum = wave_scan(sum);
-        if (lane == 63) sh.segments[r * kSampleWaves + wave] = sum;
+        if (lane == 63) sh.segments[r * (THREADS / 64) + wave] = sum;
     }
     return top;
 }
@@ -303,20 +322,21 @@ __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleR
 
 // The bucket in which the running total of sh.bins, from bucket 0 on, reaches `target`, or all there is if that is less; for targets of zero
 // and less the first that holds anything.  The totals before it and of all are left in sh.above and `all`.
-__device__ __forceinline__ int find_bucket(SampleShared& sh, double target, unsigned long long& all) {
+__device__ __forceinline__ int find_bucket(PickShared& sh, double target, unsigned long long& all) {
+    constexpr int kOwn = kBuckets / kSampleThreads;
     __syncthreads();
-    const unsigned long long a = sh.bins[2 * threadIdx.x], b = sh.bins[2 * threadIdx.x + 1];
-    const unsigned long long before = block_scan(a + b, sh.scan, all);
+    unsigned long long own[kOwn], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) sum += own[k] = sh.bins[kOwn * threadIdx.x + k];
+    unsigned long long before = block_scan(sum, sh.scan, all);
     target = fmin(target, static_cast<double>(all));
-    const auto first = [&](unsigned long long sum_before, unsigned long long own) {
-        return own > 0 && (sum_before == 0 || static_cast<double>(sum_before) < target) && static_cast<double>(sum_before + own) >= target;
-    };
-    if (first(before, a)) {
-        sh.bucket = 2 * threadIdx.x;
-        sh.above = before;
-    } else if (first(before + a, b)) {
-        sh.bucket = 2 * threadIdx.x + 1;
-        sh.above = before + a;
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) {
+        if (own[k] > 0 && (before == 0 || static_cast<double>(before) < target) && static_cast<double>(before + own[k]) >= target) {
+            sh.bucket = kOwn * static_cast<int>(threadIdx.x) + k;
+            sh.above = before;
+        }
+        before += own[k];
     }
     __syncthreads();
     return sh.bucket;
@@ -326,14 +346,13 @@ __device__ __forceinline__ int find_bucket(SampleShared& sh, double target, unsi
 // `target`.  Buckets of x relative to the largest first, then of the keys of one bucket, finer and finer, then equal keys by
 // their index.  Tokens whose w are nothing are left out.
 template <int TYPE, bool MASS>
-__device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, double scale, const Cut& kept, double target, SampleShared& sh) {
+__device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, double scale, const Cut& kept, double target, PickShared& sh) {
     const double fine = kBuckets / kLeastPower / 64;
     const auto counts = [&](float x) { return w.power64(x) > -64 * kLeastPower; };
     const auto bucket_of = [&](float x) { return min(static_cast<int>(-w.power64(x) * fine), kBuckets - 1); };
     const auto clear = [&] {
         __syncthreads();
-        sh.bins[2 * threadIdx.x] = 0;
-        sh.bins[2 * threadIdx.x + 1] = 0;
+        for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.bins[b] = 0;
         __syncthreads();
     };
     const auto amount = [&](float x) { return MASS ? whole_number(w.weight(x), scale) : 1ull; };
@@ -378,7 +397,7 @@ __device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWei
     cut.key = low;
     if (threadIdx.x == 0) sh.found = 0x7FFFFFFF;
     int counted = 0;
-    for (int from = 0; from < row.vocab && counted < take; from += kRound) {
+    for (int from = 0; from < row.vocab && counted < take; from += kSampleThreads * kVec) {
         const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
         float x[kVec];
         unsigned equal = 0;
@@ -403,10 +422,26 @@ __device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWei
 
 // ------------------------------------------------------------------------ lists
 
-// n numbers of sh.list in ascending order; what lies behind them, up to the next power of two, is overwritten.
-__device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
+// n different numbers of sh.list in ascending order; what lies behind them, up to the next power of two, is overwritten.  Few are put in their places by
+// counting how many are smaller, shared among the threads; more are sorted by pairs (each of its steps is a meeting of all).
+__device__ __forceinline__ void sort_list(PickShared& sh, int n) {
     int size = 64;
     while (size < n) size *= 2;
+    if (size <= kSampleThreads) {
+        const int e = static_cast<int>(threadIdx.x) & (size - 1), parts = kSampleThreads / size, part = static_cast<int>(threadIdx.x) / size;
+        const int each = (n + parts - 1) / parts, from = part * each, to = min(n, from + each);
+        sh.ranks[threadIdx.x] = 0;
+        __syncthreads();
+        const unsigned long long mine = sh.list[e];
+        unsigned rank = 0;
+#pragma unroll 8
+        for (int j = from; j < to; j++) rank += sh.list[j] < mine;
+        if (e < n && rank > 0) atomicAdd(&sh.ranks[e], rank);
+        __syncthreads();
+        if (part == 0 && e < n) sh.list[sh.ranks[e]] = mine;
+        __syncthreads();
+        return;
+    }
     for (int i = n + static_cast<int>(threadIdx.x); i < size; i += kSampleThreads) sh.list[i] = ~0ull;
     __syncthreads();
     for (int k = 2; k <= size; k *= 2)
@@ -423,6 +458,32 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
         }
 }
 
+// The sorted list's first n tokens' w into sh.weights, and of each thread's share of them, [from, to), the sum before it, and of all.
+__device__ __forceinline__ double weigh_list(const SampleWeights& w, int n, int& from, int& to, double& all, PickShared& sh) {
+    for (int i = threadIdx.x; i < n; i += kSampleThreads) sh.weights[i] = w.weight(key_value(~static_cast<unsigned>(sh.list[i] >> 32)));
+    __syncthreads();
+    const int each = (n + kSampleThreads - 1) / kSampleThreads;
+    from = min(n, static_cast<int>(threadIdx.x) * each);
+    to = min(n, from + each);
+    double mine = 0.0;
+    for (int i = from; i < to; i++) mine += sh.weights[i];
+    return block_scan(mine, sh.sums, all);
+}
+
+// How many of them are kept: of w above zero and at least min_p, with less than `target` before them.  All cuts leave the first of what there is: w falls
+// and the sum before it grows.
+__device__ __forceinline__ int count_kept(double before, int from, int to, double target, double min_p, bool first, PickShared& sh) {
+    int kept = 0;
+    for (int i = from; i < to; i++) {
+        const double v = sh.weights[i];
+        kept += v > 0.0 && ((first && i == 0) || (before < target && v >= min_p));
+        before += v;
+    }
+    int all;
+    (void)block_scan(kept, sh.ints, all);
+    return all;
+}
+
 // A place for each lane that `wants` one, counted in *count; one atomic for all of them.
 __device__ __forceinline__ int take_places(bool wants, int* count) {
     const unsigned long long all = __ballot(wants);
@@ -433,103 +494,172 @@ __device__ __forceinline__ int take_places(bool wants, int* count) {
     return first + __popcll(all & ((1ull << (threadIdx.x & 63)) - 1));
 }
 
-// The tokens that `may`, of the groups whose largest logit has `group_may`, into sh.list, by (key descending, index).  Returns how many; more
-// than kListed: the list is not whole.  Groups that hold one that `may` have `group_may`; `both`: the two are the same.
-template <int TYPE, typename TOPS, typename G, typename F>
-__device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS& group_top, SampleShared& sh, bool both, G&& group_may, F&& may) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = groups_of(row.vocab);
+// The groups' largest logits: the first ones in registers, the others read again each time.
+template <typename TOPS>
+struct GroupTops {
+    static constexpr int kOwn = 8;
+    const TOPS& at;
+    int groups;
+    float own[kOwn];
+    __device__ __forceinline__ GroupTops(const TOPS& tops, int n) : at(tops), groups(n) { read(0, own); }
+    __device__ __forceinline__ void read(int from, float (&v)[kOwn]) const {
+#pragma unroll
+        for (int k = 0; k < kOwn; k++) {
+            const int g = from + k * kSampleThreads + static_cast<int>(threadIdx.x);
+            v[k] = g < groups ? at(g) : -INFINITY;
+        }
+    }
+    // f called by all threads alike
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        float v[kOwn];
+#pragma unroll
+        for (int k = 0; k < kOwn; k++) v[k] = own[k];
+        for (int from = 0; from < groups; from += kOwn * kSampleThreads) {
+            if (from > 0) read(from, v);
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) {
+                if (from + k * kSampleThreads >= groups) break;
+                f(v[k], from + k * kSampleThreads + static_cast<int>(threadIdx.x));
+            }
+        }
+    }
+};
+
+// The least logit, up to `top`, that `may`, where all larger ones may: a wavefront tries 64 at a time.
+template <typename F>
+__device__ __forceinline__ float least_that(float top, F&& may) {
+    unsigned low = order_key(-3.402823466e38f), high = order_key(top);
+    while (low < high) {
+        const unsigned step = (high - low) / 64 + 1;
+        const unsigned mine = min(static_cast<unsigned long long>(high), low + static_cast<unsigned long long>(threadIdx.x & 63) * step);
+        const unsigned long long yes = __ballot(may(key_value(mine)));
+        const int first = yes ? __ffsll(yes) - 1 : 64;
+        const unsigned long long end = low + static_cast<unsigned long long>(first) * step;
+        if (first > 0) low += (first - 1) * step + 1;
+        if (end < high) high = static_cast<unsigned>(end);
+    }
+    return key_value(high);
+}
+
+// The tokens of logits from `least` to `most` into sh.list, by (key descending, index).  Returns how many; more than kListed: the list is not
+// whole.  Only groups whose largest reaches `least` are looked at.
+template <int TYPE, typename TOPS>
+__device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS& tops, PickShared& sh, float least, float most) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = sh.found = 0;
     __syncthreads();
-    for (int g0 = 64 * wave; g0 < groups; g0 += kSampleThreads) {
-        const int g = g0 + lane;
-        const float t = g < groups ? group_top(g) : -INFINITY;
-        const bool hot = t > -INFINITY && group_may(t);
+    tops.each([&](float t, int g) {
+        const bool hot = t >= least;
         const int at = take_places(hot, &sh.found);
         if (hot && at < kListed) sh.hot[at] = g;
-    }
+    });
     __syncthreads();
     const int hot = sh.found;
     const auto add = [&](float x, int index) {
-        const bool wants = x > -INFINITY && may(x);
+        const bool wants = x >= least && x <= most;
         const int at = take_places(wants, &sh.listed);
         if (wants && at < kListed) sh.list[at] = static_cast<unsigned long long>(~order_key(x)) << 32 | static_cast<unsigned>(index);
     };
     if (hot <= kListed) {
-        for (int h = wave; h < hot; h += 4 * kSampleWaves) {
-            float x[4];
-            int index[4];
+        constexpr int kDeep = 16;
+        for (int h = wave; h < hot; h += kDeep * kSampleWaves) {
+            float x[kDeep];
+            int index[kDeep];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < kDeep; k++) {
                 const int g = h + k * kSampleWaves;
                 index[k] = g < hot ? sh.hot[g] * kGroup + lane : row.vocab;
                 x[k] = row.one(index[k]);
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++) add(x[k], index[k]);
+            for (int k = 0; k < kDeep; k++) add(x[k], index[k]);
         }
-    } else if (both) {
+    } else if (most == INFINITY) {
         return hot;  // (each holds one at least)
     } else {
-        for (int from = 0; from < row.vocab; from += kRound) {
-            const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
-            float x[kVec];
-            row.load(i0, x);
-#pragma unroll
-            for (int i = 0; i < kVec; i++) add(x[i], i0 + i);
-        }
+        row.each(add);
     }
     __syncthreads();
     return sh.listed;
 }
 
-// Draws from the sorted list's first `kept` tokens, whose w are in sh.kept_weights: by their indices.
-__device__ __forceinline__ void draw_listed(const SampleParams& p, int r, int kept, SampleShared& sh) {
+__device__ __forceinline__ double target_of(const SampleParams& p, int r, double total) {
+    const float u = p.uniforms[r];
+    return (u > 0.0f ? static_cast<double>(u) : 0.0) * total;  // (NaN: 0)
+}
+
+// Draws from the sorted list's first `kept` tokens, whose w are in sh.weights: by their indices.
+__device__ __forceinline__ void draw_listed(const SampleParams& p, int r, int kept, PickShared& sh) {
     __syncthreads();
     for (int i = threadIdx.x; i < kept; i += kSampleThreads) sh.list[i] = sh.list[i] << 32 | static_cast<unsigned>(i);  // (the key goes)
-    __syncthreads();
-    sort_list(sh, kept);
-    double v[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int i = 2 * threadIdx.x + k;
-        v[k] = i < kept ? sh.kept_weights[static_cast<unsigned>(sh.list[i])] : 0.0;
-    }
-    double total;
-    const double before = block_scan(v[0] + v[1], sh.sums, total);
-    const float u = p.uniforms[r];
-    const double target = (u > 0.0f ? static_cast<double>(u) : 0.0) * total;  // (NaN: 0)
     if (threadIdx.x == 0) {
         sh.low = 0xFFFFFFFFu;
         sh.found = 0;
     }
     __syncthreads();
-    if (v[1] > 0.0 && before + v[0] + v[1] >= target) atomicMin(&sh.low, 2 * threadIdx.x + 1);
-    if (v[0] > 0.0 && before + v[0] >= target) atomicMin(&sh.low, 2 * threadIdx.x);
-    if (v[0] > 0.0) atomicMax(&sh.found, 2 * threadIdx.x + (v[1] > 0.0));
+    sort_list(sh, kept);
+    const auto weight = [&](int i) { return sh.weights[static_cast<unsigned>(sh.list[i])]; };
+    const int each = (kept + kSampleThreads - 1) / kSampleThreads, from = min(kept, static_cast<int>(threadIdx.x) * each), to = min(kept, from + each);
+    double mine = 0.0, total;
+    for (int i = from; i < to; i++) mine += weight(i);
+    double upto = block_scan(mine, sh.sums, total);
+    const double target = target_of(p, r, total);
+    for (int i = from; i < to; i++) {
+        upto += weight(i);
+        if (upto >= target) {
+            atomicMin(&sh.low, static_cast<unsigned>(i));
+            break;
+        }
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int at = sh.low != 0xFFFFFFFFu ? static_cast<int>(sh.low) : sh.found;
+        const int at = min(static_cast<int>(min(sh.low, 0x7FFFFFFFu)), kept - 1);
         p.ids[r] = static_cast<int>(sh.list[at] >> 32);
-        if (p.probs) p.probs[r] = static_cast<float>(sh.kept_weights[static_cast<unsigned>(sh.list[at])] / total);
+        if (p.probs) p.probs[r] = static_cast<float>(weight(at) / total);
     }
 }
 
 // ------------------------------------------------------------- segments of the row
 
-// Draws from what `weight` keeps, segment by segment; sh.segments holds the segments' sums of it.
+// Sums of what `weight` keeps of segments [first, first + count) into sh.segments.
 template <int TYPE, typename F>
-__device__ __forceinline__ void draw_segments(const SampleParams& p, int r, const SampleRow<TYPE>& row, SampleShared& sh, F&& weight) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = segments_of(row.vocab);
+__device__ __forceinline__ void sum_segments(const SampleRow<TYPE>& row, int first, int count, PickShared& sh, F&& weight) {
+    constexpr int kDeep = 8;
+    __syncthreads();
+    for (int s0 = threadIdx.x >> 6; s0 < count; s0 += kDeep * kSampleWaves) {
+        typename SampleRow<TYPE>::T e[kDeep][kVec];
+#pragma unroll
+        for (int k = 0; k < kDeep; k++) row.load_raw((first + s0 + k * kSampleWaves) * kSegment + static_cast<int>(threadIdx.x & 63) * kVec, e[k]);
+#pragma unroll
+        for (int k = 0; k < kDeep; k++) {
+            const int s = s0 + k * kSampleWaves;
+            if (s >= count) break;
+            const int i0 = (first + s) * kSegment + static_cast<int>(threadIdx.x & 63) * kVec;
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < kVec; i++) sum += weight(SampleRow<TYPE>::clean(e[k][i]), i0 + i);
+            sum = wave_scan(sum);
+            if ((threadIdx.x & 63) == 63) sh.segments[s] = sum;
+        }
+    }
+}
+
+// Draws from what `weight` keeps of `count` segments from `first` on, whose sums are in sh.segments: `ahead` is kept before them and `total` of the
+// whole row (negative: what they hold).
+template <int TYPE, typename F>
+__device__ __forceinline__ void draw_segments(const SampleParams& p, int r, const SampleRow<TYPE>& row, int first, int count, double ahead, double total,
+                                              PickShared& sh, F&& weight) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     const int each = (count + kSampleThreads - 1) / kSampleThreads, from = min(count, static_cast<int>(threadIdx.x) * each), to = min(count, from + each);
-    double mine = 0.0;
+    double mine = 0.0, all;
     for (int s = from; s < to; s++) mine += sh.segments[s];
     if (threadIdx.x == 0) sh.found = -1;
-    double total;
-    const double before = block_scan(mine, sh.sums, total);
-    const float u = p.uniforms[r];
-    const double target = (u > 0.0f ? static_cast<double>(u) : 0.0) * total;  // (NaN: 0)
+    const double before = block_scan(mine, sh.sums, all);
+    if (total < 0.0) total = all;
+    const double target = target_of(p, r, total) - ahead;
     // the last segment whose running total before it is below the target, among those that hold anything
     double below = before;
     for (int s = from; s < to; s++) {
@@ -545,7 +675,7 @@ __device__ __forceinline__ void draw_segments(const SampleParams& p, int r, cons
     }
     __syncthreads();
     if (wave != 0) return;
-    const int i0 = segment * kSegment + lane * kVec;
+    const int i0 = (first + segment) * kSegment + lane * kVec;
     double v[kVec], sum = 0.0;
     float x[kVec];
     row.load(i0, x);
@@ -581,15 +711,15 @@ __device__ __forceinline__ void draw_segments(const SampleParams& p, int r, cons
 // largest and only there where that is not minus infinity.
 template <int TYPE, typename GROUP, typename CHUNK, typename SEGMENT, typename MASS>
 __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const SampleRow<TYPE>& row, const SampleSettings& set, int chunk, int chunks,
-                                         const GROUP& group_top, const CHUNK& chunk_top, const SEGMENT& segment_sum, const MASS& mass, SampleShared& sh) {
-    const int groups = groups_of(p.vocab);
+                                         const GROUP& group_top, const CHUNK& chunk_top, const SEGMENT& segment_sum, const MASS& mass, PickShared& sh) {
+    const GroupTops<GROUP> tops(group_top, groups_of(p.vocab));
     float top = -INFINITY, low = INFINITY;  // of the groups' largest
-    for (int g = threadIdx.x; g < groups; g += kSampleThreads) {
-        const float t = group_top(g);
+    tops.each([&](float t, int) {
         top = fmaxf(top, t);
-        if (t > -INFINITY) low = fminf(low, t);
-    }
-    top = block_top(top, sh);
+        low = t > -INFINITY ? fminf(low, t) : low;
+    });
+    for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_tops[c] = chunk_top(c);
+    top = block_top<kSampleThreads>(top, sh.tops);
     if (top == -INFINITY) {
         if (threadIdx.x == 0) {
             p.ids[r] = -1;
@@ -600,8 +730,9 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     if (set.greedy()) {
         if (threadIdx.x == 0) sh.low = 0xFFFFFFFFu;
         __syncthreads();
-        for (int g = threadIdx.x; g < groups; g += kSampleThreads)
-            if (group_top(g) == top) atomicMin(&sh.low, static_cast<unsigned>(g));
+        tops.each([&](float t, int g) {
+            if (t == top) atomicMin(&sh.low, static_cast<unsigned>(g));
+        });
         __syncthreads();
         if (threadIdx.x < 64) {
             const int g = static_cast<int>(sh.low);
@@ -617,7 +748,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52);
     const int segments = segments_of(p.vocab);
     const auto sum_of = [&](int s) {
-        const double share = w.weight(chunk_top(s * kSegment / chunk));
+        const double share = w.weight(sh.chunk_tops[s * kSegment / chunk]);
         return share > 0.0 ? segment_sum(s) * share : 0.0;
     };
 
@@ -629,10 +760,9 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             const int s = static_cast<int>(threadIdx.x) + k * kSampleThreads;
             own[k] = s < segments ? sum_of(s) : 0.0;
         }
-        __syncthreads();
 #pragma unroll
         for (int k = 0; k < kOwn; k++) sh.segments[threadIdx.x + k * kSampleThreads] = own[k];
-        draw_segments(p, r, row, sh, [&](float x, int) { return w.weight(x); });
+        draw_segments(p, r, row, 0, segments, 0.0, -1.0, sh, [&](float x, int) { return w.weight(x); });
         return;
     }
 
@@ -642,15 +772,14 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     if (set.top_k > 0) {
         // buckets of the logits, from the largest down, and the one that holds the k-th largest of the groups' largest, or of all where groups are few
         if (set.top_k <= kListed) {
-            low = -block_top(-low, sh);
+            low = -block_top<kSampleThreads>(-low, sh.tops);
             double fine = 0.0;
             const auto bucket_of = [&](float x) { return x == top ? 0 : static_cast<int>(fmin((static_cast<double>(top) - x) * fine, 1e9)); };
             int bound = kBuckets;
-            for (int by_group = 4 * set.top_k <= 3 * groups; by_group >= 0 && bound == kBuckets; by_group--) {
+            for (int by_group = 4 * set.top_k <= 3 * tops.groups; by_group >= 0 && bound == kBuckets; by_group--) {
                 fine = by_group ? (kBuckets - 1) / fmax(static_cast<double>(top) - low, 1e-300) : kBuckets / kLeastPower / 64 * w.turn;
                 __syncthreads();
-                sh.counts[threadIdx.x] = 0;
-                sh.counts[threadIdx.x + kSampleThreads] = 0;
+                for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.counts[b] = 0;
                 if (threadIdx.x == 0) sh.bucket = kBuckets;
                 __syncthreads();
                 const auto count = [&](float x, int) {
@@ -658,22 +787,26 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                     if (const int b = bucket_of(x); b < kBuckets) atomicAdd(&sh.counts[b], 1u);
                 };
                 if (by_group) {
-                    for (int g = threadIdx.x; g < groups; g += kSampleThreads) count(group_top(g), 0);
+                    tops.each(count);
                 } else {
                     row.each(count);
                 }
                 __syncthreads();
-                const int a = static_cast<int>(sh.counts[2 * threadIdx.x]), b = static_cast<int>(sh.counts[2 * threadIdx.x + 1]);
-                int all;
-                const int before = block_scan(a + b, sh.ints, all);
-                if (before < set.top_k && before + a >= set.top_k) sh.bucket = 2 * threadIdx.x;
-                if (before + a < set.top_k && before + a + b >= set.top_k) sh.bucket = 2 * threadIdx.x + 1;
+                constexpr int kOwn = kBuckets / kSampleThreads;
+                int own[kOwn], sum = 0, all;
+#pragma unroll
+                for (int k = 0; k < kOwn; k++) sum += own[k] = static_cast<int>(sh.counts[kOwn * threadIdx.x + k]);
+                int before = block_scan(sum, sh.ints, all);
+#pragma unroll
+                for (int k = 0; k < kOwn; k++) {
+                    if (before < set.top_k && before + own[k] >= set.top_k) sh.bucket = kOwn * static_cast<int>(threadIdx.x) + k;
+                    before += own[k];
+                }
                 __syncthreads();
                 bound = sh.bucket;
             }
             // (none: fewer than k tokens have a w)
-            const auto may = [&](float x) { return bucket_of(x) <= bound; };
-            listed = make_list(row, group_top, sh, true, may, may);
+            listed = make_list(row, tops, sh, least_that(top, [&](float x) { return bucket_of(x) <= bound; }), INFINITY);
         }
         if (listed > kListed) {
             cut = find_cut<TYPE, false>(row, w, scale, cut, set.top_k, sh);
@@ -696,21 +829,30 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         const int place = grid_place(top, grid);
         if (set.on_grid(top, 0x1p29)) {
             // w by buckets, of all chunks, and the one in which their running sum reaches the target
-            double own = 0.0;
+            constexpr int kOwn = kMassBuckets / kSampleThreads;
+            double own[kOwn], sum = 0.0, all;
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) own[k] = 0.0;
             for (int c = 0; c < chunks; c++) {
-                const float t = chunk_top(c);
+                const float t = sh.chunk_tops[c];
                 const double share = w.weight(t);
                 if (!(share > 0.0)) continue;
-                const int b = static_cast<int>(threadIdx.x) - (place - grid_place(t, grid));
-                if (b >= 0) own += static_cast<double>(mass(c, b)) * share;
+                const int shift = place - grid_place(t, grid);
+#pragma unroll
+                for (int k = 0; k < kOwn; k++)
+                    if (const int b = kOwn * static_cast<int>(threadIdx.x) + k - shift; b >= 0) own[k] += static_cast<double>(mass(c, b)) * share;
             }
-            own /= scale;
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) sum += own[k] /= scale;
             if (threadIdx.x == 0) sh.bucket = kMassBuckets;
-            double all;
-            const double before = block_scan(own, sh.sums, all);
-            if (own > 0.0 && (before < target || before == 0.0) && before + own >= target) {
-                sh.bucket = threadIdx.x;
-                sh.mass_above = before;
+            double before = block_scan(sum, sh.sums, all);
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) {
+                if (own[k] > 0.0 && (before < target || before == 0.0) && before + own[k] >= target) {
+                    sh.bucket = kOwn * static_cast<int>(threadIdx.x) + k;
+                    sh.mass_above = before;
+                }
+                before += own[k];
             }
             __syncthreads();
             bound = sh.bucket;
@@ -718,28 +860,54 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         if (bound < kMassBuckets - 1) {  // (a chunk's last bucket holds what is further down as well)
             const double above = sh.mass_above;
             const auto bucket_of = [&](float x) { return w.power64(x) > -64 * kLeastPower ? place - grid_place(x, grid) : kMassBuckets; };
-            const auto reaches = [&](float x) { return bucket_of(x) <= bound; };
-            const auto may = [&](float x) { return reaches(x) && w.weight(x) >= set.min_p; };
-            listed = make_list(row, group_top, sh, true, may, may);
+            const float least = least_that(top, [&](float x) { return bucket_of(x) <= bound; });
+            listed = make_list(row, tops, sh, set.min_p > 0.0 ? fmaxf(least, least_that(top, [&](float x) { return w.weight(x) >= set.min_p; })) : least, INFINITY);
             if (listed > kListed) {  // the bucket's own tokens say where the cut is
-                const int own = make_list(row, group_top, sh, false, reaches, [&](float x) { return bucket_of(x) == bound; });
+                const float next = bound > 0 ? least_that(top, [&](float x) { return bucket_of(x) < bound; }) : INFINITY;
+                const int own = make_list(row, tops, sh, least, bound > 0 ? key_value(order_key(next) - 1) : 3.402823466e38f);
                 if (own <= kListed) {
                     sort_list(sh, own);
-                    double v[2];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int i = 2 * static_cast<int>(threadIdx.x) + k;
-                        v[k] = i < own ? w.weight(key_value(~static_cast<unsigned>(sh.list[i] >> 32))) : 0.0;
-                    }
+                    int from, to;
                     double all;
-                    const double before = above + block_scan(v[0] + v[1], sh.sums, all);
-                    if (threadIdx.x == 0) sh.found = 0;
-                    __syncthreads();
-                    if (v[1] > 0.0 && before + v[0] < target) atomicMax(&sh.found, 2 * static_cast<int>(threadIdx.x) + 1);
-                    if (v[0] > 0.0 && before < target) atomicMax(&sh.found, 2 * static_cast<int>(threadIdx.x));
-                    __syncthreads();
-                    cut.key = ~static_cast<unsigned>(sh.list[sh.found] >> 32);
-                    cut.index = static_cast<int>(static_cast<unsigned>(sh.list[sh.found]));
+                    const double before = above + weigh_list(w, own, from, to, all, sh);
+                    const int kept = count_kept(before, from, to, target, 0.0, true, sh);  // (the running sum reaches the target here: one at least)
+                    cut.key = ~static_cast<unsigned>(sh.list[kept - 1] >> 32);
+                    cut.index = static_cast<int>(static_cast<unsigned>(sh.list[kept - 1]));
+                    if (set.min_p == 0.0 || -log2(set.min_p) * kMassFine > bound + 2) {
+                        // what the chunks keep: all above the bucket, and of its own what is kept.  Only the chunk that the draw falls into is read again
+                        for (int c = static_cast<int>(threadIdx.x) >> 6; c < chunks; c += kSampleWaves) {
+                            const float t = sh.chunk_tops[c];
+                            const double share = w.weight(t);
+                            double sum = 0.0;
+                            if (share > 0.0) {
+                                const int shift = place - grid_place(t, grid);
+                                for (int b = shift + static_cast<int>(threadIdx.x & 63); b < bound; b += 64) sum += static_cast<double>(mass(c, b - shift));
+                                sum *= share / scale;
+                            }
+                            for (int i = threadIdx.x & 63; i < kept; i += 64)
+                                if (static_cast<int>(static_cast<unsigned>(sh.list[i])) / chunk == c) sum += sh.weights[i];
+                            sum = wave_scan(sum);
+                            if ((threadIdx.x & 63) == 63) sh.chunk_sums[c] = sum;
+                        }
+                        __syncthreads();
+                        double held = 0.0;
+                        for (int c = 0; c < chunks; c++) held += sh.chunk_sums[c];
+                        const double wanted = target_of(p, r, held);
+                        int here = -1;
+                        double ahead = 0.0, running = 0.0;
+                        for (int c = 0; c < chunks; c++) {
+                            if (sh.chunk_sums[c] > 0.0 && (running < wanted || running == 0.0)) {
+                                here = c;
+                                ahead = running;
+                            }
+                            running += sh.chunk_sums[c];
+                        }
+                        const auto weight = [&](float x, int i) { return cut.keeps(order_key(x), i) ? w.weight(x) : 0.0; };
+                        const int first = here * (chunk / kSegment), count = min(chunk / kSegment, segments - first);
+                        sum_segments(row, first, count, sh, weight);
+                        draw_segments(p, r, row, first, count, ahead, held, sh, weight);
+                        return;
+                    }
                     bound = -1;
                 }
             }
@@ -751,90 +919,69 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
         }
     } else {
-        const auto may = [&](float x) { return w.weight(x) >= set.min_p; };
-        listed = make_list(row, group_top, sh, true, may, may);
+        listed = make_list(row, tops, sh, least_that(top, [&](float x) { return w.weight(x) >= set.min_p; }), INFINITY);
     }
 
     if (listed <= kListed) {
         sort_list(sh, listed);
         if (set.top_k > 0) listed = min(listed, set.top_k);
-        double v[2], all;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = 2 * static_cast<int>(threadIdx.x) + k;
-            v[k] = i < listed ? w.weight(key_value(~static_cast<unsigned>(sh.list[i] >> 32))) : 0.0;
-        }
-        const double before = block_scan(v[0] + v[1], sh.sums, all);
-        if (set.top_k > 0) total = all;
-        const double target = set.top_p < 1.0 ? set.top_p * total : INFINITY;
-        // (all cuts leave the first of what there is: v falls and the sum before it grows)
-        const int kept0 = v[0] > 0.0 && (threadIdx.x == 0 || (before < target && v[0] >= set.min_p));
-        const int kept1 = v[1] > 0.0 && before + v[0] < target && v[1] >= set.min_p;
-        int kept;
-        (void)block_scan(kept0 + kept1, sh.ints, kept);
-        __syncthreads();
-        sh.kept_weights[2 * threadIdx.x] = v[0];
-        sh.kept_weights[2 * threadIdx.x + 1] = v[1];
-        draw_listed(p, r, kept, sh);
+        int from, to;
+        double all;
+        const double before = weigh_list(w, listed, from, to, all, sh);
+        const double target = set.top_p < 1.0 ? set.top_p * (set.top_k > 0 ? all : total) : INFINITY;
+        draw_listed(p, r, count_kept(before, from, to, target, set.min_p, true, sh), sh);
         return;
     }
     const auto weight = [&](float x, int i) {
         const double v = cut.keeps(order_key(x), i) ? w.weight(x) : 0.0;
         return v >= set.min_p ? v : 0.0;
     };
-    __syncthreads();
-    for (int s = threadIdx.x >> 6; s < segments; s += kSampleWaves) {
-        const int i0 = s * kSegment + static_cast<int>(threadIdx.x & 63) * kVec;
-        float x[kVec];
-        row.load(i0, x);
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < kVec; i++) sum += weight(x[i], i0 + i);
-        sum = wave_scan(sum);
-        if ((threadIdx.x & 63) == 63) sh.segments[s] = sum;
-    }
-    draw_segments(p, r, row, sh, weight);
+    sum_segments(row, 0, segments, sh, weight);
+    draw_segments(p, r, row, 0, segments, 0.0, -1.0, sh, weight);
 }
 
 // A row of one chunk, from its logits to the pick.
-template <int TYPE, int ROUNDS>
+template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const SampleParams p) {
-    __shared__ SampleShared sh;
+    __shared__ ChunkShared<kSampleThreads> left;
+    __shared__ PickShared sh;
     const int r = p.first_row + static_cast<int>(blockIdx.x);
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
-    const float top = scan_chunk<TYPE, ROUNDS>(p, row, set, 0, sh);
+    const float top = scan_chunk<TYPE, kSampleThreads>(p, row, set, 0, left);
+    if (threadIdx.x < 64) sh.powers[threadIdx.x] = left.powers[threadIdx.x];
     __syncthreads();
-    pick_row(p, r, row, set, ROUNDS * kRound, 1, [&](int g) { return sh.group_tops[g]; }, [&](int) { return top; },
-             [&](int s) { return sh.segments[s]; }, [&](int, int b) { return sh.bins[b]; }, sh);
+    pick_row(p, r, row, set, kChunk, 1, [&](int g) { return left.group_tops[g]; }, [&](int) { return top; }, [&](int s) { return left.segments[s]; },
+             [&](int, int b) { return left.masses[b]; }, sh);
 }
 
-// One chunk of a row, for sample_pick_kernel.
-template <int TYPE, int ROUNDS>
-__global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(const SampleParams p) {
-    __shared__ SampleShared sh;
-    const int c = static_cast<int>(blockIdx.x) % p.chunks, r = p.first_row + static_cast<int>(blockIdx.x) / p.chunks;
+// One chunk of a row, for sample_pick_kernel.  Two workgroups to a compute unit, so that one reads while the other computes.
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(const SampleParams p) {
+    __shared__ ChunkShared<THREADS> left;
+    constexpr int kLength = THREADS * kVec * kRounds, kGroups = kLength / kGroup, kSegments = kLength / kSegment;
+    const int c = static_cast<int>(blockIdx.x) % p.chunks, r = p.first_row + static_cast<int>(blockIdx.x) / p.chunks, t = threadIdx.x;
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
-    const float top = scan_chunk<TYPE, ROUNDS>(p, row, set, c * ROUNDS * kRound, sh);
+    const float top = scan_chunk<TYPE, THREADS>(p, row, set, c * kLength, left);
     __syncthreads();
-    constexpr int kGroups = ROUNDS * kRound / kGroup, kSegments = ROUNDS * kRound / kSegment;
-    const int t = threadIdx.x;
-    if (const int g = c * kGroups + t; t < kGroups && g < groups_of(p.vocab)) p.group_tops[static_cast<size_t>(r) * groups_of(p.vocab) + g] = sh.group_tops[t];
+    for (int g = t; g < kGroups && c * kGroups + g < groups_of(p.vocab); g += THREADS)
+        p.group_tops[static_cast<size_t>(r) * groups_of(p.vocab) + c * kGroups + g] = left.group_tops[g];
     if (t == 0) p.chunk_tops[static_cast<size_t>(r) * p.chunks + c] = top;
     if (top == -INFINITY) return;
-    if (const int s = c * kSegments + t; set.sums() && t < kSegments && s < segments_of(p.vocab))
-        p.segment_sums[static_cast<size_t>(r) * segments_of(p.vocab) + s] = sh.segments[t];
-    if (set.masses() && set.on_grid(top)) p.masses[(static_cast<size_t>(r) * p.chunks + c) * kMassBuckets + t] = sh.bins[t];
+    if (set.sums() && t < kSegments && c * kSegments + t < segments_of(p.vocab))
+        p.segment_sums[static_cast<size_t>(r) * segments_of(p.vocab) + c * kSegments + t] = left.segments[t];
+    if (set.masses() && set.on_grid(top))
+        for (int b = t; b < kMassBuckets; b += THREADS) p.masses[(static_cast<size_t>(r) * p.chunks + c) * kMassBuckets + b] = left.masses[b];
 }
 
 template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(const SampleParams p, int chunk) {
-    __shared__ SampleShared sh;
+    __shared__ PickShared sh;
     const int r = p.first_row + static_cast<int>(blockIdx.x);
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
-    fill_powers(sh);
+    fill_powers(p, sh.powers);
     const float* const group_tops = p.group_tops + static_cast<size_t>(r) * groups_of(p.vocab);
     const float* const chunk_tops = p.chunk_tops + static_cast<size_t>(r) * p.chunks;
     const double* const segment_sums = p.segment_sums + static_cast<size_t>(r) * segments_of(p.vocab);

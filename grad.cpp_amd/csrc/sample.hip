@@ -2,6 +2,8 @@
 #include "device_scope.h"
 #include "kernels_sample.h"
 
+#include <cmath>
+
 namespace gh {
 
 [[noreturn]] static void refuse(const std::string& why) { throw ApiError{GH_ERR_INVALID_ARGUMENT, "gh_sample: " + why}; }
@@ -12,23 +14,20 @@ static void check_sizes(int type, int rows, int vocab) {
     if (vocab < 1 || vocab > kMaxSampleVocab) refuse("vocab must be 1 to 2^20");
 }
 
-// Rows of one chunk are picked from by the workgroup that reads them.  Longer ones are read in chunks by as many workgroups, large chunks where
+// Rows of one chunk are picked from by the workgroup that reads them.  Longer ones are read in chunks by as many workgroups, wide chunks where
 // they keep every compute unit busy.
 struct SampleForm {
-    int rounds = 0;
+    int chunk = kChunk;
     int chunks = 1;
     size_t group_tops = 0, chunk_tops = 0, segment_sums = 0, masses = 0, bytes = 0;  // places in the workspace
 };
 
 static SampleForm form_of(int rows, int vocab) {
     SampleForm f;
-    if (vocab <= kMaxRounds * kRound) {
-        f.rounds = vocab <= kRound ? 1 : vocab <= 2 * kRound ? 2 : 4;
-        return f;
-    }
-    const auto chunks = [&](int rounds) { return (vocab + rounds * kRound - 1) / (rounds * kRound); };
-    f.rounds = static_cast<long long>(rows) * chunks(4) >= 256 ? 4 : 1;
-    f.chunks = chunks(f.rounds);
+    if (vocab <= kChunk) return f;
+    const auto chunks = [&](int length) { return (vocab + length - 1) / length; };
+    if (static_cast<long long>(rows) * chunks(kWideChunk) >= 256) f.chunk = kWideChunk;
+    f.chunks = chunks(f.chunk);
     const auto place = [&](size_t per_row) {
         const size_t at = f.bytes;
         f.bytes += (per_row * static_cast<size_t>(rows) + 15) / 16 * 16;
@@ -48,13 +47,15 @@ static void launch_sample(SampleParams p, const SampleForm& f, int rows, hipStre
     for (p.first_row = 0; p.first_row < rows; p.first_row += slice) {
         const int n = std::min(slice, rows - p.first_row);
         if (f.chunks == 1) {
-            const auto kernel = f.rounds == 1 ? sample_row_kernel<TYPE, 1> : f.rounds == 2 ? sample_row_kernel<TYPE, 2> : sample_row_kernel<TYPE, 4>;
-            hipLaunchKernelGGL(kernel, dim3(n), dim3(kSampleThreads), 0, stream, p);
+            hipLaunchKernelGGL(sample_row_kernel<TYPE>, dim3(n), dim3(kSampleThreads), 0, stream, p);
         } else {
-            const auto kernel = f.rounds == 1 ? sample_scan_kernel<TYPE, 1> : sample_scan_kernel<TYPE, 4>;
-            hipLaunchKernelGGL(kernel, dim3(n * f.chunks), dim3(kSampleThreads), 0, stream, p);
+            if (f.chunk == kChunk) {
+                hipLaunchKernelGGL((sample_scan_kernel<TYPE, kSampleThreads>), dim3(n * f.chunks), dim3(kSampleThreads), 0, stream, p);
+            } else {
+                hipLaunchKernelGGL((sample_scan_kernel<TYPE, kWideThreads>), dim3(n * f.chunks), dim3(kWideThreads), 0, stream, p);
+            }
             HIP_CHECK(hipGetLastError());
-            hipLaunchKernelGGL(sample_pick_kernel<TYPE>, dim3(n), dim3(kSampleThreads), 0, stream, p, f.rounds * kRound);
+            hipLaunchKernelGGL(sample_pick_kernel<TYPE>, dim3(n), dim3(kSampleThreads), 0, stream, p, f.chunk);
         }
         HIP_CHECK(hipGetLastError());
     }
@@ -89,6 +90,7 @@ static void sample(const gh_sample_args& a, hipStream_t stream) {
     p.uniforms = a.uniforms;
     p.ids = a.ids;
     p.probs = a.probs;
+    for (int j = 0; j < 64; j++) p.powers[j] = std::exp2(j / 64.0);
     char* const work = static_cast<char*>(a.workspace);
     p.chunks = f.chunks;
     p.group_tops = reinterpret_cast<float*>(work + f.group_tops);
