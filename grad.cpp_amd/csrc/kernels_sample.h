@@ -19,11 +19,13 @@
 
 #include "kernels_cache_attn.h"
 
+#include <type_traits>
+
 namespace gh {
 
 constexpr int kSampleThreads = 256;  // that pick: most of it is steps one behind the other, which four wavefronts take in less time than sixteen
 constexpr int kSampleWaves = kSampleThreads / 64;
-constexpr int kWideThreads = 1024;  // that read large chunks
+constexpr int kWideThreads = 512;   // that read large chunks
 constexpr int kMaxSampleVocab = 1 << 20;
 constexpr int kVec = 8;               // logits of a lane
 constexpr int kGroup = 64;            // of eight lanes
@@ -32,6 +34,8 @@ constexpr int kRounds = 4;            // vectors of a thread, in registers: a ch
 constexpr int kChunk = kSampleThreads * kVec * kRounds, kWideChunk = kWideThreads * kVec * kRounds;
 constexpr int kMaxSegments = kMaxSampleVocab / kSegment;
 constexpr int kListed = 2048;                 // tokens that are sorted
+constexpr int kPowers = 256;                  // a table of 2^(j / 256), j < 256
+static_assert(kPowers == 1 << 8, "");
 constexpr int kBuckets = 2048;                // of the histograms over the row
 constexpr double kLeastPower = 44.0;          // w below 2^-44 of the largest are nothing: all of a million tokens together are below 2^-24
 // w by buckets of x: so many to a power of two, on a grid that all chunks share
@@ -51,7 +55,7 @@ struct SampleParams {
     int* ids;
     float* probs;
     int first_row;
-    double powers[64];  // 2^(j / 64)
+    double powers[kPowers];
     // what the chunks leave, of every row: [groups], [chunks], [segments], [chunks][kMassBuckets]
     int chunks;
     float* group_tops;
@@ -142,11 +146,14 @@ struct SampleRow {
 #pragma unroll
         for (int i = 0; i < kVec; i++) x[i] = clean(e[i]);
     }
-    __device__ __forceinline__ float one(int i) const { return i < vocab ? clean(at[i]) : -INFINITY; }
+    __device__ __forceinline__ float one(int i) const {
+        const float x = clean(at[min(i, vocab - 1)]);
+        return i < vocab ? x : -INFINITY;
+    }
     // Every logit, in any order, f called by all threads alike; many loads at a time, or each would be a trip to memory of its own.
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
-        constexpr int kDeep = 16;
+        constexpr int kDeep = 4;
         for (int from = 0; from < vocab; from += kDeep * kSampleThreads * kVec) {
             T e[kDeep][kVec];
 #pragma unroll
@@ -173,7 +180,7 @@ template <int THREADS>
 struct ChunkShared {
     unsigned long long masses[kMassBuckets];
     double segments[THREADS * kVec * kRounds / kSegment];
-    double powers[64];  // 2^(j / 64)
+    double powers[kPowers];
     float group_tops[THREADS * kVec * kRounds / kGroup];
     float tops[THREADS / 64];
 };
@@ -190,7 +197,7 @@ struct PickShared {
         double weights[kListed];
     };
     unsigned ranks[kSampleThreads];
-    double powers[64];
+    double powers[kPowers];
     double chunk_sums[kMaxSampleVocab / kChunk];
     float chunk_tops[kMaxSampleVocab / kChunk];
     unsigned long long scan[kSampleWaves];
@@ -203,23 +210,27 @@ struct PickShared {
     int bucket, found, listed;
 };
 
-// exp((x - top) / T).  2^y for y = n / 64 + r, |r| <= 1 / 128: 2^(n / 64) from a table and the series of 2^r, cut off behind the
-// fourth power (relative error below 5e-14).  Exactly 1 at the top.
+// w = exp((x - top) / T) = 2^(n / 256 + r / 256), |r| <= 1/2: 2^(n / 256) from a table, the series of the rest cut off behind the third power (relative
+// error below 2e-13).  Exactly 1 at the top, 0 below 2^-44.
+constexpr double kLeastTurns = -kPowers * kLeastPower;
+constexpr double kMagic = 0x1.8p52;  // added to a number below 2^51 leaves it rounded in the last bits
+
+// 256 log2 of a w of `z`, or what is not a number.
+__device__ __forceinline__ double weight_of(double z, const double* powers) {
+    constexpr double l = 0.69314718055994530942 / kPowers, c2 = l * l / 2, c3 = l * l * l / 6;
+    z = z > kLeastTurns ? z : -1e9;
+    const double t = z + kMagic, r = z - (t - kMagic);
+    const int n = static_cast<int>(__double_as_longlong(t));
+    const double head = powers[n & (kPowers - 1)];
+    return ldexp(fma(head, r * fma(r, fma(r, c3, c2), l), head), n >> 8);
+}
+
 struct SampleWeights {
     float top;
-    double turn;  // 64 log2(e) / T
+    double turn;  // 256 log2(e) / T
     const double* powers;
-    __device__ __forceinline__ double power64(float x) const { return x == top ? 0.0 : (static_cast<double>(x) - top) * turn; }
-    __device__ __forceinline__ double weight(float x) const {
-        constexpr double kMagic = 0x1.8p52;
-        constexpr double l = 0.69314718055994530942 / 64, c2 = l * l / 2, c3 = l * l * l / 6, c4 = l * l * l * l / 24;
-        const double z = power64(x), t = z + kMagic, r = z - (t - kMagic);
-        const int n = static_cast<int>(__double_as_longlong(t));
-        const double head = powers[n & 63];
-        const double tail = r * fma(r, fma(r, fma(r, c4, c3), c2), l);
-        const double w = ldexp(fma(head, tail, head), n >> 6);
-        return z > -64.0 * kLeastPower ? w : 0.0;
-    }
+    __device__ __forceinline__ double turns(float x) const { return x == top ? 0.0 : (static_cast<double>(x) - top) * turn; }
+    __device__ __forceinline__ double weight(float x) const { return weight_of(turns(x), powers); }
 };
 
 __device__ __forceinline__ unsigned long long whole_number(double w, double scale) {
@@ -241,7 +252,7 @@ struct SampleSettings {
         min_p = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
     }
     __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f); }
-    __device__ __forceinline__ double turn() const { return 64 * 1.44269504088896340736 / temperature; }
+    __device__ __forceinline__ double turn() const { return fmax(kPowers * 1.44269504088896340736 / temperature, 1e-290); }
     // the whole row's sum: by segments; by buckets as well
     __device__ __forceinline__ bool sums() const { return !greedy() && top_k == 0 && (top_p < 1.0 || min_p == 0.0); }
     __device__ __forceinline__ bool masses() const { return !greedy() && top_k == 0 && top_p < 1.0; }
@@ -251,10 +262,10 @@ struct SampleSettings {
 };
 
 // The place on the grid: larger logits have larger ones.
-__device__ __forceinline__ int grid_place(float x, double grid) { return static_cast<int>(__double_as_longlong(fma(static_cast<double>(x), grid, 0x1.8p52))); }
+__device__ __forceinline__ int grid_place(float x, double grid) { return static_cast<int>(__double_as_longlong(fma(static_cast<double>(x), grid, kMagic))); }
 
 __device__ __forceinline__ void fill_powers(const SampleParams& p, double* powers) {
-    if (threadIdx.x < 64) powers[threadIdx.x] = p.powers[threadIdx.x];
+    if (threadIdx.x < kPowers) powers[threadIdx.x] = p.powers[threadIdx.x];
 }
 
 template <int THREADS>
@@ -274,7 +285,8 @@ __device__ __forceinline__ float block_top(float v, float* tops) {
 template <int TYPE, int THREADS>
 __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, ChunkShared<THREADS>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    typename SampleRow<TYPE>::T raw[kRounds][kVec];
+    using T = typename SampleRow<TYPE>::T;
+    T raw[kRounds][kVec];
 #pragma unroll
     for (int r = 0; r < kRounds; r++) row.load_raw(first + (r * THREADS + static_cast<int>(threadIdx.x)) * kVec, raw[r]);
     fill_powers(p, sh.powers);
@@ -283,7 +295,7 @@ __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleR
     for (int r = 0; r < kRounds; r++) {
         float high = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kVec; i++) high = fmaxf(high, SampleRow<TYPE>::clean(raw[r][i]));
+        for (int i = 0; i < kVec; i++) high = fmaxf(high, static_cast<float>(raw[r][i]));  // (not a NaN)
         high = fmaxf(high, dpp_move<0xB1, 0xF>(high, high));   // over the eight lanes of a group
         high = fmaxf(high, dpp_move<0x4E, 0xF>(high, high));
         high = fmaxf(high, dpp_move<0x141, 0xF>(high, high));  // row_half_mirror
@@ -295,25 +307,39 @@ __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleR
         for (int b = threadIdx.x; b < kMassBuckets; b += THREADS) sh.masses[b] = 0;
     top = block_top<THREADS>(top, sh.tops);
     if (!set.sums() || top == -INFINITY) return top;
-    const SampleWeights w{top, set.turn(), sh.powers};
-    const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52), grid = set.grid();
+    float base = top;
+    if (top == INFINITY) {  // infinity less infinity is none
+        base = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRounds; r++)
+#pragma unroll
+            for (int i = 0; i < kVec; i++) raw[r][i] = static_cast<T>(static_cast<float>(raw[r][i]) == INFINITY ? 0.0f : -INFINITY);
+    }
+    const double turn = set.turn(), scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52), grid = set.grid();
     const int place = grid_place(top, grid);
-    const bool counts = masses && set.on_grid(top);
+    const auto sum_up = [&](auto counted) {
 #pragma unroll
-    for (int r = 0; r < kRounds; r++) {
-        double sum = 0.0;
+        for (int r = 0; r < kRounds; r++) {
+            double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kVec; i++) {
-            const float x = SampleRow<TYPE>::clean(raw[r][i]);
-            const double v = w.weight(x);
-            sum += v;
-            if (counts && v > 0.0) {
-                const unsigned b = static_cast<unsigned>(place - grid_place(x, grid));
-                atomicAdd(&sh.masses[min(b, kMassBuckets - 1u)], whole_number(v, scale));
+            for (int i = 0; i < kVec; i++) {
+                const float x = static_cast<float>(raw[r][i]);  // (NaN: nothing)
+                const double v = weight_of((static_cast<double>(x) - base) * turn, sh.powers);
+                sum += v;
+                if constexpr (decltype(counted)::value) {
+                    // (what is no number on the grid has a w of nothing)
+                    const unsigned b = static_cast<unsigned>(place - grid_place(x, grid));
+                    if (b < kMassBuckets && v > 0.0) atomicAdd(&sh.masses[b], whole_number(v, scale));
+                }
             }
+            sum = wave_scan(sum);
+            if (lane == 63) sh.segments[r * (THREADS / 64) + wave] = sum;
         }
-        sum = wave_scan(sum);
-        if (lane == 63) sh.segments[r * (THREADS / 64) + wave] = sum;
+    };
+    if (masses && set.on_grid(top)) {
+        sum_up(std::true_type{});
+    } else {
+        sum_up(std::false_type{});
     }
     return top;
 }
@@ -347,9 +373,9 @@ __device__ __forceinline__ int find_bucket(PickShared& sh, double target, unsign
 // their index.  Tokens whose w are nothing are left out.
 template <int TYPE, bool MASS>
 __device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, double scale, const Cut& kept, double target, PickShared& sh) {
-    const double fine = kBuckets / kLeastPower / 64;
-    const auto counts = [&](float x) { return w.power64(x) > -64 * kLeastPower; };
-    const auto bucket_of = [&](float x) { return min(static_cast<int>(-w.power64(x) * fine), kBuckets - 1); };
+    const double fine = kBuckets / -kLeastTurns;
+    const auto counts = [&](float x) { return w.turns(x) > kLeastTurns; };
+    const auto bucket_of = [&](float x) { return min(static_cast<int>(-w.turns(x) * fine), kBuckets - 1); };
     const auto clear = [&] {
         __syncthreads();
         for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.bins[b] = 0;
@@ -579,10 +605,102 @@ __device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS&
     } else if (most == INFINITY) {
         return hot;  // (each holds one at least)
     } else {
-        row.each(add);
+        // the whole row: which of a thread's logits, then places for all of a wavefront's at once
+        using T = typename SampleRow<TYPE>::T;
+        constexpr int kDeep = 16, kStep = kSampleThreads * kVec;
+        for (int from = 0; from < row.vocab; from += kDeep * kStep) {
+            const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
+            T e[kDeep][kVec];
+            unsigned mask[kDeep * kVec / 32];
+#pragma unroll
+            for (int k = 0; k < kDeep; k++) row.load_raw(i0 + k * kStep, e[k]);
+            int wants = 0;
+#pragma unroll
+            for (int m = 0; m < kDeep * kVec / 32; m++) {
+                mask[m] = 0;
+#pragma unroll
+                for (int b = 0; b < 32; b++) {
+                    const float x = static_cast<float>(e[m * 32 / kVec + b / kVec][b % kVec]);
+                    mask[m] |= x >= least && x <= most ? 1u << b : 0u;
+                }
+                wants += __popc(mask[m]);
+            }
+            const int upto = wave_scan(wants);
+            int first = 0;
+            if (lane == 63 && upto > 0) first = atomicAdd(&sh.listed, upto);
+            int at = __builtin_amdgcn_readlane(first, 63) + upto - wants;
+#pragma unroll
+            for (int m = 0; m < kDeep * kVec / 32; m++)
+                for (; mask[m]; mask[m] &= mask[m] - 1, at++) {
+                    const int b = m * 32 + __ffs(mask[m]) - 1, index = i0 + b / kVec * kStep + b % kVec;
+                    if (at < kListed) sh.list[at] = static_cast<unsigned long long>(~order_key(row.one(index))) << 32 | static_cast<unsigned>(index);
+                }
+        }
     }
     __syncthreads();
     return sh.listed;
+}
+
+// The cut among the list's n tokens behind which the running sum of w, `above` before the first of them, reaches `target`; one is kept at least.  The
+// tokens are left, in any order, in sh.bins.  Many are first told apart by buckets of their keys.
+__device__ __forceinline__ Cut cut_list(const SampleWeights& w, int n, double above, double target, double scale, PickShared& sh) {
+    constexpr int kOwn = kListed / kSampleThreads;
+    unsigned long long own[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) {
+        const int i = static_cast<int>(threadIdx.x) + k * kSampleThreads;
+        own[k] = i < n ? sh.list[i] : 0;
+    }
+    const auto key_of = [&](int k) { return ~static_cast<unsigned>(own[k] >> 32); };
+    const auto there = [&](int k) { return static_cast<int>(threadIdx.x) + k * kSampleThreads < n; };
+    int bucket = 0, shift = 31;
+    unsigned high = 0;
+    if (n > kSampleThreads) {
+        if (threadIdx.x == 0) {
+            sh.low = 0xFFFFFFFFu;
+            sh.high = 0;
+        }
+        for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.bins[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kOwn; k++)
+            if (there(k)) {
+                atomicMin(&sh.low, key_of(k));
+                atomicMax(&sh.high, key_of(k));
+            }
+        __syncthreads();
+        high = sh.high;
+        shift = max(0, 32 - __clz(high - sh.low) - 11);
+#pragma unroll
+        for (int k = 0; k < kOwn; k++)
+            if (there(k)) atomicAdd(&sh.bins[(high - key_of(k)) >> shift], whole_number(w.weight(key_value(key_of(k))), scale));
+        unsigned long long all;
+        bucket = find_bucket(sh, (target - above) * scale, all);
+        above += static_cast<double>(sh.above) / scale;
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) {
+        const int i = static_cast<int>(threadIdx.x) + k * kSampleThreads;
+        if (i < n) sh.bins[i] = own[k];
+        if (n > kSampleThreads) {
+            const bool wants = there(k) && static_cast<int>((high - key_of(k)) >> shift) == bucket;
+            const int at = take_places(wants, &sh.listed);
+            if (wants) sh.list[at] = own[k];
+        }
+    }
+    __syncthreads();
+    if (n > kSampleThreads) n = sh.listed;
+    sort_list(sh, n);
+    int from, to;
+    double all;
+    const double before = above + weigh_list(w, n, from, to, all, sh);
+    const int kept = count_kept(before, from, to, target, 0.0, true, sh);
+    Cut cut;
+    cut.key = ~static_cast<unsigned>(sh.list[kept - 1] >> 32);
+    cut.index = static_cast<int>(static_cast<unsigned>(sh.list[kept - 1]));
+    return cut;
 }
 
 __device__ __forceinline__ double target_of(const SampleParams& p, int r, double total) {
@@ -777,7 +895,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             const auto bucket_of = [&](float x) { return x == top ? 0 : static_cast<int>(fmin((static_cast<double>(top) - x) * fine, 1e9)); };
             int bound = kBuckets;
             for (int by_group = 4 * set.top_k <= 3 * tops.groups; by_group >= 0 && bound == kBuckets; by_group--) {
-                fine = by_group ? (kBuckets - 1) / fmax(static_cast<double>(top) - low, 1e-300) : kBuckets / kLeastPower / 64 * w.turn;
+                fine = by_group ? (kBuckets - 1) / fmax(static_cast<double>(top) - low, 1e-300) : kBuckets / -kLeastTurns * w.turn;
                 __syncthreads();
                 for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.counts[b] = 0;
                 if (threadIdx.x == 0) sh.bucket = kBuckets;
@@ -827,20 +945,32 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         int bound = kMassBuckets;
         const double grid = set.grid();
         const int place = grid_place(top, grid);
+        // how far a chunk's buckets lie behind the row's; all of them where it has none
+        const auto shift_of = [&](int c) { return w.weight(sh.chunk_tops[c]) > 0.0 ? place - grid_place(sh.chunk_tops[c], grid) : kMassBuckets; };
         if (set.on_grid(top, 0x1p29)) {
             // w by buckets, of all chunks, and the one in which their running sum reaches the target
             constexpr int kOwn = kMassBuckets / kSampleThreads;
             double own[kOwn], sum = 0.0, all;
 #pragma unroll
             for (int k = 0; k < kOwn; k++) own[k] = 0.0;
-            for (int c = 0; c < chunks; c++) {
-                const float t = sh.chunk_tops[c];
-                const double share = w.weight(t);
-                if (!(share > 0.0)) continue;
-                const int shift = place - grid_place(t, grid);
+            constexpr int kDeep = 4;  // chunks
+            for (int c0 = 0; c0 < chunks; c0 += kDeep) {
+                unsigned long long v[kDeep][kOwn];
 #pragma unroll
-                for (int k = 0; k < kOwn; k++)
-                    if (const int b = kOwn * static_cast<int>(threadIdx.x) + k - shift; b >= 0) own[k] += static_cast<double>(mass(c, b)) * share;
+                for (int d = 0; d < kDeep; d++) {
+                    const int shift = c0 + d < chunks ? shift_of(c0 + d) : kMassBuckets;
+#pragma unroll
+                    for (int k = 0; k < kOwn; k++) {
+                        const int b = kOwn * static_cast<int>(threadIdx.x) + k - shift;
+                        v[d][k] = b >= 0 ? mass(c0 + d, b) : 0;
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < kDeep; d++) {
+                    const double share = c0 + d < chunks ? w.weight(sh.chunk_tops[c0 + d]) : 0.0;
+#pragma unroll
+                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(v[d][k]) * share;
+                }
             }
 #pragma unroll
             for (int k = 0; k < kOwn; k++) sum += own[k] /= scale;
@@ -857,35 +987,35 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             __syncthreads();
             bound = sh.bucket;
         }
-        if (bound < kMassBuckets - 1) {  // (a chunk's last bucket holds what is further down as well)
+        if (bound < kMassBuckets) {  // (buckets end there)
             const double above = sh.mass_above;
-            const auto bucket_of = [&](float x) { return w.power64(x) > -64 * kLeastPower ? place - grid_place(x, grid) : kMassBuckets; };
+            const auto bucket_of = [&](float x) { return w.turns(x) > kLeastTurns ? place - grid_place(x, grid) : kMassBuckets; };
             const float least = least_that(top, [&](float x) { return bucket_of(x) <= bound; });
             listed = make_list(row, tops, sh, set.min_p > 0.0 ? fmaxf(least, least_that(top, [&](float x) { return w.weight(x) >= set.min_p; })) : least, INFINITY);
             if (listed > kListed) {  // the bucket's own tokens say where the cut is
                 const float next = bound > 0 ? least_that(top, [&](float x) { return bucket_of(x) < bound; }) : INFINITY;
                 const int own = make_list(row, tops, sh, least, bound > 0 ? key_value(order_key(next) - 1) : 3.402823466e38f);
                 if (own <= kListed) {
-                    sort_list(sh, own);
-                    int from, to;
-                    double all;
-                    const double before = above + weigh_list(w, own, from, to, all, sh);
-                    const int kept = count_kept(before, from, to, target, 0.0, true, sh);  // (the running sum reaches the target here: one at least)
-                    cut.key = ~static_cast<unsigned>(sh.list[kept - 1] >> 32);
-                    cut.index = static_cast<int>(static_cast<unsigned>(sh.list[kept - 1]));
+                    cut = cut_list(w, own, above, target, scale, sh);
                     if (set.min_p == 0.0 || -log2(set.min_p) * kMassFine > bound + 2) {
                         // what the chunks keep: all above the bucket, and of its own what is kept.  Only the chunk that the draw falls into is read again
                         for (int c = static_cast<int>(threadIdx.x) >> 6; c < chunks; c += kSampleWaves) {
-                            const float t = sh.chunk_tops[c];
-                            const double share = w.weight(t);
+                            constexpr int kDeep = 8;
+                            const int shift = shift_of(c);
                             double sum = 0.0;
-                            if (share > 0.0) {
-                                const int shift = place - grid_place(t, grid);
-                                for (int b = shift + static_cast<int>(threadIdx.x & 63); b < bound; b += 64) sum += static_cast<double>(mass(c, b - shift));
-                                sum *= share / scale;
+                            for (int b0 = shift + static_cast<int>(threadIdx.x & 63); b0 < bound; b0 += 64 * kDeep) {
+                                unsigned long long v[kDeep];
+#pragma unroll
+                                for (int d = 0; d < kDeep; d++) v[d] = b0 + 64 * d < bound ? mass(c, b0 + 64 * d - shift) : 0;
+#pragma unroll
+                                for (int d = 0; d < kDeep; d++) sum += static_cast<double>(v[d]);
                             }
-                            for (int i = threadIdx.x & 63; i < kept; i += 64)
-                                if (static_cast<int>(static_cast<unsigned>(sh.list[i])) / chunk == c) sum += sh.weights[i];
+                            sum *= w.weight(sh.chunk_tops[c]) / scale;
+                            for (int i = threadIdx.x & 63; i < own; i += 64) {
+                                const unsigned key = ~static_cast<unsigned>(sh.bins[i] >> 32);
+                                const int index = static_cast<int>(static_cast<unsigned>(sh.bins[i]));
+                                if (index / chunk == c && cut.keeps(key, index)) sum += w.weight(key_value(key));
+                            }
                             sum = wave_scan(sum);
                             if ((threadIdx.x & 63) == 63) sh.chunk_sums[c] = sum;
                         }
@@ -949,15 +1079,16 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const Sample
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
     const float top = scan_chunk<TYPE, kSampleThreads>(p, row, set, 0, left);
-    if (threadIdx.x < 64) sh.powers[threadIdx.x] = left.powers[threadIdx.x];
+    sh.powers[threadIdx.x] = left.powers[threadIdx.x];
+    static_assert(kPowers == kSampleThreads, "");
     __syncthreads();
     pick_row(p, r, row, set, kChunk, 1, [&](int g) { return left.group_tops[g]; }, [&](int) { return top; }, [&](int s) { return left.segments[s]; },
              [&](int, int b) { return left.masses[b]; }, sh);
 }
 
-// One chunk of a row, for sample_pick_kernel.  Two workgroups to a compute unit, so that one reads while the other computes.
+// One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute.
 template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS, 6) void sample_scan_kernel(const SampleParams p) {
     __shared__ ChunkShared<THREADS> left;
     constexpr int kLength = THREADS * kVec * kRounds, kGroups = kLength / kGroup, kSegments = kLength / kSegment;
     const int c = static_cast<int>(blockIdx.x) % p.chunks, r = p.first_row + static_cast<int>(blockIdx.x) / p.chunks, t = threadIdx.x;

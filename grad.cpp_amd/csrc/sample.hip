@@ -2,6 +2,7 @@
 #include "device_scope.h"
 #include "kernels_sample.h"
 
+#include <array>
 #include <cmath>
 
 namespace gh {
@@ -90,7 +91,12 @@ static void sample(const gh_sample_args& a, hipStream_t stream) {
     p.uniforms = a.uniforms;
     p.ids = a.ids;
     p.probs = a.probs;
-    for (int j = 0; j < 64; j++) p.powers[j] = std::exp2(j / 64.0);
+    static const std::array<double, kPowers> powers = [] {
+        std::array<double, kPowers> t;
+        for (int j = 0; j < kPowers; j++) t[static_cast<size_t>(j)] = std::exp2(static_cast<double>(j) / kPowers);
+        return t;
+    }();
+    std::copy(powers.begin(), powers.end(), p.powers);
     char* const work = static_cast<char*>(a.workspace);
     p.chunks = f.chunks;
     p.group_tops = reinterpret_cast<float*>(work + f.group_tops);
