@@ -62,6 +62,10 @@ struct SampleParams {
     float* chunk_tops;
     double* segment_sums;
     unsigned long long* masses;
+    // where several workgroups look through a row of many groups: [2] (listed, arrived), [kListed]
+    int shares;
+    unsigned* counters;
+    unsigned long long* lists;
 };
 
 constexpr int groups_of(int vocab) { return (vocab + kGroup - 1) / kGroup; }
@@ -132,10 +136,10 @@ struct SampleRow {
         const float x = static_cast<float>(e);
         return x == x ? x + 0.0f : -INFINITY;
     }
+    // (Without a condition but for the row's end, so that many loads can be under way at once.)
     __device__ __forceinline__ void load_raw(int i0, T (&e)[kVec]) const {
-        if (i0 + kVec <= vocab) {
-            __builtin_memcpy(e, at + i0, sizeof(e));
-        } else {
+        if (vocab >= kVec) __builtin_memcpy(e, at + min(i0, vocab - kVec), sizeof(e));
+        if (i0 + kVec > vocab) {
 #pragma unroll
             for (int i = 0; i < kVec; i++) e[i] = i0 + i < vocab ? at[i0 + i] : static_cast<T>(-INFINITY);
         }
@@ -180,7 +184,6 @@ template <int THREADS>
 struct ChunkShared {
     unsigned long long masses[kMassBuckets];
     double segments[THREADS * kVec * kRounds / kSegment];
-    double powers[kPowers];
     float group_tops[THREADS * kVec * kRounds / kGroup];
     float tops[THREADS / 64];
 };
@@ -197,13 +200,15 @@ struct PickShared {
         double weights[kListed];
     };
     unsigned ranks[kSampleThreads];
-    double powers[kPowers];
     double chunk_sums[kMaxSampleVocab / kChunk];
     float chunk_tops[kMaxSampleVocab / kChunk];
+    double chunk_shares[kMaxSampleVocab / kChunk];  // of a w relative to its chunk's largest, relative to the row's
+    int chunk_shifts[kMaxSampleVocab / kChunk];     // how far its buckets lie behind the row's; all of them where it has none
     unsigned long long scan[kSampleWaves];
     double sums[kSampleWaves];
     int ints[kSampleWaves];
-    float tops[kSampleWaves];
+    float tops[kSampleWaves], lows[kSampleWaves];
+    unsigned long long chunk_wholes[kMaxSampleVocab / kChunk];
     unsigned low, high;
     unsigned long long above;  // of the histogram, before the bucket that was found
     double mass_above;
@@ -218,7 +223,7 @@ constexpr double kMagic = 0x1.8p52;  // added to a number below 2^51 leaves it r
 // 256 log2 of a w of `z`, or what is not a number.
 __device__ __forceinline__ double weight_of(double z, const double* powers) {
     constexpr double l = 0.69314718055994530942 / kPowers, c2 = l * l / 2, c3 = l * l * l / 6;
-    z = z > kLeastTurns ? z : -1e9;
+    z = z > kLeastTurns ? z : -1e9;  // (at 0 then)
     const double t = z + kMagic, r = z - (t - kMagic);
     const int n = static_cast<int>(__double_as_longlong(t));
     const double head = powers[n & (kPowers - 1)];
@@ -280,16 +285,35 @@ __device__ __forceinline__ float block_top(float v, float* tops) {
     return v;
 }
 
-// One chunk of a row, from `first` on.  Leaves the groups' largest logits, and where they are wanted the segments' sums, relative to the largest of
-// the chunk, and w by buckets of x, from the chunk's largest down.  Returns the largest.
+// The largest and the least of the workgroup's. (Of the threads that pick.)
+__device__ __forceinline__ void block_ends(float& high, float& low, PickShared& sh) {
+    high = wave_max(high);
+    low = -wave_max(-low);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        sh.tops[threadIdx.x >> 6] = high;
+        sh.lows[threadIdx.x >> 6] = low;
+    }
+    __syncthreads();
+    high = sh.tops[0];
+    low = sh.lows[0];
+#pragma unroll
+    for (int w = 1; w < kSampleWaves; w++) {
+        high = fmaxf(high, sh.tops[w]);
+        low = fminf(low, sh.lows[w]);
+    }
+}
+
+// One chunk of a row, from `first` on.  Leaves the groups' largest logits, and where they are wanted the segments' sums (with buckets, the wavefronts'), relative
+// to the largest of the chunk, and w by buckets of x, from the chunk's largest down.  Returns the largest.
 template <int TYPE, int THREADS>
-__device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, ChunkShared<THREADS>& sh) {
+__device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, const double* powers,
+                                            ChunkShared<THREADS>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     using T = typename SampleRow<TYPE>::T;
     T raw[kRounds][kVec];
 #pragma unroll
     for (int r = 0; r < kRounds; r++) row.load_raw(first + (r * THREADS + static_cast<int>(threadIdx.x)) * kVec, raw[r]);
-    fill_powers(p, sh.powers);
     float top = -INFINITY;
 #pragma unroll
     for (int r = 0; r < kRounds; r++) {
@@ -318,24 +342,34 @@ __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleR
     const double turn = set.turn(), scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52), grid = set.grid();
     const int place = grid_place(top, grid);
     const auto sum_up = [&](auto counted) {
+        double all = 0.0;
 #pragma unroll
         for (int r = 0; r < kRounds; r++) {
             double sum = 0.0;
 #pragma unroll
             for (int i = 0; i < kVec; i++) {
                 const float x = static_cast<float>(raw[r][i]);  // (NaN: nothing)
-                const double v = weight_of((static_cast<double>(x) - base) * turn, sh.powers);
+                const double z = (static_cast<double>(x) - base) * turn, v = weight_of(z, powers);
                 sum += v;
                 if constexpr (decltype(counted)::value) {
-                    // (what is no number on the grid has a w of nothing)
+                    // (what has no place on the grid has a w of nothing)
                     const unsigned b = static_cast<unsigned>(place - grid_place(x, grid));
-                    if (b < kMassBuckets && v > 0.0) atomicAdd(&sh.masses[b], whole_number(v, scale));
+                    if (z > kLeastTurns && b < kMassBuckets) atomicAdd(&sh.masses[b], whole_number(v, scale));
                 }
             }
-            sum = wave_scan(sum);
-            if (lane == 63) sh.segments[r * (THREADS / 64) + wave] = sum;
+            if constexpr (decltype(counted)::value) {
+                all += sum;
+            } else {
+                sum = wave_scan(sum);
+                if (lane == 63) sh.segments[r * (THREADS / 64) + wave] = sum;
+            }
+        }
+        if constexpr (decltype(counted)::value) {
+            all = wave_scan(all);
+            if (lane == 63) sh.segments[wave] = all;
         }
     };
+    // (with buckets the first THREADS / 64 sums are those of the wavefronts over the whole chunk)
     if (masses && set.on_grid(top)) {
         sum_up(std::true_type{});
     } else {
@@ -532,7 +566,8 @@ struct GroupTops {
 #pragma unroll
         for (int k = 0; k < kOwn; k++) {
             const int g = from + k * kSampleThreads + static_cast<int>(threadIdx.x);
-            v[k] = g < groups ? at(g) : -INFINITY;
+            const float t = at(min(g, groups - 1));
+            v[k] = g < groups ? t : -INFINITY;
         }
     }
     // f called by all threads alike
@@ -566,6 +601,57 @@ __device__ __forceinline__ float least_that(float top, F&& may) {
         if (end < high) high = static_cast<unsigned>(end);
     }
     return key_value(high);
+}
+
+// A float a little below x.
+__device__ __forceinline__ float below(double x) {
+    constexpr float kMost = 3.402823466e38f;
+    const unsigned key = order_key(static_cast<float>(fmin(fmax(x, -kMost), kMost)));
+    return key_value(max(key - 2, order_key(-kMost)));
+}
+
+// Which of the row's logits are from `least` to `most`: f(set bits' count) gives a thread's first place, put(place, index) takes each.  `share` of `shares`.
+template <int TYPE, typename F, typename G>
+__device__ __forceinline__ void look_through(const SampleRow<TYPE>& row, float least, float most, int share, int shares, F&& places, G&& put) {
+    using T = typename SampleRow<TYPE>::T;
+    constexpr int kDeep = 8, kStep = kSampleThreads * kVec, kMasks = kDeep * kVec / 32;
+    for (int from = share * kDeep * kStep; from < row.vocab; from += shares * kDeep * kStep) {
+        const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
+        T e[kDeep][kVec];
+        unsigned mask[kMasks];
+#pragma unroll
+        for (int k = 0; k < kDeep; k++) row.load_raw(i0 + k * kStep, e[k]);
+        int wants = 0;
+#pragma unroll
+        for (int m = 0; m < kMasks; m++) {
+            mask[m] = 0;
+#pragma unroll
+            for (int b = 0; b < 32; b++) {
+                const float x = static_cast<float>(e[m * 32 / kVec + b / kVec][b % kVec]);
+                mask[m] |= x >= least && x <= most ? 1u << b : 0u;
+            }
+            wants += __popc(mask[m]);
+        }
+        int at = places(wants);
+#pragma unroll
+        for (int m = 0; m < kMasks; m++)
+            for (; mask[m]; mask[m] &= mask[m] - 1, at++) {
+                const int b = m * 32 + __ffs(mask[m]) - 1;
+                put(at, i0 + b / kVec * kStep + b % kVec);
+            }
+    }
+}
+// Places for all that a wavefront's lanes want, from a counter that `add` adds to.
+template <typename F>
+__device__ __forceinline__ int wave_places(int wants, F&& add) {
+    const int upto = wave_scan(wants);
+    int first = 0;
+    if ((threadIdx.x & 63) == 63 && upto > 0) first = add(upto);
+    return __builtin_amdgcn_readlane(first, 63) + upto - wants;
+}
+template <int TYPE>
+__device__ __forceinline__ unsigned long long list_entry(const SampleRow<TYPE>& row, int index) {
+    return static_cast<unsigned long long>(~order_key(row.one(index))) << 32 | static_cast<unsigned>(index);
 }
 
 // The tokens of logits from `least` to `most` into sh.list, by (key descending, index).  Returns how many; more than kListed: the list is not
@@ -605,40 +691,40 @@ __device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS&
     } else if (most == INFINITY) {
         return hot;  // (each holds one at least)
     } else {
-        // the whole row: which of a thread's logits, then places for all of a wavefront's at once
-        using T = typename SampleRow<TYPE>::T;
-        constexpr int kDeep = 16, kStep = kSampleThreads * kVec;
-        for (int from = 0; from < row.vocab; from += kDeep * kStep) {
-            const int i0 = from + static_cast<int>(threadIdx.x) * kVec;
-            T e[kDeep][kVec];
-            unsigned mask[kDeep * kVec / 32];
-#pragma unroll
-            for (int k = 0; k < kDeep; k++) row.load_raw(i0 + k * kStep, e[k]);
-            int wants = 0;
-#pragma unroll
-            for (int m = 0; m < kDeep * kVec / 32; m++) {
-                mask[m] = 0;
-#pragma unroll
-                for (int b = 0; b < 32; b++) {
-                    const float x = static_cast<float>(e[m * 32 / kVec + b / kVec][b % kVec]);
-                    mask[m] |= x >= least && x <= most ? 1u << b : 0u;
-                }
-                wants += __popc(mask[m]);
-            }
-            const int upto = wave_scan(wants);
-            int first = 0;
-            if (lane == 63 && upto > 0) first = atomicAdd(&sh.listed, upto);
-            int at = __builtin_amdgcn_readlane(first, 63) + upto - wants;
-#pragma unroll
-            for (int m = 0; m < kDeep * kVec / 32; m++)
-                for (; mask[m]; mask[m] &= mask[m] - 1, at++) {
-                    const int b = m * 32 + __ffs(mask[m]) - 1, index = i0 + b / kVec * kStep + b % kVec;
-                    if (at < kListed) sh.list[at] = static_cast<unsigned long long>(~order_key(row.one(index))) << 32 | static_cast<unsigned>(index);
-                }
-        }
+        look_through(row, least, most, 0, 1, [&](int wants) { return wave_places(wants, [&](int n) { return atomicAdd(&sh.listed, n); }); },
+                     [&](int at, int index) {
+                         if (at < kListed) sh.list[at] = list_entry(row, index);
+                     });
     }
     __syncthreads();
     return sh.listed;
+}
+
+// The same for rows that p.shares workgroups look through: -1 to all but the last of them to end.
+template <int TYPE>
+__device__ __forceinline__ int make_list_together(const SampleParams& p, int r, const SampleRow<TYPE>& row, int share, PickShared& sh, float least, float most) {
+    unsigned* const counters = p.counters + 2 * static_cast<size_t>(r);
+    unsigned long long* const list = p.lists + static_cast<size_t>(r) * kListed;
+    look_through(row, least, most, share, p.shares,
+                 [&](int wants) {
+                     return wave_places(wants, [&](int n) {
+                         return static_cast<int>(__hip_atomic_fetch_add(counters, static_cast<unsigned>(n), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                     });
+                 },
+                 [&](int at, int index) {
+                     if (at < kListed) __hip_atomic_store(list + at, list_entry(row, index), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                 });
+    // the stores have to be out before the workgroup counts as arrived
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        sh.found = __hip_atomic_fetch_add(counters + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<unsigned>(p.shares - 1);
+    __syncthreads();
+    if (!sh.found) return -1;
+    const int listed = static_cast<int>(__hip_atomic_load(counters, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    for (int i = threadIdx.x; i < min(listed, kListed); i += kSampleThreads) sh.list[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return listed;
 }
 
 // The cut among the list's n tokens behind which the running sum of w, `above` before the first of them, reaches `target`; one is kept at least.  The
@@ -656,21 +742,17 @@ __device__ __forceinline__ Cut cut_list(const SampleWeights& w, int n, double ab
     int bucket = 0, shift = 31;
     unsigned high = 0;
     if (n > kSampleThreads) {
-        if (threadIdx.x == 0) {
-            sh.low = 0xFFFFFFFFu;
-            sh.high = 0;
-        }
-        for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.bins[b] = 0;
-        __syncthreads();
+        float most = -INFINITY, least = INFINITY;
 #pragma unroll
         for (int k = 0; k < kOwn; k++)
             if (there(k)) {
-                atomicMin(&sh.low, key_of(k));
-                atomicMax(&sh.high, key_of(k));
+                most = fmaxf(most, key_value(key_of(k)));
+                least = fminf(least, key_value(key_of(k)));
             }
-        __syncthreads();
-        high = sh.high;
-        shift = max(0, 32 - __clz(high - sh.low) - 11);
+        for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.bins[b] = 0;
+        block_ends(most, least, sh);
+        high = order_key(most);
+        shift = max(0, 32 - __clz(high - order_key(least)) - 11);
 #pragma unroll
         for (int k = 0; k < kOwn; k++)
             if (there(k)) atomicAdd(&sh.bins[(high - key_of(k)) >> shift], whole_number(w.weight(key_value(key_of(k))), scale));
@@ -736,6 +818,43 @@ __device__ __forceinline__ void draw_listed(const SampleParams& p, int r, int ke
         const int at = min(static_cast<int>(min(sh.low, 0x7FFFFFFFu)), kept - 1);
         p.ids[r] = static_cast<int>(sh.list[at] >> 32);
         if (p.probs) p.probs[r] = static_cast<float>(weight(at) / total);
+    }
+}
+
+__device__ __forceinline__ unsigned long long read_lane(unsigned long long v, int lane) {
+    return static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32
+           | static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ unsigned long long to_lane(unsigned long long v, int lane) {
+    return static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_ds_permute(lane * 4, static_cast<int>(v >> 32)))) << 32
+           | static_cast<unsigned>(__builtin_amdgcn_ds_permute(lane * 4, static_cast<int>(v)));
+}
+
+// A list of at most 64 tokens from its order to the pick, by one wavefront, a token to a lane.
+__device__ __forceinline__ void pick_few(const SampleParams& p, int r, const SampleWeights& w, const SampleSettings& set, int n, double total, const PickShared& sh) {
+    const int lane = threadIdx.x;
+    unsigned long long item = lane < n ? sh.list[lane] : ~0ull << 32 | static_cast<unsigned>(lane);
+    int rank = 0;
+    for (int j = 0; j < 64; j++) rank += read_lane(item, j) < item;
+    item = to_lane(item, rank);
+    if (set.top_k > 0) n = min(n, set.top_k);
+    double v = lane < n ? w.weight(key_value(~static_cast<unsigned>(item >> 32))) : 0.0;
+    double upto = wave_scan(v), before = __shfl_up(upto, 1);
+    if (lane == 0) before = 0.0;
+    const double target = set.top_p < 1.0 ? set.top_p * (set.top_k > 0 ? __shfl(upto, 63) : total) : INFINITY;
+    const int kept = __popcll(__ballot(v > 0.0 && (lane == 0 || (before < target && v >= set.min_p))));
+    // by their indices
+    unsigned long long index = lane < kept ? static_cast<unsigned>(item) : 1ull << 32 | static_cast<unsigned>(lane);
+    rank = 0;
+    for (int j = 0; j < 64; j++) rank += read_lane(index, j) < index;
+    index = to_lane(index, rank);
+    v = __longlong_as_double(static_cast<long long>(to_lane(static_cast<unsigned long long>(__double_as_longlong(lane < kept ? v : 0.0)), rank)));
+    upto = wave_scan(v);
+    const double all = __shfl(upto, 63);
+    const unsigned long long hits = __ballot(lane < kept && upto >= target_of(p, r, all));
+    if (lane == (hits ? __ffsll(hits) - 1 : kept - 1)) {
+        p.ids[r] = static_cast<int>(static_cast<unsigned>(index));
+        if (p.probs) p.probs[r] = static_cast<float>(v / all);
     }
 }
 
@@ -826,10 +945,10 @@ __device__ __forceinline__ void draw_segments(const SampleParams& p, int r, cons
 // ----------------------------------------------------------------------- a row
 
 // From what the chunks left to the pick.  group_top(g), chunk_top(c), segment_sum(s) and mass(c, b), the last two relative to their chunk's
-// largest and only there where that is not minus infinity.
+// largest and only there where that is not minus infinity.  `share`: this workgroup's of the row's (p.shares).
 template <int TYPE, typename GROUP, typename CHUNK, typename SEGMENT, typename MASS>
-__device__ __forceinline__ void pick_row(const SampleParams& p, int r, const SampleRow<TYPE>& row, const SampleSettings& set, int chunk, int chunks,
-                                         const GROUP& group_top, const CHUNK& chunk_top, const SEGMENT& segment_sum, const MASS& mass, PickShared& sh) {
+__device__ __forceinline__ void pick_row(const SampleParams& p, int r, const SampleRow<TYPE>& row, const SampleSettings& set, int chunk, int chunks, int share,
+                                         const GROUP& group_top, const CHUNK& chunk_top, const SEGMENT& segment_sum, const MASS& mass, const double* powers, PickShared& sh) {
     const GroupTops<GROUP> tops(group_top, groups_of(p.vocab));
     float top = -INFINITY, low = INFINITY;  // of the groups' largest
     tops.each([&](float t, int) {
@@ -837,7 +956,8 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         low = t > -INFINITY ? fminf(low, t) : low;
     });
     for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_tops[c] = chunk_top(c);
-    top = block_top<kSampleThreads>(top, sh.tops);
+    if (share > 0 && !set.masses()) return;  // (the first alone has work)
+    block_ends(top, low, sh);
     if (top == -INFINITY) {
         if (threadIdx.x == 0) {
             p.ids[r] = -1;
@@ -862,12 +982,14 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         }
         return;
     }
-    const SampleWeights w{top, set.turn(), sh.powers};
+    const SampleWeights w{top, set.turn(), powers};
     const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52);
     const int segments = segments_of(p.vocab);
+    for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_shares[c] = w.weight(sh.chunk_tops[c]);  // (its own thread's)
+    __syncthreads();
     const auto sum_of = [&](int s) {
-        const double share = w.weight(sh.chunk_tops[s * kSegment / chunk]);
-        return share > 0.0 ? segment_sum(s) * share : 0.0;
+        const double chunk_share = sh.chunk_shares[s * kSegment / chunk];
+        return chunk_share > 0.0 ? segment_sum(s) * chunk_share : 0.0;
     };
 
     if (set.sums() && set.top_p == 1.0) {  // nothing is cut
@@ -884,13 +1006,13 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         return;
     }
 
+    const auto min_p_reach = [&] { return top + kPowers * log2(set.min_p) / w.turn; };  // the logit of w = min_p
     Cut cut;
     double total = 0.0;  // of what top-p is a share of
     int listed = kListed + 1;
     if (set.top_k > 0) {
         // buckets of the logits, from the largest down, and the one that holds the k-th largest of the groups' largest, or of all where groups are few
         if (set.top_k <= kListed) {
-            low = -block_top<kSampleThreads>(-low, sh.tops);
             double fine = 0.0;
             const auto bucket_of = [&](float x) { return x == top ? 0 : static_cast<int>(fmin((static_cast<double>(top) - x) * fine, 1e9)); };
             int bound = kBuckets;
@@ -924,7 +1046,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                 bound = sh.bucket;
             }
             // (none: fewer than k tokens have a w)
-            listed = make_list(row, tops, sh, least_that(top, [&](float x) { return bucket_of(x) <= bound; }), INFINITY);
+            listed = make_list(row, tops, sh, below(static_cast<double>(top) - (bound + 1) / fine), INFINITY);
         }
         if (listed > kListed) {
             cut = find_cut<TYPE, false>(row, w, scale, cut, set.top_k, sh);
@@ -939,41 +1061,45 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         }
     } else if (set.top_p < 1.0) {
         double mine = 0.0;
-        for (int s = threadIdx.x; s < segments; s += kSampleThreads) mine += sum_of(s);
+        const int waves = chunk / (kVec * kRounds * 64);
+        for (int i = threadIdx.x; i < chunks * waves; i += kSampleThreads)
+            if (const int s = i / waves * (chunk / kSegment) + i % waves; s < segments) mine += sum_of(s);
         (void)block_scan(mine, sh.sums, total);
         const double target = set.top_p * total;
         int bound = kMassBuckets;
         const double grid = set.grid();
         const int place = grid_place(top, grid);
-        // how far a chunk's buckets lie behind the row's; all of them where it has none
-        const auto shift_of = [&](int c) { return w.weight(sh.chunk_tops[c]) > 0.0 ? place - grid_place(sh.chunk_tops[c], grid) : kMassBuckets; };
+        for (int c = threadIdx.x; c < chunks; c += kSampleThreads)
+            sh.chunk_shifts[c] = sh.chunk_shares[c] > 0.0 ? place - grid_place(sh.chunk_tops[c], grid) : kMassBuckets;
+        __syncthreads();
         if (set.on_grid(top, 0x1p29)) {
             // w by buckets, of all chunks, and the one in which their running sum reaches the target
             constexpr int kOwn = kMassBuckets / kSampleThreads;
             double own[kOwn], sum = 0.0, all;
 #pragma unroll
             for (int k = 0; k < kOwn; k++) own[k] = 0.0;
-            constexpr int kDeep = 4;  // chunks
+            constexpr int kDeep = 8;  // chunks
             for (int c0 = 0; c0 < chunks; c0 += kDeep) {
                 unsigned long long v[kDeep][kOwn];
 #pragma unroll
                 for (int d = 0; d < kDeep; d++) {
-                    const int shift = c0 + d < chunks ? shift_of(c0 + d) : kMassBuckets;
+                    const int shift = c0 + d < chunks ? sh.chunk_shifts[c0 + d] : kMassBuckets;
 #pragma unroll
                     for (int k = 0; k < kOwn; k++) {
                         const int b = kOwn * static_cast<int>(threadIdx.x) + k - shift;
-                        v[d][k] = b >= 0 ? mass(c0 + d, b) : 0;
+                        const unsigned long long held = mass(min(c0 + d, chunks - 1), max(b, 0));
+                        v[d][k] = b >= 0 ? held : 0;
                     }
                 }
 #pragma unroll
                 for (int d = 0; d < kDeep; d++) {
-                    const double share = c0 + d < chunks ? w.weight(sh.chunk_tops[c0 + d]) : 0.0;
+                    const double chunk_share = c0 + d < chunks ? sh.chunk_shares[c0 + d] : 0.0;
 #pragma unroll
-                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(v[d][k]) * share;
+                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(v[d][k]) * chunk_share;
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kOwn; k++) sum += own[k] /= scale;
+            for (int k = 0; k < kOwn; k++) sum += own[k] *= 1.0 / scale;
             if (threadIdx.x == 0) sh.bucket = kMassBuckets;
             double before = block_scan(sum, sh.sums, all);
 #pragma unroll
@@ -990,34 +1116,55 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         if (bound < kMassBuckets) {  // (buckets end there)
             const double above = sh.mass_above;
             const auto bucket_of = [&](float x) { return w.turns(x) > kLeastTurns ? place - grid_place(x, grid) : kMassBuckets; };
-            const float least = least_that(top, [&](float x) { return bucket_of(x) <= bound; });
-            listed = make_list(row, tops, sh, set.min_p > 0.0 ? fmaxf(least, least_that(top, [&](float x) { return w.weight(x) >= set.min_p; })) : least, INFINITY);
+            const double reach = (place - bound - 0.5) / grid;
+            listed = make_list(row, tops, sh, below(fmax(reach, set.min_p > 0.0 ? min_p_reach() : reach)), INFINITY);
             if (listed > kListed) {  // the bucket's own tokens say where the cut is
+                const float least = least_that(top, [&](float x) { return bucket_of(x) <= bound; });
                 const float next = bound > 0 ? least_that(top, [&](float x) { return bucket_of(x) < bound; }) : INFINITY;
-                const int own = make_list(row, tops, sh, least, bound > 0 ? key_value(order_key(next) - 1) : 3.402823466e38f);
+                const float most = bound > 0 ? key_value(order_key(next) - 1) : 3.402823466e38f;
+                const bool together = p.shares > 1 && sh.found > kListed;  // (found: the groups that reach so far)
+                if (share > 0 && !together) return;
+                const int own = together ? make_list_together(p, r, row, share, sh, least, most) : make_list(row, tops, sh, least, most);
+                if (own < 0) return;
+                share = 0;  // (the last of them goes on)
                 if (own <= kListed) {
                     cut = cut_list(w, own, above, target, scale, sh);
                     if (set.min_p == 0.0 || -log2(set.min_p) * kMassFine > bound + 2) {
                         // what the chunks keep: all above the bucket, and of its own what is kept.  Only the chunk that the draw falls into is read again
-                        for (int c = static_cast<int>(threadIdx.x) >> 6; c < chunks; c += kSampleWaves) {
-                            constexpr int kDeep = 8;
-                            const int shift = shift_of(c);
+                        constexpr int kDeep = 8, kOwn = kMassBuckets / kSampleThreads;  // chunks
+                        for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_wholes[c] = 0;
+                        __syncthreads();
+                        for (int i = threadIdx.x; i < own; i += kSampleThreads) {
+                            const unsigned key = ~static_cast<unsigned>(sh.bins[i] >> 32);
+                            const int index = static_cast<int>(static_cast<unsigned>(sh.bins[i]));
+                            if (cut.keeps(key, index)) atomicAdd(&sh.chunk_wholes[index / chunk], whole_number(w.weight(key_value(key)), scale));
+                        }
+                        for (int c0 = 0; c0 < chunks; c0 += kDeep) {
+                            unsigned long long v[kDeep][kOwn];
+#pragma unroll
+                            for (int d = 0; d < kDeep; d++) {
+                                const int shift = c0 + d < chunks ? sh.chunk_shifts[c0 + d] : kMassBuckets;
+#pragma unroll
+                                for (int k = 0; k < kOwn; k++) {
+                                    const int b = static_cast<int>(threadIdx.x) + k * kSampleThreads;
+                                    const unsigned long long held = mass(min(c0 + d, chunks - 1), max(b - shift, 0));
+                                    v[d][k] = b >= shift && b < bound ? held : 0;
+                                }
+                            }
+#pragma unroll
+                            for (int d = 0; d < kDeep; d++) {
+                                double sum = 0.0;
+#pragma unroll
+                                for (int k = 0; k < kOwn; k++) sum += static_cast<double>(v[d][k]);
+                                sum = wave_scan(sum);
+                                if (c0 + d < chunks && (threadIdx.x & 63) == 63) sh.segments[(c0 + d) * kSampleWaves + (threadIdx.x >> 6)] = sum;
+                            }
+                        }
+                        __syncthreads();
+                        for (int c = threadIdx.x; c < chunks; c += kSampleThreads) {
                             double sum = 0.0;
-                            for (int b0 = shift + static_cast<int>(threadIdx.x & 63); b0 < bound; b0 += 64 * kDeep) {
-                                unsigned long long v[kDeep];
-#pragma unroll
-                                for (int d = 0; d < kDeep; d++) v[d] = b0 + 64 * d < bound ? mass(c, b0 + 64 * d - shift) : 0;
-#pragma unroll
-                                for (int d = 0; d < kDeep; d++) sum += static_cast<double>(v[d]);
-                            }
-                            sum *= w.weight(sh.chunk_tops[c]) / scale;
-                            for (int i = threadIdx.x & 63; i < own; i += 64) {
-                                const unsigned key = ~static_cast<unsigned>(sh.bins[i] >> 32);
-                                const int index = static_cast<int>(static_cast<unsigned>(sh.bins[i]));
-                                if (index / chunk == c && cut.keeps(key, index)) sum += w.weight(key_value(key));
-                            }
-                            sum = wave_scan(sum);
-                            if ((threadIdx.x & 63) == 63) sh.chunk_sums[c] = sum;
+                            for (int k = 0; k < kSampleWaves; k++) sum += sh.segments[c * kSampleWaves + k];
+                            sh.chunk_sums[c] = (sum * sh.chunk_shares[c] + static_cast<double>(sh.chunk_wholes[c])) / scale;
                         }
                         __syncthreads();
                         double held = 0.0;
@@ -1049,9 +1196,14 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
         }
     } else {
-        listed = make_list(row, tops, sh, least_that(top, [&](float x) { return w.weight(x) >= set.min_p; }), INFINITY);
+        listed = make_list(row, tops, sh, below(min_p_reach()), INFINITY);
     }
+    if (share > 0) return;
 
+    if (listed <= 64) {
+        if (threadIdx.x < 64) pick_few(p, r, w, set, listed, total, sh);
+        return;
+    }
     if (listed <= kListed) {
         sort_list(sh, listed);
         if (set.top_k > 0) listed = min(listed, set.top_k);
@@ -1075,29 +1227,32 @@ template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const SampleParams p) {
     __shared__ ChunkShared<kSampleThreads> left;
     __shared__ PickShared sh;
+    __shared__ double powers[kPowers];
+    fill_powers(p, powers);
     const int r = p.first_row + static_cast<int>(blockIdx.x);
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
-    const float top = scan_chunk<TYPE, kSampleThreads>(p, row, set, 0, left);
-    sh.powers[threadIdx.x] = left.powers[threadIdx.x];
-    static_assert(kPowers == kSampleThreads, "");
+    const float top = scan_chunk<TYPE, kSampleThreads>(p, row, set, 0, powers, left);
     __syncthreads();
-    pick_row(p, r, row, set, kChunk, 1, [&](int g) { return left.group_tops[g]; }, [&](int) { return top; }, [&](int s) { return left.segments[s]; },
-             [&](int, int b) { return left.masses[b]; }, sh);
+    pick_row(p, r, row, set, kChunk, 1, 0, [&](int g) { return left.group_tops[g]; }, [&](int) { return top; }, [&](int s) { return left.segments[s]; },
+             [&](int, int b) { return left.masses[b]; }, powers, sh);
 }
 
 // One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute.
 template <int TYPE, int THREADS>
 __global__ __launch_bounds__(THREADS, 6) void sample_scan_kernel(const SampleParams p) {
     __shared__ ChunkShared<THREADS> left;
+    __shared__ double powers[kPowers];
+    fill_powers(p, powers);
     constexpr int kLength = THREADS * kVec * kRounds, kGroups = kLength / kGroup, kSegments = kLength / kSegment;
     const int c = static_cast<int>(blockIdx.x) % p.chunks, r = p.first_row + static_cast<int>(blockIdx.x) / p.chunks, t = threadIdx.x;
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
-    const float top = scan_chunk<TYPE, THREADS>(p, row, set, c * kLength, left);
+    const float top = scan_chunk<TYPE, THREADS>(p, row, set, c * kLength, powers, left);
     __syncthreads();
     for (int g = t; g < kGroups && c * kGroups + g < groups_of(p.vocab); g += THREADS)
         p.group_tops[static_cast<size_t>(r) * groups_of(p.vocab) + c * kGroups + g] = left.group_tops[g];
+    if (p.shares > 1 && c == 0 && t < 2) p.counters[2 * static_cast<size_t>(r) + t] = 0;
     if (t == 0) p.chunk_tops[static_cast<size_t>(r) * p.chunks + c] = top;
     if (top == -INFINITY) return;
     if (set.sums() && t < kSegments && c * kSegments + t < segments_of(p.vocab))
@@ -1109,16 +1264,17 @@ __global__ __launch_bounds__(THREADS, 6) void sample_scan_kernel(const SamplePar
 template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(const SampleParams p, int chunk) {
     __shared__ PickShared sh;
-    const int r = p.first_row + static_cast<int>(blockIdx.x);
+    __shared__ double powers[kPowers];
+    const int r = p.first_row + static_cast<int>(blockIdx.x) / p.shares, share = static_cast<int>(blockIdx.x) % p.shares;
     const SampleRow<TYPE> row(p, r);
     const SampleSettings set(p, r);
-    fill_powers(p, sh.powers);
+    fill_powers(p, powers);
     const float* const group_tops = p.group_tops + static_cast<size_t>(r) * groups_of(p.vocab);
     const float* const chunk_tops = p.chunk_tops + static_cast<size_t>(r) * p.chunks;
     const double* const segment_sums = p.segment_sums + static_cast<size_t>(r) * segments_of(p.vocab);
     const unsigned long long* const masses = p.masses + static_cast<size_t>(r) * p.chunks * kMassBuckets;
-    pick_row(p, r, row, set, chunk, p.chunks, [&](int g) { return group_tops[g]; }, [&](int c) { return chunk_tops[c]; },
-             [&](int s) { return segment_sums[s]; }, [&](int c, int b) { return masses[c * kMassBuckets + b]; }, sh);
+    pick_row(p, r, row, set, chunk, p.chunks, share, [&](int g) { return group_tops[g]; }, [&](int c) { return chunk_tops[c]; },
+             [&](int s) { return segment_sums[s]; }, [&](int c, int b) { return masses[c * kMassBuckets + b]; }, powers, sh);
 }
 
 }  // namespace gh

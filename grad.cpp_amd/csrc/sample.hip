@@ -20,7 +20,8 @@ static void check_sizes(int type, int rows, int vocab) {
 struct SampleForm {
     int chunk = kChunk;
     int chunks = 1;
-    size_t group_tops = 0, chunk_tops = 0, segment_sums = 0, masses = 0, bytes = 0;  // places in the workspace
+    int shares = 1;  // workgroups that look through a row
+    size_t group_tops = 0, chunk_tops = 0, segment_sums = 0, masses = 0, counters = 0, lists = 0, bytes = 0;  // places in the workspace
 };
 
 static SampleForm form_of(int rows, int vocab) {
@@ -38,6 +39,11 @@ static SampleForm form_of(int rows, int vocab) {
     f.chunk_tops = place(sizeof(float) * f.chunks);
     f.segment_sums = place(sizeof(double) * segments_of(vocab));
     f.masses = place(sizeof(unsigned long long) * kMassBuckets * f.chunks);
+    if (groups_of(vocab) > kListed && rows < 512) {
+        f.shares = std::min(8, 512 / rows);
+        f.counters = place(2 * sizeof(unsigned));
+        f.lists = place(sizeof(unsigned long long) * kListed);
+    }
     return f;
 }
 
@@ -56,7 +62,7 @@ static void launch_sample(SampleParams p, const SampleForm& f, int rows, hipStre
                 hipLaunchKernelGGL((sample_scan_kernel<TYPE, kWideThreads>), dim3(n * f.chunks), dim3(kWideThreads), 0, stream, p);
             }
             HIP_CHECK(hipGetLastError());
-            hipLaunchKernelGGL(sample_pick_kernel<TYPE>, dim3(n), dim3(kSampleThreads), 0, stream, p, f.chunk);
+            hipLaunchKernelGGL(sample_pick_kernel<TYPE>, dim3(n * f.shares), dim3(kSampleThreads), 0, stream, p, f.chunk);
         }
         HIP_CHECK(hipGetLastError());
     }
@@ -103,6 +109,9 @@ static void sample(const gh_sample_args& a, hipStream_t stream) {
     p.chunk_tops = reinterpret_cast<float*>(work + f.chunk_tops);
     p.segment_sums = reinterpret_cast<double*>(work + f.segment_sums);
     p.masses = reinterpret_cast<unsigned long long*>(work + f.masses);
+    p.shares = f.shares;
+    p.counters = reinterpret_cast<unsigned*>(work + f.counters);
+    p.lists = reinterpret_cast<unsigned long long*>(work + f.lists);
     if (a.type == GH_F32) launch_sample<kCacheF32>(p, f, a.rows, stream);
     else if (a.type == GH_BF16) launch_sample<kCacheBf16>(p, f, a.rows, stream);
     else launch_sample<kCacheF16>(p, f, a.rows, stream);
