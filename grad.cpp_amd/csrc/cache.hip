@@ -329,11 +329,15 @@ private:
             // save (128 rows, bf16: 1 k positions 31 us in 4 parts, 34 in 8; 4 k 44 in 8, 75 in 32; 16 k 75 in 16, 142 in 64;
             // fp32 products take some six times as long: 4 k 48 in 16, 57 in 8, 54 in 32; 16 k 90 in 32, 98 in 16, 121 in 64).
             const int resident = o.head_dim > 128 ? 256 : 512;
-            const int workgroups = tiles ? resident : bytes == 4 ? 1024 : 2048;
-            const int least = tiles ? 128 : bytes == 4 ? 256 : 384;
+            // Windows and sinks: few rows' spans are of one length, nothing has to be evened out, so one workgroup to a compute unit and
+            // nothing split that ends no sooner for it (16 sequences with windows of 4 k, 32/8 heads of 128 in bf16: 54 us, with 512
+            // workgroups 60, 768 63, 2048 77; 4 sequences 20.2 and 25.8; 64 with windows of 512, 12 heads of 64 in fp32: 40.4 us, in two parts
+            // each 47.8; only ragged ones lose a little, 16 of 1 to 4 k, fp32: 95 us, with 512 91).
+            const int workgroups = tiles ? resident : sinks > 0 ? 256 : bytes == 4 ? 1024 : 2048;
+            const int least = tiles ? 128 : bytes == 4 || sinks > 0 ? 256 : 384;
             l.cut = plan_attend(seqs, mine,
                                 AttendCut{group, o.kv_heads, l.form.height, causal, window, workgroups, least, 64,
-                                          !tiles ? 0 : bytes == 4 ? 16 : 64, tiles ? resident : 0, sinks},
+                                          !tiles ? 0 : bytes == 4 ? 16 : 64, tiles ? resident : 0, sinks, !tiles && sinks > 0 ? 1 : 0},
                                 many ? std::vector<SharedPrefix>{} : prefixes);
             room.parts = std::max(room.parts, static_cast<size_t>(l.cut.parts) * o.kv_heads * l.form.part_floats * sizeof(float));
             room.counters = std::max(room.counters, l.cut.joins.size() * o.kv_heads * sizeof(unsigned));

@@ -107,6 +107,7 @@ struct AttendCut {
                        // positions / n + square n.  A tile of 1 / r-th the height has a join of 1 / r-th the time
     int resident = 0;  // if not 0: no more workgroups than this many where there are fewer tiles (one more is a round of its own)
     int sinks = 0;     // first positions that rows see beside their window; only with a window
+    int slack = 0;     // quarters of a part's length that one part may be longer before there are two
 };
 
 // Tiles of `height` rows; a tile's positions are cut into parts of one length.  `shared`: prefixes whose members (of at
@@ -154,7 +155,7 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
     const auto cut_up = [&](int n, int k0, int k1, int& run) {
         int most = cut.most;
         if (cut.square > 0) most = std::min(most, static_cast<int>(std::sqrt(static_cast<double>(k1 - k0) * height / n / cut.square) + 0.5));
-        const int parts = std::max(1, static_cast<int>(std::min<long long>(most, (k1 - k0 + span - 1) / span)));
+        const int parts = std::max(1, static_cast<int>(std::min<long long>(most, (k1 - k0 + span - cut.slack * span / 4 - 1) / span)));
         run = (((k1 - k0 + parts - 1) / parts) + 31) / 32 * 32;
         return std::max(1, (k1 - k0 + run - 1) / run);
     };

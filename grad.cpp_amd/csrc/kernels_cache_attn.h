@@ -118,10 +118,16 @@ template <bool SINKS>
 __device__ __forceinline__ int position_of(const AttendParams& p, const AttendItem& it, int v) {
     return SINKS && v >= p.lead ? v + it.gap : v;
 }
+// What a row at `pos` sees of an item's positions, as bounds: two comparisons an element, where the conditions themselves are some ten.
 template <bool SINKS>
-__device__ __forceinline__ bool sees(const AttendParams& p, int t, int pos) {
-    return (!p.causal || t <= pos) && (p.window <= 0 || t > pos - p.window || (SINKS && t < p.sinks));
-}
+struct Visible {
+    int low, high, sinks;
+    __device__ __forceinline__ Visible(const AttendParams& p, const AttendItem& it, int pos)
+        : low(p.window > 0 ? pos - p.window + 1 : 0), high(position_of<SINKS>(p, it, it.k1 - 1)), sinks(p.sinks) {
+        if (p.causal) high = min(high, pos);
+    }
+    __device__ __forceinline__ bool at(int t) const { return (t <= high) & ((t >= low) | (SINKS && t < sinks)); }
+};
 // Whether a mask cuts `tokens` places from `at` on, for rows at positions first to final; whether none of the rows sees any of them.
 // Without conditional evaluation: where a branch of its own stands between a matrix product and what reads the result, the compiler puts
 // the product's wait states on one of the two paths only.
@@ -570,10 +576,10 @@ __global__ __launch_bounds__(64 * attend_waves(TYPE, DH), DH <= 64 ? 4 : 1) void
         unsigned seen = 0;
         bool hidden = false;
         if (cut) {
+            const Visible<SINKS> visible(p, it, pos);
 #pragma unroll
             for (int i = 0; i < 4 * G::kBlocks; i++) {
-                const int place = 4 * quarter + (i & 3), t = position_of<SINKS>(p, it, at + 16 * (i / 4)) + place;
-                const bool see = at + 16 * (i / 4) + place < it.k1 && sees<SINKS>(p, t, pos);
+                const bool see = visible.at(position_of<SINKS>(p, it, at + 16 * (i / 4)) + 4 * quarter + (i & 3));
                 z[i] = see ? z[i] : -INFINITY;
                 seen |= see ? 1u << i : 0u;
             }

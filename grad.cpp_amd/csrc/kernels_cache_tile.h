@@ -91,7 +91,7 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
         for (int t0 = begin; t0 < end; t0 += 64) {
             const int n = min(64, end - t0);
             float z = -INFINITY;
-            const bool seen = lane < n && (!SINKS || sees<true>(p, position_of<true>(p, it, t0 + lane), pos));
+            const bool seen = lane < n && (!SINKS || Visible<true>(p, it, pos).at(position_of<true>(p, it, t0 + lane)));
             if (seen) {
                 const T* key = at(0, position_of<SINKS>(p, it, t0 + lane));
                 z = 0.0f;
@@ -287,12 +287,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
         ahead_of_products<kBlocks * kSteps, 1, 6>();
         const bool cut = (at + TOKENS > it.k1) | cuts<SINKS>(p, it, at, TOKENS, first, final);
         if (cut) {
+            const Visible<SINKS> visible(p, it, pos);
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int block = at + 32 * b + 16 * (i / 8), place = 8 * (i / 4 & 1) + 4 * half + (i & 3);
-                    const bool see = block + place < it.k1 && sees<SINKS>(p, position_of<SINKS>(p, it, block) + place, pos);
+                    const bool see = visible.at(position_of<SINKS>(p, it, block) + place);
                     z[b][i] = see ? z[b][i] : -INFINITY;
                 }
         }
@@ -560,12 +561,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
         }
         const bool cut = (at + TOKENS > it.k1) | cuts<SINKS>(p, it, at, TOKENS, first, final);
         if (cut) {
+            const Visible<SINKS> visible(p, it, pos);
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int block = at + 32 * b + 16 * (i / 8), place = 8 * (i / 4 & 1) + 4 * half + (i & 3);
-                    const bool see = block + place < it.k1 && sees<SINKS>(p, position_of<SINKS>(p, it, block) + place, pos);
+                    const bool see = visible.at(position_of<SINKS>(p, it, block) + place);
                     z[b][i] = see ? z[b][i] : -INFINITY;
                 }
         }

@@ -199,7 +199,6 @@ struct PickShared {
         int hot[kListed];  // groups
         double weights[kListed];
     };
-    unsigned ranks[kSampleThreads];
     double chunk_sums[kMaxSampleVocab / kChunk];
     float chunk_tops[kMaxSampleVocab / kChunk];
     double chunk_shares[kMaxSampleVocab / kChunk];  // of a w relative to its chunk's largest, relative to the row's
@@ -482,26 +481,47 @@ __device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWei
 
 // ------------------------------------------------------------------------ lists
 
-// n different numbers of sh.list in ascending order; what lies behind them, up to the next power of two, is overwritten.  Few are put in their places by
-// counting how many are smaller, shared among the threads; more are sorted by pairs (each of its steps is a meeting of all).
+__device__ __forceinline__ unsigned long long read_lane(unsigned long long v, int lane) {
+    return static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32
+           | static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ unsigned long long to_lane(unsigned long long v, int lane) {
+    return static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_ds_permute(lane * 4, static_cast<int>(v >> 32)))) << 32
+           | static_cast<unsigned>(__builtin_amdgcn_ds_permute(lane * 4, static_cast<int>(v)));
+}
+
+// A number of each lane's, all different: how many are smaller among the first n lanes'.
+__device__ __forceinline__ int rank_in_wave(unsigned long long mine, int n) {
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += read_lane(mine, j) < mine;
+    return rank;
+}
+
+// n different numbers of sh.list in ascending order; what lies behind them, up to the next power of two, is overwritten.  Up to a number for each thread:
+// every wavefront orders its own, and each finds its place among the others' by halves.  More are sorted by pairs, each of whose steps is a meeting of all.
 __device__ __forceinline__ void sort_list(PickShared& sh, int n) {
-    int size = 64;
-    while (size < n) size *= 2;
-    if (size <= kSampleThreads) {
-        const int e = static_cast<int>(threadIdx.x) & (size - 1), parts = kSampleThreads / size, part = static_cast<int>(threadIdx.x) / size;
-        const int each = (n + parts - 1) / parts, from = part * each, to = min(n, from + each);
-        sh.ranks[threadIdx.x] = 0;
+    if (n <= kSampleThreads) {
+        const int wave = static_cast<int>(threadIdx.x) >> 6, runs = (n + 63) / 64;
         __syncthreads();
-        const unsigned long long mine = sh.list[e];
-        unsigned rank = 0;
-#pragma unroll 8
-        for (int j = from; j < to; j++) rank += sh.list[j] < mine;
-        if (e < n && rank > 0) atomicAdd(&sh.ranks[e], rank);
+        const unsigned long long mine = static_cast<int>(threadIdx.x) < n ? sh.list[threadIdx.x] : ~0ull << 11 | threadIdx.x;  // (behind all others)
+        const int rank = wave < runs ? rank_in_wave(mine, 64) : 0;
+        sh.list[wave * 64 + rank] = mine;  // (a wavefront's own places)
         __syncthreads();
-        if (part == 0 && e < n) sh.list[sh.ranks[e]] = mine;
+        int place = rank;
+        for (int run = 0; run < runs; run++) {
+            if (run == wave) continue;
+            int before = 0;
+#pragma unroll
+            for (int step = 32; step > 0; step /= 2) before += sh.list[run * 64 + before + step - 1] < mine ? step : 0;
+            place += before + (sh.list[run * 64 + before] < mine);
+        }
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < n) sh.list[place] = mine;
         __syncthreads();
         return;
     }
+    int size = 64;
+    while (size < n) size *= 2;
     for (int i = n + static_cast<int>(threadIdx.x); i < size; i += kSampleThreads) sh.list[i] = ~0ull;
     __syncthreads();
     for (int k = 2; k <= size; k *= 2)
@@ -669,16 +689,13 @@ __device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS&
     });
     __syncthreads();
     const int hot = sh.found;
-    const auto add = [&](float x, int index) {
-        const bool wants = x >= least && x <= most;
-        const int at = take_places(wants, &sh.listed);
-        if (wants && at < kListed) sh.list[at] = static_cast<unsigned long long>(~order_key(x)) << 32 | static_cast<unsigned>(index);
-    };
+    const auto add = [&](int n) { return atomicAdd(&sh.listed, n); };
     if (hot <= kListed) {
-        constexpr int kDeep = 16;
+        constexpr int kDeep = 32;
         for (int h = wave; h < hot; h += kDeep * kSampleWaves) {
             float x[kDeep];
             int index[kDeep];
+            unsigned wants = 0;
 #pragma unroll
             for (int k = 0; k < kDeep; k++) {
                 const int g = h + k * kSampleWaves;
@@ -686,12 +703,19 @@ __device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS&
                 x[k] = row.one(index[k]);
             }
 #pragma unroll
-            for (int k = 0; k < kDeep; k++) add(x[k], index[k]);
+            for (int k = 0; k < kDeep; k++) wants |= x[k] >= least && x[k] <= most ? 1u << k : 0u;
+            int at = wave_places(__popc(wants), add);
+#pragma unroll
+            for (int k = 0; k < kDeep; k++)
+                if (wants >> k & 1) {
+                    if (at < kListed) sh.list[at] = static_cast<unsigned long long>(~order_key(x[k])) << 32 | static_cast<unsigned>(index[k]);
+                    at++;
+                }
         }
     } else if (most == INFINITY) {
         return hot;  // (each holds one at least)
     } else {
-        look_through(row, least, most, 0, 1, [&](int wants) { return wave_places(wants, [&](int n) { return atomicAdd(&sh.listed, n); }); },
+        look_through(row, least, most, 0, 1, [&](int wants) { return wave_places(wants, add); },
                      [&](int at, int index) {
                          if (at < kListed) sh.list[at] = list_entry(row, index);
                      });
@@ -821,22 +845,11 @@ __device__ __forceinline__ void draw_listed(const SampleParams& p, int r, int ke
     }
 }
 
-__device__ __forceinline__ unsigned long long read_lane(unsigned long long v, int lane) {
-    return static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32
-           | static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
-}
-__device__ __forceinline__ unsigned long long to_lane(unsigned long long v, int lane) {
-    return static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_ds_permute(lane * 4, static_cast<int>(v >> 32)))) << 32
-           | static_cast<unsigned>(__builtin_amdgcn_ds_permute(lane * 4, static_cast<int>(v)));
-}
-
 // A list of at most 64 tokens from its order to the pick, by one wavefront, a token to a lane.
 __device__ __forceinline__ void pick_few(const SampleParams& p, int r, const SampleWeights& w, const SampleSettings& set, int n, double total, const PickShared& sh) {
     const int lane = threadIdx.x;
     unsigned long long item = lane < n ? sh.list[lane] : ~0ull << 32 | static_cast<unsigned>(lane);
-    int rank = 0;
-    for (int j = 0; j < 64; j++) rank += read_lane(item, j) < item;
-    item = to_lane(item, rank);
+    item = to_lane(item, lane < n ? rank_in_wave(item, n) : lane);
     if (set.top_k > 0) n = min(n, set.top_k);
     double v = lane < n ? w.weight(key_value(~static_cast<unsigned>(item >> 32))) : 0.0;
     double upto = wave_scan(v), before = __shfl_up(upto, 1);
@@ -845,8 +858,7 @@ __device__ __forceinline__ void pick_few(const SampleParams& p, int r, const Sam
     const int kept = __popcll(__ballot(v > 0.0 && (lane == 0 || (before < target && v >= set.min_p))));
     // by their indices
     unsigned long long index = lane < kept ? static_cast<unsigned>(item) : 1ull << 32 | static_cast<unsigned>(lane);
-    rank = 0;
-    for (int j = 0; j < 64; j++) rank += read_lane(index, j) < index;
+    const int rank = lane < kept ? rank_in_wave(index, kept) : lane;
     index = to_lane(index, rank);
     v = __longlong_as_double(static_cast<long long>(to_lane(static_cast<unsigned long long>(__double_as_longlong(lane < kept ? v : 0.0)), rank)));
     upto = wave_scan(v);
@@ -1240,7 +1252,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const Sample
 
 // One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute.
 template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS, 6) void sample_scan_kernel(const SampleParams p) {
+__global__ __launch_bounds__(THREADS, 5) void sample_scan_kernel(const SampleParams p) {
     __shared__ ChunkShared<THREADS> left;
     __shared__ double powers[kPowers];
     fill_powers(p, powers);
