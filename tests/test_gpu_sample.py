@@ -190,6 +190,70 @@ def test_wide_spreads_and_far_values(torch):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [2500, 9001, 33000, 140003, 262144, 2 ** 20])
+def test_nuclei_of_any_size(torch, dtype, vocab):
+    """From one token to most of the row: lists, cuts found among one bucket's tokens, by one workgroup and by several, and by histograms (no
+    place on the grid at low temperatures, whole rows in a few buckets at high ones)."""
+    rows = 6 if vocab < 200000 else 2
+    x, u = rows_of(torch, dtype, rows, vocab, seed=vocab + 1)
+    for top_p in (0.01, 0.6, 0.98, 0.99999):
+        check(torch, x, u, f"top_p {top_p}", top_p=top_p)
+    check(torch, x, u, "and min_p", top_p=0.97, min_p=1e-5)
+    check(torch, x, u, "and min_p below", top_p=0.3, min_p=1e-7)
+    check(torch, x, u, "min_p alone", min_p=1e-4)
+    for temperature in (1e-12, 0.05, 3.0, 50.0, 1e9, float("inf")):
+        check(torch, x, u, f"temperature {temperature}", temperature=temperature, top_p=0.7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lists_of_every_length(torch, dtype):
+    for vocab in (3000, 8192, 8193, 40000, 150000):
+        x, u = rows_of(torch, dtype, 4, vocab, seed=vocab + 2)
+        for k in (1, 2, 63, 64, 65, 128, 129, 255, 256, 257, 1000, 2047, 2048, 2049, 2999):
+            check(torch, x, u, f"vocab {vocab} top_k {k}", top_k=k)
+        check(torch, x, u, "two filters", top_k=300, top_p=0.9)
+        for m in (0.5, 0.1, 0.03, 0.005, 0.0004):
+            check(torch, x, u, f"vocab {vocab} min_p {m}", min_p=m)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_are_mostly_forbidden(torch, dtype):
+    """Whole chunks and groups without a token: all but a few, all but the last, all but one chunk's."""
+    t = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    for vocab in (5000, 40001, 140001):
+        x, u = rows_of(torch, dtype, 8, vocab, seed=vocab + 3)
+        y = torch.full_like(x, -float("inf"))
+        y[1] = torch.finfo(t).min
+        y[2] = float("nan")
+        for r in (0, 1, 2):
+            y[r, 17::4999] = x[r, 17::4999]
+        y[3, -1] = 0.5
+        y[4, vocab // 2:vocab // 2 + 700] = x[4, :700]
+        y[5, :3] = x[5, :3]
+        y[6, -9:] = x[6, :9]
+        y[6, 0] = float("inf")
+        y[7, 100:4000] = x[7, 100:4000]
+        y[7, 4200] = torch.finfo(t).max
+        for s in (dict(), dict(top_k=5), dict(top_k=900), dict(top_p=0.9), dict(top_p=0.9999), dict(min_p=0.01), dict(top_k=50, top_p=0.8, min_p=0.001), dict(temperature=0.0),
+                  dict(temperature=20.0, top_p=0.95)):
+            check(torch, y, u, f"vocab {vocab} {s}", **s)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 70, 300, 600])
+def test_nuclei_of_many_rows(torch, rows):
+    """Chunks of both sizes, rows looked through by one to eight workgroups beside rows that need none."""
+    x, u = rows_of(torch, "bf16", rows, 135000, seed=rows)
+    rng = np.random.default_rng(rows)
+    some = rng.choice(rows, min(rows, 12), replace=False)
+    top_p = [0.98 if r % 3 else 0.2 for r in range(rows)]
+    temperature = [1.0 if r % 5 else 0.0 for r in range(rows)]
+    ids, probs = call(torch, x, u, temperature=temperature, top_p=top_p)
+    for r in some:
+        want, p = R.pick(x[r].cpu().double().numpy(), float(np.float32(u[r])), temperature=temperature[r], top_p=float(np.float32(top_p[r])))
+        assert ids[r] == want and abs(probs[r] - p) <= p * (2.0 ** -24 + 2.0 ** -40), (r, ids[r], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_one_row_of_logits_for_many_draws(torch, dtype):
     """A stride of zero: the draws' shares are the probabilities that are returned."""
     x, _ = rows_of(torch, dtype, 1, 800, seed=21, std=1.5)
