@@ -496,6 +496,11 @@ __device__ __forceinline__ int rank_in_wave(unsigned long long mine, int n) {
     for (int j = 0; j < n; j++) rank += read_lane(mine, j) < mine;
     return rank;
 }
+__device__ __forceinline__ int rank_in_wave(unsigned mine, int n) {
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) < mine;
+    return rank;
+}
 
 // n different numbers of sh.list in ascending order; what lies behind them, up to the next power of two, is overwritten.  Up to a number for each thread:
 // every wavefront orders its own, and each finds its place among the others' by halves.  More are sorted by pairs, each of whose steps is a meeting of all.
@@ -675,13 +680,15 @@ __device__ __forceinline__ unsigned long long list_entry(const SampleRow<TYPE>& 
 }
 
 // The tokens of logits from `least` to `most` into sh.list, by (key descending, index).  Returns how many; more than kListed: the list is not
-// whole.  Only groups whose largest reaches `least` are looked at.
+// whole.  Only groups whose largest reaches `least` are looked at.  `fresh`: sh.listed and sh.found are zero already.
 template <int TYPE, typename TOPS>
-__device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS& tops, PickShared& sh, float least, float most) {
+__device__ __forceinline__ int make_list(const SampleRow<TYPE>& row, const TOPS& tops, PickShared& sh, float least, float most, bool fresh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();
-    if (threadIdx.x == 0) sh.listed = sh.found = 0;
-    __syncthreads();
+    if (!fresh) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.listed = sh.found = 0;
+        __syncthreads();
+    }
     tops.each([&](float t, int g) {
         const bool hot = t >= least;
         const int at = take_places(hot, &sh.found);
@@ -814,8 +821,26 @@ __device__ __forceinline__ double target_of(const SampleParams& p, int r, double
     return (u > 0.0f ? static_cast<double>(u) : 0.0) * total;  // (NaN: 0)
 }
 
+// Draws from the tokens of a wavefront's first `kept` lanes, of indices `index` and w `v`.
+__device__ __forceinline__ void draw_few(const SampleParams& p, int r, int index, double v, int kept) {
+    const int lane = threadIdx.x & 63;
+    const int rank = lane < kept ? rank_in_wave(static_cast<unsigned>(index), kept) : lane;
+    index = __builtin_amdgcn_ds_permute(rank * 4, index);
+    v = __longlong_as_double(static_cast<long long>(to_lane(static_cast<unsigned long long>(__double_as_longlong(lane < kept ? v : 0.0)), rank)));
+    const double upto = wave_scan(v), all = __shfl(upto, 63);
+    const unsigned long long hits = __ballot(lane < kept && upto >= target_of(p, r, all));
+    if (lane == (hits ? __ffsll(hits) - 1 : kept - 1)) {
+        p.ids[r] = index;
+        if (p.probs) p.probs[r] = static_cast<float>(v / all);
+    }
+}
+
 // Draws from the sorted list's first `kept` tokens, whose w are in sh.weights: by their indices.
 __device__ __forceinline__ void draw_listed(const SampleParams& p, int r, int kept, PickShared& sh) {
+    if (kept <= 64) {
+        if (threadIdx.x < 64) draw_few(p, r, static_cast<int>(static_cast<unsigned>(sh.list[threadIdx.x])), sh.weights[threadIdx.x], kept);
+        return;
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < kept; i += kSampleThreads) sh.list[i] = sh.list[i] << 32 | static_cast<unsigned>(i);  // (the key goes)
     if (threadIdx.x == 0) {
@@ -856,18 +881,7 @@ __device__ __forceinline__ void pick_few(const SampleParams& p, int r, const Sam
     if (lane == 0) before = 0.0;
     const double target = set.top_p < 1.0 ? set.top_p * (set.top_k > 0 ? __shfl(upto, 63) : total) : INFINITY;
     const int kept = __popcll(__ballot(v > 0.0 && (lane == 0 || (before < target && v >= set.min_p))));
-    // by their indices
-    unsigned long long index = lane < kept ? static_cast<unsigned>(item) : 1ull << 32 | static_cast<unsigned>(lane);
-    const int rank = lane < kept ? rank_in_wave(index, kept) : lane;
-    index = to_lane(index, rank);
-    v = __longlong_as_double(static_cast<long long>(to_lane(static_cast<unsigned long long>(__double_as_longlong(lane < kept ? v : 0.0)), rank)));
-    upto = wave_scan(v);
-    const double all = __shfl(upto, 63);
-    const unsigned long long hits = __ballot(lane < kept && upto >= target_of(p, r, all));
-    if (lane == (hits ? __ffsll(hits) - 1 : kept - 1)) {
-        p.ids[r] = static_cast<int>(static_cast<unsigned>(index));
-        if (p.probs) p.probs[r] = static_cast<float>(v / all);
-    }
+    draw_few(p, r, static_cast<int>(static_cast<unsigned>(item)), v, kept);
 }
 
 // ------------------------------------------------------------- segments of the row
@@ -968,6 +982,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         low = t > -INFINITY ? fminf(low, t) : low;
     });
     for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_tops[c] = chunk_top(c);
+    if (threadIdx.x == 0) sh.listed = sh.found = 0;
     if (share > 0 && !set.masses()) return;  // (the first alone has work)
     block_ends(top, low, sh);
     if (top == -INFINITY) {
@@ -997,8 +1012,10 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     const SampleWeights w{top, set.turn(), powers};
     const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52);
     const int segments = segments_of(p.vocab);
-    for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_shares[c] = w.weight(sh.chunk_tops[c]);  // (its own thread's)
-    __syncthreads();
+    if (set.sums()) {
+        for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_shares[c] = w.weight(sh.chunk_tops[c]);  // (its own thread's)
+        __syncthreads();
+    }
     const auto sum_of = [&](int s) {
         const double chunk_share = sh.chunk_shares[s * kSegment / chunk];
         return chunk_share > 0.0 ? segment_sum(s) * chunk_share : 0.0;
@@ -1030,7 +1047,6 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             int bound = kBuckets;
             for (int by_group = 4 * set.top_k <= 3 * tops.groups; by_group >= 0 && bound == kBuckets; by_group--) {
                 fine = by_group ? (kBuckets - 1) / fmax(static_cast<double>(top) - low, 1e-300) : kBuckets / -kLeastTurns * w.turn;
-                __syncthreads();
                 for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.counts[b] = 0;
                 if (threadIdx.x == 0) sh.bucket = kBuckets;
                 __syncthreads();
@@ -1058,7 +1074,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                 bound = sh.bucket;
             }
             // (none: fewer than k tokens have a w)
-            listed = make_list(row, tops, sh, below(static_cast<double>(top) - (bound + 1) / fine), INFINITY);
+            listed = make_list(row, tops, sh, below(static_cast<double>(top) - (bound + 1) / fine), INFINITY, true);
         }
         if (listed > kListed) {
             cut = find_cut<TYPE, false>(row, w, scale, cut, set.top_k, sh);
@@ -1129,14 +1145,14 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             const double above = sh.mass_above;
             const auto bucket_of = [&](float x) { return w.turns(x) > kLeastTurns ? place - grid_place(x, grid) : kMassBuckets; };
             const double reach = (place - bound - 0.5) / grid;
-            listed = make_list(row, tops, sh, below(fmax(reach, set.min_p > 0.0 ? min_p_reach() : reach)), INFINITY);
+            listed = make_list(row, tops, sh, below(fmax(reach, set.min_p > 0.0 ? min_p_reach() : reach)), INFINITY, true);
             if (listed > kListed) {  // the bucket's own tokens say where the cut is
                 const float least = least_that(top, [&](float x) { return bucket_of(x) <= bound; });
                 const float next = bound > 0 ? least_that(top, [&](float x) { return bucket_of(x) < bound; }) : INFINITY;
                 const float most = bound > 0 ? key_value(order_key(next) - 1) : 3.402823466e38f;
                 const bool together = p.shares > 1 && sh.found > kListed;  // (found: the groups that reach so far)
                 if (share > 0 && !together) return;
-                const int own = together ? make_list_together(p, r, row, share, sh, least, most) : make_list(row, tops, sh, least, most);
+                const int own = together ? make_list_together(p, r, row, share, sh, least, most) : make_list(row, tops, sh, least, most, false);
                 if (own < 0) return;
                 share = 0;  // (the last of them goes on)
                 if (own <= kListed) {
@@ -1208,7 +1224,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
         }
     } else {
-        listed = make_list(row, tops, sh, below(min_p_reach()), INFINITY);
+        listed = make_list(row, tops, sh, below(min_p_reach()), INFINITY, true);
     }
     if (share > 0) return;
 
