@@ -1035,7 +1035,8 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         return;
     }
 
-    const auto min_p_reach = [&] { return top + kPowers * log2(set.min_p) / w.turn; };  // the logit of w = min_p
+    // The logit of w = min_p, or one a little below it, by more than the error of a w: of a hot row (T of 1e38) many logits have the same
+    const auto min_p_reach = [&] { return top + (kPowers * log2(set.min_p) - 1e-9) / w.turn; };
     Cut cut;
     double total = 0.0;  // of what top-p is a share of
     int listed = kListed + 1;
@@ -1217,6 +1218,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                 }
             }
         }
+        if (share > 0) return;
         if (listed > kListed && bound >= 0) {
             unsigned long long whole = 0, all;
             row.each([&](float x, int) { whole += whole_number(w.weight(x), scale); });
@@ -1226,7 +1228,6 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     } else {
         listed = make_list(row, tops, sh, below(min_p_reach()), INFINITY, true);
     }
-    if (share > 0) return;
 
     if (listed <= 64) {
         if (threadIdx.x < 64) pick_few(p, r, w, set, listed, total, sh);

@@ -175,6 +175,17 @@ def test_uniforms_at_their_ends(torch, dtype):
         check(torch, x, u, f"{s}", **s)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [3, 600, 5207, 31801])
+def test_logits_too_close_to_differ(torch, dtype, vocab):
+    # w that are all 1 in 64 bits, though the logits differ: min_p = 1 keeps every one
+    logits, u = rows_of(torch, dtype, 4, vocab, seed=vocab)
+    for temperature in (float("inf"), 1e30):
+        for more in (dict(), dict(top_k=500), dict(top_p=0.5)):
+            check(torch, logits, u, (temperature, more), temperature=temperature, min_p=1.0, **more)
+    check(torch, (logits.float() * 1e-39).to(logits.dtype), u, "close", min_p=1.0)
+
+
 def test_wide_spreads_and_far_values(torch):
     """Logits over the whole range of fp32, of one sign, next to each other in their last digits."""
     gen = torch.Generator().manual_seed(3)
