@@ -16,7 +16,8 @@ static void check_sizes(int type, int rows, int vocab) {
 }
 
 // Rows of one chunk are picked from by the workgroup that reads them.  Longer ones are read in chunks by as many workgroups, wide chunks where
-// they keep every compute unit busy.
+// they keep every compute unit busy.  Rows of more groups than a list holds are looked through by up to eight workgroups, as many as the GPU has room for.
+constexpr int kUnits = 256, kMostShared = 512;
 struct SampleForm {
     int chunk = kChunk;
     int chunks = 1;
@@ -28,7 +29,7 @@ static SampleForm form_of(int rows, int vocab) {
     SampleForm f;
     if (vocab <= kChunk) return f;
     const auto chunks = [&](int length) { return (vocab + length - 1) / length; };
-    if (static_cast<long long>(rows) * chunks(kWideChunk) >= 256) f.chunk = kWideChunk;
+    if (static_cast<long long>(rows) * chunks(kWideChunk) >= kUnits) f.chunk = kWideChunk;
     f.chunks = chunks(f.chunk);
     const auto place = [&](size_t per_row) {
         const size_t at = f.bytes;
@@ -39,12 +40,20 @@ static SampleForm form_of(int rows, int vocab) {
     f.chunk_tops = place(sizeof(float) * f.chunks);
     f.segment_sums = place(sizeof(double) * segments_of(vocab));
     f.masses = place(sizeof(unsigned long long) * kMassBuckets * f.chunks);
-    if (groups_of(vocab) > kListed && rows < 512) {
-        f.shares = std::min(8, 512 / rows);
+    if (rows > 0 && groups_of(vocab) > kListed && rows < kMostShared) {
+        f.shares = std::min(8, kMostShared / rows);
         f.counters = place(2 * sizeof(unsigned));
         f.lists = place(sizeof(unsigned long long) * kListed);
     }
     return f;
+}
+
+// Enough for so many rows and for fewer: between the borders of the rules more rows need more.
+static size_t workspace_of(int rows, int vocab) {
+    size_t bytes = 0;
+    const int wide = (kUnits - 1) / ((vocab + kWideChunk - 1) / kWideChunk);  // rows: the most of smaller chunks
+    for (int n : {rows, std::min(rows, wide), std::min(rows, kMostShared - 1)}) bytes = std::max(bytes, form_of(n, vocab).bytes);
+    return bytes;
 }
 
 template <int TYPE>
@@ -127,7 +136,7 @@ gh_status gh_sample_workspace(int32_t type, int32_t rows, int32_t vocab, size_t*
     return guard([&] {
         if (!bytes) throw ApiError{GH_ERR_INVALID_ARGUMENT, "null argument"};
         check_sizes(type, rows, vocab);
-        *bytes = form_of(rows, vocab).bytes;
+        *bytes = workspace_of(rows, vocab);
     });
 }
 

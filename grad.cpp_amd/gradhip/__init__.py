@@ -746,7 +746,7 @@ class Cache:
 
 
 def sample_workspace(rows, vocab, dtype="f32") -> int:
-    """Bytes of the workspace that sample() wants for so many rows of logits."""
+    """Bytes of the workspace that sample() wants for so many rows of logits or fewer."""
     if dtype not in CACHE_TYPES:
         raise ValueError(f"sample: unknown element type {dtype!r}")
     out = C.c_size_t()

@@ -374,6 +374,7 @@ typedef struct gh_sample_args {
     size_t workspace_bytes;
 } gh_sample_args;
 
+/* Bytes of workspace for any call with so many rows or fewer. */
 gh_status gh_sample_workspace(int32_t type, int32_t rows, int32_t vocab, size_t* bytes);
 gh_status gh_sample(const gh_sample_args* args, void* hip_stream);
 

@@ -311,6 +311,20 @@ def test_calls_that_need_a_workspace_refuse_without_one(torch):
     assert int(ids[0]) == -5
 
 
+@pytest.mark.parametrize("vocab", [9001, 32000, 140003])
+def test_a_workspace_of_many_rows_does_for_few(torch, vocab):
+    most = 600
+    x, u = rows_of(torch, "bf16", most, vocab, seed=47)
+    u, p = torch.tensor(u, device="cuda"), torch.full((most,), 0.9, device="cuda")
+    work = torch.empty(G.sample_workspace(most, vocab, "bf16"), dtype=torch.uint8, device="cuda").fill_(255)
+    ids = [torch.full((most,), -5, dtype=torch.int32, device="cuda") for _ in range(2)]
+    G.sample(x, u, ids[0], top_p=p, workspace=work)
+    for rows in (511, 255, 127, 85, 64, 27, 1):  # on either side of where other launches are used
+        ids[1].fill_(-5)
+        G.sample(x[:rows], u[:rows], ids[1][:rows], top_p=p[:rows], workspace=work)
+        assert torch.equal(ids[1][:rows], ids[0][:rows]) and (ids[1][rows:] == -5).all(), rows
+
+
 def test_memory_of_the_host_is_refused(torch):
     import ctypes as C
     host = np.zeros(400, np.float32)

@@ -64,6 +64,13 @@ def test_workspaces():
         G.sample_workspace(1, 10, "f64")
 
 
+def test_a_workspace_does_for_fewer_rows():
+    for vocab in (100, 8192, 8193, 16384, 32000, 50257, 131072, 131073, 201001, 2 ** 20):
+        needs = [G.sample_workspace(rows, vocab) for rows in range(0, 700)]
+        assert needs == sorted(needs), vocab
+        assert needs[0] == 0 and (needs[1] > 0) == (vocab > 8192)
+
+
 def tensor(*shape, dtype="torch.float32", device="cuda:0", stride=None):
     if stride is None:
         stride = [int(np.prod(shape[i + 1:])) for i in range(len(shape))]
