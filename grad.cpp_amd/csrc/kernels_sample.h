@@ -8,13 +8,15 @@
 // 16-bit row has thousands) share one error, and one draw in a hundred from 128 k tokens of a flat row would be
 // another token than the definition's.  The card's 64-bit instructions have the rate of plain 32-bit ones.
 //
-// The row is read once, in chunks: largest logits of groups of 64; where the sum of all w matters (no top-k), sums of segments of 512
-// relative to the chunk's largest; with top-p, w by buckets of x.  From these follows a bound below which nothing is kept:
-//   top-k: k groups have a logit of at least the k-th largest of the groups' largest;
+// A row is read once, in chunks, all of it in registers: what stays of it are the largest logits of groups of 64, and where the sum of all w
+// matters (no top-k), sums relative to the chunk's largest: with top-p w by buckets of x, without it those of segments of 512.  From these
+// follows a bound below which nothing is kept:
+//   top-k: k groups have a logit of at least the k-th largest of the groups' largest (so buckets of these will do; where groups are few, of all logits);
 //   top-p: the bucket in which the running sum of w reaches p of the whole;   min-p: the logarithm.
-// Only groups that reach the bound are looked at again, the tokens above it become a list, are sorted, cut and drawn from.  What does not fit a list
-// (a nucleus of thousands of tokens) is cut by the bucket's tokens alone, or, where that is not enough, by histograms over the row,
-// and drawn from segment by segment.
+// Only groups that reach the bound are looked at again; the tokens above it become a list, which is put in order, cut and drawn from.  What does
+// not fit a list (a nucleus of thousands of tokens) is cut among the bucket's own tokens, and only the chunk that the draw falls into is read again;
+// where a bucket's tokens do not fit a list either (thousands of equal logits, k of thousands), histograms over the row find the cut.
+// Bucket sums are whole numbers, so the order in which atomics arrive changes nothing.
 #pragma once
 
 #include "kernels_cache_attn.h"
@@ -305,6 +307,9 @@ __device__ __forceinline__ void block_ends(float& high, float& low, PickShared& 
 
 // One chunk of a row, from `first` on.  Leaves the groups' largest logits, and where they are wanted the segments' sums (with buckets, the wavefronts'), relative
 // to the largest of the chunk, and w by buckets of x, from the chunk's largest down.  Returns the largest.
+//
+// The logits are loaded in one go, kept as they are, and gone through twice, because the exponentials need the chunk's largest first.  With w and
+// buckets it is bound by vector instructions (some 39 a logit, half of them the 64-bit exponential, and an atomic on shared memory), without them by reading.
 template <int TYPE, int THREADS>
 __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, const double* powers,
                                             ChunkShared<THREADS>& sh) {
@@ -1251,7 +1256,9 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     draw_segments(p, r, row, 0, segments, 0.0, -1.0, sh, weight);
 }
 
-// A row of one chunk, from its logits to the pick.
+// A row of one chunk, from its logits to the pick: up to 8192 tokens, one launch.  Nothing in it is bound by memory or arithmetic: it is some 20 steps
+// one behind the other (loads, meetings of the workgroup, look-ups in shared memory), which is why few threads do it (5000 tokens in fp32, top-k 40 and
+// top-p 0.95: 12 us, of which a launch that does nothing is 4.5).
 template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const SampleParams p) {
     __shared__ ChunkShared<kSampleThreads> left;
@@ -1267,7 +1274,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const Sample
              [&](int, int b) { return left.masses[b]; }, powers, sh);
 }
 
-// One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute.
+// One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute: registers for
+// five wavefronts on a SIMD (six cost min-p alone no spills, 27 us for 30, but w and buckets some: 106 for 99; eight 128).
+//   256 x 128000 bf16, min-p: 17 us, 3.8 TB/s; 100 x 201001 fp32, top-p: 34 us, 2.4 TB/s, bound by its vector instructions; 64 x 50257 bf16, top-p: 9.5.
 template <int TYPE, int THREADS>
 __global__ __launch_bounds__(THREADS, 5) void sample_scan_kernel(const SampleParams p) {
     __shared__ ChunkShared<THREADS> left;
@@ -1290,6 +1299,10 @@ __global__ __launch_bounds__(THREADS, 5) void sample_scan_kernel(const SamplePar
         for (int b = t; b < kMassBuckets; b += THREADS) p.masses[(static_cast<size_t>(r) * p.chunks + c) * kMassBuckets + b] = left.masses[b];
 }
 
+// What follows: a workgroup to a row, or several where rows have more groups than a list holds and a nucleus may have to be looked for in all of
+// them (launch rules in sample.hip).  Short lists are steps one behind the other, 13 us (64 rows of 50257, top-p 0.9; 256 of 128000, min-p); 13 rows of
+// 32000 with settings of every kind 22, the time of the row with the longest list; 100 flat rows of 201001, top-p 0.98, 69: the row is looked through
+// (80 MB), then the chunk of the draw, and what the chunks left is read by every workgroup of the row (50 MB).
 template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(const SampleParams p, int chunk) {
     __shared__ PickShared sh;
