@@ -62,7 +62,7 @@ static void launch_sample(SampleParams p, const SampleForm& f, int rows, hipStre
     const int slice = (1 << 21) / f.chunks;
     for (p.first_row = 0; p.first_row < rows; p.first_row += slice) {
         const int n = std::min(slice, rows - p.first_row);
-        if (f.chunks == 1) {
+        if (p.vocab <= kChunk) {
             hipLaunchKernelGGL(sample_row_kernel<TYPE>, dim3(n), dim3(kSampleThreads), 0, stream, p);
         } else {
             if (f.chunk == kChunk) {

@@ -311,6 +311,14 @@ def test_calls_that_need_a_workspace_refuse_without_one(torch):
     assert int(ids[0]) == -5
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(300, 8193), (260, 9001), (256, 16384), (129, 16385)])
+def test_many_rows_of_one_or_two_chunks(torch, dtype, rows, vocab):
+    x, u = rows_of(torch, dtype, rows, vocab, seed=vocab)
+    for settings in (dict(), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.02), dict(temperature=0.0)):
+        check(torch, x, u, settings, **settings)
+
+
 @pytest.mark.parametrize("vocab", [9001, 32000, 140003])
 def test_a_workspace_of_many_rows_does_for_few(torch, vocab):
     most = 600
