@@ -178,7 +178,7 @@ struct SampleRow {
 struct Cut {
     unsigned key = 0;
     int index = 0x7FFFFFFF;
-    __device__ __forceinline__ bool keeps(unsigned k, int i) const { return k > key || (k == key && i <= index); }
+    __device__ __forceinline__ bool keeps(unsigned k, int i) const { return (k > key) | ((k == key) & (i <= index)); }
 };
 
 // What a chunk leaves.
@@ -202,7 +202,6 @@ struct PickShared {
         double weights[kListed];
     };
     double chunk_sums[kMaxSampleVocab / kChunk];
-    float chunk_tops[kMaxSampleVocab / kChunk];
     double chunk_shares[kMaxSampleVocab / kChunk];  // of a w relative to its chunk's largest, relative to the row's
     int chunk_shifts[kMaxSampleVocab / kChunk];     // how far its buckets lie behind the row's; all of them where it has none
     unsigned long long scan[kSampleWaves];
@@ -267,7 +266,7 @@ struct SampleSettings {
     __device__ __forceinline__ double grid() const { return kMassFine * 1.44269504088896340736 / temperature; }
 };
 
-// The place on the grid: larger logits have larger ones.
+// The place on the grid: larger logits have larger ones.  Chunks leave a bucket at its place modulo kMassBuckets, which does not depend on what is largest.
 __device__ __forceinline__ int grid_place(float x, double grid) { return static_cast<int>(__double_as_longlong(fma(static_cast<double>(x), grid, kMagic))); }
 
 __device__ __forceinline__ void fill_powers(const SampleParams& p, double* powers) {
@@ -975,21 +974,29 @@ __device__ __forceinline__ void draw_segments(const SampleParams& p, int r, cons
 
 // ----------------------------------------------------------------------- a row
 
-// From what the chunks left to the pick.  group_top(g), chunk_top(c), segment_sum(s) and mass(c, b), the last two relative to their chunk's
+// From what the chunks left to the pick.  group_top(g), chunk_top(c), segment_sum(s) and mass(c, place on the grid), the last two relative to their chunk's
 // largest and only there where that is not minus infinity.  `share`: this workgroup's of the row's (p.shares).
 template <int TYPE, typename GROUP, typename CHUNK, typename SEGMENT, typename MASS>
 __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const SampleRow<TYPE>& row, const SampleSettings& set, int chunk, int chunks, int share,
                                          const GROUP& group_top, const CHUNK& chunk_top, const SEGMENT& segment_sum, const MASS& mass, const double* powers, PickShared& sh) {
-    const GroupTops<GROUP> tops(group_top, groups_of(p.vocab));
-    float top = -INFINITY, low = INFINITY;  // of the groups' largest
-    tops.each([&](float t, int) {
-        top = fmaxf(top, t);
-        low = t > -INFINITY ? fminf(low, t) : low;
-    });
-    for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_tops[c] = chunk_top(c);
-    if (threadIdx.x == 0) sh.listed = sh.found = 0;
+    const int lane = threadIdx.x & 63;
     if (share > 0 && !set.masses()) return;  // (the first alone has work)
-    block_ends(top, low, sh);
+    // what the chunks left is requested in the order in which it is wanted, all of it before the first is there
+    static_assert(kMaxSampleVocab / kChunk <= 128, "");
+    const float tops_here = fmaxf(chunk_top(min(lane, chunks - 1)), chunk_top(min(lane + 64, chunks - 1)));
+    const float own_top = chunk_top(min(static_cast<int>(threadIdx.x), chunks - 1));
+    constexpr int kOwnMasses = kMassBuckets / kSampleThreads, kFirst = 8;
+    unsigned long long masses_here[kFirst][kOwnMasses];
+    const auto read_masses = [&](int c0, unsigned long long (&v)[kFirst][kOwnMasses]) {
+#pragma unroll
+        for (int d = 0; d < kFirst; d++)
+#pragma unroll
+            for (int k = 0; k < kOwnMasses; k++) v[d][k] = mass(min(c0 + d, chunks - 1), static_cast<int>(threadIdx.x) + k * kSampleThreads);
+    };
+    if (set.masses()) read_masses(0, masses_here);
+    const GroupTops<GROUP> tops(group_top, groups_of(p.vocab));
+    const float top = wave_max(tops_here);
+    if (threadIdx.x == 0) sh.listed = sh.found = 0;
     if (top == -INFINITY) {
         if (threadIdx.x == 0) {
             p.ids[r] = -1;
@@ -1017,10 +1024,14 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     const SampleWeights w{top, set.turn(), powers};
     const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52);
     const int segments = segments_of(p.vocab);
-    if (set.sums()) {
-        for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_shares[c] = w.weight(sh.chunk_tops[c]);  // (its own thread's)
-        __syncthreads();
+    const double grid = set.grid();
+    const int place = grid_place(top, grid);
+    if (set.sums() && static_cast<int>(threadIdx.x) < chunks) {
+        const double chunk_share = w.weight(own_top);
+        sh.chunk_shares[threadIdx.x] = chunk_share;
+        sh.chunk_shifts[threadIdx.x] = chunk_share > 0.0 ? place - grid_place(own_top, grid) : kMassBuckets;
     }
+    __syncthreads();
     const auto sum_of = [&](int s) {
         const double chunk_share = sh.chunk_shares[s * kSegment / chunk];
         return chunk_share > 0.0 ? segment_sum(s) * chunk_share : 0.0;
@@ -1048,6 +1059,9 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     if (set.top_k > 0) {
         // buckets of the logits, from the largest down, and the one that holds the k-th largest of the groups' largest, or of all where groups are few
         if (set.top_k <= kListed) {
+            float high = top, low = INFINITY;
+            tops.each([&](float t, int) { low = t > -INFINITY ? fminf(low, t) : low; });
+            block_ends(high, low, sh);
             double fine = 0.0;
             const auto bucket_of = [&](float x) { return x == top ? 0 : static_cast<int>(fmin((static_cast<double>(top) - x) * fine, 1e9)); };
             int bound = kBuckets;
@@ -1101,39 +1115,29 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         (void)block_scan(mine, sh.sums, total);
         const double target = set.top_p * total;
         int bound = kMassBuckets;
-        const double grid = set.grid();
-        const int place = grid_place(top, grid);
-        for (int c = threadIdx.x; c < chunks; c += kSampleThreads)
-            sh.chunk_shifts[c] = sh.chunk_shares[c] > 0.0 ? place - grid_place(sh.chunk_tops[c], grid) : kMassBuckets;
-        __syncthreads();
+        // a thread's places on the grid, and how far they lie behind the row's largest
+        const auto bucket_at = [&](int k) { return (place - static_cast<int>(threadIdx.x) - k * kSampleThreads) & (kMassBuckets - 1); };
         if (set.on_grid(top, 0x1p29)) {
             // w by buckets, of all chunks, and the one in which their running sum reaches the target
-            constexpr int kOwn = kMassBuckets / kSampleThreads;
+            constexpr int kOwn = kOwnMasses;
             double own[kOwn], sum = 0.0, all;
 #pragma unroll
             for (int k = 0; k < kOwn; k++) own[k] = 0.0;
-            constexpr int kDeep = 8;  // chunks
-            for (int c0 = 0; c0 < chunks; c0 += kDeep) {
-                unsigned long long v[kDeep][kOwn];
+            for (int c0 = 0; c0 < chunks; c0 += kFirst) {
+                if (c0 > 0) read_masses(c0, masses_here);
 #pragma unroll
-                for (int d = 0; d < kDeep; d++) {
+                for (int d = 0; d < kFirst; d++) {
                     const int shift = c0 + d < chunks ? sh.chunk_shifts[c0 + d] : kMassBuckets;
-#pragma unroll
-                    for (int k = 0; k < kOwn; k++) {
-                        const int b = kOwn * static_cast<int>(threadIdx.x) + k - shift;
-                        const unsigned long long held = mass(min(c0 + d, chunks - 1), max(b, 0));
-                        v[d][k] = b >= 0 ? held : 0;
-                    }
-                }
-#pragma unroll
-                for (int d = 0; d < kDeep; d++) {
                     const double chunk_share = c0 + d < chunks ? sh.chunk_shares[c0 + d] : 0.0;
 #pragma unroll
-                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(v[d][k]) * chunk_share;
+                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(bucket_at(k) >= shift ? masses_here[d][k] : 0) * chunk_share;
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kOwn; k++) sum += own[k] *= 1.0 / scale;
+            for (int k = 0; k < kOwn; k++) sh.weights[bucket_at(k)] = own[k] * (1.0 / scale);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kOwn; k++) sum += own[k] = sh.weights[kOwn * threadIdx.x + k];
             if (threadIdx.x == 0) sh.bucket = kMassBuckets;
             double before = block_scan(sum, sh.sums, all);
 #pragma unroll
@@ -1165,7 +1169,6 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                     cut = cut_list(w, own, above, target, scale, sh);
                     if (set.min_p == 0.0 || -log2(set.min_p) * kMassFine > bound + 2) {
                         // what the chunks keep: all above the bucket, and of its own what is kept.  Only the chunk that the draw falls into is read again
-                        constexpr int kDeep = 8, kOwn = kMassBuckets / kSampleThreads;  // chunks
                         for (int c = threadIdx.x; c < chunks; c += kSampleThreads) sh.chunk_wholes[c] = 0;
                         __syncthreads();
                         for (int i = threadIdx.x; i < own; i += kSampleThreads) {
@@ -1173,25 +1176,17 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                             const int index = static_cast<int>(static_cast<unsigned>(sh.bins[i]));
                             if (cut.keeps(key, index)) atomicAdd(&sh.chunk_wholes[index / chunk], whole_number(w.weight(key_value(key)), scale));
                         }
-                        for (int c0 = 0; c0 < chunks; c0 += kDeep) {
-                            unsigned long long v[kDeep][kOwn];
+                        for (int c0 = 0; c0 < chunks; c0 += kFirst) {
+                            read_masses(c0, masses_here);
 #pragma unroll
-                            for (int d = 0; d < kDeep; d++) {
+                            for (int d = 0; d < kFirst; d++) {
                                 const int shift = c0 + d < chunks ? sh.chunk_shifts[c0 + d] : kMassBuckets;
-#pragma unroll
-                                for (int k = 0; k < kOwn; k++) {
-                                    const int b = static_cast<int>(threadIdx.x) + k * kSampleThreads;
-                                    const unsigned long long held = mass(min(c0 + d, chunks - 1), max(b - shift, 0));
-                                    v[d][k] = b >= shift && b < bound ? held : 0;
-                                }
-                            }
-#pragma unroll
-                            for (int d = 0; d < kDeep; d++) {
                                 double sum = 0.0;
 #pragma unroll
-                                for (int k = 0; k < kOwn; k++) sum += static_cast<double>(v[d][k]);
+                                for (int k = 0; k < kOwnMasses; k++)
+                                    if (const int b = bucket_at(k); (b >= shift) & (b < bound)) sum += static_cast<double>(masses_here[d][k]);
                                 sum = wave_scan(sum);
-                                if (c0 + d < chunks && (threadIdx.x & 63) == 63) sh.segments[(c0 + d) * kSampleWaves + (threadIdx.x >> 6)] = sum;
+                                if (c0 + d < chunks && lane == 63) sh.segments[(c0 + d) * kSampleWaves + (threadIdx.x >> 6)] = sum;
                             }
                         }
                         __syncthreads();
@@ -1213,7 +1208,8 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                             }
                             running += sh.chunk_sums[c];
                         }
-                        const auto weight = [&](float x, int i) { return cut.keeps(order_key(x), i) ? w.weight(x) : 0.0; };
+                        // (a logit that is left out has a w of nothing: a branch around each exponential would make them follow each other)
+                        const auto weight = [&](float x, int i) { return w.weight(cut.keeps(order_key(x), i) ? x : -INFINITY); };
                         const int first = here * (chunk / kSegment), count = min(chunk / kSegment, segments - first);
                         sum_segments(row, first, count, sh, weight);
                         draw_segments(p, r, row, first, count, ahead, held, sh, weight);
@@ -1249,7 +1245,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         return;
     }
     const auto weight = [&](float x, int i) {
-        const double v = cut.keeps(order_key(x), i) ? w.weight(x) : 0.0;
+        const double v = w.weight(cut.keeps(order_key(x), i) ? x : -INFINITY);
         return v >= set.min_p ? v : 0.0;
     };
     sum_segments(row, 0, segments, sh, weight);
@@ -1270,8 +1266,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const Sample
     const SampleSettings set(p, r);
     const float top = scan_chunk<TYPE, kSampleThreads>(p, row, set, 0, powers, left);
     __syncthreads();
+    const int place = grid_place(top, set.grid());
     pick_row(p, r, row, set, kChunk, 1, 0, [&](int g) { return left.group_tops[g]; }, [&](int) { return top; }, [&](int s) { return left.segments[s]; },
-             [&](int, int b) { return left.masses[b]; }, powers, sh);
+             [&](int, int at) { return left.masses[(place - at) & (kMassBuckets - 1)]; }, powers, sh);
 }
 
 // One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute: registers for
@@ -1295,8 +1292,10 @@ __global__ __launch_bounds__(THREADS, 5) void sample_scan_kernel(const SamplePar
     if (top == -INFINITY) return;
     if (set.sums() && t < kSegments && c * kSegments + t < segments_of(p.vocab))
         p.segment_sums[static_cast<size_t>(r) * segments_of(p.vocab) + c * kSegments + t] = left.segments[t];
+    const int place = grid_place(top, set.grid());
     if (set.masses() && set.on_grid(top))
-        for (int b = t; b < kMassBuckets; b += THREADS) p.masses[(static_cast<size_t>(r) * p.chunks + c) * kMassBuckets + b] = left.masses[b];
+        for (int b = t; b < kMassBuckets; b += THREADS)
+            p.masses[(static_cast<size_t>(r) * p.chunks + c) * kMassBuckets + ((place - b) & (kMassBuckets - 1))] = left.masses[b];
 }
 
 // What follows: a workgroup to a row, or several where rows have more groups than a list holds and a nucleus may have to be looked for in all of
@@ -1316,7 +1315,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(const Sampl
     const double* const segment_sums = p.segment_sums + static_cast<size_t>(r) * segments_of(p.vocab);
     const unsigned long long* const masses = p.masses + static_cast<size_t>(r) * p.chunks * kMassBuckets;
     pick_row(p, r, row, set, chunk, p.chunks, share, [&](int g) { return group_tops[g]; }, [&](int c) { return chunk_tops[c]; },
-             [&](int s) { return segment_sums[s]; }, [&](int c, int b) { return masses[c * kMassBuckets + b]; }, powers, sh);
+             [&](int s) { return segment_sums[s]; }, [&](int c, int at) { return masses[c * kMassBuckets + at]; }, powers, sh);
 }
 
 }  // namespace gh
