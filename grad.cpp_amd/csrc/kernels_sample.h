@@ -942,14 +942,29 @@ __device__ __forceinline__ void draw_segments(const SampleParams& p, int r, cons
     }
     __syncthreads();
     if (wave != 0) return;
-    const int i0 = (first + segment) * kSegment + lane * kVec;
-    double v[kVec], sum = 0.0;
-    float x[kVec];
-    row.load(i0, x);
+    // A chunk's sums hold what is nothing beside the row's largest: a segment that has nothing else gives way to the next that has a kept token, or
+    // to the last one before it.
+    int here = segment, step = 1, i0;
+    double v[kVec], sum;
+    for (;;) {
+        i0 = (first + here) * kSegment + lane * kVec;
+        float x[kVec];
+        row.load(i0, x);
+        sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kVec; i++) sum += v[i] = weight(x[i], i0 + i);
+        for (int i = 0; i < kVec; i++) sum += v[i] = weight(x[i], i0 + i);
+        if (__ballot(sum > 0.0)) break;
+        do {
+            here += step;
+            if (here == count) {
+                step = -1;
+                here = segment - 1;
+            }
+        } while (here >= 0 && !(sh.segments[here] > 0.0));
+        if (here < 0) return;  // (not reached: the row's largest has a w of 1)
+    }
     const double upto = wave_scan(sum), shifted = __shfl_up(upto, 1);
-    double running = sh.sums[0] + (lane == 0 ? 0.0 : shifted);
+    double running = (here == segment ? sh.sums[0] : here > segment ? target : -INFINITY) + (lane == 0 ? 0.0 : shifted);
     int hit = -1, last = -1;
     double hit_weight = 0.0, last_weight = 0.0;
 #pragma unroll

@@ -348,7 +348,8 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  *   their whole sum (a uniform of 0 and less, or NaN: the first that is kept; of 1 and more: the last).
  * A temperature of 0 and less, or NaN, picks the largest logit, of equal ones the first, with probability 1.  NaN in a setting is
  * as if it were off.  NaN among the logits is never picked, nor is minus infinity: a row that has nothing else
- * gives -1 with probability 0.  Infinite logits share the row among themselves.  w below 2^-44 count as nothing.
+ * gives -1 with probability 0.  Infinite logits share the row among themselves.  w below 2^-44 are never picked
+ * (and count as nothing, or in the sums as what they are).
  * Sums and exponentials are 64-bit: a pick is the definition's wherever the uniform is not within some 2^-40
  * of a border.  The same call gives the same bits.
  *

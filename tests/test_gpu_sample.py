@@ -175,6 +175,22 @@ def test_uniforms_at_their_ends(torch, dtype):
         check(torch, x, u, f"{s}", **s)
 
 
+@pytest.mark.parametrize("vocab", [5000, 20000, 150000])
+def test_segments_that_hold_next_to_nothing(torch, vocab):
+    # w of 2^-44.5 count as nothing, however large they are beside what stands near them; uniforms that fall where they would be
+    x = torch.full((4, vocab), -float("inf"))
+    step = float(np.log(2.0))
+    x[:, 0:2000:7] = -44.5 * step
+    x[0, 4000], x[0, vocab - 1] = -43.0 * step, 0.0  # before the first token that is kept
+    x[1, 4000], x[1, 600] = -43.0 * step, 0.0        # behind the only one of its stretch
+    x[2, 1000], x[2, vocab - 900:vocab] = 0.0, -44.5 * step  # behind the last
+    x[2, vocab - 1300] = -43.0 * step
+    x[3, vocab - 1] = 0.0
+    for u in (0.0, 2.0 ** -45, 2.0 ** -43, 1 - 2.0 ** -24, 1.0):
+        for settings in (dict(), dict(top_p=0.999999), dict(min_p=1e-30)):
+            check(torch, x.cuda(), [u] * 4, (u, settings), **settings)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("vocab", [3, 600, 5207, 31801])
 def test_logits_too_close_to_differ(torch, dtype, vocab):
