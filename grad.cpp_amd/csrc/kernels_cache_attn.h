@@ -482,7 +482,7 @@ constexpr int attend_waves(int type, int dh) { return type == kCacheF32 && dh <=
 // to 2 k, 12 heads of 64 in fp32, 457 MB: 85 us, 5.4 TB/s).  A short pass is bound by its trips one behind the other, items, pages, keys
 // and values, joins (one token over 96 positions 5.8 us, of which a launch that does nothing is 4.5).
 // With windows and sinks the same: 16 sequences with windows of 4 k and 4 sinks, heads as above, 269 MB: 47 us, 5.8 TB/s; 64 with windows of 512,
-// 12 heads of 64 in fp32, 198 MB: 35 us, 5.7 TB/s; one token with a window of 256: 9.0 us, the trips, one part.
+// 12 heads of 64 in fp32, 195 MB: 35 us, 5.5 TB/s; one token with a window of 256: 9.0 us, the trips, one part.
 template <int TYPE, int DH, bool FULL, bool SINKS>
 __global__ __launch_bounds__(64 * attend_waves(TYPE, DH), DH <= 64 ? 4 : 1) void attend_rows_kernel(const AttendParams p) {
     constexpr int kAttendWaves = attend_waves(TYPE, DH);
