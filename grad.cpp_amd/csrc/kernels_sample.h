@@ -1042,6 +1042,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     const int segments = segments_of(p.vocab);
     const double grid = set.grid();
     const int place = grid_place(top, grid);
+    __syncthreads();  // (the table of powers, which every wavefront filled a part of, is whole; loads go on)
     if (set.sums() && static_cast<int>(threadIdx.x) < chunks) {
         const double chunk_share = w.weight(own_top);
         sh.chunk_shares[threadIdx.x] = chunk_share;
