@@ -16,7 +16,8 @@
 // Only groups that reach the bound are looked at again; the tokens above it become a list, which is put in order, cut and drawn from.  What does
 // not fit a list (a nucleus of thousands of tokens) is cut among the bucket's own tokens, and only the chunk that the draw falls into is read again;
 // where a bucket's tokens do not fit a list either (thousands of equal logits, k of thousands), histograms over the row find the cut.
-// Bucket sums are whole numbers, so the order in which atomics arrive changes nothing.
+// Bucket sums are whole numbers, so the order in which atomics arrive changes nothing.  A bucket's are of a unit of its own, 2^-48 and less of its
+// w: with one unit for a row a tail of a million equal w of 2^-26 would be rounded alike, and its cut be off by tokens.
 #pragma once
 
 #include "kernels_cache_attn.h"
@@ -43,12 +44,14 @@ constexpr double kLeastPower = 44.0;          // w below 2^-44 of the largest ar
 // w by buckets of x: so many to a power of two, on a grid that all chunks share
 constexpr int kMassBuckets = 1024;
 constexpr double kMassFine = 40.0;
+constexpr int kMassBits = 47;  // of a w in its bucket's unit: a chunk's 2^14 tokens sum to less than 2^63
+static_assert(kWideChunk <= 1 << 14, "");
 
 struct SampleParams {
     const void* logits;
     long long row_stride;
     int vocab;
-    int scale_bits;  // of the histograms' whole numbers: vocab * 2^scale_bits < 2^63
+    int scale_bits;  // of a w in the unit of its bucket, for the histograms over the row: vocab * 2^scale_bits < 2^63
     const float* temperature;
     const int* top_k;
     const float* top_p;
@@ -204,6 +207,7 @@ struct PickShared {
     double chunk_sums[kMaxSampleVocab / kChunk];
     double chunk_shares[kMaxSampleVocab / kChunk];  // of a w relative to its chunk's largest, relative to the row's
     int chunk_shifts[kMaxSampleVocab / kChunk];     // how far its buckets lie behind the row's; all of them where it has none
+    double chunk_scales[kMaxSampleVocab / kChunk];  // of its buckets' units, relative to the row's
     unsigned long long scan[kSampleWaves];
     double sums[kSampleWaves];
     int ints[kSampleWaves];
@@ -211,7 +215,7 @@ struct PickShared {
     unsigned long long chunk_wholes[kMaxSampleVocab / kChunk];
     unsigned low, high;
     unsigned long long above;  // of the histogram, before the bucket that was found
-    double mass_above;
+    double mass_above, mass_upto;
     int bucket, found, listed;
 };
 
@@ -240,6 +244,17 @@ struct SampleWeights {
 
 __device__ __forceinline__ unsigned long long whole_number(double w, double scale) {
     return static_cast<unsigned long long>(__double_as_longlong(fma(w, scale, 0x1p52))) & 0xFFFFFFFFFFFFFull;
+}
+
+__device__ __forceinline__ double power_of_two(int n) { return __longlong_as_double(static_cast<long long>(1023 + n) << 52); }
+
+// The unit of a bucket is 2^-kMassBits of the power of two that its place on the grid falls into: kMassFine places to each.  Seen from a larger logit's place
+// these are `octaves_to(b, rest)` powers of two down, for the bucket b places down (not beyond kMassBuckets); all chunks cut the grid alike.
+constexpr int kOctave = static_cast<int>(kMassFine);
+__device__ __forceinline__ int octave_rest(int place) { return kOctave - 1 - ((place % kOctave + kOctave) % kOctave); }
+__device__ __forceinline__ int octaves_to(int b, int rest) {
+    static_assert(kOctave == 40 && kMassBuckets == 1024, "1639 / 2^16: (b + rest) / 40 up to 2600");
+    return (b + rest) * 1639 >> 16;
 }
 
 // What a row's settings come to.
@@ -343,8 +358,8 @@ __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleR
 #pragma unroll
             for (int i = 0; i < kVec; i++) raw[r][i] = static_cast<T>(static_cast<float>(raw[r][i]) == INFINITY ? 0.0f : -INFINITY);
     }
-    const double turn = set.turn(), scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52), grid = set.grid();
-    const int place = grid_place(top, grid);
+    const double turn = set.turn(), grid = set.grid();
+    const int place = grid_place(top, grid), rest = octave_rest(place);
     const auto sum_up = [&](auto counted) {
         double all = 0.0;
 #pragma unroll
@@ -358,7 +373,7 @@ __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleR
                 if constexpr (decltype(counted)::value) {
                     // (what has no place on the grid has a w of nothing)
                     const unsigned b = static_cast<unsigned>(place - grid_place(x, grid));
-                    if (z > kLeastTurns && b < kMassBuckets) atomicAdd(&sh.masses[b], whole_number(v, scale));
+                    if (z > kLeastTurns && b < kMassBuckets) atomicAdd(&sh.masses[b], whole_number(v, power_of_two(kMassBits + octaves_to(static_cast<int>(b), rest))));
                 }
             }
             if constexpr (decltype(counted)::value) {
@@ -406,12 +421,53 @@ __device__ __forceinline__ int find_bucket(PickShared& sh, double target, unsign
     return sh.bucket;
 }
 
-// The cut behind which the running total, in the order of the tokens, of 1 (MASS: of w as whole numbers) per token that `kept` keeps reaches
+// The same for w of `buckets` buckets, value(b) of each, of which one is above zero: the last in front of which the running total is below the
+// target (a total that rounding leaves between two threads' takes the same one in every thread).  Leaves the total before it in sh.mass_above, with it in
+// sh.mass_upto.
+template <int BUCKETS, typename F>
+__device__ __forceinline__ int find_mass(PickShared& sh, double target, F&& value) {
+    constexpr int kOwn = BUCKETS / kSampleThreads;
+    const int first = kOwn * static_cast<int>(threadIdx.x);
+    __syncthreads();
+    double own[kOwn], sum = 0.0, all;
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) sum += own[k] = value(first + k);
+    if (threadIdx.x == 0) sh.bucket = 0;
+    const double before = block_scan(sum, sh.sums, all);
+    double running = before;
+    int last = -1;
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) {
+        if (own[k] > 0.0 && (running == 0.0 || running < target)) last = first + k;
+        running += own[k];
+    }
+    // (one atomic a wavefront: one for each bucket before the target took 7 us of a flat row of 201001)
+    const unsigned long long any = __ballot(last >= 0);
+    if (any && static_cast<int>(threadIdx.x & 63) == 63 - __clzll(any)) atomicMax(&sh.bucket, last);
+    __syncthreads();
+    const int bucket = sh.bucket;
+    running = before;
+#pragma unroll
+    for (int k = 0; k < kOwn; k++) {
+        if (first + k == bucket) {
+            sh.mass_above = running;
+            sh.mass_upto = running + own[k];
+        }
+        running += own[k];
+    }
+    __syncthreads();
+    return bucket;
+}
+
+// The cut behind which the running total, in the order of the tokens, of 1 (MASS: of w) per token that `kept` keeps reaches
 // `target`.  Buckets of x relative to the largest first, then of the keys of one bucket, finer and finer, then equal keys by
 // their index.  Tokens whose w are nothing are left out.
 template <int TYPE, bool MASS>
-__device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, double scale, const Cut& kept, double target, PickShared& sh) {
+__device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWeights& w, int scale_bits, const Cut& kept, double target, PickShared& sh) {
     const double fine = kBuckets / -kLeastTurns;
+    // w of bucket b are 2^(-44 b / kBuckets) and less; the whole powers of two in it
+    static_assert(kLeastPower * 512 == 22528.0 && kBuckets == 2048, "");
+    const auto octaves = [](int b) { return b * 11 >> 9; };
     const auto counts = [&](float x) { return w.turns(x) > kLeastTurns; };
     const auto bucket_of = [&](float x) { return min(static_cast<int>(-w.turns(x) * fine), kBuckets - 1); };
     const auto clear = [&] {
@@ -419,15 +475,25 @@ __device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWei
         for (int b = threadIdx.x; b < kBuckets; b += kSampleThreads) sh.bins[b] = 0;
         __syncthreads();
     };
-    const auto amount = [&](float x) { return MASS ? whole_number(w.weight(x), scale) : 1ull; };
     clear();
     row.each([&](float x, int i) {
-        if (counts(x) && kept.keeps(order_key(x), i)) atomicAdd(&sh.bins[bucket_of(x)], amount(x));
+        if (!counts(x) || !kept.keeps(order_key(x), i)) return;
+        const int b = bucket_of(x);
+        atomicAdd(&sh.bins[b], MASS ? whole_number(w.weight(x), power_of_two(scale_bits + octaves(b))) : 1ull);
     });
-    unsigned long long all;
-    const int bucket = find_bucket(sh, target, all);
-    if (!MASS && static_cast<double>(all) < target) return kept;  // (there are fewer)
-    unsigned long long above = sh.above;
+    int bucket;
+    unsigned long long above = 0, all;
+    double scale = 1.0;  // of the bucket
+    if constexpr (MASS) {
+        bucket = find_mass<kBuckets>(sh, target, [&](int b) { return static_cast<double>(sh.bins[b]) * power_of_two(-scale_bits - octaves(b)); });
+        scale = power_of_two(scale_bits + octaves(bucket));
+        target = (target - sh.mass_above) * scale;
+    } else {
+        bucket = find_bucket(sh, target, all);
+        if (static_cast<double>(all) < target) return kept;  // (there are fewer)
+        above = sh.above;
+    }
+    const auto amount = [&](float x) { return MASS ? whole_number(w.weight(x), scale) : 1ull; };
     if (threadIdx.x == 0) {
         sh.low = 0xFFFFFFFFu;
         sh.high = 0;
@@ -454,7 +520,7 @@ __device__ __noinline__ Cut find_cut(const SampleRow<TYPE>& row, const SampleWei
         if (high - low > (1u << shift) - 1) low = high - ((1u << shift) - 1);
     }
     // equal keys: so many of them, the lowest indices
-    const double each = static_cast<double>(amount(key_value(low)));
+    const double each = MASS ? w.weight(key_value(low)) * scale : 1.0;
     const double wanted = ceil((target - static_cast<double>(above)) / each);
     const int take = wanted < 1.0 ? 1 : wanted > 1e9 ? 1000000000 : static_cast<int>(wanted);
     Cut cut;
@@ -764,7 +830,7 @@ __device__ __forceinline__ int make_list_together(const SampleParams& p, int r, 
 }
 
 // The cut among the list's n tokens behind which the running sum of w, `above` before the first of them, reaches `target`; one is kept at least.  The
-// tokens are left, in any order, in sh.bins.  Many are first told apart by buckets of their keys.
+// tokens are left, in any order, in sh.bins.  Many are first told apart by buckets of their keys, in whole numbers of w times `scale`.
 __device__ __forceinline__ Cut cut_list(const SampleWeights& w, int n, double above, double target, double scale, PickShared& sh) {
     constexpr int kOwn = kListed / kSampleThreads;
     unsigned long long own[kOwn];
@@ -1038,15 +1104,16 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         return;
     }
     const SampleWeights w{top, set.turn(), powers};
-    const double scale = __longlong_as_double(static_cast<long long>(1023 + p.scale_bits) << 52);
     const int segments = segments_of(p.vocab);
     const double grid = set.grid();
-    const int place = grid_place(top, grid);
+    const int place = grid_place(top, grid), rest = octave_rest(place);
     __syncthreads();  // (the table of powers, which every wavefront filled a part of, is whole; loads go on)
     if (set.sums() && static_cast<int>(threadIdx.x) < chunks) {
         const double chunk_share = w.weight(own_top);
         sh.chunk_shares[threadIdx.x] = chunk_share;
-        sh.chunk_shifts[threadIdx.x] = chunk_share > 0.0 ? place - grid_place(own_top, grid) : kMassBuckets;
+        const int shift = chunk_share > 0.0 ? min(place - grid_place(own_top, grid), kMassBuckets) : kMassBuckets;
+        sh.chunk_shifts[threadIdx.x] = shift;
+        sh.chunk_scales[threadIdx.x] = chunk_share * power_of_two(octaves_to(shift, rest));
     }
     __syncthreads();
     const auto sum_of = [&](int s) {
@@ -1114,14 +1181,12 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
             listed = make_list(row, tops, sh, below(static_cast<double>(top) - (bound + 1) / fine), INFINITY, true);
         }
         if (listed > kListed) {
-            cut = find_cut<TYPE, false>(row, w, scale, cut, set.top_k, sh);
+            cut = find_cut<TYPE, false>(row, w, p.scale_bits, cut, set.top_k, sh);
             if (set.top_p < 1.0) {
-                unsigned long long mine = 0, all;
-                row.each([&](float x, int i) {
-                    if (cut.keeps(order_key(x), i)) mine += whole_number(w.weight(x), scale);
-                });
-                (void)block_scan(mine, sh.scan, all);
-                cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
+                double mine = 0.0, all;
+                row.each([&](float x, int i) { mine += w.weight(cut.keeps(order_key(x), i) ? x : -INFINITY); });
+                (void)block_scan(mine, sh.sums, all);
+                cut = find_cut<TYPE, true>(row, w, p.scale_bits, cut, set.top_p * all, sh);
             }
         }
     } else if (set.top_p < 1.0) {
@@ -1134,10 +1199,11 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         int bound = kMassBuckets;
         // a thread's places on the grid, and how far they lie behind the row's largest
         const auto bucket_at = [&](int k) { return (place - static_cast<int>(threadIdx.x) - k * kSampleThreads) & (kMassBuckets - 1); };
+        const auto unit_at = [&](int k) { return power_of_two(-kMassBits - octaves_to(bucket_at(k), rest)); };
         if (set.on_grid(top, 0x1p29)) {
             // w by buckets, of all chunks, and the one in which their running sum reaches the target
             constexpr int kOwn = kOwnMasses;
-            double own[kOwn], sum = 0.0, all;
+            double own[kOwn];
 #pragma unroll
             for (int k = 0; k < kOwn; k++) own[k] = 0.0;
             for (int c0 = 0; c0 < chunks; c0 += kFirst) {
@@ -1145,28 +1211,15 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
 #pragma unroll
                 for (int d = 0; d < kFirst; d++) {
                     const int shift = c0 + d < chunks ? sh.chunk_shifts[c0 + d] : kMassBuckets;
-                    const double chunk_share = c0 + d < chunks ? sh.chunk_shares[c0 + d] : 0.0;
+                    const double chunk_scale = c0 + d < chunks ? sh.chunk_scales[c0 + d] : 0.0;
 #pragma unroll
-                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(bucket_at(k) >= shift ? masses_here[d][k] : 0) * chunk_share;
+                    for (int k = 0; k < kOwn; k++) own[k] += static_cast<double>(bucket_at(k) >= shift ? masses_here[d][k] : 0) * chunk_scale;
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kOwn; k++) sh.weights[bucket_at(k)] = own[k] * (1.0 / scale);
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kOwn; k++) sum += own[k] = sh.weights[kOwn * threadIdx.x + k];
-            if (threadIdx.x == 0) sh.bucket = kMassBuckets;
-            double before = block_scan(sum, sh.sums, all);
-#pragma unroll
-            for (int k = 0; k < kOwn; k++) {
-                if (own[k] > 0.0 && (before < target || before == 0.0) && before + own[k] >= target) {
-                    sh.bucket = kOwn * static_cast<int>(threadIdx.x) + k;
-                    sh.mass_above = before;
-                }
-                before += own[k];
-            }
-            __syncthreads();
-            bound = sh.bucket;
+            for (int k = 0; k < kOwn; k++) sh.weights[bucket_at(k)] = own[k] * unit_at(k);
+            const int bucket = find_mass<kMassBuckets>(sh, target, [&](int b) { return sh.weights[b]; });
+            if (sh.mass_upto >= target) bound = bucket;
         }
         if (bound < kMassBuckets) {  // (buckets end there)
             const double above = sh.mass_above;
@@ -1183,6 +1236,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                 if (own < 0) return;
                 share = 0;  // (the last of them goes on)
                 if (own <= kListed) {
+                    const double scale = power_of_two(kMassBits + octaves_to(bound, rest));
                     cut = cut_list(w, own, above, target, scale, sh);
                     if (set.min_p == 0.0 || -log2(set.min_p) * kMassFine > bound + 2) {
                         // what the chunks keep: all above the bucket, and of its own what is kept.  Only the chunk that the draw falls into is read again
@@ -1201,7 +1255,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                                 double sum = 0.0;
 #pragma unroll
                                 for (int k = 0; k < kOwnMasses; k++)
-                                    if (const int b = bucket_at(k); (b >= shift) & (b < bound)) sum += static_cast<double>(masses_here[d][k]);
+                                    if (const int b = bucket_at(k); (b >= shift) & (b < bound)) sum += static_cast<double>(masses_here[d][k]) * unit_at(k);
                                 sum = wave_scan(sum);
                                 if (c0 + d < chunks && lane == 63) sh.segments[(c0 + d) * kSampleWaves + (threadIdx.x >> 6)] = sum;
                             }
@@ -1210,7 +1264,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                         for (int c = threadIdx.x; c < chunks; c += kSampleThreads) {
                             double sum = 0.0;
                             for (int k = 0; k < kSampleWaves; k++) sum += sh.segments[c * kSampleWaves + k];
-                            sh.chunk_sums[c] = (sum * sh.chunk_shares[c] + static_cast<double>(sh.chunk_wholes[c])) / scale;
+                            sh.chunk_sums[c] = sum * sh.chunk_scales[c] + static_cast<double>(sh.chunk_wholes[c]) / scale;
                         }
                         __syncthreads();
                         double held = 0.0;
@@ -1238,10 +1292,10 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
         }
         if (share > 0) return;
         if (listed > kListed && bound >= 0) {
-            unsigned long long whole = 0, all;
-            row.each([&](float x, int) { whole += whole_number(w.weight(x), scale); });
-            (void)block_scan(whole, sh.scan, all);
-            cut = find_cut<TYPE, true>(row, w, scale, cut, set.top_p * static_cast<double>(all), sh);
+            double mine = 0.0, all;
+            row.each([&](float x, int) { mine += w.weight(x); });
+            (void)block_scan(mine, sh.sums, all);
+            cut = find_cut<TYPE, true>(row, w, p.scale_bits, cut, set.top_p * all, sh);
         }
     } else {
         listed = make_list(row, tops, sh, below(min_p_reach()), INFINITY, true);

@@ -348,10 +348,10 @@ gh_status gh_pick_noalloc(const float* logits, int32_t batch, int32_t vocab, con
  *   their whole sum (a uniform of 0 and less, or NaN: the first that is kept; of 1 and more: the last).
  * A temperature of 0 and less, or NaN, picks the largest logit, of equal ones the first, with probability 1.  NaN in a setting is
  * as if it were off.  NaN among the logits is never picked, nor is minus infinity: a row that has nothing else
- * gives -1 with probability 0.  Infinite logits share the row among themselves.  w below 2^-44 are never picked
- * (and count as nothing, or in the sums as what they are).
- * Sums and exponentials are 64-bit: a pick is the definition's wherever the uniform is not within some 2^-40
- * of a border.  The same call gives the same bits.
+ * gives -1 with probability 0.  Infinite logits share the row among themselves.  w below 2^-44 are never picked;
+ * the sums hold them or not, and borders are moved by what they amount to: nothing in most rows, less than vocab x 2^-44 of the largest w in any.
+ * Exponentials are 64-bit, sums 64-bit or of whole numbers that hold every w to 2^-42 of itself and better: a pick is the definition's wherever
+ * neither its uniform nor top_p is within some 2^-40 of a border.  The same call gives the same bits.
  *
  * Every pointer is DEVICE memory of the caller's, on one device, which need not be the current one.  The work is enqueued
  * on hip_stream (a hipStream_t of that device, NULL for its default stream) and the call returns without waiting; nothing
