@@ -1141,10 +1141,13 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
     double total = 0.0;  // of what top-p is a share of
     int listed = kListed + 1;
     if (set.top_k > 0) {
-        // buckets of the logits, from the largest down, and the one that holds the k-th largest of the groups' largest, or of all where groups are few
+        // Buckets of the logits, from the largest down, and the one that holds the k-th largest of the groups' largest, or of all where groups are few.
+        // Groups without a w are left out: one of nothing but forbidden tokens, at the type's lowest value, would stretch the first bucket over all the others
+        // (32 x 50257, fp32, k = 40: 17 us, with them 198)
         if (set.top_k <= kListed) {
+            const float nothing = below(static_cast<double>(top) + kLeastTurns / w.turn);
             float high = top, low = INFINITY;
-            tops.each([&](float t, int) { low = t > -INFINITY ? fminf(low, t) : low; });
+            tops.each([&](float t, int) { low = t >= nothing ? fminf(low, t) : low; });
             block_ends(high, low, sh);
             double fine = 0.0;
             const auto bucket_of = [&](float x) { return x == top ? 0 : static_cast<int>(fmin((static_cast<double>(top) - x) * fine, 1e9)); };
@@ -1155,7 +1158,7 @@ __device__ __forceinline__ void pick_row(const SampleParams& p, int r, const Sam
                 if (threadIdx.x == 0) sh.bucket = kBuckets;
                 __syncthreads();
                 const auto count = [&](float x, int) {
-                    if (!(x > -INFINITY)) return;
+                    if (!(x >= nothing)) return;
                     if (const int b = bucket_of(x); b < kBuckets) atomicAdd(&sh.counts[b], 1u);
                 };
                 if (by_group) {
