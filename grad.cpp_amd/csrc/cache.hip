@@ -441,7 +441,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
         const int length = c.book.at(seqs[i]).length;
         if (counts[i] < 0) refuse("negative number of positions");
         rows += counts[i];
-        pages += (static_cast<long long>(length) + counts[i] + c.o.page_tokens - 1) / c.o.page_tokens;
+        pages += (static_cast<long long>(length) + counts[i] + c.o.page_tokens - 1) / c.o.page_tokens - c.book.hole_of(c.book.at(seqs[i])).pages();
         if (rows > (1 << 23) || rows * c.group > (1 << 30) || pages > (1 << 28)) refuse("a pass of more than 2^23 rows");
     }
     const Cache::Turn turn(c, stream);
@@ -454,9 +454,10 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     for (int i = 0; i < n; i++) {
         const int first = c.book.at(seqs[i]).length;
         if (counts[i] > INT_MAX - kMaxPageTokens - first) throw ApiError{GH_ERR_OUT_OF_RANGE, "cache: a sequence of more than 2^31 positions"};
-        c.seqs[static_cast<size_t>(i)] = {first + counts[i], first, row0, table};
+        const int hole = c.book.hole_of(c.book.at(seqs[i])).pages();
+        c.seqs[static_cast<size_t>(i)] = {first + counts[i], first, row0, table, hole};
         row0 += counts[i];
-        table += c.book.pages_for(first + counts[i]);
+        table += c.book.pages_for(first + counts[i]) - hole;
     }
     // prefixes that sequences of few rows share are read once for all of them
     std::vector<const std::vector<int>*> pages_of(static_cast<size_t>(n));
@@ -486,7 +487,7 @@ static void extend_cache(Cache& c, const int32_t* seqs, const int32_t* counts, i
     int* page = reinterpret_cast<int*>(host + table_at);
     for (int i = 0; i < n; i++) {
         const PageBook::Sequence& s = c.book.at(seqs[i]);
-        for (int p : s.pages) *page++ = p == PageBook::kNone ? 0 : p;  // (of a forgotten page nothing is read)
+        page = c.book.write_list(s, page);
         for (int t = s.length - counts[i]; t < s.length; t++)
             *row++ = {s.pages[static_cast<size_t>(t >> c.layout.page_shift)] * c.o.page_tokens + (t & (c.o.page_tokens - 1)), t};
     }

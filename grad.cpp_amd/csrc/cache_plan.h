@@ -20,6 +20,7 @@ struct PassSeq {
     int first;  // position of its first new row
     int row0;   // index of that row
     int table;  // where its page list begins
+    int hole = 0;  // pages that it has forgotten and that the list leaves out: all that rows see lies before or behind them
 };
 
 struct RowAt {
@@ -29,15 +30,16 @@ struct RowAt {
 
 // One workgroup's work for one kv head: `rows` rows over the positions [k0, k1) of a page list.  Where rows see a sequence's first
 // positions beside a window far from them, [k0, k1) counts the positions that are left when what lies between is taken out:
-// those from `lead` (the sinks, rounded up to 16) on are `gap` further on.
+// those from `lead` (the sinks, rounded up to 16) on are `gap` further on, and their pages hole() places nearer to the list's front.
 struct AttendItem {
     int r0, rows;  // of a sequence's tile axis, or (map >= 0) as the map has them
     int k0, k1;
     int part;          // the place in memory that its result goes to, -1: it is whole and goes to the caller
     int join, joins;   // the joins that wait for it
     int first, row0, table;  // the sequence's; for a map, a position behind all others
-    int map;           // rows of several sequences: where their (pass row * group + head of the group) are listed
+    int map;           // rows of several sequences: where their (pass row * group + head of the group) are listed; if not, -1 - hole()
     int gap;           // a multiple of 16
+    constexpr int hole() const { return map < 0 ? -1 - map : 0; }
 };
 
 // A tile whose positions were dealt to several workgroups: the last of them to finish puts it together, first the parts of a
@@ -181,13 +183,14 @@ inline AttendPlan plan_attend(const std::vector<PassSeq>& seqs, const std::vecto
             if (it.part >= 0) it.part++;
         }
     };
+    // (a hole lies behind the sinks and before the first row's window: without sinks before everything that is read)
     const auto add_tile = [&](size_t i, int r0, AttendJoin join) {
         int n, k0, k1, run;
         const int gap = tile_span(i, r0, n, k0, k1);
         const int parts = cut_up(n, k0, k1, run);
         const bool whole = parts == 1 && join.shared_parts == 0;
         AttendItem it{r0, n, 0, 0, whole ? -1 : plan.parts, static_cast<int>(plan.joins.size()), whole ? 0 : 1,
-                      seqs[i].first, seqs[i].row0, seqs[i].table, -1, gap};
+                      seqs[i].first, seqs[i].row0, seqs[i].table - (lead == 0 ? seqs[i].hole : 0), -1 - (lead == 0 ? 0 : seqs[i].hole), gap};
         add_items(it, k0, k1, parts, run);
         if (whole) return;
         join.r0 = r0;

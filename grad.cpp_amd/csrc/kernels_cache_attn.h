@@ -118,6 +118,11 @@ template <bool SINKS>
 __device__ __forceinline__ int position_of(const AttendParams& p, const AttendItem& it, int v) {
     return SINKS && v >= p.lead ? v + it.gap : v;
 }
+// Its page.
+template <bool SINKS>
+__device__ __forceinline__ int page_of(const AttendParams& p, const AttendItem& it, const int* table, int v) {
+    return table[(position_of<SINKS>(p, it, v) >> p.cache.page_shift) - (SINKS && v >= p.lead ? it.hole() : 0)];
+}
 // What a row at `pos` sees of an item's positions, as bounds: two comparisons an element, where the conditions themselves are some ten.
 template <bool SINKS>
 struct Visible {
@@ -160,7 +165,7 @@ struct Granule {
 template <bool SINKS, int BLOCKS>
 __device__ __forceinline__ void look_up(const AttendParams& p, const AttendItem& it, const int* table, int at, int (&pages)[BLOCKS]) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) pages[b] = table[position_of<SINKS>(p, it, min(at + 16 * b, it.k1 - 1)) >> p.cache.page_shift];
+    for (int b = 0; b < BLOCKS; b++) pages[b] = page_of<SINKS>(p, it, table, min(at + 16 * b, it.k1 - 1));
 }
 
 // FULL: the head has DH dims.  Otherwise lanes whose dims do not exist read past the end of the run: zeros.

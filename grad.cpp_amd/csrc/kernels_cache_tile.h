@@ -76,8 +76,9 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
     using T = typename C::T;
     constexpr int kPad = DH + 4, kOwn = DH / 64;
     const int lane = threadIdx.x & 63, dims = p.cache.dim, mask = (1 << p.cache.page_shift) - 1;
-    const auto at = [&](int which, int t) {
-        return reinterpret_cast<const T*>(cache_run(p.cache, table[t >> p.cache.page_shift], p.layer, which, head)) + static_cast<size_t>(t & mask) * dims;
+    const auto at = [&](int which, int v) {  // of a place
+        return reinterpret_cast<const T*>(cache_run(p.cache, page_of<SINKS>(p, it, table, v), p.layer, which, head))
+               + static_cast<size_t>(position_of<SINKS>(p, it, v) & mask) * dims;
     };
 #pragma unroll 1
     for (int i = from; i < from + rows; i++) {
@@ -94,7 +95,7 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
             float z = -INFINITY;
             const bool seen = lane < n && (!SINKS || Visible<true>(p, it, pos).at(position_of<true>(p, it, t0 + lane)));
             if (seen) {
-                const T* key = at(0, position_of<SINKS>(p, it, t0 + lane));
+                const T* key = at(0, t0 + lane);
                 z = 0.0f;
 #pragma unroll 1
                 for (int d = 0; d < dims; d++) z = fmaf(static_cast<float>(query[d]), static_cast<float>(key[d]), z);
@@ -111,7 +112,7 @@ __device__ void rows_one_by_one(const AttendParams& p, const AttendItem& it, con
             for (int j = 0; j < n; j++) {
                 if (SINKS && __shfl(static_cast<int>(seen), j) == 0) continue;
                 const float w = __shfl(prob, j);
-                const T* value = at(1, position_of<SINKS>(p, it, t0 + j));
+                const T* value = at(1, t0 + j);
 #pragma unroll
                 for (int k = 0; k < kOwn; k++)
                     if (lane + 64 * k < dims) o[k] = fmaf(w, static_cast<float>(value[lane + 64 * k]), o[k]);
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_tile
     const auto row_of = [&](int i) { return 64 * (kTileWaves * i + wave) / kUnits; };
     const auto look = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < kLoads; i++) pages[i] = table[position_of<SINKS>(p, it, min(at + row_of(i), it.k1 - 1)) >> p.cache.page_shift];
+        for (int i = 0; i < kLoads; i++) pages[i] = page_of<SINKS>(p, it, table, min(at + row_of(i), it.k1 - 1));
     };
     const auto fetch = [&](int at) {
 #pragma unroll
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DH > 128 ? 1 : 2) void attend_wide
     const auto row_of = [&](int i) { return 64 * (kTileWaves * i + wave) / kUnits; };
     const auto look = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < kLoads; i++) pages[i] = table[position_of<SINKS>(p, it, min(at + row_of(i), it.k1 - 1)) >> p.cache.page_shift];
+        for (int i = 0; i < kLoads; i++) pages[i] = page_of<SINKS>(p, it, table, min(at + row_of(i), it.k1 - 1));
     };
     const auto fetch = [&](int at) {
 #pragma unroll

@@ -38,6 +38,24 @@ public:
         bool forgot(int from, int to) const { return std::max(from, gone_from) < std::min(to, gone_to); }  // any of those
     };
 
+    // The places of a sequence's list whose pages it has forgotten, but for the last one of a sequence cut off inside what was forgotten.
+    struct Hole {
+        int from, to;
+        int pages() const { return to - from; }
+    };
+    Hole hole_of(const Sequence& s) const {
+        const int from = pages_for(s.gone_from);
+        return {from, std::max(from, s.gone_to / page_tokens_)};
+    }
+    // The list without its hole, which is as long as a stream is: what a pass takes along.  (A last page may be nobody's: it has no rows, nothing of it is read.)
+    int* write_list(const Sequence& s, int* to) const {
+        const Hole hole = hole_of(s);
+        const int n = static_cast<int>(s.pages.size());
+        for (int i = 0; i < hole.from && i < n; i++) *to++ = std::max(s.pages[static_cast<size_t>(i)], 0);
+        for (int i = hole.to; i < n; i++) *to++ = std::max(s.pages[static_cast<size_t>(i)], 0);
+        return to;
+    }
+
     PageBook(int pages, int page_tokens) : page_tokens_(page_tokens), held_(static_cast<size_t>(pages), 0) {
         free_.reserve(held_.size());
         for (int p = 0; p < pages; p++) free_.push_back(p);  // ascending: a heap with the lowest on top
@@ -114,11 +132,14 @@ public:
             throw std::invalid_argument("cache: sequence " + std::to_string(seq) + " has forgotten positions " + std::to_string(s.gone_from) + " to "
                                         + std::to_string(s.gone_to) + ": what else it forgets has to touch them");
         const bool any = s.gone_from < s.gone_to;
+        const Hole before = hole_of(s);
         s.gone_from = any ? std::min(s.gone_from, from) : from;
         s.gone_to = any ? std::max(s.gone_to, to) : to;
-        // (only pages with a position of this call can have become wholly forgotten)
+        // (only pages with a position of this call can have become wholly forgotten, and those of the hole are: a stream's is as long as the stream)
         const int first = std::max(pages_for(s.gone_from), from / page_tokens_), end = std::min(s.gone_to / page_tokens_, pages_for(to));
         for (int i = first; i < end; i++) {
+            if (i >= before.from && i < before.to) i = before.to;
+            if (i >= end) break;
             int& p = s.pages[static_cast<size_t>(i)];
             if (p != kNone) release(p);
             p = kNone;
@@ -159,8 +180,9 @@ public:
         std::vector<PageCopy> copies;
         copies.reserve(static_cast<size_t>(n));
         for (int i = 0; i < n; i++) {  // (memory for the page lists first: what follows does not throw)
-            const Sequence& s = at(seqs[i]);
-            seqs_[static_cast<size_t>(seqs[i])].pages.reserve(static_cast<size_t>(pages_for(s.length + counts[i])));
+            std::vector<int>& list = seqs_[static_cast<size_t>(seqs[i])].pages;
+            const size_t want = static_cast<size_t>(pages_for(at(seqs[i]).length + counts[i]));
+            if (want > list.capacity()) list.reserve(std::max(want, list.capacity() + list.capacity() / 2));
         }
         for (int i = 0; i < n; i++) {
             if (counts[i] == 0) continue;
