@@ -332,7 +332,8 @@ private:
             // Windows and sinks: few rows' spans are of one length, nothing has to be evened out, so one workgroup to a compute unit and
             // nothing split that ends no sooner for it (16 sequences with windows of 4 k, 32/8 heads of 128 in bf16: 54 us, with 512
             // workgroups 60, 768 63, 2048 77; 4 sequences 20.2 and 25.8; 64 with windows of 512, 12 heads of 64 in fp32: 40.4 us, in two parts
-            // each 47.8; only ragged ones lose a little, 16 of 1 to 4 k, fp32: 95 us, with 512 91).
+            // each 47.8; only ragged ones lose a little, 16 of 1 to 4 k, fp32: 95 us, with 512 91).  Windows alone have the rule of all positions, which is
+            // not the quickest for them (the same calls on one set of inputs, with sinks and without: 47 and 67 us, 35 and 41).
             const int workgroups = tiles ? resident : sinks > 0 ? 256 : bytes == 4 ? 1024 : 2048;
             const int least = tiles ? 128 : bytes == 4 || sinks > 0 ? 256 : 384;
             l.cut = plan_attend(seqs, mine,

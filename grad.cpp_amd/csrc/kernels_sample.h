@@ -323,7 +323,7 @@ __device__ __forceinline__ void block_ends(float& high, float& low, PickShared& 
 // to the largest of the chunk, and w by buckets of x, from the chunk's largest down.  Returns the largest.
 //
 // The logits are loaded in one go, kept as they are, and gone through twice, because the exponentials need the chunk's largest first.  Without w it is bound
-// by reading; with w and buckets (some 39 vector instructions a logit, a look-up and an atomic in shared memory) by neither alone: what is resident
+// by reading; with w and buckets (some 44 vector instructions a logit, a look-up and an atomic in shared memory) by neither alone: what is resident
 // loads, then computes.
 template <int TYPE, int THREADS>
 __device__ __forceinline__ float scan_chunk(const SampleParams& p, const SampleRow<TYPE>& row, const SampleSettings& set, int first, const double* powers,
@@ -1347,8 +1347,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(const Sample
 
 // One chunk of a row, for sample_pick_kernel.  Several workgroups to a compute unit, so that one reads while the others compute: registers for
 // five wavefronts on a SIMD (six cost min-p alone no spills, 27 us for 30, but w and buckets some: 106 for 99; eight 128).
-//   256 x 128000 bf16, min-p: 17 us, 3.8 TB/s; 100 x 201001 fp32, top-p: 33 us, 2.4 TB/s (as long with 25 instructions a logit, turns and rest by one
-//   rounding each); 64 x 50257 bf16, top-p: 9.6.
+//   256 x 128000 bf16, min-p: 17 us, 3.8 TB/s; 100 x 201001 fp32, top-p: 36 us, 2.2 TB/s, of which the buckets' own units are 2 to 3 (without
+//   them 33, and as long with 25 instructions a logit instead of 39, turns and rest by one rounding each); 64 x 50257 bf16, top-p: 9.9.
 template <int TYPE, int THREADS>
 __global__ __launch_bounds__(THREADS, 5) void sample_scan_kernel(const SampleParams p) {
     __shared__ ChunkShared<THREADS> left;
@@ -1374,8 +1374,8 @@ __global__ __launch_bounds__(THREADS, 5) void sample_scan_kernel(const SamplePar
 }
 
 // What follows: a workgroup to a row, or several where rows have more groups than a list holds and a nucleus may have to be looked for in all of
-// them (launch rules in sample.hip).  Short lists are steps one behind the other, 12.5 us (64 rows of 50257, top-p 0.9; 256 of 128000, min-p); 13 rows of
-// 32000 with settings of every kind 22, the time of the row with the longest list; 100 flat rows of 201001, top-p 0.98, 64: 13 for what the chunks
+// them (launch rules in sample.hip).  Short lists are steps one behind the other, 12.0 to 12.8 us (256 rows of 128000, min-p; 64 of 50257, top-p 0.9); 13 rows of
+// 32000 with settings of every kind 22, the time of the row with the longest list; 100 flat rows of 201001, top-p 0.98, 65: 13 for what the chunks
 // left (50 MB, read by every workgroup of a row), 16 to look the rows through (80 MB), then 28 of the last workgroup of each: the cut 7, sums of the
 // chunks 6, those of the draw's chunk 8, the draw.
 template <int TYPE>

@@ -17,6 +17,8 @@ static void check_sizes(int type, int rows, int vocab) {
 
 // Rows of one chunk are picked from by the workgroup that reads them.  Longer ones are read in chunks by as many workgroups, wide chunks where
 // they keep every compute unit busy.  Rows of more groups than a list holds are looked through by up to eight workgroups, as many as the GPU has room for.
+// (Flat rows, fp32, top-p 0.98, 1 and 64 of them: 140000 tokens 51 and 83 us.  Below that border one workgroup does it from a list of groups: 32000 tokens 62 and
+// 65, 64000 93 and 104, 128000 161 and 175.)
 constexpr int kUnits = 256, kMostShared = 512;
 struct SampleForm {
     int chunk = kChunk;

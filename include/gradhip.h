@@ -499,7 +499,10 @@ gh_status gh_cache_attend(gh_cache* c, int32_t layer, const gh_rows* q, const gh
 /* gh_cache_attend whose rows see, beside the last `window` positions, the first `sinks` of their sequence: positions u with
  * u > t - window or u < sinks (and u <= t if causal).  What lies between is not read.  window = 0 sees everything, whatever
  * `sinks` is; sinks = 0 is gh_cache_attend.  A row that would see a position that its sequence has forgotten is refused
- * (GH_ERR_OUT_OF_RANGE): with a window, what lies from `sinks` on and before the window of the pass's first row may be forgotten. */
+ * (GH_ERR_OUT_OF_RANGE): with a window, what lies from `sinks` on and before the window of the pass's first row may be forgotten.
+ * Positions are those in the text, for the sinks too: keys stay rotated to the places at which they were appended, so the distance from
+ * a stream's newest row to its sinks grows with the stream.  Schemes that number what is left in the cache instead, to keep that distance
+ * within what a rotary model was trained on, are not offered: a model that holds only up to some distance should not be run beyond it. */
 gh_status gh_cache_attend_sinks(gh_cache* c, int32_t layer, const gh_rows* q, const gh_rows* out, float scale, int32_t causal,
                                 int32_t window, int32_t sinks, void* hip_stream);
 
